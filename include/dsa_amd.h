@@ -486,6 +486,120 @@ DSA_API int dsa_sparse_mla_prefill(const void* q, int64_t q_token_stride, int64_
                                    int num_heads, int topk, float sm_scale, void* out,
                                    float* max_logits, float* lse, void* stream);
 
+/* ---- 4-bit caches ------------------------------------------------------------
+ * Blocks of 32 elements: e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign bit;
+ * element 2i in the low nibble of byte i) with one UE8M0 scale byte a block,
+ * value = code * 2^(byte - 127), byte 255 = a block of NaN.
+ *   MLA row, 400 bytes:   [256 B codes of the 512 nope dims][16 scale bytes]
+ *                         [64 x bf16 rope]
+ *   indexer page, page_size x 68 bytes: [page_size x 64 B codes of 128 dims]
+ *                         [page_size x 4 scale bytes]
+ * The writers take the smallest scale 2^k with amax <= 6 * 2^k, k in [-40, 125],
+ * and round to the nearest code, ties to the even one; larger magnitudes (and
+ * infinities) become the largest code, and a block that holds a NaN gets byte 255
+ * and zero codes. Slots that are negative or past the cache are skipped by the
+ * writers and read as zeros by the readers. When two tokens of one call name the
+ * same slot, the row holds pieces of either. The reference has no 4-bit caches;
+ * these entry points stand beside their fp8 counterparts, named in each. */
+
+/* Quantise and store MLA KV rows (counterpart of dsa_mla_kv_store).
+ *   kv       [num_tokens, 576] bf16, row stride kv_row_stride elements, rows 16-byte aligned
+ *   slots    [num_tokens] int32, or int64 when slot_is_64
+ *   kv_cache block b row r at kv_cache + b*kv_block_stride_bytes + r*400; 16-byte
+ *            aligned base and block stride */
+DSA_API int dsa_mla_kv_store_fp4(const void* kv, int64_t kv_row_stride, const void* slots,
+                                 int slot_is_64, int num_tokens, uint8_t* kv_cache,
+                                 int64_t kv_block_stride_bytes, int kv_block_size,
+                                 int64_t kv_num_blocks, void* stream);
+
+/* The rows at `slots` as bf16 [num_tokens, 576] (exact), row stride
+ * out_row_stride elements: the keys of a prefill over cached tokens, for
+ * dsa_sparse_mla_prefill (counterpart of the cached part of dsa_mla_prefill_kv). */
+DSA_API int dsa_mla_kv_load_fp4(const uint8_t* kv_cache, int64_t kv_block_stride_bytes,
+                                int kv_block_size, int64_t kv_num_blocks, const void* slots,
+                                int slot_is_64, int num_tokens, void* out,
+                                int64_t out_row_stride, void* stream);
+
+/* Sparse MLA decode over the 4-bit MLA cache (counterpart of
+ * dsa_sparse_mla_decode: same arguments, outputs, split counts and workspace;
+ * rows of 400 bytes). A head whose valid keys hold a NaN gets NaN outputs. */
+DSA_API int dsa_sparse_mla_decode_fp4(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                      const uint8_t* kv_cache, int64_t kv_block_stride_bytes,
+                                      int kv_block_size, int64_t kv_num_blocks,
+                                      const int32_t* indices, int64_t idx_stride,
+                                      int num_tokens, int num_heads, int topk, float sm_scale,
+                                      void* out, float* lse, int num_splits,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Quantise and store indexer keys (counterpart of dsa_indexer_k_store).
+ *   k        [num_tokens, 128] bf16, row stride k_row_stride elements, rows 16-byte aligned
+ *   cache    [num_pages, page_size*68] bytes, contiguous, 4-byte aligned */
+DSA_API int dsa_indexer_k_store_fp4(const void* k, int64_t k_row_stride, const void* slots,
+                                    int slot_is_64, int num_tokens, uint8_t* cache,
+                                    int page_size, int64_t num_pages, void* stream);
+
+/* The keys at `slots` as fp8 with one f32 scale each, the operands of
+ * dsa_mqa_logits and dsa_mqa_topk (counterpart of dsa_gather_indexer_cache).
+ *   key_out   [num_tokens, 128] e4m3fn bytes;  scale_out [num_tokens] f32
+ * scale = 2^-6 of the key's largest block scale (2^-126 at least), key = value /
+ * scale: exact for blocks whose scale is at most 2^14 below the key's largest,
+ * else rounded to e4m3's smallest step. NaN blocks give fp8 NaNs. */
+DSA_API int dsa_indexer_k_load_fp4(const uint8_t* cache, int page_size, int64_t num_pages,
+                                   const void* slots, int slot_is_64, int num_tokens,
+                                   uint8_t* key_out, float* scale_out, void* stream);
+
+/* Indexer logits over the 4-bit paged key cache (counterpart of
+ * dsa_indexer_logits).
+ *   q_fp8, weights, context_lens, block_tables, logits as there
+ *   kv_cache  [num_pages, 64*68] bytes, 16-byte aligned
+ * logits[b*n+j, t] = sum_h weights[b*n+j, h] * relu(q[b,j,h,:] . k[t,:])
+ * for t < context_lens[b, j], products exact and sums in f32. A key that is NaN
+ * scores NaN; positions on a page that is not in [0, num_pages) score -inf.
+ * Positions from the context length on: -inf up to max_context_len with
+ * clean_logits, else up to the end of the entry's last page only. */
+DSA_API int dsa_indexer_logits_fp4(const uint8_t* q_fp8, const uint8_t* kv_cache, int64_t num_pages,
+                                   const float* weights, const int32_t* context_lens,
+                                   const int32_t* block_tables, int64_t block_table_stride,
+                                   int batch, int next_n, int num_heads, int head_dim,
+                                   int page_size, int64_t max_context_len, float* logits,
+                                   int64_t logits_stride, int clean_logits, void* stream);
+
+/* Block tables and slot maps of a batch from its requests' lengths, on the device.
+ *   cached_lens, new_lens [batch] int32: tokens of request b in the cache (c_b)
+ *                and added by this step (n_b)
+ *   block_tables [batch, bt_width] int32, row stride bt_stride; holds request b's
+ *                first ceil(c_b / page_size) blocks, and gets the blocks of the
+ *                pages that its new tokens open. Other entries are left alone
+ *   free_blocks  [num_free] int32: those blocks are taken from it in request
+ *                order, from entry *free_head on (NULL: 0). NULL: the caller has
+ *                written the new pages' entries; nothing is taken or written
+ *   slots        [num_rows] int32, or int64: row r is new token j of request b (r =
+ *                n_0 + .. + n_(b-1) + j) at position p = c_b + j:
+ *                block_tables[b, p / page_size] * page_size + p % page_size.
+ *                Rows past the new tokens (a padded batch) get -1
+ *   positions    [num_rows] int32 or int64: p; 0 past the new tokens (may be NULL)
+ *   seq_lens     [num_rows] int32: p + 1, the causal length that the decode
+ *                entries take; 0 past the new tokens (may be NULL)
+ *   cu_seqlens_q, cu_seqlens_k [batch + 1] int32 or int64: prefix sums of n_b and of
+ *                c_b + n_b (either may be NULL)
+ *   status       [4] int64: {fault bits, new tokens, blocks taken, longest c_b + n_b}
+ * Fault bits: 1 a length is negative or c_b + n_b passes int32 (that request is
+ * taken as empty); 2 a request has more pages than bt_width; 4 the free list is too
+ * short; 8 more new tokens than num_rows; 16 a prefix sum does not fit int32 (it is
+ * stored as the largest). A token without a block (bits 2 and 4, or a negative
+ * block number), or whose slot does not fit int32, gets slot -1. With bit 8 only
+ * the first num_rows tokens are mapped and their blocks written.
+ * At most 8192 requests. No counterpart in the reference, whose host scheduler
+ * builds these (SequenceBatch block tables and slot_mapping, read by
+ * dlengine/runtime/context/batch.py:10-80). */
+DSA_API int dsa_batch_tables(const int32_t* cached_lens, const int32_t* new_lens, int batch,
+                             int32_t* block_tables, int64_t bt_stride, int bt_width,
+                             int page_size, const int32_t* free_blocks, int64_t num_free,
+                             const int32_t* free_head, void* slots, int slots_are_64,
+                             void* positions, int positions_are_64, int32_t* seq_lens,
+                             int64_t num_rows, void* cu_seqlens_q, void* cu_seqlens_k,
+                             int cu_is_64, int64_t* status, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

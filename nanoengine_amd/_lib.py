@@ -61,6 +61,16 @@ SIGNATURES = {
     "dsa_prefill_windows": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P, _P, _P, _P]),
     "dsa_indexer_k_transform_store": (c_int, [_P, c_int64, _P, _P, c_float, _P, c_int64, _P, c_int, _P, c_int,
                                               c_int, _P, c_int, _P]),
+    "dsa_batch_tables": (c_int, [_P, _P, c_int, _P, c_int64, c_int, c_int, _P, c_int64, _P, _P, c_int, _P, c_int, _P,
+                                 c_int64, _P, _P, c_int, _P, _P]),
+    "dsa_mla_kv_store_fp4": (c_int, [_P, c_int64, _P, c_int, c_int, _P, c_int64, c_int, c_int64, _P]),
+    "dsa_mla_kv_load_fp4": (c_int, [_P, c_int64, c_int, c_int64, _P, c_int, c_int, _P, c_int64, _P]),
+    "dsa_sparse_mla_decode_fp4": (c_int, [_P, c_int64, c_int64, _P, c_int64, c_int, c_int64, _P, c_int64, c_int,
+                                          c_int, c_int, c_float, _P, _P, c_int, _P, c_size_t, _P]),
+    "dsa_indexer_k_store_fp4": (c_int, [_P, c_int64, _P, c_int, c_int, _P, c_int, c_int64, _P]),
+    "dsa_indexer_k_load_fp4": (c_int, [_P, c_int, c_int64, _P, c_int, c_int, _P, _P, _P]),
+    "dsa_indexer_logits_fp4": (c_int, [_P, _P, c_int64, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int,
+                                       c_int64, _P, c_int64, c_int, _P]),
 }
 
 _lib = None

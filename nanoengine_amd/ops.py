@@ -18,6 +18,9 @@ MLA_D_V = 512
 INDEXER_HEADS = 64
 INDEXER_HEAD_DIM = 128
 INDEXER_ROW_BYTES = INDEXER_HEAD_DIM + 4
+# the 4-bit caches: e2m1 codes and one scale byte per 32 elements (include/dsa_amd.h)
+MLA_FP4_ROW_BYTES = MLA_D_V // 2 + MLA_D_V // 32 + 2 * (MLA_D_QK - MLA_D_V)
+INDEXER_FP4_ROW_BYTES = INDEXER_HEAD_DIM // 2 + INDEXER_HEAD_DIM // 32
 
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -740,3 +743,237 @@ def sparse_mla_prefill_paged(q: torch.Tensor, k_cache: torch.Tensor, block_table
               topk, float(sm_scale), out.data_ptr(), max_logits.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
               workspace.numel(), _stream(dev))
     return out, max_logits, lse
+
+
+# --------------------------------------------------------------------------- 4-bit caches
+def _launch(dev: torch.device, name: str, *args) -> None:
+    """Call ``name`` with the current stream of ``dev`` as its last argument, on ``dev``."""
+    if dev.index == torch.cuda.current_device():
+        _lib.call(name, *args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _stream(dev))
+
+
+def mla_fp4_geometry(k_cache: torch.Tensor) -> tuple[int, int]:
+    """(block stride in bytes, rows per block) of a 4-bit MLA cache view
+    [num_blocks, block_size, (1,) 400] whose block stride may include a padding row."""
+    if not (k_cache.dtype == torch.uint8 and k_cache.dim() in (3, 4)
+            and k_cache.shape[-1] == MLA_FP4_ROW_BYTES and k_cache.stride(-1) == 1):
+        _fail(f"k_cache must be uint8 [blocks, block_size, (1,) {MLA_FP4_ROW_BYTES}] with contiguous rows, "
+              f"got {k_cache.dtype} {tuple(k_cache.shape)}")
+    if k_cache.dim() == 4 and k_cache.shape[2] != 1:
+        _fail("MLA cache has one KV head")
+    block_size = k_cache.shape[1]
+    if block_size > 1 and k_cache.stride(1) != MLA_FP4_ROW_BYTES:
+        _fail(f"rows inside a block must be {MLA_FP4_ROW_BYTES} B apart")
+    return (k_cache.stride(0) if k_cache.shape[0] > 1 else block_size * MLA_FP4_ROW_BYTES), block_size
+
+
+def _fp4_pages(cache: torch.Tensor, page_size: int) -> int:
+    """Pages of a contiguous 4-bit indexer cache."""
+    page_bytes = int(page_size) * INDEXER_FP4_ROW_BYTES
+    if not (page_bytes > 0 and cache.dtype == torch.uint8 and cache.is_contiguous()
+            and cache.numel() % page_bytes == 0):
+        _fail(f"cache must be contiguous uint8 pages of page_size*{INDEXER_FP4_ROW_BYTES} bytes")
+    return cache.numel() // page_bytes
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Row stride of a 2-D tensor (torch leaves that of a single row free)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def mla_kv_store_fp4(kv: torch.Tensor, k_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """Quantise kv [N, (1,) 576] bf16 into the 4-bit MLA cache [blocks, block_size, (1,) 400] at
+    slot_mapping; slots that are negative or past the cache are skipped (see dsa_mla_kv_store_fp4)."""
+    if not (kv.dim() in (2, 3) and kv.dtype == torch.bfloat16 and kv.shape[-1] == MLA_D_QK and kv.stride(-1) == 1
+            and (kv.dim() == 2 or kv.shape[1] == 1)):
+        _fail(f"kv must be bf16 [N, (1,) {MLA_D_QK}] with a contiguous last dim")
+    blk_stride, block_size = mla_fp4_geometry(k_cache)
+    n = kv.shape[0]
+    slots, is64 = _slots(slot_mapping, n)
+    dev = _check_cuda(kv, k_cache, slots)
+    _launch(dev, "dsa_mla_kv_store_fp4", kv.data_ptr(), kv.stride(0) if n > 1 else MLA_D_QK, slots.data_ptr(), is64, n,
+            k_cache.data_ptr(), blk_stride, block_size, k_cache.shape[0])
+
+
+def mla_kv_load_fp4(k_cache: torch.Tensor, slots: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The 4-bit MLA rows at slots [N] as bf16 [N, 576] (exact; zeros for slots that are negative or
+    past the cache): the cached keys of a prefill for ``sparse_mla_prefill`` (see dsa_mla_kv_load_fp4)."""
+    blk_stride, block_size = mla_fp4_geometry(k_cache)
+    s, is64 = _slots(slots, 0)
+    n = s.shape[0]
+    dev = _check_cuda(k_cache, s)
+    if out is None:
+        out = torch.empty(n, MLA_D_QK, dtype=torch.bfloat16, device=dev)
+    if not (out.dtype == torch.bfloat16 and tuple(out.shape) == (n, MLA_D_QK) and out.stride(1) == 1):
+        _fail(f"out must be bf16 [{n}, {MLA_D_QK}] with a contiguous last dim")
+    _check_cuda(k_cache, out)
+    _launch(dev, "dsa_mla_kv_load_fp4", k_cache.data_ptr(), blk_stride, block_size, k_cache.shape[0], s.data_ptr(), is64, n,
+            out.data_ptr(), _row_stride(out))
+    return out
+
+
+def sparse_mla_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, indices: torch.Tensor, sm_scale: float,
+                          out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                          num_splits: int | None = None,
+                          workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``sparse_mla_decode`` over the 4-bit MLA cache: q [T,H,576] bf16, k_cache [blocks, block_size,
+    (1,) 400] uint8, indices [T,topk] int32 physical slots -> (o [T,H,512] bf16, lse [T,H] f32)."""
+    if not (q.dim() == 3 and q.shape[2] == MLA_D_QK and q.dtype == torch.bfloat16 and q.stride(2) == 1):
+        _fail(f"q must be bf16 [T, H, {MLA_D_QK}] with a contiguous last dim")
+    T, H, _ = q.shape
+    if not (indices.dim() == 2 and indices.shape[0] == T and indices.dtype == torch.int32
+            and indices.stride(1) == 1):
+        _fail("indices must be int32 [T, topk] with unit column stride")
+    topk = indices.shape[1]
+    blk_stride, block_size = mla_fp4_geometry(k_cache)
+    dev = _check_cuda(q, k_cache, indices)
+    if out is None:
+        out = torch.empty(T, H, MLA_D_V, dtype=torch.bfloat16, device=dev)
+    if lse is None:
+        lse = torch.empty(T, H, dtype=torch.float32, device=dev)
+    if not (out.dtype == torch.bfloat16 and tuple(out.shape) == (T, H, MLA_D_V) and out.is_contiguous()):
+        _fail("out must be contiguous bf16 [T, H, 512]")
+    if not (lse.dtype == torch.float32 and tuple(lse.shape) == (T, H) and lse.is_contiguous()):
+        _fail("lse must be contiguous f32 [T, H]")
+    _check_cuda(q, out, lse)
+    if num_splits is None:
+        num_splits = sparse_mla_num_splits(T, H, topk, dev)
+    need = sparse_mla_workspace_bytes(T, H, num_splits)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    _launch(dev, "dsa_sparse_mla_decode_fp4", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), blk_stride,
+            block_size, k_cache.shape[0], indices.data_ptr(), indices.stride(0), T, H, topk, float(sm_scale),
+            out.data_ptr(), lse.data_ptr(), int(num_splits), workspace.data_ptr() if need else None,
+            workspace.numel() * workspace.element_size() if need else 0)
+    return out, lse
+
+
+def indexer_k_store_fp4(key: torch.Tensor, cache: torch.Tensor, slot_mapping: torch.Tensor, page_size: int) -> None:
+    """Quantise indexer keys [N, 128] bf16 into the 4-bit pages [pages, page_size*68]; slots that are
+    negative or past the cache are skipped (see dsa_indexer_k_store_fp4)."""
+    if not (key.dim() == 2 and key.shape[1] == INDEXER_HEAD_DIM and key.dtype == torch.bfloat16
+            and key.stride(1) == 1):
+        _fail("key must be bf16 [N, 128] with a contiguous last dim")
+    pages = _fp4_pages(cache, page_size)
+    slots, is64 = _slots(slot_mapping, key.shape[0])
+    dev = _check_cuda(key, cache, slots)
+    _launch(dev, "dsa_indexer_k_store_fp4", key.data_ptr(), _row_stride(key), slots.data_ptr(), is64, key.shape[0],
+            cache.data_ptr(), int(page_size), pages)
+
+
+def indexer_k_load_fp4(cache: torch.Tensor, slots: torch.Tensor, page_size: int, key_out: torch.Tensor | None = None,
+                       scale_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The 4-bit indexer keys at slots [N] as (fp8 keys [N, 128] float8_e4m3fn, scales [N] f32), the
+    operands of ``mqa_logits`` and ``mqa_topk`` (see dsa_indexer_k_load_fp4)."""
+    pages = _fp4_pages(cache, page_size)
+    s, is64 = _slots(slots, 0)
+    n = s.shape[0]
+    dev = _check_cuda(cache, s)
+    if key_out is None:
+        key_out = torch.empty(n, INDEXER_HEAD_DIM, dtype=torch.float8_e4m3fn, device=dev)
+    if scale_out is None:
+        scale_out = torch.empty(n, dtype=torch.float32, device=dev)
+    if not (key_out.dtype in (torch.float8_e4m3fn, torch.uint8) and tuple(key_out.shape) == (n, INDEXER_HEAD_DIM)
+            and key_out.is_contiguous()):
+        _fail(f"key_out must be contiguous fp8 [{n}, 128]")
+    if not (scale_out.dtype == torch.float32 and scale_out.numel() == n and scale_out.is_contiguous()):
+        _fail(f"scale_out must be contiguous f32 [{n}]")
+    _check_cuda(cache, key_out, scale_out)
+    _launch(dev, "dsa_indexer_k_load_fp4", cache.data_ptr(), int(page_size), pages, s.data_ptr(), is64, n,
+            key_out.data_ptr(), scale_out.data_ptr())
+    return key_out, scale_out
+
+
+def indexer_logits_fp4(q_fp8: torch.Tensor, kv_cache: torch.Tensor, weights: torch.Tensor,
+                       context_lens: torch.Tensor, block_tables: torch.Tensor, max_context_len: int,
+                       out: torch.Tensor | None = None, clean_logits: bool = True) -> torch.Tensor:
+    """Indexer logits [B*n, max_context_len] f32 over the 4-bit pages [num_pages, 64*68] (see
+    dsa_indexer_logits_fp4). With ``clean_logits`` the positions past each row's length are -inf; without
+    it only those up to the end of its last page are written."""
+    if not (q_fp8.dim() == 4 and q_fp8.dtype in (torch.float8_e4m3fn, torch.uint8) and q_fp8.is_contiguous()):
+        _fail(f"q_fp8 must be contiguous fp8 [B, next_n, H, D], got {q_fp8.dtype} {tuple(q_fp8.shape)}")
+    B, n, H, D = q_fp8.shape
+    page_size = 64
+    pages = _fp4_pages(kv_cache, page_size)
+    if not (weights.dtype == torch.float32 and tuple(weights.shape) == (B * n, H)):
+        _fail(f"weights must be f32 [{B * n}, {H}], got {weights.dtype} {tuple(weights.shape)}")
+    weights = weights.contiguous()
+    if not (context_lens.numel() == B * n):
+        _fail(f"context_lens must be [B, next_n]={B, n}, got {tuple(context_lens.shape)}")
+    cl = context_lens.to(torch.int32).contiguous()
+    if not (block_tables.dim() == 2 and block_tables.shape[0] == B):
+        _fail("block_tables must be [B, M]")
+    bt = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
+    if not (bt.stride(1) == 1):
+        _fail("block_tables rows must be contiguous")
+    if not (max_context_len >= 0 and bt.shape[1] * page_size >= max_context_len):
+        _fail("block_tables too narrow for max_context_len")
+    dev = _check_cuda(q_fp8, kv_cache, weights, cl, bt)
+    if out is None:
+        out = torch.empty(B * n, max_context_len, dtype=torch.float32, device=dev)
+    if not (out.dtype == torch.float32 and out.dim() == 2 and out.shape[0] == B * n
+            and out.shape[1] >= max_context_len and (out.shape[1] < 2 or out.stride(1) == 1)):
+        _fail("logits output must be f32 [B*n, >=max_ctx] with unit column stride")
+    _check_cuda(q_fp8, out)
+    _launch(dev, "dsa_indexer_logits_fp4", q_fp8.data_ptr(), kv_cache.data_ptr(), pages, weights.data_ptr(), cl.data_ptr(),
+            bt.data_ptr(), bt.stride(0), B, n, H, D, page_size, int(max_context_len), out.data_ptr(),
+            _row_stride(out), int(bool(clean_logits)))
+    return out
+
+
+# --------------------------------------------------------------------------- batch tables
+def _int_out(t: torch.Tensor | None, n: int, name: str, dtypes=(torch.int32, torch.int64)) -> int:
+    """1 when the optional output is int64."""
+    if t is None:
+        return 0
+    if not (t.dtype in dtypes and tuple(t.shape) == (n,) and t.is_contiguous()):
+        _fail(f"{name} must be contiguous {' or '.join(str(d).replace('torch.', '') for d in dtypes)} [{n}]")
+    return int(t.dtype == torch.int64)
+
+
+def batch_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor, page_size: int,
+                 slot_mapping: torch.Tensor, status: torch.Tensor, *, free_blocks: torch.Tensor | None = None,
+                 free_head: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                 seq_lens: torch.Tensor | None = None, cu_seqlens_q: torch.Tensor | None = None,
+                 cu_seqlens_k: torch.Tensor | None = None) -> None:
+    """Extend a batch's block tables and map its new tokens to cache slots, on the device, from each
+    request's cached and new token counts [B] int32 (see dsa_batch_tables for every output and for the
+    fault bits of ``status`` [4] int64, which the caller reads when it next synchronises)."""
+    if not (cached_lens.dim() == 1 and cached_lens.dtype == torch.int32 and cached_lens.is_contiguous()
+            and new_lens.shape == cached_lens.shape and new_lens.dtype == torch.int32 and new_lens.is_contiguous()):
+        _fail("cached_lens and new_lens must be contiguous int32 [B]")
+    B = cached_lens.shape[0]
+    if not (block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.dtype == torch.int32
+            and (block_tables.stride(1) == 1 or block_tables.shape[1] < 2)):
+        _fail("block_tables must be int32 [B, M] with unit column stride")
+    if B > 1 and block_tables.stride(0) < block_tables.shape[1]:
+        _fail("block_tables rows must not overlap")
+    if page_size <= 0:
+        raise ValueError("page_size must be positive")
+    rows = slot_mapping.shape[0] if slot_mapping.dim() == 1 else -1
+    s64 = _int_out(slot_mapping, rows, "slot_mapping")
+    p64 = _int_out(positions, rows, "positions")
+    _int_out(seq_lens, rows, "seq_lens", (torch.int32,))
+    c64 = _int_out(cu_seqlens_q, B + 1, "cu_seqlens_q")
+    k64 = _int_out(cu_seqlens_k, B + 1, "cu_seqlens_k")
+    if cu_seqlens_q is not None and cu_seqlens_k is not None and c64 != k64:
+        _fail("cu_seqlens_q and cu_seqlens_k must share one dtype")
+    if not (status.dtype == torch.int64 and status.numel() == 4 and status.is_contiguous()):
+        _fail("status must be contiguous int64 [4]")
+    if free_blocks is not None and not (free_blocks.dim() == 1 and free_blocks.dtype == torch.int32
+                                        and free_blocks.is_contiguous()):
+        _fail("free_blocks must be contiguous int32 [F]")
+    if free_head is not None and not (free_head.dtype == torch.int32 and free_head.numel() == 1):
+        _fail("free_head must be int32 with one element")
+    dev = _check_cuda(*(t for t in (cached_lens, new_lens, block_tables, slot_mapping, status, free_blocks, free_head,
+                                    positions, seq_lens, cu_seqlens_q, cu_seqlens_k) if t is not None))
+    # an empty free list still means that blocks are taken from it
+    free_ptr = None if free_blocks is None else (free_blocks.data_ptr() or status.data_ptr())
+    _launch(dev, "dsa_batch_tables", cached_lens.data_ptr(), new_lens.data_ptr(), B, block_tables.data_ptr(),
+            _row_stride(block_tables), block_tables.shape[1], int(page_size), free_ptr,
+            0 if free_blocks is None else free_blocks.shape[0], _ptr(free_head), slot_mapping.data_ptr(), s64,
+            _ptr(positions), p64, _ptr(seq_lens), rows, _ptr(cu_seqlens_q), _ptr(cu_seqlens_k), c64 or k64,
+            status.data_ptr())

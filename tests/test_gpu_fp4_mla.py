@@ -1,0 +1,151 @@
+"""Sparse MLA decode over the 4-bit cache on the GPU, against float64 with the oracle's bounds."""
+import pytest
+import torch
+
+from nanoengine_amd import ops
+from oracle import fp4_oracle as F
+
+pytestmark = pytest.mark.gpu
+SCALE = 192 ** -0.5
+
+
+def _cache(blocks, seed, device, block_size=64, pad=1, spread=0.0):
+    """[blocks, block_size, 1, 400] view (rows of quantised normal values, channels of different size) and its values."""
+    g = torch.Generator(device=device).manual_seed(seed)
+    kv = torch.randn(blocks * block_size, 576, generator=g, device=device)
+    kv = kv * torch.exp(spread * torch.randn(576, generator=g, device=device))
+    rows = F.mla_rows(kv.to(torch.bfloat16))
+    buf = torch.full((blocks, block_size + pad, 1, 400), 0xff, dtype=torch.uint8, device=device)
+    buf[:, :block_size, 0] = rows.view(blocks, block_size, 400)
+    return buf[:, :block_size], F.mla_values(rows)
+
+
+def _query(T, H, seed, device):
+    return torch.randn(T, H, 576, generator=torch.Generator(device=device).manual_seed(seed + 1),
+                       device=device).to(torch.bfloat16)
+
+
+def _indices(T, K, total, seed, device, invalid=0.0):
+    g = torch.Generator().manual_seed(seed)
+    idx = torch.stack([torch.randperm(max(total, K), generator=g)[:K] for _ in range(T)])
+    idx[torch.rand(T, K, generator=g) < invalid] = -1
+    return idx.to(torch.int32).to(device)
+
+
+def _check(o, lse, q, values, idx, scale):
+    for t in range(q.shape[0]):
+        at = idx[t].long()
+        at = at[(at >= 0) & (at < values.shape[0])]
+        eo, el, ot, lt = F.attend(q[t], values[at], scale)
+        assert torch.all((o[t].double() - eo).abs() <= ot + 1e-30), (t, (o[t].double() - eo).abs().max())
+        if at.numel() == 0:
+            assert torch.all(o[t] == 0) and torch.all(torch.isneginf(lse[t]))
+        else:
+            assert torch.all((lse[t].double() - el).abs() <= lt), (t, (lse[t].double() - el).abs().max())
+
+
+@pytest.mark.parametrize("T,H,K,invalid", [(1, 16, 64, 0.0), (3, 32, 192, 0.3), (2, 48, 320, 0.1), (5, 64, 512, 0.0),
+                                           (2, 80, 2048, 0.5), (3, 128, 2048, 0.0), (9, 128, 576, 0.05),
+                                           (130, 128, 64, 0.2), (300, 16, 512, 0.1)])
+def test_matches_float64(cuda, T, H, K, invalid):
+    print(f"mla fp4 T={T} H={H} K={K}", flush=True)
+    cache, values = _cache(40, T * 1000 + K, cuda)
+    q, idx = _query(T, H, T, cuda), _indices(T, K, 40 * 64, K, cuda, invalid)
+    o, lse = ops.sparse_mla_decode_fp4(q, cache, idx, SCALE)
+    torch.cuda.synchronize()
+    _check(o, lse, q, values, idx, SCALE)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 4, 8, 32])
+def test_split_counts(cuda, splits):
+    cache, values = _cache(40, 3, cuda)
+    q, idx = _query(2, 128, 3, cuda), _indices(2, 2048, 2560, 3, cuda, 0.02)
+    idx[1, 64:] = -1                                # every split but the first has no key
+    o, lse = ops.sparse_mla_decode_fp4(q, cache, idx, SCALE, num_splits=splits)
+    torch.cuda.synchronize()
+    _check(o, lse, q, values, idx, SCALE)
+
+
+def test_rows_without_keys_and_short_rows(cuda):
+    cache, values = _cache(40, 4, cuda)
+    q, idx = _query(6, 64, 4, cuda), _indices(6, 512, 2560, 4, cuda)
+    idx[0] = -1                                     # nothing
+    idx[1, 1:] = -1                                 # one key, the first
+    idx[2, :511] = -1                               # one key, the last
+    idx[3, :32] = -1                                # no key in the first half of the first block
+    idx[4, 40:] = 10 ** 6                           # stale slots past the cache
+    idx[5, ::2] = -5
+    for splits in (1, 2, 8):
+        o, lse = ops.sparse_mla_decode_fp4(q, cache, idx, SCALE, num_splits=splits)
+        torch.cuda.synchronize()
+        _check(o, lse, q, values, idx, SCALE)
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.0, 1e-4])
+@pytest.mark.parametrize("order", ["random", "rising", "falling"])
+def test_far_apart_scores(cuda, scale, order):
+    """A softmax scale of 1 spreads the scores over hundreds of powers of two; in rising order every block moves
+    the running maximum, in falling order (interleaved by halves of a block) the second half stays far below."""
+    cache, values = _cache(40, 5, cuda, spread=0.5)
+    q, idx = _query(2, 64, 5, cuda), _indices(2, 1024, 2560, 5, cuda)
+    if order != "random":
+        s = (values[idx.long()] @ q[:, 0].double()[..., None]).squeeze(-1)
+        by = s.argsort(dim=1, descending=order == "falling")
+        if order == "falling":
+            a, b = by[:, :512].view(2, 16, 32), by[:, 512:].flip(1).view(2, 16, 32)
+            by = torch.stack([a, b], dim=2).view(2, 1024)
+        idx = idx.gather(1, by)
+    o, lse = ops.sparse_mla_decode_fp4(q, cache, idx, scale)
+    torch.cuda.synchronize()
+    _check(o, lse, q, values, idx, scale)
+
+
+@pytest.mark.parametrize("block_size,pad", [(64, 0), (48, 1), (1, 0), (256, 3)])
+def test_cache_geometries(cuda, block_size, pad):
+    blocks = 4096 // block_size + 1
+    cache, values = _cache(blocks, 6, cuda, block_size, pad)
+    q, idx = _query(3, 32, 6, cuda), _indices(3, 256, blocks * block_size, 6, cuda)
+    o, lse = ops.sparse_mla_decode_fp4(q, cache, idx, SCALE)
+    torch.cuda.synchronize()
+    _check(o, lse, q, values, idx, SCALE)
+
+
+def test_strided_query_indices_and_given_outputs(cuda):
+    cache, values = _cache(40, 7, cuda)
+    q = _query(4, 128, 7, cuda).view(4, 2, 64, 576)[:, 1]                       # 64 of 128 heads
+    idx = torch.nn.functional.pad(_indices(4, 512, 2560, 7, cuda), (3, 5), value=1)[:, 3:515]
+    o = torch.empty(4, 64, 512, dtype=torch.bfloat16, device=cuda)
+    lse = torch.empty(4, 64, device=cuda)
+    got = ops.sparse_mla_decode_fp4(q, cache, idx, SCALE, out=o, lse=lse)
+    torch.cuda.synchronize()
+    assert got[0] is o and got[1] is lse
+    _check(o, lse, q, values, idx, SCALE)
+
+
+def test_scale_bytes_far_apart(cuda):
+    """Rows whose blocks differ by up to 2^40 in size, and rows of zeros."""
+    g = torch.Generator(device=cuda).manual_seed(8)
+    kv = torch.randn(2560, 576, generator=g, device=cuda)
+    kv[:, :512] *= torch.exp2(torch.randint(-20, 6, (2560, 16), generator=g, device=cuda).float()).repeat_interleave(32, 1)
+    kv[::7, :512] = 0
+    rows = F.mla_rows(kv.to(torch.bfloat16))
+    q, idx = _query(3, 64, 8, cuda), _indices(3, 512, 2560, 8, cuda)
+    o, lse = ops.sparse_mla_decode_fp4(q, rows.view(40, 64, 400), idx, 0.002)
+    torch.cuda.synchronize()
+    _check(o, lse, q, F.mla_values(rows), idx, 0.002)
+
+
+def test_nan_rows(cuda):
+    """A NaN in a selected row makes its token's outputs NaN; in a row that no token selects, or behind a skipped
+    index, it does nothing."""
+    cache, values = _cache(40, 9, cuda)
+    idx = torch.stack([torch.arange(0, 256), torch.arange(1000, 1256), torch.arange(0, 256)]).to(torch.int32).to(cuda)
+    idx[2, 17] = -1
+    cache[0, 17, 0, 256 + 3] = 255                  # slot 17: selected by token 0 only
+    cache[30, 1, 0, 256 + 3] = 255                  # by none
+    q = _query(3, 128, 9, cuda)
+    for splits in (1, 4):
+        o, lse = ops.sparse_mla_decode_fp4(q, cache, idx, SCALE, num_splits=splits)
+        torch.cuda.synchronize()
+        assert torch.all(torch.isnan(o[0])) and torch.all(torch.isnan(lse[0]))
+        _check(o[1:], lse[1:], q[1:], values, idx[1:], SCALE)
