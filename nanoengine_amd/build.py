@@ -19,7 +19,7 @@ MICROBENCH_SRC = "microbench.hip"
 MICROBENCH_LIB = PKG_DIR / "libdsa_microbench.so"
 SOURCES = ["capi.hip", "topk.hip", "indexer.hip", "sparse_mla.hip", "cache_store.hip",
            "indexer_prologue.hip", "prefill_logits.hip", "sparse_mla_prefill.hip",
-           "prefill_topk.hip", "cache_store_fp4.hip", "indexer_fp4.hip", "sparse_mla_fp4.hip", "batch_tables.hip"]
+           "prefill_topk.hip", "cache_store_fp4.hip", "indexer_fp4.hip", "batch_tables.hip"]
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -50,7 +50,6 @@ PER_FILE_FLAGS = {
     "prefill_topk.hip": VGPR_FORM,
     "cache_store_fp4.hip": [],
     "indexer_fp4.hip": VGPR_FORM,
-    "sparse_mla_fp4.hip": [],
     "batch_tables.hip": [],
 }
 

@@ -151,12 +151,14 @@ struct MlaFresh {
 // Sparse MLA decode over physical slots of the paged fp8 cache (the body of
 // dsa_sparse_mla_decode), with the fresh rows of a chunked prefill where `fresh`
 // is given. max_out (splits == 1 only) receives each head's largest scaled score
-// in natural units.
+// in natural units. fp4: the cache's rows are the 400-byte ones of fp4.h (no
+// fresh rows then).
 int sparse_mla_decode_impl(const void* q, int64_t q_token_stride, int64_t q_head_stride, const uint8_t* kv_cache,
                            int64_t kv_block_stride_bytes, int kv_block_size, int64_t kv_num_blocks,
                            const int32_t* indices, int64_t idx_stride, int num_tokens, int num_heads, int topk,
                            float sm_scale, void* out, float* lse, int num_splits, void* workspace,
-                           size_t workspace_bytes, void* stream, float* max_out, const MlaFresh* fresh);
+                           size_t workspace_bytes, void* stream, float* max_out, const MlaFresh* fresh,
+                           bool fp4 = false);
 
 // The same kernel over bf16 rows only: token t attends over rows[indices[t][i]]
 // (row stride in elements), i < topk, a multiple of 32; an index outside

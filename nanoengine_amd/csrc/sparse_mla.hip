@@ -59,6 +59,7 @@
 #include <cmath>
 
 #include "dsa_common.h"
+#include "fp4.h"
 #include "../../include/dsa_amd.h"
 
 namespace dsa {
@@ -73,7 +74,6 @@ constexpr int kMlaWaves = kMlaThreads / 64;
 constexpr int kMlaHeadsPerWG = 64;
 constexpr int kMlaKeys = 64;              // rows per block
 constexpr int kMlaRowBytes = 656;
-constexpr int kMlaRowPieces = kMlaRowBytes / 16;      // 41
 constexpr int kMlaDv = 512;
 constexpr int kBufBytes = kMlaKeys * kMlaRowBytes;    // 41984: one block of packed raw rows
 // A chunked prefill's fresh keys are bf16 rows [576] (1152 B), 32 to a block:
@@ -83,7 +83,6 @@ constexpr int kFreshRowBytes = 576 * 2;
 constexpr int kFreshRowPieces = kFreshRowBytes / 16;  // 72
 constexpr int kFreshDma = kFreshKeys * kFreshRowBytes / 1024;  // 36
 static_assert(kFreshKeys * kFreshRowBytes <= kBufBytes, "a fresh block must fit a row buffer");
-constexpr int kDmaPerBlock = kBufBytes / 1024;        // 41 wave-wide 16-byte loads per block
 constexpr int kNumBufs = 3;
 // LDS map (bytes)
 constexpr int kPOff = kNumBufs * kBufBytes;            // P, two blocks: [2][2 hp][4 k-steps][64 lanes][8 bf16]
@@ -117,10 +116,17 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr float kMinLogP = -30.0f;
 constexpr int kDropExp = -30;
 // The keys of an instantiation: cache slots (decode), cache slots then bf16
-// rows (paged prefill), bf16 rows only (prefill over assembled keys).
-enum KeyKind : int { kSlots = 0, kSlotsThenRows = 1, kRows = 2 };
+// rows (paged prefill), bf16 rows only (prefill over assembled keys), slots of a
+// 4-bit cache (decode).
+enum KeyKind : int { kSlots = 0, kSlotsThenRows = 1, kRows = 2, kSlots4 = 3 };
 template <int kKeys>
-constexpr int buf_bytes() { return kKeys == kRows ? kRowsBufBytes : kBufBytes; }
+constexpr int row_bytes() { return kKeys == kSlots4 ? kMla4RowBytes : kMlaRowBytes; }
+template <int kKeys>
+constexpr int buf_bytes() { return kKeys == kRows ? kRowsBufBytes : kMlaKeys * row_bytes<kKeys>(); }
+template <int kKeys>
+constexpr int row_pieces() { return row_bytes<kKeys>() / 16; }  // 41, or 25 of 4-bit rows
+template <int kKeys>
+constexpr int block_dma() { return kMlaKeys * row_bytes<kKeys>() / 1024; }  // wave-wide loads of a block
 constexpr int kIdxWave = 3;                // the wave that fetches the row indices (a QK wave)
 
 // Output staging of a PV wave: 32 heads x 128 dims, rows 16 bytes apart from a
@@ -128,7 +134,8 @@ constexpr int kIdxWave = 3;                // the wave that fetches the row indi
 constexpr int kStageRow16 = 128 * 2 + 16, kStageRow32 = 128 * 4 + 16;
 constexpr int kStageOut = 32 * kStageRow32;
 static_assert(4 * kStageOut <= kEOff, "the output staging lies in the row and P buffers");
-static_assert(kBufBytes % 1024 == 0, "a block of rows must be whole wave-wide loads");
+static_assert(buf_bytes<kSlots>() % 1024 == 0 && buf_bytes<kSlots4>() % 1024 == 0,
+              "a block of rows must be whole wave-wide loads");
 static_assert(kMlaSmemBytes <= 160 * 1024 && kRowsSmemBytes <= 160 * 1024, "LDS budget");
 static_assert(4 * kStageOut <= kRowsXOff, "the output staging lies in the row buffers");
 
@@ -246,7 +253,9 @@ constexpr int kTabWave = 2;  // the wave that builds the row-address table (a QK
 constexpr int kQRowBytes = 576 * 2;
 constexpr int kQPieces = kQRowBytes / 16;                          // 72
 constexpr int kQDma = kMlaHeadsPerWG * kQRowBytes / 1024;          // 72 wave-wide copies
-static_assert(kMlaHeadsPerWG * kQRowBytes <= 2 * kRowsBufBytes, "the query fits two row buffers of either size");
+static_assert(kMlaHeadsPerWG * kQRowBytes <= 2 * kRowsBufBytes &&
+                  buf_bytes<kSlots4>() + kMlaHeadsPerWG * kQRowBytes <= kPOff,
+              "the query fits what lies between row buffer 0 and P");
 static_assert(kQDma % kMlaWaves == 0 && kQPieces % 8 == 0, "query copies per wave, swizzle groups");
 
 // Wave-uniform state of one workgroup's loop. Blocks [0, ncached) are 64 cache
@@ -273,6 +282,7 @@ __device__ __forceinline__ bool slot_valid(const MlaParams& P, int32_t slot) {
   return slot >= 0 && slot_block(P, slot) < P.kv_num_blocks;
 }
 
+template <int kKeys>
 __device__ __forceinline__ uint64_t row_address(const MlaParams& P, int32_t slot) {
   if (!slot_valid(P, slot)) return reinterpret_cast<uint64_t>(g_mla_zero_row);
   int64_t blk, in_blk;
@@ -283,7 +293,7 @@ __device__ __forceinline__ uint64_t row_address(const MlaParams& P, int32_t slot
     blk = slot / P.kv_block_size;
     in_blk = slot % P.kv_block_size;
   }
-  return reinterpret_cast<uint64_t>(P.kv + blk * P.kv_blk_stride + in_blk * kMlaRowBytes);
+  return reinterpret_cast<uint64_t>(P.kv + blk * P.kv_blk_stride + in_blk * row_bytes<kKeys>());
 }
 
 // A fresh row index is used when it is in [0, fresh_rows); a fresh block's
@@ -299,7 +309,7 @@ __device__ __forceinline__ void build_addr_table(const MlaParams& P, uint8_t* sm
   const int32_t slot = reinterpret_cast<const int32_t*>(smem + kRingOff + (j % kRingSlots) * 256)[lane];
   uint64_t a;
   if (!rows_block<kKeys>(c, j))
-    a = row_address(P, slot);
+    a = row_address<kKeys>(P, slot);
   else
     a = fresh_valid(P, slot, lane) ? reinterpret_cast<uint64_t>(P.fresh + (int64_t)slot * P.fresh_row_stride)
                                    : reinterpret_cast<uint64_t>(g_mla_zero_row);
@@ -307,15 +317,20 @@ __device__ __forceinline__ void build_addr_table(const MlaParams& P, uint8_t* sm
 }
 
 // Wave w sends loads [first(w), first(w) + count(w)) of the block: six for
-// wave 0, five for the others, in runs that share one M0 (LDS base) value.
+// wave 0, five for the others (4-bit rows: four and three), in runs that share
+// one M0 (LDS base) value.
+template <int kKeys>
 __device__ __forceinline__ int dma_count(int wave) {
-  return kDmaPerBlock / kMlaWaves + (wave < kDmaPerBlock % kMlaWaves ? 1 : 0);
+  return block_dma<kKeys>() / kMlaWaves + (wave < block_dma<kKeys>() % kMlaWaves ? 1 : 0);
 }
+template <int kKeys>
 __device__ __forceinline__ int dma_first(int wave) {
-  return wave * (kDmaPerBlock / kMlaWaves) + min(wave, kDmaPerBlock % kMlaWaves);
+  return wave * (block_dma<kKeys>() / kMlaWaves) + min(wave, block_dma<kKeys>() % kMlaWaves);
 }
-static_assert(kDmaPerBlock / kMlaWaves == 5 && kDmaPerBlock % kMlaWaves == 1,
+static_assert(block_dma<kSlots>() / kMlaWaves == 5 && block_dma<kSlots>() % kMlaWaves == 1,
               "six loads for wave 0, five for the others");
+static_assert(block_dma<kSlots4>() / kMlaWaves == 3 && block_dma<kSlots4>() % kMlaWaves == 1,
+              "four loads for wave 0, three for the others");
 
 // Load i of this lane: table byte offset 8 * row in bits 0-15, byte offset
 // within the row in bits 16-31.
@@ -323,13 +338,14 @@ struct DmaLanes {
   uint32_t pk[6];
 };
 
+template <int kKeys>
 __device__ __forceinline__ DmaLanes dma_lanes(int wave, int lane) {
   DmaLanes d;
 #pragma unroll
   for (int i = 0; i < 6; ++i) {
-    const int c = 64 * (dma_first(wave) + i) + lane;
-    const int r = min(c / kMlaRowPieces, kMlaKeys - 1);
-    d.pk[i] = (uint32_t)(8 * r) | ((uint32_t)(16 * (c - r * kMlaRowPieces)) << 16);
+    const int c = 64 * (dma_first<kKeys>(wave) + i) + lane;
+    const int r = min(c / row_pieces<kKeys>(), kMlaKeys - 1);
+    d.pk[i] = (uint32_t)(8 * r) | ((uint32_t)(16 * (c - r * row_pieces<kKeys>())) << 16);
   }
   return d;
 }
@@ -341,20 +357,27 @@ __device__ __forceinline__ uint64_t dma_addr(const uint8_t* tab, uint32_t pk) {
 // Send this wave's loads of a block into `buf` (the table must hold its rows):
 // runs of up to four share one M0 value, the immediate offset moving both the
 // global and the LDS address by 1 KB steps.
+template <int kKeys>
 __device__ __forceinline__ void issue_block(const uint8_t* smem, int j, const DmaLanes& d, const uint8_t* buf,
                                             int wave) {
   const uint8_t* tab = smem + kAddrOff + (j & 1) * 512;
-  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_addr(buf) + 1024 * dma_first(wave));
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_addr(buf) + 1024 * dma_first<kKeys>(wave));
   const uint64_t a0 = dma_addr(tab, d.pk[0]);
   const uint64_t a1 = dma_addr(tab, d.pk[1]) - 1024;
   const uint64_t a2 = dma_addr(tab, d.pk[2]) - 2048;
+  if (kKeys == kSlots4 && dma_count<kKeys>(wave) == 3) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off\n\tglobal_load_lds_dwordx4 %1, off offset:1024\n\t"
+                 "global_load_lds_dwordx4 %2, off offset:2048" ::"v"(a0), "v"(a1), "v"(a2), "{m0}"(m0) : "memory");
+    return;
+  }
   const uint64_t a3 = dma_addr(tab, d.pk[3]) - 3072;
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off\n\tglobal_load_lds_dwordx4 %1, off offset:1024\n\t"
                "global_load_lds_dwordx4 %2, off offset:2048\n\tglobal_load_lds_dwordx4 %3, off offset:3072"
                ::"v"(a0), "v"(a1), "v"(a2), "v"(a3), "{m0}"(m0) : "memory");
-  const uint32_t m1 = __builtin_amdgcn_readfirstlane(lds_addr(buf) + 1024 * (dma_first(wave) + 4));
+  if (kKeys == kSlots4) return;
+  const uint32_t m1 = __builtin_amdgcn_readfirstlane(lds_addr(buf) + 1024 * (dma_first<kKeys>(wave) + 4));
   const uint64_t b0 = dma_addr(tab, d.pk[4]);
-  if (dma_count(wave) == 6) {
+  if (dma_count<kKeys>(wave) == 6) {
     const uint64_t b1 = dma_addr(tab, d.pk[5]) - 1024;
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off\n\tglobal_load_lds_dwordx4 %1, off offset:1024"
                  ::"v"(b0), "v"(b1), "{m0}"(m1) : "memory");
@@ -401,7 +424,7 @@ __device__ __forceinline__ void iteration_start(const MlaParams& P, uint8_t* sme
   if (c.wave == kIdxWave && t + 4 < c.nblk) issue_index<kKeys>(P, smem, c, t + 4);
   if (t + 1 < c.nblk) {
     uint8_t* buf = smem + ((t + 1) % kNumBufs) * buf_bytes<kKeys>();
-    if (!rows_block<kKeys>(c, t + 1)) issue_block(smem, t + 1, dl, buf, c.wave);
+    if (!rows_block<kKeys>(c, t + 1)) issue_block<kKeys>(smem, t + 1, dl, buf, c.wave);
     else issue_fresh_block(smem, t + 1, buf, c.wave, c.lane);
   }
 }
@@ -449,7 +472,7 @@ __device__ __forceinline__ void qk_waves(const MlaParams& P, uint8_t* smem, cons
   v4i qr[4];
   {
     const int r = 32 * hp + c32;
-    const uint8_t* qrow = smem + kBufBytes + r * kQRowBytes;
+    const uint8_t* qrow = smem + buf_bytes<kKeys>() + r * kQRowBytes;
     const int sw = 16 * (r & 7);
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -473,7 +496,7 @@ __device__ __forceinline__ void qk_waves(const MlaParams& P, uint8_t* smem, cons
     // a fresh block has 32 keys, all in key half 0
     const bool fresh = rows_block<kKeys>(c, t);
     if (t < c.nblk && !(fresh && kh == 1) && hp < kTiles) {
-      const uint8_t* buf = smem + (t % kNumBufs) * kBufBytes;
+      const uint8_t* buf = smem + (t % kNumBufs) * buf_bytes<kKeys>();
       const int32_t slot_t = reinterpret_cast<const int32_t*>(smem + kRingOff + (t % kRingSlots) * 256)[lane];
       const uint64_t vmask = __ballot(fresh ? fresh_valid(P, slot_t, lane) : slot_valid(P, slot_t));
       // s[r]: key 32kh + 8(r/4) + 4h + r%4, head c32
@@ -510,6 +533,38 @@ __device__ __forceinline__ void qk_waves(const MlaParams& P, uint8_t* smem, cons
                                                         0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);
         }
+      } else if constexpr (kKeys == kSlots4) {
+        // chunk k: dims 64k + 32h .. +31 are 16 bytes of codes and one scale, byte 2k + h of the row's
+        // sixteen; read D chunks ahead
+        const uint8_t* row = buf + (32 * kh + c32) * kMla4RowBytes;
+        const v4i sb = *reinterpret_cast<const v4i*>(row + kMla4ScaleOff);
+        const uint8_t* krow = row + 16 * h;
+        uint32_t sbh[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sbh[i] = (uint32_t)sb[i] >> (8 * h);
+        constexpr int D = 2;
+        v4i kraw[D + 1];
+        v4i rope[4];
+#pragma unroll
+        for (int k = 0; k < D; ++k) kraw[k] = *reinterpret_cast<const v4i*>(krow + 32 * k);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k + D < 8) kraw[(k + D) % (D + 1)] = *reinterpret_cast<const v4i*>(krow + 32 * (k + D));
+          else
+#pragma unroll
+            for (int r = 2 * (k + D - 8); r < 2 * (k + D - 8) + 2; ++r)
+              rope[r] = *reinterpret_cast<const v4i*>(row + kMla4RopeOff + 32 * r + 16 * h);
+          __builtin_amdgcn_sched_barrier(0);
+          const float sc = fp4_scale((sbh[k >> 1] >> (16 * (k & 1))) & 255u);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_v8bf(fp4x8_to_bf16((uint32_t)kraw[k % (D + 1)][j], sc)),
+                                                        as_v8bf(qn[k][j]), s, 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_v8bf(rope[r]), as_v8bf(qr[r]), s, 0, 0, 0);
       } else {
       const uint8_t* row = buf + (32 * kh + c32) * kMlaRowBytes;
       const v4f ksc = *reinterpret_cast<const v4f*>(row + 512);
@@ -581,7 +636,10 @@ __device__ __forceinline__ void qk_waves(const MlaParams& P, uint8_t* smem, cons
       float pv[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        pv[r] = __builtin_amdgcn_exp2f(fmaxf(fmaf(s[r], P.scale_log2, -m_use), kMinLogP));
+        // (over 4-bit rows P may be as small as it is: P' is formed by a subtraction that stops at 0,
+        // and a NaN score stays one)
+        pv[r] = kKeys == kSlots4 ? __builtin_amdgcn_exp2f(fmaf(s[r], P.scale_log2, -m_use))
+                                 : __builtin_amdgcn_exp2f(fmaxf(fmaf(s[r], P.scale_log2, -m_use), kMinLogP));
       if (!all_valid) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -787,6 +845,80 @@ __device__ __forceinline__ void qk_waves_rows(const MlaParams& P, uint8_t* smem,
   barrier();
 }
 
+// O += P' . V of one block of 4-bit rows. A transposing 8-bit read gives a lane
+// one byte column, two dims, of eight keys; each byte becomes the two dims' bf16
+// values with its key's scale, and two permutes a key pair sort them into the B
+// operands of the even and the odd dims (lane c32: dims 2 c32 and 2 c32 + 1 of 64).
+// (The alternative, a transposing 4-bit read whose pairs are keys of one dim, needs
+// no permutes but converts two keys with one scale, so that P would have to carry
+// the scales: four times the additions, as a 32-dim tile has a scale of its own.)
+// P' = P * 2^(m_kh - R): a subtraction from the exponent field that stops at zero.
+template <int kTiles>
+__device__ __forceinline__ void pv_block4(v16f (&o)[kTiles][4], const int (&fx)[kTiles][2], const uint8_t* pb,
+                                          const uint16_t* et, uint32_t vb, int lane) {
+  typedef int v4i_alias __attribute__((ext_vector_type(4), may_alias));
+  const int h = lane >> 5, half = (lane >> 4) & 1;
+  const uint16_t* etl = et + 64 * half + 8 * h;  // scale block 2u + half of 64-dim group u
+  auto vaddr = [&](int ks) {
+    uint32_t a = vb + (16 * ks) * kMla4RowBytes;
+    asm volatile("" : "+v"(a));
+    return a;
+  };
+  v2i vq[2][2];
+  v4i pq[2][kTiles], eq[2][2];
+  auto read_step = [&](int ks) {
+    const int b = ks & 1;
+    const uint32_t a = vaddr(ks);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      vq[b][u] = lds_read_tr8_at(a + 32 * u);
+      eq[b][u] = *reinterpret_cast<const v4i_alias*>(etl + 128 * u + 16 * ks);
+    }
+#pragma unroll
+    for (int mt = 0; mt < kTiles; ++mt) pq[b][mt] = *reinterpret_cast<const v4i*>(pb + mt * 4096 + (ks * 64 + lane) * 16);
+  };
+  read_step(0);
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    const int cur = ks & 1;
+    if (ks + 1 < 4) read_step(ks + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    v4i pa[kTiles];
+#pragma unroll
+    for (int mt = 0; mt < kTiles; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int pe = pq[cur][mt][e];
+        pa[mt][e] = __builtin_bit_cast(int, __builtin_elementwise_sub_sat(__builtin_bit_cast(v2u16, pe),
+                                                                          __builtin_bit_cast(v2u16, fx[mt][ks >> 1])));
+      }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      v4i even, odd;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        // keys 2d and 2d + 1: the conversion uses its scale's exponent field only, so the upper entry is
+        // taken with the lower one in its mantissa
+        const uint32_t raw = (uint32_t)vq[cur][u][d >> 1], e2 = (uint32_t)eq[cur][u][d];
+        const uint32_t k0 = __builtin_bit_cast(
+            uint32_t, d & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(raw, __uint_as_float(e2 << 16), 2)
+                            : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(raw, __uint_as_float(e2 << 16), 0));
+        const uint32_t k1 = __builtin_bit_cast(
+            uint32_t, d & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(raw, __uint_as_float(e2), 3)
+                            : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(raw, __uint_as_float(e2), 1));
+        even[d] = (int)__builtin_amdgcn_perm(k1, k0, 0x05040100u);
+        odd[d] = (int)__builtin_amdgcn_perm(k1, k0, 0x07060302u);
+      }
+#pragma unroll
+      for (int mt = 0; mt < kTiles; ++mt) {
+        o[mt][2 * u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_v8bf(pa[mt]), as_v8bf(even), o[mt][2 * u], 0, 0, 0);
+        o[mt][2 * u + 1] =
+            __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_v8bf(pa[mt]), as_v8bf(odd), o[mt][2 * u + 1], 0, 0, 0);
+      }
+    }
+  }
+}
+
 // PV waves: O += P'(t-1) . V(t-1) against R, then the normalised output.
 // Wave dq = w - 4 owns O[64 heads x dims 128dq .. 128dq+127], exactly V tile
 // dq, as two head tiles (the head halves): each V byte is converted once per
@@ -801,7 +933,9 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
   // may alias them (so the reads stay after the writes)
   typedef int v4i_alias __attribute__((ext_vector_type(4), may_alias));
   uint16_t* et = reinterpret_cast<uint16_t*>(smem + kEOff) + dq * 256;
-  v16f o[kTiles][4];  // o[mt][nn][r]: head 32mt + 8(r/4) + 4h + r%4 of the workgroup, dim 128dq + 32nn + c32
+  // o[mt][nn][r]: head 32mt + 8(r/4) + 4h + r%4 of the workgroup, dim 128dq + 32nn + c32 (4-bit rows: dim
+  // 128dq + 64(nn/2) + 2 c32 + nn%2)
+  v16f o[kTiles][4];
 #pragma unroll
   for (int mt = 0; mt < kTiles; ++mt)
 #pragma unroll
@@ -815,8 +949,8 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
   // 8(e/4) + 4h + e%4 (e = m/2) and dims (G%2)*16 + 8(m%2) of each 32-dim tile
   const int m16 = lane & 15, G = lane >> 4;
   const int e8 = m16 >> 1;
-  const uint32_t vlane = (uint32_t)((8 * (e8 >> 2) + 4 * h + (e8 & 3)) * kMlaRowBytes + 128 * dq + (G & 1) * 16 +
-                                    8 * (m16 & 1));
+  const uint32_t vlane = (uint32_t)((8 * (e8 >> 2) + 4 * h + (e8 & 3)) * row_bytes<kKeys>() +
+                                    (kKeys == kSlots4 ? 64 : 128) * dq + (G & 1) * 16 + 8 * (m16 & 1));
   // transposing bf16 reads of a fresh block: lane (G = lane/16, m = lane%16)
   // addresses key row 4h + m/4 (+8) and dims 16(G%2) + 4(m%4) .. +3 of each
   // 32-dim tile, and receives dim 16(G%2) + m of four consecutive keys
@@ -831,7 +965,15 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
       const int par = (t - 1) & 1;
       const uint8_t* bufp = smem + ((t - 1) % kNumBufs) * buf_bytes<kKeys>();
       const bool fresh = rows_block<kKeys>(c, t - 1);
-      if (!fresh) {
+      if constexpr (kKeys == kSlots4) {
+        // scale table of block t-1, dims 128dq .. +127 (lane = key): four blocks' scales in the exponent
+        // field of a 16-bit entry, [4 blocks][the key's position, as below]
+        const int key = lane;
+        const uint32_t sb = *reinterpret_cast<const uint32_t*>(bufp + key * kMla4RowBytes + kMla4ScaleOff + 4 * dq);
+        const int pos = ((key >> 4) * 2 + ((key >> 2) & 1)) * 8 + 4 * ((key >> 3) & 1) + (key & 3);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) et[64 * i + pos] = (uint16_t)(((sb >> (8 * i)) & 255u) << 7);
+      } else if (!fresh) {
         // exponent table of block t-1, tile dq (lane = key): the tile scale's
         // exponent in the bf16 exponent field, at the PV A operand position of
         // the key (k-step key/16, lane half (key/4)%2, element 4((key/8)%2) + key%4)
@@ -876,6 +1018,12 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2) {
           const float mk = k2 == 0 ? m0 : m1;
+          if constexpr (kKeys == kSlots4) {
+            // R - m_kh, taken off P's exponent field (a half without a key has no P)
+            const int f4 = mk == -__builtin_inff() ? 0 : (int)fminf(R[mt] - mk, 255.f);
+            fx[mt][k2] = (f4 << 7) | (f4 << 23);
+            continue;
+          }
           const int f = mk == -__builtin_inff() ? 0 : max((int)(mk - R[mt]), kDropExp);
           fx[mt][k2] = (f << 7) & 0xffff;
           fx[mt][k2] |= fx[mt][k2] << 16;
@@ -893,6 +1041,9 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
         return a;
       };
       constexpr int kSteps = kKeys == kRows ? kFreshKeys / 16 : kMlaKeys / 16;
+      if constexpr (kKeys == kSlots4) {
+        pv_block4<kTiles>(o, fx, pb, et, vb, lane);
+      } else {
       // k-step ks: its P (both head tiles), exponent and V reads issued one
       // k-step ahead
       v2i vq[2][4];
@@ -960,6 +1111,7 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
             o[mt][nn] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_v8bf(pa[mt]), vop, o[mt][nn], 0, 0, 0);
         }
       }
+      }
     } else if (kKeys == kRows) {
       barrier();
     }
@@ -984,9 +1136,10 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
       const float lk = fin[(mt * 2 + k2) * 32 + c32];
       const float mk = fin[128 + (mt * 2 + k2) * 32 + c32];
       if (mk != -__builtin_inff()) lt += lk * __builtin_amdgcn_exp2f(mk - R[mt]);
+      else if (kKeys == kSlots4) lt += lk;  // 0, or the NaN of a half whose every key is one
       mm = fmaxf(mm, fin[256 + (mt * 2 + k2) * 32 + c32]);
     }
-    const bool any = lt > 0.f;
+    const bool any = kKeys == kSlots4 ? lt != 0.f : lt > 0.f;  // (a NaN sum gives NaN outputs)
     const float inv = any ? 1.f / lt : 0.f;
     const float lse = any ? (R[mt] + __builtin_amdgcn_logf(lt)) * kLn2 : -__builtin_inff();
     const int h_half = hg_base + 32 * mt;
@@ -1002,8 +1155,14 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
       for (int r = 0; r < 16; ++r) {
         const float ir = __shfl(inv, 8 * (r >> 2) + hb + (r & 3), 64);
         uint16_t* srow = reinterpret_cast<uint16_t*>(st + (8 * (r >> 2) + 4 * h + (r & 3)) * kStageRow16) + c32;
+        if constexpr (kKeys == kSlots4) {
+          uint32_t* srow4 = reinterpret_cast<uint32_t*>(srow + c32);  // dims 2 c32, 2 c32 + 1
 #pragma unroll
-        for (int nn = 0; nn < 4; ++nn) srow[32 * nn] = (uint16_t)f32_to_bf16_rne(o[mt][nn][r] * ir);
+          for (int nn = 0; nn < 4; nn += 2) srow4[16 * nn] = pack_bf16_rne(o[mt][nn][r] * ir, o[mt][nn + 1][r] * ir);
+        } else {
+#pragma unroll
+          for (int nn = 0; nn < 4; ++nn) srow[32 * nn] = (uint16_t)f32_to_bf16_rne(o[mt][nn][r] * ir);
+        }
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -1024,8 +1183,14 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
       for (int r = 0; r < 16; ++r) {
         const float ir = __shfl(inv, 8 * (r >> 2) + hb + (r & 3), 64);
         float* srow = reinterpret_cast<float*>(st + (8 * (r >> 2) + 4 * h + (r & 3)) * kStageRow32) + c32;
+        if constexpr (kKeys == kSlots4) {
 #pragma unroll
-        for (int nn = 0; nn < 4; ++nn) srow[32 * nn] = o[mt][nn][r] * ir;
+          for (int nn = 0; nn < 4; nn += 2)
+            *reinterpret_cast<v2f*>(srow + c32 + 32 * nn) = v2f{o[mt][nn][r] * ir, o[mt][nn + 1][r] * ir};
+        } else {
+#pragma unroll
+          for (int nn = 0; nn < 4; ++nn) srow[32 * nn] = o[mt][nn][r] * ir;
+        }
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -1095,7 +1260,7 @@ sparse_mla_kernel(const MlaParams P) {
   if (c.wave == kIdxWave)
     for (int j = 0; j < 4 && j < c.nblk; ++j) issue_index<kKeys>(P, smem, c, j);
   issue_query<kKeys>(P, smem, c, hg * kMlaHeadsPerWG);
-  const DmaLanes dl = dma_lanes(c.wave, c.lane);
+  const DmaLanes dl = dma_lanes<kKeys>(c.wave, c.lane);
   if (c.wave == kIdxWave)  // its index copies landed (the query's may still be on their way)
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kQDma / kMlaWaves) : "memory");
   barrier();
@@ -1106,7 +1271,7 @@ sparse_mla_kernel(const MlaParams P) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's query copies
   barrier();
   if (c.nblk > 0) {
-    if (!rows_block<kKeys>(c, 0)) issue_block(smem, 0, dl, smem, c.wave);
+    if (!rows_block<kKeys>(c, 0)) issue_block<kKeys>(smem, 0, dl, smem, c.wave);
     else issue_fresh_block(smem, 0, smem, c.wave, c.lane);
   }
   // both roles run the same number of iterations and barriers
@@ -1149,9 +1314,15 @@ sparse_mla_combine_kernel(const float* __restrict__ ws_o, const float* __restric
   float l = load_lse(0);
   load_group(0);
   float m = l;
-  for (int s0 = 64; s0 < splits; s0 += 64) m = fmaxf(m, load_lse(s0));
+  bool nan = l != l;
+  for (int s0 = 64; s0 < splits; s0 += 64) {
+    const float x = load_lse(s0);
+    m = fmaxf(m, x);
+    nan |= x != x;
+  }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+  if (__ballot(nan)) m = __builtin_nanf("");  // a part of 4-bit rows with a NaN: every weight becomes one
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   float wsum = 0.f;
   if (m != -__builtin_inff()) {
@@ -1174,12 +1345,12 @@ sparse_mla_combine_kernel(const float* __restrict__ ws_o, const float* __restric
         }
     }
   }
-  const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+  const float inv = wsum != 0.f ? 1.f / wsum : 0.f;
   v4i v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = (int)pack_bf16_rne(acc[2 * e] * inv, acc[2 * e + 1] * inv);
   *reinterpret_cast<v4i*>(out + th * kMlaDv + lane * 8) = v;
-  if (lane == 0 && lse_out) lse_out[th] = wsum > 0.f ? m + logf(wsum) : -__builtin_inff();
+  if (lane == 0 && lse_out) lse_out[th] = wsum != 0.f ? m + logf(wsum) : -__builtin_inff();
 }
 
 static int64_t mla_items(int num_tokens, int num_heads) {
@@ -1270,6 +1441,17 @@ int dsa_sparse_mla_decode(const void* q, int64_t q_token_stride, int64_t q_head_
                                      nullptr);
 }
 
+int dsa_sparse_mla_decode_fp4(const void* q, int64_t q_token_stride, int64_t q_head_stride, const uint8_t* kv_cache,
+                              int64_t kv_block_stride_bytes, int kv_block_size, int64_t kv_num_blocks,
+                              const int32_t* indices, int64_t idx_stride, int num_tokens, int num_heads, int topk,
+                              float sm_scale, void* out, float* lse, int num_splits, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  return dsa::sparse_mla_decode_impl(q, q_token_stride, q_head_stride, kv_cache, kv_block_stride_bytes,
+                                     kv_block_size, kv_num_blocks, indices, idx_stride, num_tokens, num_heads, topk,
+                                     sm_scale, out, lse, num_splits, workspace, workspace_bytes, stream, nullptr,
+                                     nullptr, true);
+}
+
 }  // extern "C"
 
 namespace dsa {
@@ -1281,16 +1463,18 @@ static int launch_mla(const MlaParams& P, KeyKind keys, int64_t nwg, hipStream_t
     for (const void* k : {(const void*)sparse_mla_kernel<kSlots, 1>, (const void*)sparse_mla_kernel<kSlots, 2>,
                           (const void*)sparse_mla_kernel<kSlotsThenRows, 1>,
                           (const void*)sparse_mla_kernel<kSlotsThenRows, 2>, (const void*)sparse_mla_kernel<kRows, 1>,
-                          (const void*)sparse_mla_kernel<kRows, 2>})
+                          (const void*)sparse_mla_kernel<kRows, 2>, (const void*)sparse_mla_kernel<kSlots4, 1>,
+                          (const void*)sparse_mla_kernel<kSlots4, 2>})
       if (hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kRowsSmemBytes) != hipSuccess)
         smem_status = 1;
   }
   if (smem_status) return set_error(kLaunchFailed, "sparse_mla: cannot reserve %zu B of LDS", kRowsSmemBytes);
   if (nwg > INT32_MAX) return set_error(kInvalidArgument, "%s: grid too large", what);
-  void (*const kernels[3][2])(MlaParams) = {
+  void (*const kernels[4][2])(MlaParams) = {
       {sparse_mla_kernel<kSlots, 1>, sparse_mla_kernel<kSlots, 2>},
       {sparse_mla_kernel<kSlotsThenRows, 1>, sparse_mla_kernel<kSlotsThenRows, 2>},
-      {sparse_mla_kernel<kRows, 1>, sparse_mla_kernel<kRows, 2>}};
+      {sparse_mla_kernel<kRows, 1>, sparse_mla_kernel<kRows, 2>},
+      {sparse_mla_kernel<kSlots4, 1>, sparse_mla_kernel<kSlots4, 2>}};
   hipLaunchKernelGGL(kernels[keys][P.H <= 32 ? 0 : 1], dim3((unsigned)nwg), dim3(kMlaThreads),
                      keys == kRows ? kRowsSmemBytes : kMlaSmemBytes, stream, P);
   return check_launch(what);
@@ -1325,14 +1509,15 @@ int sparse_mla_decode_impl(const void* q, int64_t q_token_stride, int64_t q_head
                            int64_t kv_block_stride_bytes, int kv_block_size, int64_t kv_num_blocks,
                            const int32_t* indices, int64_t idx_stride, int num_tokens, int num_heads, int topk,
                            float sm_scale, void* out, float* lse, int num_splits, void* workspace,
-                           size_t workspace_bytes, void* stream, float* max_out, const MlaFresh* fresh) {
+                           size_t workspace_bytes, void* stream, float* max_out, const MlaFresh* fresh, bool fp4) {
   if (num_tokens < 0 || num_heads <= 0 || (num_heads % 16) != 0)
     return set_error(kUnsupported, "sparse_mla: num_heads=%d must be a positive multiple of 16", num_heads);
   if (topk <= 0 || topk % kMlaKeys != 0)
     return set_error(kUnsupported, "sparse_mla: topk=%d must be a positive multiple of %d", topk, kMlaKeys);
-  if (kv_block_size <= 0 || kv_block_stride_bytes < (int64_t)kv_block_size * kMlaRowBytes)
-    return set_error(kInvalidArgument, "sparse_mla: kv block stride %lld < %d rows x 656 B",
-                     (long long)kv_block_stride_bytes, kv_block_size);
+  const int row_b = fp4 ? kMla4RowBytes : kMlaRowBytes;
+  if (kv_block_size <= 0 || kv_block_stride_bytes < (int64_t)kv_block_size * row_b)
+    return set_error(kInvalidArgument, "sparse_mla: kv block stride %lld < %d rows x %d B",
+                     (long long)kv_block_stride_bytes, kv_block_size, row_b);
   if (kv_block_stride_bytes % 16 != 0)
     return set_error(kInvalidArgument, "sparse_mla: kv block stride must be a multiple of 16 bytes");
   if (kv_num_blocks < 0) return set_error(kInvalidArgument, "sparse_mla: kv_num_blocks < 0");
@@ -1420,7 +1605,7 @@ int sparse_mla_decode_impl(const void* q, int64_t q_token_stride, int64_t q_head
     P.ws_lse = P.ws_o + (size_t)num_splits * part.rows * kMlaDv;
   }
   const int64_t nwg = whole + (items - whole) * num_splits;
-  if (int rc = launch_mla(P, fresh ? kSlotsThenRows : kSlots, nwg, (hipStream_t)stream, "dsa_sparse_mla_decode"))
+  if (int rc = launch_mla(P, fp4 ? kSlots4 : fresh ? kSlotsThenRows : kSlots, nwg, (hipStream_t)stream, "dsa_sparse_mla_decode"))
     return rc;
   if (num_splits > 1) {
     hipLaunchKernelGGL(sparse_mla_combine_kernel, dim3((unsigned)((items - whole) * kMlaHeadsPerWG)), dim3(64), 0,
