@@ -11,15 +11,18 @@
 //
 // Persistent kernel, one workgroup of 8 waves per CU; every wave owns one contiguous
 // range of the flattened (batch entry, page) space and no barrier after the start.
-//   pages : straight from HBM into the wave's ring of page buffers in LDS, kBufs - 1
-//           pages ahead, 1 KB of whole 64-byte keys to an instruction. Lane l's
-//           source piece is swizzled so that 16 consecutive keys' reads of one
-//           block fall on all banks.
+//   pages : straight from HBM into the wave's two page buffers in LDS, one page
+//           ahead, 1 KB of whole 64-byte keys to an instruction. Lane l's source
+//           piece is swizzled so that 16 consecutive keys' reads of one block fall
+//           on all banks. (Three and four buffers, three waves a SIMD, and pages dealt
+//           out one by one to the waves of a workgroup all take the same time.)
 //   keys  : the B operand of v_mfma_f32_32x32x16_bf16. Lane (c32, h) reads 16 bytes
 //           of codes, one 32-dim block with one scale: dims 64c + 32h .. +31 of key c32 of
 //           a 32-key tile, converted eight at a time into the operands of four k-steps.
 //   query : the A operand, 64 heads in the same order of dims, resident in registers
 //           with the head weights.
+//   order : the sums of one eight-product unit stand between the products of the
+//           next (150 -> 141 us).
 //   sum   : a lane ends up with 32 of a key's 64 heads; the lane halves' sums of the
 //           two key tiles change places in one swap, so that lane t holds key t.
 #include <algorithm>
@@ -38,9 +41,9 @@ constexpr int kPage = 64, kDim = 128, kHeads = 64;
 constexpr int kCodeBytes = kPage * kIdx4KeyBytes;                        // 4096
 constexpr int kPageBytes4 = kPage * (kIdx4KeyBytes + kIdx4KeyScales);    // 4352
 constexpr int kWaves = 8, kThreads = 64 * kWaves;
-constexpr int kBufs = 4;            // page buffers a wave, kBufs - 1 pages in flight
+constexpr int kBufs = 2;            // page buffers a wave: one page in flight, one multiplied
 constexpr int kPageLoads = 5;       // instructions of a page: 4 x 1 KB of codes, the scales
-constexpr int kWindow = 64, kAdvance = 60;  // block-table entries a wave holds, pages per refill
+constexpr int kAdvance = 62;        // pages per refill of a wave's 64 block-table entries
 constexpr int kMaxBatch = 4096;     // entries of a launch (their page prefix lies in LDS)
 constexpr int kFillChunk = 4096;    // positions past a row's pages that a wave fills at a time
 constexpr int kWeightBytes = 2 * kHeads * sizeof(float);  // a wave's head weights (two query tokens only)
@@ -49,7 +52,7 @@ constexpr size_t smem_bytes(int next_n, int batch) {
          ((size_t)batch + 1 + kWaves) * sizeof(int32_t);
 }
 static_assert(smem_bytes(2, kMaxBatch) <= 160 * 1024, "LDS budget");
-static_assert(kAdvance % kBufs == 0 && kAdvance + kBufs - 1 < kWindow, "window refill geometry");
+static_assert(kAdvance + kBufs - 1 < 64, "window refill geometry");
 
 // Source of a page outside the cache (its scores are replaced by -inf).
 __device__ __align__(16) uint8_t g_idx4_zero_page[kPageBytes4];
@@ -162,6 +165,9 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
       bl = lo;
       page = P.bt[(int64_t)bl * P.bt_stride + (p - prefix[bl])];
     }
+    // the load's wait belongs here: left to the first use, it stands in the page loop and drains the
+    // pages in flight at every turn
+    asm volatile("" : "+v"(page));
     win_b = bl;
     win_page = page;
   };
@@ -220,46 +226,98 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
     const uint8_t* buf = ring + (k % kBufs) * kPageBytes4;
     int c32_o = c32;
     asm volatile("" : "+v"(c32_o));
-    float part[NQ][2] = {};
-    // (a loop for two query tokens: unrolled, the second tile's operands would take the registers of the first's)
-#pragma unroll(NQ == 1 ? 2 : 1)
-    for (int tt = 0; tt < 2; ++tt) {
+    // A unit is the eight products of one key tile, query token and head tile. The vector work, the sum of
+    // the unit before (and the next tile's conversions), is spread between its products: done in
+    // turns, one wave's products and the other's vector work covered each other only by chance.
+    float part[NQ][2];
+    v16f acc[2];
+    auto read_key = [&](int tt, v4i (&raw)[2], uint32_t& sb) {
       const int key = 32 * tt + c32_o;
-      const uint32_t sb = *reinterpret_cast<const uint32_t*>(buf + kCodeBytes + 4 * key) >> (8 * h);
-      v8bf kb[8];
+      sb = *reinterpret_cast<const uint32_t*>(buf + kCodeBytes + 4 * key) >> (8 * h);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const v4i raw = *reinterpret_cast<const v4i*>(buf + 64 * key + 16 * ((2 * c + h) ^ ((key >> 2) & 3)));
-        const float sc = fp4_scale((sb >> (16 * c)) & 255u);
+      for (int c = 0; c < 2; ++c)
+        raw[c] = *reinterpret_cast<const v4i*>(buf + 64 * key + 16 * ((2 * c + h) ^ ((key >> 2) & 3)));
+    };
+    auto convert = [&](v8bf (&kb)[8], const v4i (&raw)[2], uint32_t sb, int c) {
+      const float sc = fp4_scale((sb >> (16 * c)) & 255u);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) kb[4 * c + j] = __builtin_bit_cast(v8bf, fp4x8_to_bf16((uint32_t)raw[j], sc));
+      for (int i = 0; i < 4; ++i) kb[4 * c + i] = __builtin_bit_cast(v8bf, fp4x8_to_bf16((uint32_t)raw[c][i], sc));
+    };
+    auto products = [&](v16f& c, const v8bf (&q8)[8], const v8bf (&kb)[8]) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) c[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(q8[ks], kb[ks], c, 0, 0, 0);
+    };
+    auto weigh = [&](const v16f& c, int j, int ht) {
+      float a = 0.f, b2 = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        v4f wv;
+        if constexpr (kWLds) wv = *reinterpret_cast<const v4f*>(wl + j * kHeads + 32 * ht + 8 * g + 4 * h);
+        else wv = v4f{w[ht][4 * g], w[ht][4 * g + 1], w[ht][4 * g + 2], w[ht][4 * g + 3]};
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          a = fmaf(wv[r], relu_nan(c[4 * g + r]), a);
+          b2 = fmaf(wv[r + 1], relu_nan(c[4 * g + r + 1]), b2);
+        }
       }
+      return a + b2;
+    };
+    auto spread = [&]() {
 #pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        v16f c[2];
+      for (int i = 0; i < 8; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // one MFMA
+        __builtin_amdgcn_sched_group_barrier(0x2, 6, 0);  // up to six vector operations
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (NQ == 1) {
+      v4i raw[2][2];
+      uint32_t sb[2];
+      read_key(0, raw[0], sb[0]);
+      read_key(1, raw[1], sb[1]);
+      v8bf kb[2][8];
+      convert(kb[0], raw[0], sb[0], 0);
+      convert(kb[0], raw[0], sb[0], 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int ht = 0; ht < 2; ++ht)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) c[ht][r] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-          for (int ht = 0; ht < 2; ++ht)
-            c[ht] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa[j][ht][ks], kb[ks], c[ht], 0, 0, 0);
-        float acc[2] = {0.f, 0.f};
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-          for (int ht = 0; ht < 2; ++ht) {
-            v4f wv;
-            if constexpr (kWLds) wv = *reinterpret_cast<const v4f*>(wl + j * kHeads + 32 * ht + 8 * g + 4 * h);
-            else wv = v4f{w[ht][4 * g], w[ht][4 * g + 1], w[ht][4 * g + 2], w[ht][4 * g + 3]};
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[ht] = fmaf(wv[r], relu_nan(c[ht][4 * g + r]), acc[ht]);
-          }
-        if (tt == 0) part[j][0] = acc[0] + acc[1];
-        else part[j][1] = acc[0] + acc[1];
+      for (int u = 0; u < 4; ++u) {  // tile u / 2, head tile u % 2
+        products(acc[u & 1], qa[0][u & 1], kb[u >> 1]);
+        if (u < 2) convert(kb[1], raw[1], sb[1], u);
+        if (u == 1) part[0][0] = weigh(acc[0], 0, 0);
+        if (u == 2) part[0][0] += weigh(acc[1], 0, 1);
+        if (u == 3) part[0][1] = weigh(acc[0], 0, 0);
+        spread();
+      }
+      part[0][1] += weigh(acc[1], 0, 1);
+    } else {
+      // a loop over the tiles: unrolled, the second one's operands would take the registers of the first's
+#pragma unroll 1
+      for (int tt = 0; tt < 2; ++tt) {
+        v4i raw[2];
+        uint32_t sb;
+        read_key(tt, raw, sb);
+        v8bf kb[8];
+        convert(kb, raw, sb, 0);
+        convert(kb, raw, sb, 1);
         __builtin_amdgcn_sched_barrier(0);
+        float sum[NQ];
+#pragma unroll
+        for (int u = 0; u < 2 * NQ; ++u) {  // query token u / 2, head tile u % 2
+          products(acc[u & 1], qa[u >> 1][u & 1], kb);
+          if (u > 0) {
+            const float x = weigh(acc[(u - 1) & 1], (u - 1) >> 1, (u - 1) & 1);
+            sum[(u - 1) >> 1] = (u - 1) & 1 ? sum[(u - 1) >> 1] + x : x;
+          }
+          spread();
+        }
+        sum[NQ - 1] += weigh(acc[1], NQ - 1, 1);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          if (tt == 0) part[j][0] = sum[j];
+          else part[j][1] = sum[j];
+        }
       }
     }
     const int64_t t = (p0 + k - first) * kPage + lane;
@@ -274,18 +332,7 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
     }
   };
 
-  // The loads of page k have landed when no more than those of the pages after it,
-  // and their stores, are outstanding (all return in order).
-  auto wait_for = [&](int younger) {
-    if (younger >= kBufs - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kBufs - 1) * (kPageLoads + NQ)) : "memory");
-    else if (younger == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kPageLoads) : "memory");
-    else if (younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kPageLoads) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  };
-  static_assert(kBufs == 4, "wait_for's cases");
-#pragma unroll
-  for (int u = 0; u < kBufs - 1; ++u)
-    if (u < n) issue(u);
+  issue(0);
   // entry by entry, so that the query's registers are the inner loop's constants
   for (int k = 0; k < n;) {
     const int b = __builtin_amdgcn_readlane(win_b, k - wb);
@@ -293,9 +340,16 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
     const int k_end = (int)min((int64_t)n, __builtin_amdgcn_readfirstlane(prefix[b + 1]) - p0);
     enter(b);
     for (; k < k_end; ++k) {
-      if (k + kBufs - 1 < n) issue(k + kBufs - 1);
-      // the first pages have no stores behind their loads
-      wait_for(k < kBufs - 1 ? min(n - 1 - k, kBufs - 2) : n - 1 - k);
+      // Page k has landed when no more is outstanding than what was issued after it:
+      // the loads of page k + 1 and, but for the first page, the stores of page k - 1
+      // (all return in order; whatever else the compiler put between only waits longer).
+      if (k + 1 < n) {
+        issue(k + 1);
+        if (k == 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kPageLoads) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kPageLoads + NQ) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
       compute(k, b, first);
       if (k + 1 - wb == kAdvance) {
         // the pages loaded ahead came from this window's last lanes
