@@ -8,6 +8,9 @@ Modules mirror the reference interfaces they replace:
   indexer      - the decode selection of Indexer.forward, IndexerCache
   mla_backend  - MlaAttentionBase-compatible sparse MLA backend + "mi355x" tier
   pipeline     - the fused three-launch decode step
+  batch_tables - block tables and slot maps from request lengths, on the device
+The MLA and indexer caches are fp8 as the reference's, or 4-bit (e2m1 blocks of 32
+with a power-of-two scale: ops.*_fp4, indexer.IndexerCacheFp4).
 The kernels live in libdsa_amd.so (C ABI in include/dsa_amd.h); there is no
 CPU fallback.
 """

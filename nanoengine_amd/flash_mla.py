@@ -57,10 +57,12 @@ def flash_mla_with_kvcache(q: torch.Tensor, k_cache: torch.Tensor, block_table, 
                            causal: bool = False, is_fp8_kvcache: bool = False,
                            indices: torch.Tensor | None = None):
     """Sparse MLA decode. q [B, n, H, 576] bf16; k_cache [blocks, block_size, 1, 656]
-    fp8 bytes (block stride may include the padding row); indices [B, n, topk]
+    fp8 bytes (block stride may include the padding row), or [.., 1, 400] bytes of
+    4-bit rows, which is_fp8_kvcache says nothing about; indices [B, n, topk]
     int32 physical slots (-1 = skip). Returns (o [B, n, H, 512] bf16,
     lse [B, H, n] f32, natural log)."""
-    if indices is None or not is_fp8_kvcache:
+    fp4 = k_cache.shape[-1] == ops.MLA_FP4_ROW_BYTES
+    if indices is None or not (is_fp8_kvcache or fp4):
         raise NotImplementedError("only the sparse fp8 MLA decode (indices=..., is_fp8_kvcache=True) "
                                   "is implemented on MI355X")
     if causal:
@@ -80,7 +82,8 @@ def flash_mla_with_kvcache(q: torch.Tensor, k_cache: torch.Tensor, block_table, 
         splits, ws = sched.num_splits, sched.workspace
     if num_splits is not None:
         splits = int(num_splits)
-    o, lse = ops.sparse_mla_decode(q3, k_cache, idx, softmax_scale, num_splits=splits, workspace=ws)
+    decode = ops.sparse_mla_decode_fp4 if fp4 else ops.sparse_mla_decode
+    o, lse = decode(q3, k_cache, idx, softmax_scale, num_splits=splits, workspace=ws)
     return o.view(B, n, H, ops.MLA_D_V), lse.view(B, n, H).permute(0, 2, 1)
 
 

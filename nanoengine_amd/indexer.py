@@ -71,6 +71,45 @@ class IndexerCache:
         ops.indexer_k_store(key_bf16, self.buffer[layer_id], slot_mapping, self.page_size)
 
 
+class IndexerCacheFp4:
+    """Per-layer indexer key cache in 4 bits, one contiguous uint8 buffer
+    ``[num_layers, num_pages, page_size * 68]``; each page holds ``page_size`` keys
+    of 64 code bytes followed by ``page_size`` x 4 scale bytes. The counterpart of
+    ``IndexerCache`` at about half its size; ``indexer_decode_topk`` and
+    ``DsaDecodeStep(indexer_format="fp4")`` score it."""
+
+    def __init__(self, num_layers: int, num_pages: int, page_size: int, head_dim: int = 128,
+                 device: str | torch.device = "cuda", buffer: torch.Tensor | None = None):
+        if head_dim != ops.INDEXER_HEAD_DIM:
+            raise ValueError(f"the 4-bit indexer cache holds {ops.INDEXER_HEAD_DIM}-dim keys, got {head_dim}")
+        self.num_layers = num_layers
+        self.num_pages = num_pages
+        self.page_size = page_size
+        self.head_dim = head_dim
+        self.bytes_per_token = ops.INDEXER_FP4_ROW_BYTES
+        shape = (num_layers, num_pages, page_size * self.bytes_per_token)
+        self.buffer = torch.zeros(shape, dtype=torch.uint8, device=device) if buffer is None else buffer
+        if tuple(self.buffer.shape) != shape or self.buffer.dtype != torch.uint8:
+            raise ValueError(f"IndexerCacheFp4 buffer must be uint8 with shape {shape}, "
+                             f"got dtype={self.buffer.dtype}, shape={tuple(self.buffer.shape)}")
+
+    @property
+    def buffers(self) -> list[torch.Tensor]:
+        return [self.buffer[i] for i in range(self.num_layers)]
+
+    def get_buffer(self, layer_id: int) -> torch.Tensor:
+        return self.buffer[layer_id]
+
+    def store_key(self, layer_id: int, key_bf16: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+        """Quantise keys [N, head_dim] bf16 and write them at slot_mapping."""
+        ops.indexer_k_store_fp4(key_bf16, self.buffer[layer_id], slot_mapping, self.page_size)
+
+    def load_key_fp8(self, layer_id: int, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """The keys at ``slots`` as (fp8 [N, head_dim], f32 scales [N]), which
+        ``deep_gemm.fp8_mqa_logits`` and ``ops.mqa_topk`` take in prefill."""
+        return ops.indexer_k_load_fp4(self.buffer[layer_id], slots, self.page_size)
+
+
 def indexer_decode_topk(q_fp8: torch.Tensor, weights: torch.Tensor, kv_cache_buf: torch.Tensor,
                         context_lens: torch.Tensor, block_tables: torch.Tensor, index_topk: int,
                         page_size: int = 64, *, is_prefill: bool = False, schedule_meta=None,
@@ -79,7 +118,8 @@ def indexer_decode_topk(q_fp8: torch.Tensor, weights: torch.Tensor, kv_cache_buf
     """Steps 8-9 of ``Indexer.forward`` for decode (lightning.py:1357-1492).
 
     q_fp8 [num_tokens, 64, 128] (num_tokens = batch * next_n); weights
-    [num_tokens, 64] f32; kv_cache_buf [num_pages, page_size * 132] uint8;
+    [num_tokens, 64] f32; kv_cache_buf [num_pages, page_size * 132] uint8, or
+    [num_pages, page_size * 68] of 4-bit keys;
     context_lens [batch] int (length after the last query token); block_tables
     [batch, M] int32. Returns logical top-k positions [num_tokens, index_topk]
     int32 (ascending, -1 padded), or (logical, physical) when ``translate_topk``.
@@ -90,15 +130,19 @@ def indexer_decode_topk(q_fp8: torch.Tensor, weights: torch.Tensor, kv_cache_buf
     ntps = num_tokens // batch
     n_heads, head_dim = q_fp8.shape[1], q_fp8.shape[2]
     q4 = q_fp8.view(batch, ntps, n_heads, head_dim)
-    kv_cache = kv_cache_buf.view(kv_cache_buf.shape[0], page_size, 1, -1)
+    fp4 = kv_cache_buf.shape[-1] == page_size * ops.INDEXER_FP4_ROW_BYTES  # else fp8
+    kv_cache = kv_cache_buf if fp4 else kv_cache_buf.view(kv_cache_buf.shape[0], page_size, 1, -1)
     max_context_len = block_tables.shape[-1] * page_size
     ctx = _expand_decode_context_lens(context_lens.to(torch.int32), ntps)
     bt = block_tables.to(torch.int32)
     # schedule_meta is taken as the reference takes it; the logits kernels balance
     # their pages themselves, so none is built here
-    logits = deep_gemm.fp8_paged_mqa_logits(q4, kv_cache, weights, ctx, bt, schedule_meta,
-                                            max_context_len, clean_logits=False) \
-        if logits_out is None else _logits_into(q4, kv_cache, weights, ctx, bt, max_context_len, logits_out)
+    if fp4:
+        logits = _logits_fp4(q4, kv_cache, weights, ctx, bt, max_context_len, logits_out)
+    else:
+        logits = deep_gemm.fp8_paged_mqa_logits(q4, kv_cache, weights, ctx, bt, schedule_meta,
+                                                max_context_len, clean_logits=False) \
+            if logits_out is None else _logits_into(q4, kv_cache, weights, ctx, bt, max_context_len, logits_out)
 
     seq_lens = ctx.reshape(-1).contiguous()
     logical = torch.empty((num_tokens, index_topk), dtype=torch.int32, device=q_fp8.device)
@@ -138,6 +182,20 @@ def _select_other_k(logits: torch.Tensor, seq_lens: torch.Tensor, index_topk: in
 def _logits_into(q4, kv_cache, weights, ctx, bt, max_context_len, out):
     kv = kv_cache.reshape(kv_cache.shape[0], -1)
     return ops.indexer_logits(q4, kv, weights, ctx, bt, max_context_len, out=out)
+
+
+def _logits_fp4(q4, kv_cache, weights, ctx, bt, max_context_len, out):
+    """The 4-bit pages' logits; more than two query tokens position by position, as the fp8 route does."""
+    B, n = ctx.shape
+    if n <= 2:
+        return ops.indexer_logits_fp4(q4, kv_cache, weights, ctx, bt, max_context_len, out=out, clean_logits=False)
+    if out is None:
+        out = torch.empty(B * n, max_context_len, dtype=torch.float32, device=q4.device)
+    w, rows = weights.view(B, n, -1), out.view(B, n, -1)
+    for j in range(n):
+        ops.indexer_logits_fp4(q4[:, j:j + 1].contiguous(), kv_cache, w[:, j], ctx[:, j:j + 1], bt, max_context_len,
+                               out=rows[:, j], clean_logits=False)
+    return out
 
 
 # Logits workspace of one prefill call: at most this fraction of the device's

@@ -1,4 +1,5 @@
-"""MLA attention backend for the "mi355x" hardware tier (sparse fp8 decode).
+"""MLA attention backend for the "mi355x" hardware tier (sparse decode over the
+fp8 cache, or over a 4-bit one: the injected cache's row width says which).
 
 Mirrors the reference contract:
 - ``MlaAttentionBase`` (dlengine/runtime/layers/backends/mla/base.py:18-49);
@@ -72,8 +73,9 @@ class MlaAttentionBase(nn.Module):
 
 
 class Mi355xSparseMlaAttention(MlaAttentionBase):
-    """Sparse fp8 MLA decode on MI355X (the DSA decode branch of
-    FlashMlaAttention.forward, flash_mla.py:30-99)."""
+    """Sparse MLA decode on MI355X (the DSA decode branch of
+    FlashMlaAttention.forward, flash_mla.py:30-99), over a cache of 656-byte fp8
+    rows or of 400-byte 4-bit rows."""
 
     def __init__(self, *args, **kwargs) -> None:
         kwargs.pop("mla_qk_nope_head_dim", None)
@@ -88,7 +90,10 @@ class Mi355xSparseMlaAttention(MlaAttentionBase):
         if write_kv_cache and k is not None and k_cache.numel() and not context.is_dummy:
             slot_mapping = (context.hisparse_slot_mapping if context.hisparse_slot_mapping is not None
                             else context.slot_mapping)
-            ops.mla_kv_store(k, k_cache, slot_mapping)
+            if k_cache.shape[-1] == ops.MLA_FP4_ROW_BYTES:
+                ops.mla_kv_store_fp4(k, k_cache, slot_mapping)
+            else:
+                ops.mla_kv_store(k, k_cache, slot_mapping)
         if context.is_prefill:
             raise RuntimeError("Mi355xSparseMlaAttention.forward serves decode only; MLA prefill is "
                                "handled by the model's non-absorbed path.")

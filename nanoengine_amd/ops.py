@@ -896,8 +896,13 @@ def indexer_logits_fp4(q_fp8: torch.Tensor, kv_cache: torch.Tensor, weights: tor
     if not (q_fp8.dim() == 4 and q_fp8.dtype in (torch.float8_e4m3fn, torch.uint8) and q_fp8.is_contiguous()):
         _fail(f"q_fp8 must be contiguous fp8 [B, next_n, H, D], got {q_fp8.dtype} {tuple(q_fp8.shape)}")
     B, n, H, D = q_fp8.shape
-    page_size = 64
-    pages = _fp4_pages(kv_cache, page_size)
+    pages = kv_cache.shape[0]
+    page_bytes = kv_cache.numel() // max(pages, 1)
+    page_size = page_bytes // INDEXER_FP4_ROW_BYTES if pages else 64
+    if not (kv_cache.dtype == torch.uint8 and kv_cache.is_contiguous()
+            and page_bytes % INDEXER_FP4_ROW_BYTES == 0):
+        _fail(f"kv_cache must be contiguous uint8 [pages, page_size*{INDEXER_FP4_ROW_BYTES}], "
+              f"got {kv_cache.dtype} {tuple(kv_cache.shape)}")
     if not (weights.dtype == torch.float32 and tuple(weights.shape) == (B * n, H)):
         _fail(f"weights must be f32 [{B * n}, {H}], got {weights.dtype} {tuple(weights.shape)}")
     weights = weights.contiguous()

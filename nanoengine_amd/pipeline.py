@@ -11,7 +11,9 @@ take their split partials' buffer from torch's allocator). By default the
 indexer and the top-k run fused (``ops.indexer_topk``: the logits of long
 contexts are never written to memory, those of short ones and small batches go
 to the workspace); ``fused=False`` runs them as the two separate reference
-operators over a logits buffer.
+operators over a logits buffer, and so does ``indexer_format="fp4"``, whose indexer
+cache holds 4-bit pages. The MLA cache's row width says whether its rows are fp8
+(656 bytes) or 4-bit (400 bytes).
 
 Buffer ownership: a call returns views of the object's own buffers (o, lse,
 logical, physical), and the next call on the same object overwrites them. A
@@ -33,7 +35,12 @@ from .state import IndexerTopKState
 
 class DsaDecodeStep:
     def __init__(self, batch: int, next_n: int, max_context_len: int, num_heads: int = 128,
-                 index_topk: int = 2048, page_size: int = 64, device="cuda", fused: bool = True):
+                 index_topk: int = 2048, page_size: int = 64, device="cuda", fused: bool = True,
+                 indexer_format: str = "fp8"):
+        if indexer_format not in ("fp8", "fp4"):
+            raise ValueError(f"indexer_format must be fp8 or fp4, got {indexer_format!r}")
+        self.indexer_format = indexer_format
+        fused = fused and indexer_format == "fp8"
         self.batch, self.next_n, self.max_ctx = batch, next_n, max_context_len
         self.num_heads, self.topk, self.page_size = num_heads, index_topk, page_size
         self.fused = fused
@@ -83,10 +90,10 @@ class DsaDecodeStep:
                  layer_idx: int | None = None, indexer_state: IndexerTopKState | None = None,
                  shared: bool = False, out: torch.Tensor | None = None, lse: torch.Tensor | None = None):
         """q_idx_fp8 [B*n, 64, 128] fp8; weights [B*n, 64] f32; indexer_cache
-        [pages, 8448] uint8; seq_lens [B*n] int32 per-query lengths;
+        [pages, 8448] uint8 (4-bit pages: [pages, 4352]); seq_lens [B*n] int32 per-query lengths;
         block_tables [B, M] int32; page_tables [B*n, M] int32 (block_tables
         repeated per query token); q_mla [B*n, H, 576] bf16; kv_cache
-        [blocks, 64, 1, 656] fp8 bytes. Returns (o, lse, logical, physical).
+        [blocks, 64, 1, 656] fp8 bytes (4-bit rows: [blocks, 64, 1, 400]). Returns (o, lse, logical, physical).
 
         With an ``indexer_state``, a full layer (``shared=False``) publishes its
         (logical, physical) pair under ``layer_idx``; a shared layer
@@ -95,6 +102,7 @@ class DsaDecodeStep:
         indexer inputs are not read on a shared layer and may be None.
         ``out`` [B*n, H, 512] bf16 and ``lse`` [B*n, H] f32, when given, receive
         this call's attention output instead of the object's own buffers."""
+        decode = ops.sparse_mla_decode_fp4 if kv_cache.shape[-1] == ops.MLA_FP4_ROW_BYTES else ops.sparse_mla_decode
         o_buf = self.out if out is None else out
         lse_buf = self.lse if lse is None else lse
         if shared:
@@ -102,8 +110,8 @@ class DsaDecodeStep:
                 raise ValueError("a shared indexer layer needs the indexer_state of a preceding full layer")
             logical, physical = indexer_state.require(layer_idx, self.batch * self.next_n, self.topk,
                                                       require_physical=True)
-            ops.sparse_mla_decode(q_mla, kv_cache, physical, sm_scale, out=o_buf, lse=lse_buf,
-                                  num_splits=self.num_splits, workspace=self._split_workspace())
+            decode(q_mla, kv_cache, physical, sm_scale, out=o_buf, lse=lse_buf,
+                   num_splits=self.num_splits, workspace=self._split_workspace())
             return o_buf, lse_buf, logical, physical
         B, n = self.batch, self.next_n
         q4 = q_idx_fp8.view(B, n, *q_idx_fp8.shape[1:])
@@ -111,12 +119,16 @@ class DsaDecodeStep:
             ops.indexer_topk(q4, indexer_cache, weights, seq_lens.view(B, n), block_tables, self.max_ctx,
                              self.topk, self.physical, self.logical, workspace=self.fused_workspace)
         else:
-            ops.indexer_logits(q4, indexer_cache, weights, seq_lens.view(B, n), block_tables, self.max_ctx,
-                               out=self.logits)
+            if self.indexer_format == "fp4":
+                ops.indexer_logits_fp4(q4, indexer_cache, weights, seq_lens, block_tables, self.max_ctx,
+                                       out=self.logits, clean_logits=False)
+            else:
+                ops.indexer_logits(q4, indexer_cache, weights, seq_lens.view(B, n), block_tables, self.max_ctx,
+                                   out=self.logits)
             ops.topk_transform(self.logits, seq_lens, page_tables, self.physical, self.page_size, self.topk,
                                self.logical, workspace=self.topk_workspace)
         if indexer_state is not None:
             indexer_state.publish(layer_idx, self.logical, self.physical)
-        ops.sparse_mla_decode(q_mla, kv_cache, self.physical, sm_scale, out=o_buf, lse=lse_buf,
-                              num_splits=self.num_splits, workspace=self._split_workspace())
+        decode(q_mla, kv_cache, self.physical, sm_scale, out=o_buf, lse=lse_buf,
+               num_splits=self.num_splits, workspace=self._split_workspace())
         return o_buf, lse_buf, self.logical, self.physical

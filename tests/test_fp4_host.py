@@ -179,3 +179,37 @@ def test_tables_adapter_refuses_bad_tensors():
             ops.batch_tables(**{**args, **kw})
     with pytest.raises(ValueError, match="page_size"):
         ops.batch_tables(lens, lens, bt, 0, slots, status)
+
+
+# ------------------------------------------------------------------ the classes around them
+def test_cache_class_checks():
+    from nanoengine_amd import indexer
+    c = indexer.IndexerCacheFp4(2, 16, 64, device="cpu")
+    assert c.bytes_per_token == 68 and c.get_buffer(1).shape == (16, 64 * 68) and len(c.buffers) == 2
+    with pytest.raises(ValueError, match="128-dim"):
+        indexer.IndexerCacheFp4(1, 4, 64, 64, device="cpu")
+    with pytest.raises(ValueError, match="uint8"):
+        indexer.IndexerCacheFp4(1, 4, 64, device="cpu", buffer=torch.zeros(1, 4, 64 * 132, dtype=torch.uint8))
+
+
+def test_step_refuses_an_unknown_format():
+    from nanoengine_amd.pipeline import DsaDecodeStep
+    with pytest.raises(ValueError, match="indexer_format"):
+        DsaDecodeStep(1, 1, 64, device="cpu", indexer_format="int4")
+
+
+def test_batch_tables_report_their_faults():
+    from nanoengine_amd.batch_tables import BatchTables
+    t = BatchTables(3, 5, 4, device="cpu")
+    t.status.copy_(torch.tensor([0, 5, 2, 77]))
+    assert t.check() == (5, 2, 77)
+    t.status[0] = 2 | 8
+    with pytest.raises(RuntimeError, match="more pages than its block table; more new tokens than rows"):
+        t.check()
+    with pytest.raises(ValueError, match="cannot hold 2 tokens of 3"):
+        t.context_fields(2)
+    t.seq_lens.copy_(torch.tensor([9, 4, 0, 0, 0]))
+    fields = t.context_fields()
+    assert fields["context_lens"].tolist() == [[9, 4, 0]] and fields["block_tables"].shape == (1, 3, 4)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        t.plan(torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
