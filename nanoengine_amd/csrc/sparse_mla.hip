@@ -683,6 +683,132 @@ __device__ __forceinline__ void qk_waves(const MlaParams& P, uint8_t* smem, cons
   barrier();
 }
 
+// QK waves over 4-bit rows for at most 32 heads (a tensor-parallel rank's 16 or
+// 32; NT tiles of 16 heads): with 32-head tiles half of these waves would idle and
+// the others set the block time. Each of the four waves owns 16 keys of a block, over
+// all dims, as 18 v_mfma_f32_16x16x32_bf16 a head tile: A = the keys, lane (n16, g)
+// reading 16 bytes of key n16, its 32-dim blocks 4c + g with one scale each, for four
+// k-steps (dims 128c + 32g + 8i .. +7); B = the query in the same order. The shape
+// has 55% of the 32x32x16's rate, but the wave converts half the keys and takes a
+// quarter of the exponentials. A reference per wave, that is per k-step of P.V.
+template <int NT>
+__device__ __forceinline__ void qk_waves4_narrow(const MlaParams& P, uint8_t* smem, const MlaCtx& c,
+                                                 const DmaLanes& dl) {
+  const int lane = c.lane, w = c.wave, n16 = lane & 15, g = lane >> 4;
+  v4i qn[NT][4][4], qr[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = 16 * nt + n16;
+    const uint8_t* qrow = smem + buf_bytes<kSlots4>() + r * kQRowBytes;
+    const int sw = 16 * (r & 7);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qn[nt][k][i] = *reinterpret_cast<const v4i*>(qrow + ((16 * (16 * k + 4 * g + i)) ^ sw));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) qr[nt][i] = *reinterpret_cast<const v4i*>(qrow + ((16 * (64 + 4 * i + g)) ^ sw));
+  }
+  prologue_end();
+  float* ref = reinterpret_cast<float*>(smem + kRefOff);
+  float m_run[NT], m_max[NT], l_run[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m_run[nt] = m_max[nt] = -__builtin_inff();
+    l_run[nt] = 0.f;
+  }
+  for (int t = 0; t <= c.nblk; ++t) {
+    iteration_start<kSlots4>(P, smem, c, dl, t);
+    if (c.wave == kTabWave && t + 2 < c.nblk) build_addr_table<kSlots4>(P, smem, c, t + 2);
+    if (t < c.nblk) {
+      const uint8_t* row = smem + (t % kNumBufs) * buf_bytes<kSlots4>() + (16 * w + n16) * kMla4RowBytes;
+      const v4i sb = *reinterpret_cast<const v4i*>(row + kMla4ScaleOff);
+      v4i kraw[4], rope[2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) kraw[k] = *reinterpret_cast<const v4i*>(row + 64 * k + 16 * g);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) rope[i] = *reinterpret_cast<const v4i*>(row + kMla4RopeOff + 64 * i + 16 * g);
+      const int32_t slot_t = reinterpret_cast<const int32_t*>(smem + kRingOff + (t % kRingSlots) * 256)[lane];
+      const uint64_t vmask = __ballot(slot_valid(P, slot_t));
+      __builtin_amdgcn_sched_barrier(0);
+      // s[nt][r]: key 16w + 4g + r, head 16nt + n16; two chains a tile
+      v4f s[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float sc = fp4_scale(((uint32_t)sb[k] >> (8 * g)) & 255u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const v8bf kb = as_v8bf(fp4x8_to_bf16((uint32_t)kraw[k][i], sc));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            s[nt][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb, as_v8bf(qn[nt][k][i]), s[nt][i & 1], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          s[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_v8bf(rope[i]), as_v8bf(qr[nt][i]), s[nt][i], 0, 0, 0);
+      const bool all_valid = vmask == ~0ull;
+      const uint32_t vm = (uint32_t)(vmask >> (16 * w + 4 * g)) & 15u;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float sv[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sv[r] = s[nt][0][r] + s[nt][1][r];
+        if (!all_valid) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!((vm >> r) & 1u)) sv[r] = -__builtin_inff();
+        }
+        float mloc = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
+        {
+          const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
+          mloc = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+          const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
+          mloc = fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+        }
+        const float mblk = mloc * P.scale_log2;
+        m_max[nt] = fmaxf(m_max[nt], mblk);
+        const bool need = mblk > m_run[nt] + kRescaleThreshold;
+        if (__ballot(need)) {
+          const float m_new = need ? ceilf(mblk) : m_run[nt];
+          l_run[nt] *= __builtin_amdgcn_exp2f(m_run[nt] - m_new);  // a power of two (0 from -inf)
+          m_run[nt] = m_new;
+        }
+        const float m_use = m_run[nt] == -__builtin_inff() ? 0.f : m_run[nt];
+        float pv[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) pv[r] = __builtin_amdgcn_exp2f(fmaf(sv[r], P.scale_log2, -m_use));
+        if (!all_valid) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!((vm >> r) & 1u)) pv[r] = 0.f;
+        }
+        l_run[nt] += (pv[0] + pv[1]) + (pv[2] + pv[3]);
+        // k-step w of P.V: lane (head, h = g % 2) holds keys 8(j/4) + 4h + j%4 in eight bf16
+        *reinterpret_cast<v2i*>(smem + kPOff + (t & 1) * 8192 + (w * 64 + 32 * (g & 1) + 16 * nt + n16) * 16 + 8 * (g >> 1)) =
+            v2i{cvt_pk_bf16(pv[0], pv[1]), cvt_pk_bf16(pv[2], pv[3])};
+        if (g == 0) ref[((t & 1) * 4 + w) * 32 + 16 * nt + n16] = m_run[nt];
+      }
+    }
+    iteration_end();
+  }
+  float* fin = reinterpret_cast<float*>(smem + kFinOff);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float l2 = l_run[nt] + shfl_xor(l_run[nt], 16);
+    l2 += shfl_xor(l2, 32);
+    if (g == 0) {
+      fin[w * 32 + 16 * nt + n16] = l2;
+      fin[128 + w * 32 + 16 * nt + n16] = m_run[nt];
+      fin[256 + w * 32 + 16 * nt + n16] = m_max[nt];
+    }
+  }
+  barrier();
+}
+
 // QK waves over bf16 rows only (kRows): a block has 32 keys, so the four waves
 // split the dims instead of the keys. Wave (hp, dh = c.kh) forms the partial
 // S^T[32 keys x 32 heads] over quarters 2dh and 2dh + 1 of the dims (a quarter:
@@ -852,9 +978,10 @@ __device__ __forceinline__ void qk_waves_rows(const MlaParams& P, uint8_t* smem,
 // (The alternative, a transposing 4-bit read whose pairs are keys of one dim, needs
 // no permutes but converts two keys with one scale, so that P would have to carry
 // the scales: four times the additions, as a 32-dim tile has a scale of its own.)
-// P' = P * 2^(m_kh - R): a subtraction from the exponent field that stops at zero.
+// P' = P * 2^(m - R), m the reference of the k-step's keys: fx is taken off the
+// exponent field, stopping at zero.
 template <int kTiles>
-__device__ __forceinline__ void pv_block4(v16f (&o)[kTiles][4], const int (&fx)[kTiles][2], const uint8_t* pb,
+__device__ __forceinline__ void pv_block4(v16f (&o)[kTiles][4], const int (&fx)[kTiles][4], const uint8_t* pb,
                                           const uint16_t* et, uint32_t vb, int lane) {
   typedef int v4i_alias __attribute__((ext_vector_type(4), may_alias));
   const int h = lane >> 5, half = (lane >> 4) & 1;
@@ -890,7 +1017,7 @@ __device__ __forceinline__ void pv_block4(v16f (&o)[kTiles][4], const int (&fx)[
       for (int e = 0; e < 4; ++e) {
         const int pe = pq[cur][mt][e];
         pa[mt][e] = __builtin_bit_cast(int, __builtin_elementwise_sub_sat(__builtin_bit_cast(v2u16, pe),
-                                                                          __builtin_bit_cast(v2u16, fx[mt][ks >> 1])));
+                                                                          __builtin_bit_cast(v2u16, fx[mt][ks])));
       }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -923,7 +1050,7 @@ __device__ __forceinline__ void pv_block4(v16f (&o)[kTiles][4], const int (&fx)[
 // Wave dq = w - 4 owns O[64 heads x dims 128dq .. 128dq+127], exactly V tile
 // dq, as two head tiles (the head halves): each V byte is converted once per
 // workgroup, and one exponent per key scales both tiles' P.
-template <int kKeys, int kTiles>
+template <int kKeys, int kTiles, int kNarrow>
 __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, const MlaCtx& c, const DmaLanes& dl,
                                          int split) {
   const int lane = c.lane, h = c.h, c32 = c.c32, dq = c.wave - 4;
@@ -984,12 +1111,18 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
       }
       // each head tile's O follows the larger of its key-half references, moving
       // by a power of two; over bf16 rows only it follows the one reference
-      int fx[kTiles][2];
+      int fx[kTiles][kKeys == kSlots4 ? 4 : 2];
 #pragma unroll
       for (int mt = 0; mt < kTiles; ++mt) {
         float m0, m1 = 0.f, mn;
+        float mq[4];  // narrow scores: a reference per k-step
         if constexpr (kKeys == kRows) {
           mn = m0 = ref[(par * 2 + mt) * 32 + c32];
+        } else if constexpr (kNarrow > 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mq[i] = ref[(par * 4 + i) * 32 + c32];
+          mn = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
+          m0 = mn;
         } else {
           m0 = ref[((par * 2 + mt) * 2 + 0) * 32 + c32];
           m1 = ref[((par * 2 + mt) * 2 + 1) * 32 + c32];
@@ -1011,6 +1144,16 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
             for (int r = 0; r < 16; ++r) o[mt][nn][r] *= ar[r];
         }
         if constexpr (kKeys == kRows) continue;
+        if constexpr (kKeys == kSlots4) {
+          // R - m per k-step (one without a valid key so far has no P)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            const float mk = kNarrow > 0 ? mq[ks] : ks < 2 ? m0 : m1;
+            const int f4 = mk == -__builtin_inff() ? 0 : (int)fminf(R[mt] - mk, 255.f);
+            fx[mt][ks] = (f4 << 7) | (f4 << 23);
+          }
+          continue;
+        }
         // per key half: m_kh - R (<= 0) for the bf16 exponent field (a key half
         // with no valid key yet has only zero rows in this block, so any finite
         // P' is fine there; a half more than 2^30 below R is scaled by 2^-30
@@ -1018,12 +1161,6 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2) {
           const float mk = k2 == 0 ? m0 : m1;
-          if constexpr (kKeys == kSlots4) {
-            // R - m_kh, taken off P's exponent field (a half without a key has no P)
-            const int f4 = mk == -__builtin_inff() ? 0 : (int)fminf(R[mt] - mk, 255.f);
-            fx[mt][k2] = (f4 << 7) | (f4 << 23);
-            continue;
-          }
           const int f = mk == -__builtin_inff() ? 0 : max((int)(mk - R[mt]), kDropExp);
           fx[mt][k2] = (f << 7) & 0xffff;
           fx[mt][k2] |= fx[mt][k2] << 16;
@@ -1132,7 +1269,7 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
       mm = fin[256 + mt * 32 + c32];
     }
 #pragma unroll
-    for (int k2 = 0; k2 < 2 && kKeys != kRows; ++k2) {
+    for (int k2 = 0; k2 < (kNarrow > 0 ? 4 : 2) && kKeys != kRows; ++k2) {
       const float lk = fin[(mt * 2 + k2) * 32 + c32];
       const float mk = fin[128 + (mt * 2 + k2) * 32 + c32];
       if (mk != -__builtin_inff()) lt += lk * __builtin_amdgcn_exp2f(mk - R[mt]);
@@ -1209,7 +1346,8 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
 // tensor-parallel rank's 16) the second tile would be padding: its score waves
 // idle and its P.V products are left out. (As a run-time condition this cost
 // the 64-head kernel 5%: the branches stop the P.V loop's read-ahead.)
-template <int kKeys, int kTiles>
+// kNarrow: 4-bit rows and at most 32 heads, as that many tiles of 16.
+template <int kKeys, int kTiles, int kNarrow = 0>
 __global__ void __launch_bounds__(kMlaThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 sparse_mla_kernel(const MlaParams P) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -1277,8 +1415,9 @@ sparse_mla_kernel(const MlaParams P) {
   // both roles run the same number of iterations and barriers
   if (c.wave < 4) {
     if constexpr (kKeys == kRows) qk_waves_rows<kTiles>(P, smem, c, dl);
+    else if constexpr (kNarrow > 0) qk_waves4_narrow<kNarrow>(P, smem, c, dl);
     else qk_waves<kKeys, kTiles>(P, smem, c, dl);
-  } else pv_waves<kKeys, kTiles>(P, smem, c, dl, split);
+  } else pv_waves<kKeys, kTiles, kNarrow>(P, smem, c, dl, split);
 }
 
 // One wave per (split item, head): merge the split partials. Bound by the
@@ -1463,19 +1602,20 @@ static int launch_mla(const MlaParams& P, KeyKind keys, int64_t nwg, hipStream_t
     for (const void* k : {(const void*)sparse_mla_kernel<kSlots, 1>, (const void*)sparse_mla_kernel<kSlots, 2>,
                           (const void*)sparse_mla_kernel<kSlotsThenRows, 1>,
                           (const void*)sparse_mla_kernel<kSlotsThenRows, 2>, (const void*)sparse_mla_kernel<kRows, 1>,
-                          (const void*)sparse_mla_kernel<kRows, 2>, (const void*)sparse_mla_kernel<kSlots4, 1>,
-                          (const void*)sparse_mla_kernel<kSlots4, 2>})
+                          (const void*)sparse_mla_kernel<kRows, 2>, (const void*)sparse_mla_kernel<kSlots4, 1, 1>,
+                          (const void*)sparse_mla_kernel<kSlots4, 1, 2>, (const void*)sparse_mla_kernel<kSlots4, 2>})
       if (hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kRowsSmemBytes) != hipSuccess)
         smem_status = 1;
   }
   if (smem_status) return set_error(kLaunchFailed, "sparse_mla: cannot reserve %zu B of LDS", kRowsSmemBytes);
   if (nwg > INT32_MAX) return set_error(kInvalidArgument, "%s: grid too large", what);
-  void (*const kernels[4][2])(MlaParams) = {
-      {sparse_mla_kernel<kSlots, 1>, sparse_mla_kernel<kSlots, 2>},
-      {sparse_mla_kernel<kSlotsThenRows, 1>, sparse_mla_kernel<kSlotsThenRows, 2>},
-      {sparse_mla_kernel<kRows, 1>, sparse_mla_kernel<kRows, 2>},
-      {sparse_mla_kernel<kSlots4, 1>, sparse_mla_kernel<kSlots4, 2>}};
-  hipLaunchKernelGGL(kernels[keys][P.H <= 32 ? 0 : 1], dim3((unsigned)nwg), dim3(kMlaThreads),
+  // at most 16 heads, at most 32, more
+  void (*const kernels[4][3])(MlaParams) = {
+      {sparse_mla_kernel<kSlots, 1>, sparse_mla_kernel<kSlots, 1>, sparse_mla_kernel<kSlots, 2>},
+      {sparse_mla_kernel<kSlotsThenRows, 1>, sparse_mla_kernel<kSlotsThenRows, 1>, sparse_mla_kernel<kSlotsThenRows, 2>},
+      {sparse_mla_kernel<kRows, 1>, sparse_mla_kernel<kRows, 1>, sparse_mla_kernel<kRows, 2>},
+      {sparse_mla_kernel<kSlots4, 1, 1>, sparse_mla_kernel<kSlots4, 1, 2>, sparse_mla_kernel<kSlots4, 2>}};
+  hipLaunchKernelGGL(kernels[keys][P.H <= 16 ? 0 : P.H <= 32 ? 1 : 2], dim3((unsigned)nwg), dim3(kMlaThreads),
                      keys == kRows ? kRowsSmemBytes : kMlaSmemBytes, stream, P);
   return check_launch(what);
 }
