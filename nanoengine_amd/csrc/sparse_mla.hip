@@ -683,6 +683,23 @@ __device__ __forceinline__ void qk_waves(const MlaParams& P, uint8_t* smem, cons
   barrier();
 }
 
+// Scale table of a block's dims 128dq .. +127 (lane = key): the four 32-dim blocks'
+// scales in the exponent field of a 16-bit entry, [4 blocks][the key's position in
+// the P.V operand: k-step key/16, lane half (key/4)%2, element 4((key/8)%2) + key%4].
+__device__ __forceinline__ void scale_table4(const uint8_t* buf, uint16_t* et, int dq, int lane) {
+  const uint32_t sb = *reinterpret_cast<const uint32_t*>(buf + lane * kMla4RowBytes + kMla4ScaleOff + 4 * dq);
+  const int pos = ((lane >> 4) * 2 + ((lane >> 2) & 1)) * 8 + 4 * ((lane >> 3) & 1) + (lane & 3);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) et[64 * i + pos] = (uint16_t)(((sb >> (8 * i)) & 255u) << 7);
+}
+// Where the narrow score waves put the scale tables of the blocks of parity `par`
+// (the row buffers of 4-bit rows end before).
+constexpr int kEt4Off = kNumBufs * kMlaKeys * kMla4RowBytes;
+static_assert(kEt4Off + 2 * 4 * 512 <= kPOff, "the scale tables lie between the row buffers and P");
+__device__ __forceinline__ uint16_t* et_block4(uint8_t* smem, int par, int dq) {
+  return reinterpret_cast<uint16_t*>(smem + kEt4Off + par * 2048 + dq * 512);
+}
+
 // QK waves over 4-bit rows for at most 32 heads (a tensor-parallel rank's 16 or
 // 32; NT tiles of 16 heads): with 32-head tiles half of these waves would idle and
 // the others set the block time. Each of the four waves owns 16 keys of a block, over
@@ -729,6 +746,9 @@ __device__ __forceinline__ void qk_waves4_narrow(const MlaParams& P, uint8_t* sm
       for (int i = 0; i < 2; ++i) rope[i] = *reinterpret_cast<const v4i*>(row + kMla4RopeOff + 64 * i + 16 * g);
       const int32_t slot_t = reinterpret_cast<const int32_t*>(smem + kRingOff + (t % kRingSlots) * 256)[lane];
       const uint64_t vmask = __ballot(slot_valid(P, slot_t));
+      // the P.V waves' scale table of this block, for the dims 128w .. +127: theirs is the longer chain
+      // (each building its own: 31.0 us where this takes 29.4, 90 tokens of 16 heads)
+      scale_table4(smem + (t % kNumBufs) * buf_bytes<kSlots4>(), et_block4(smem, t & 1, w), w, lane);
       __builtin_amdgcn_sched_barrier(0);
       // s[nt][r]: key 16w + 4g + r, head 16nt + n16; two chains a tile
       v4f s[NT][2];
@@ -980,8 +1000,8 @@ __device__ __forceinline__ void qk_waves_rows(const MlaParams& P, uint8_t* smem,
 // the scales: four times the additions, as a 32-dim tile has a scale of its own.)
 // P' = P * 2^(m - R), m the reference of the k-step's keys: fx is taken off the
 // exponent field, stopping at zero.
-template <int kTiles>
-__device__ __forceinline__ void pv_block4(v16f (&o)[kTiles][4], const int (&fx)[kTiles][4], const uint8_t* pb,
+template <int kTiles, int kParts>
+__device__ __forceinline__ void pv_block4(v16f (&o)[kTiles][4], const int (&fx)[kTiles][kParts], const uint8_t* pb,
                                           const uint16_t* et, uint32_t vb, int lane) {
   typedef int v4i_alias __attribute__((ext_vector_type(4), may_alias));
   const int h = lane >> 5, half = (lane >> 4) & 1;
@@ -1017,7 +1037,7 @@ __device__ __forceinline__ void pv_block4(v16f (&o)[kTiles][4], const int (&fx)[
       for (int e = 0; e < 4; ++e) {
         const int pe = pq[cur][mt][e];
         pa[mt][e] = __builtin_bit_cast(int, __builtin_elementwise_sub_sat(__builtin_bit_cast(v2u16, pe),
-                                                                          __builtin_bit_cast(v2u16, fx[mt][ks])));
+                                                                          __builtin_bit_cast(v2u16, fx[mt][ks * kParts / 4])));
       }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -1093,13 +1113,7 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
       const uint8_t* bufp = smem + ((t - 1) % kNumBufs) * buf_bytes<kKeys>();
       const bool fresh = rows_block<kKeys>(c, t - 1);
       if constexpr (kKeys == kSlots4) {
-        // scale table of block t-1, dims 128dq .. +127 (lane = key): four blocks' scales in the exponent
-        // field of a 16-bit entry, [4 blocks][the key's position, as below]
-        const int key = lane;
-        const uint32_t sb = *reinterpret_cast<const uint32_t*>(bufp + key * kMla4RowBytes + kMla4ScaleOff + 4 * dq);
-        const int pos = ((key >> 4) * 2 + ((key >> 2) & 1)) * 8 + 4 * ((key >> 3) & 1) + (key & 3);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) et[64 * i + pos] = (uint16_t)(((sb >> (8 * i)) & 255u) << 7);
+        if constexpr (kNarrow == 0) scale_table4(bufp, et, dq, lane);
       } else if (!fresh) {
         // exponent table of block t-1, tile dq (lane = key): the tile scale's
         // exponent in the bf16 exponent field, at the PV A operand position of
@@ -1111,7 +1125,8 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
       }
       // each head tile's O follows the larger of its key-half references, moving
       // by a power of two; over bf16 rows only it follows the one reference
-      int fx[kTiles][kKeys == kSlots4 ? 4 : 2];
+      constexpr int kParts = kNarrow > 0 ? 4 : 2;  // references of a block: per key half, or per 16 keys
+      int fx[kTiles][kParts];
 #pragma unroll
       for (int mt = 0; mt < kTiles; ++mt) {
         float m0, m1 = 0.f, mn;
@@ -1145,12 +1160,12 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
         }
         if constexpr (kKeys == kRows) continue;
         if constexpr (kKeys == kSlots4) {
-          // R - m per k-step (one without a valid key so far has no P)
+          // R - m of each part (one without a valid key so far has no P)
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const float mk = kNarrow > 0 ? mq[ks] : ks < 2 ? m0 : m1;
+          for (int k = 0; k < kParts; ++k) {
+            const float mk = kNarrow > 0 ? mq[k] : k == 0 ? m0 : m1;
             const int f4 = mk == -__builtin_inff() ? 0 : (int)fminf(R[mt] - mk, 255.f);
-            fx[mt][ks] = (f4 << 7) | (f4 << 23);
+            fx[mt][k] = (f4 << 7) | (f4 << 23);
           }
           continue;
         }
@@ -1179,7 +1194,7 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
       };
       constexpr int kSteps = kKeys == kRows ? kFreshKeys / 16 : kMlaKeys / 16;
       if constexpr (kKeys == kSlots4) {
-        pv_block4<kTiles>(o, fx, pb, et, vb, lane);
+        pv_block4<kTiles, kParts>(o, fx, pb, kNarrow > 0 ? et_block4(smem, par, dq) : et, vb, lane);
       } else {
       // k-step ks: its P (both head tiles), exponent and V reads issued one
       // k-step ahead
