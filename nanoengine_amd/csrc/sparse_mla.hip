@@ -51,6 +51,15 @@
 // QK waves split the dims instead of the keys and exchange their partial scores
 // in the middle of an iteration. Every key of a block shares one reference, the
 // largest score when it last moved, so P needs no exponent adds.
+// 4-bit rows (kSlots4: 400 bytes, fp4.h): the same roles and loop. A QK lane reads
+// 16 bytes of codes a chunk, one 32-dim block with one scale, and converts them with it.
+// A PV wave's 128 dims have four scales a key instead of one, so P carries none: the
+// codes are converted with their scales (pv_block4), and P needs only its reference's
+// exponent, subtracted with saturation. Either way every converted value is the bf16
+// the row stands for. The row is 61% of the fp8 one and the time the same (128
+// tokens of 128 heads, 2048 keys: 77 us from a graph, 1.84 TB/s, 0.95 PFLOP/s): the
+// block time follows the SIMDs' instructions, not the bytes. With at most 32 heads
+// the score waves take 16 keys each on 16x16x32 products (qk_waves4_narrow).
 // Splits over the key list (the items of the last, partial round of the CUs)
 // write normalised partial outputs and LSEs to a caller-provided workspace; a
 // combine kernel merges them with the LSE rule of merge_attention_states.
@@ -708,6 +717,9 @@ __device__ __forceinline__ uint16_t* et_block4(uint8_t* smem, int par, int dq) {
 // k-steps (dims 128c + 32g + 8i .. +7); B = the query in the same order. The shape
 // has 55% of the 32x32x16's rate, but the wave converts half the keys and takes a
 // quarter of the exponentials. A reference per wave, that is per k-step of P.V.
+// (90 tokens of 16 heads: 36.4 us on 32x32 tiles, 31.0 so; 256 tokens 61 and 54,
+// 4.1 TB/s of rows. The P.V waves' conversions, ~1600 of an iteration's ~2300 cycles,
+// set the block time then; a second block of rows in flight gains nothing.)
 template <int NT>
 __device__ __forceinline__ void qk_waves4_narrow(const MlaParams& P, uint8_t* smem, const MlaCtx& c,
                                                  const DmaLanes& dl) {
@@ -747,7 +759,7 @@ __device__ __forceinline__ void qk_waves4_narrow(const MlaParams& P, uint8_t* sm
       const int32_t slot_t = reinterpret_cast<const int32_t*>(smem + kRingOff + (t % kRingSlots) * 256)[lane];
       const uint64_t vmask = __ballot(slot_valid(P, slot_t));
       // the P.V waves' scale table of this block, for the dims 128w .. +127: theirs is the longer chain
-      // (each building its own: 31.0 us where this takes 29.4, 90 tokens of 16 heads)
+      // (256 tokens of 16 heads: 54.7 us with each building its own, 53.6 so)
       scale_table4(smem + (t % kNumBufs) * buf_bytes<kSlots4>(), et_block4(smem, t & 1, w), w, lane);
       __builtin_amdgcn_sched_barrier(0);
       // s[nt][r]: key 16w + 4g + r, head 16nt + n16; two chains a tile

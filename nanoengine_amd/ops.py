@@ -746,9 +746,12 @@ def sparse_mla_prefill_paged(q: torch.Tensor, k_cache: torch.Tensor, block_table
 
 
 # --------------------------------------------------------------------------- 4-bit caches
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _launch(dev: torch.device, name: str, *args) -> None:
     """Call ``name`` with the current stream of ``dev`` as its last argument, on ``dev``."""
-    if dev.index == torch.cuda.current_device():
+    if dev.index == _CURRENT_DEVICE():
         _lib.call(name, *args, _stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -934,7 +937,7 @@ def _int_out(t: torch.Tensor | None, n: int, name: str, dtypes=(torch.int32, tor
     """1 when the optional output is int64."""
     if t is None:
         return 0
-    if not (t.dtype in dtypes and tuple(t.shape) == (n,) and t.is_contiguous()):
+    if not (t.dtype in dtypes and t.dim() == 1 and t.numel() == n and t.is_contiguous()):
         _fail(f"{name} must be contiguous {' or '.join(str(d).replace('torch.', '') for d in dtypes)} [{n}]")
     return int(t.dtype == torch.int64)
 
@@ -973,8 +976,11 @@ def batch_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables
         _fail("free_blocks must be contiguous int32 [F]")
     if free_head is not None and not (free_head.dtype == torch.int32 and free_head.numel() == 1):
         _fail("free_head must be int32 with one element")
-    dev = _check_cuda(*(t for t in (cached_lens, new_lens, block_tables, slot_mapping, status, free_blocks, free_head,
-                                    positions, seq_lens, cu_seqlens_q, cu_seqlens_k) if t is not None))
+    dev = _check_cuda(cached_lens)
+    for t in (new_lens, block_tables, slot_mapping, status, free_blocks, free_head, positions, seq_lens, cu_seqlens_q,
+              cu_seqlens_k):
+        if t is not None and t.device != dev:
+            _fail(f"tensors on different devices: {t.device} vs {dev}")
     # an empty free list still means that blocks are taken from it
     free_ptr = None if free_blocks is None else (free_blocks.data_ptr() or status.data_ptr())
     _launch(dev, "dsa_batch_tables", cached_lens.data_ptr(), new_lens.data_ptr(), B, block_tables.data_ptr(),
