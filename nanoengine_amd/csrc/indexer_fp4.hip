@@ -45,7 +45,7 @@ constexpr int kBufs = 2;            // page buffers a wave: one page in flight, 
 constexpr int kPageLoads = 5;       // instructions of a page: 4 x 1 KB of codes, the scales
 constexpr int kAdvance = 62;        // pages per refill of a wave's 64 block-table entries
 constexpr int kMaxBatch = 4096;     // entries of a launch (their page prefix lies in LDS)
-constexpr int kFillChunk = 4096;    // positions past a row's pages that a wave fills at a time
+constexpr int kFillChunk = 1024;    // positions past a row's pages that a wave fills at a time
 constexpr int kWeightBytes = 2 * kHeads * sizeof(float);  // a wave's head weights (two query tokens only)
 constexpr size_t smem_bytes(int next_n, int batch) {
   return (size_t)kWaves * (kBufs * kPageBytes4 + (next_n == 2 ? kWeightBytes : 0)) +
@@ -131,25 +131,9 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
   const int64_t total = carry;
   const int64_t nwaves = (int64_t)gridDim.x * kWaves, gw = (int64_t)blockIdx.x * kWaves + wave;
 
-  // positions past the rows' pages
-  if (P.clean) {
-    const int64_t chunks = (P.max_ctx + kFillChunk - 1) / kFillChunk, tasks = (int64_t)P.batch * chunks;
-    for (int64_t i = gw; i < tasks; i += nwaves) {
-      const int b = (int)(i / chunks);
-      const int64_t at = (i - b * chunks) * kFillChunk;
-      const int64_t begin = max(at, (int64_t)(prefix[b + 1] - prefix[b]) * kPage);
-      const int64_t end = min(at + kFillChunk, P.max_ctx);
-#pragma unroll
-      for (int j = 0; j < NQ; ++j)
-        for (int64_t t = begin + lane; t < end; t += 64)
-          P.logits[((int64_t)b * NQ + j) * P.stride + t] = -__builtin_inff();
-    }
-  }
-
   // this wave's range of the flattened pages
   const int64_t p0 = total * gw / nwaves, p1 = total * (gw + 1) / nwaves;
   const int n = (int)(p1 - p0);
-  if (n <= 0) return;
 
   // block-table window: lane l holds page p0 + wb + l as (batch entry, cache page)
   int wb = 0, win_b = 0, win_page = -1;
@@ -171,7 +155,7 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
     win_b = bl;
     win_page = page;
   };
-  refill(0);
+  if (n > 0) refill(0);
 
   const uint32_t lane_off = 64u * (lane >> 2) + 16u * ((lane & 3) ^ (lane >> 4));
   auto issue = [&](int k) {
@@ -332,7 +316,7 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
     }
   };
 
-  issue(0);
+  if (n > 0) issue(0);
   // entry by entry, so that the query's registers are the inner loop's constants
   for (int k = 0; k < n;) {
     const int b = __builtin_amdgcn_readlane(win_b, k - wb);
@@ -356,6 +340,21 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
         wb += kAdvance;
         refill(wb);
       }
+    }
+  }
+
+  // positions past the rows' pages, after the pages: the waits above would wait for these stores too
+  if (P.clean) {
+    const int64_t chunks = (P.max_ctx + kFillChunk - 1) / kFillChunk, tasks = (int64_t)P.batch * chunks;
+    for (int64_t i = gw; i < tasks; i += nwaves) {
+      const int b = (int)(i / chunks);
+      const int64_t at = (i - b * chunks) * kFillChunk;
+      const int64_t begin = max(at, (int64_t)(prefix[b + 1] - prefix[b]) * kPage);
+      const int64_t end = min(at + kFillChunk, P.max_ctx);
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+        for (int64_t t = begin + lane; t < end; t += 64)
+          P.logits[((int64_t)b * NQ + j) * P.stride + t] = -__builtin_inff();
     }
   }
 }
