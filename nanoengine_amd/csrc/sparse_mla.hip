@@ -1612,6 +1612,11 @@ int dsa_sparse_mla_decode_fp4(const void* q, int64_t q_token_stride, int64_t q_h
                               const int32_t* indices, int64_t idx_stride, int num_tokens, int num_heads, int topk,
                               float sm_scale, void* out, float* lse, int num_splits, void* workspace,
                               size_t workspace_bytes, void* stream) {
+  // the running maximum is one of unscaled scores
+  if (!(sm_scale >= 0.f) || !std::isfinite(sm_scale))
+    return dsa::set_error(dsa::kInvalidArgument, "sparse_mla: sm_scale must be finite and not negative");
+  if (reinterpret_cast<uintptr_t>(workspace) & 15)
+    return dsa::set_error(dsa::kInvalidArgument, "sparse_mla: the workspace must be 16-byte aligned");
   return dsa::sparse_mla_decode_impl(q, q_token_stride, q_head_stride, kv_cache, kv_block_stride_bytes,
                                      kv_block_size, kv_num_blocks, indices, idx_stride, num_tokens, num_heads, topk,
                                      sm_scale, out, lse, num_splits, workspace, workspace_bytes, stream, nullptr,

@@ -749,13 +749,25 @@ def sparse_mla_prefill_paged(q: torch.Tensor, k_cache: torch.Tensor, block_table
 _CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _launch(dev: torch.device, name: str, *args) -> None:
-    """Call ``name`` with the current stream of ``dev`` as its last argument, on ``dev``."""
-    if dev.index == _CURRENT_DEVICE():
-        _lib.call(name, *args, _stream(dev))
+def _gpu(*tensors: torch.Tensor) -> int:
+    """Index of the one GPU that holds every tensor (the checks of ``_check_cuda`` by device number: a
+    device object per tensor is most of a small call's checks)."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if index < 0 or t.get_device() != index:
+            _check_cuda(*tensors)
+    return index
+
+
+def _launch(index: int, name: str, *args) -> None:
+    """Call ``name`` on GPU ``index`` with its current stream as the last argument."""
+    if index != _CURRENT_DEVICE():
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+    elif _RAW_STREAM is not None:
+        _lib.call(name, *args, _RAW_STREAM(index))
     else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, _stream(dev))
+        _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
 
 
 def mla_fp4_geometry(k_cache: torch.Tensor) -> tuple[int, int]:
@@ -796,7 +808,7 @@ def mla_kv_store_fp4(kv: torch.Tensor, k_cache: torch.Tensor, slot_mapping: torc
     blk_stride, block_size = mla_fp4_geometry(k_cache)
     n = kv.shape[0]
     slots, is64 = _slots(slot_mapping, n)
-    dev = _check_cuda(kv, k_cache, slots)
+    dev = _gpu(kv, k_cache, slots)
     _launch(dev, "dsa_mla_kv_store_fp4", kv.data_ptr(), kv.stride(0) if n > 1 else MLA_D_QK, slots.data_ptr(), is64, n,
             k_cache.data_ptr(), blk_stride, block_size, k_cache.shape[0])
 
@@ -807,12 +819,12 @@ def mla_kv_load_fp4(k_cache: torch.Tensor, slots: torch.Tensor, out: torch.Tenso
     blk_stride, block_size = mla_fp4_geometry(k_cache)
     s, is64 = _slots(slots, 0)
     n = s.shape[0]
-    dev = _check_cuda(k_cache, s)
+    dev = _gpu(k_cache, s)
     if out is None:
         out = torch.empty(n, MLA_D_QK, dtype=torch.bfloat16, device=dev)
     if not (out.dtype == torch.bfloat16 and tuple(out.shape) == (n, MLA_D_QK) and out.stride(1) == 1):
         _fail(f"out must be bf16 [{n}, {MLA_D_QK}] with a contiguous last dim")
-    _check_cuda(k_cache, out)
+    _gpu(k_cache, out)
     _launch(dev, "dsa_mla_kv_load_fp4", k_cache.data_ptr(), blk_stride, block_size, k_cache.shape[0], s.data_ptr(), is64, n,
             out.data_ptr(), _row_stride(out))
     return out
@@ -832,7 +844,7 @@ def sparse_mla_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, indices: torch
         _fail("indices must be int32 [T, topk] with unit column stride")
     topk = indices.shape[1]
     blk_stride, block_size = mla_fp4_geometry(k_cache)
-    dev = _check_cuda(q, k_cache, indices)
+    dev = _gpu(q, k_cache, indices)
     if out is None:
         out = torch.empty(T, H, MLA_D_V, dtype=torch.bfloat16, device=dev)
     if lse is None:
@@ -841,13 +853,20 @@ def sparse_mla_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, indices: torch
         _fail("out must be contiguous bf16 [T, H, 512]")
     if not (lse.dtype == torch.float32 and tuple(lse.shape) == (T, H) and lse.is_contiguous()):
         _fail("lse must be contiguous f32 [T, H]")
-    _check_cuda(q, out, lse)
+    _gpu(q, out, lse)
     if num_splits is None:
         num_splits = sparse_mla_num_splits(T, H, topk, dev)
-    need = sparse_mla_workspace_bytes(T, H, num_splits)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+    need = 0
+    if num_splits > 1:
+        if dev == _CURRENT_DEVICE():
+            need = sparse_mla_workspace_bytes(T, H, num_splits)
+        else:  # the size goes by the current device's CUs
+            with torch.cuda.device(dev):
+                need = sparse_mla_workspace_bytes(T, H, num_splits)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need
+                 or workspace.data_ptr() % 16 or workspace.get_device() != dev):
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    _launch(dev, "dsa_sparse_mla_decode_fp4", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), blk_stride,
+    _launch(dev, "dsa_sparse_mla_decode_fp4", q.data_ptr(), q.stride(0) if T > 1 else 0, q.stride(1), k_cache.data_ptr(), blk_stride,
             block_size, k_cache.shape[0], indices.data_ptr(), indices.stride(0), T, H, topk, float(sm_scale),
             out.data_ptr(), lse.data_ptr(), int(num_splits), workspace.data_ptr() if need else None,
             workspace.numel() * workspace.element_size() if need else 0)
@@ -862,7 +881,7 @@ def indexer_k_store_fp4(key: torch.Tensor, cache: torch.Tensor, slot_mapping: to
         _fail("key must be bf16 [N, 128] with a contiguous last dim")
     pages = _fp4_pages(cache, page_size)
     slots, is64 = _slots(slot_mapping, key.shape[0])
-    dev = _check_cuda(key, cache, slots)
+    dev = _gpu(key, cache, slots)
     _launch(dev, "dsa_indexer_k_store_fp4", key.data_ptr(), _row_stride(key), slots.data_ptr(), is64, key.shape[0],
             cache.data_ptr(), int(page_size), pages)
 
@@ -874,7 +893,7 @@ def indexer_k_load_fp4(cache: torch.Tensor, slots: torch.Tensor, page_size: int,
     pages = _fp4_pages(cache, page_size)
     s, is64 = _slots(slots, 0)
     n = s.shape[0]
-    dev = _check_cuda(cache, s)
+    dev = _gpu(cache, s)
     if key_out is None:
         key_out = torch.empty(n, INDEXER_HEAD_DIM, dtype=torch.float8_e4m3fn, device=dev)
     if scale_out is None:
@@ -884,7 +903,7 @@ def indexer_k_load_fp4(cache: torch.Tensor, slots: torch.Tensor, page_size: int,
         _fail(f"key_out must be contiguous fp8 [{n}, 128]")
     if not (scale_out.dtype == torch.float32 and scale_out.numel() == n and scale_out.is_contiguous()):
         _fail(f"scale_out must be contiguous f32 [{n}]")
-    _check_cuda(cache, key_out, scale_out)
+    _gpu(cache, key_out, scale_out)
     _launch(dev, "dsa_indexer_k_load_fp4", cache.data_ptr(), int(page_size), pages, s.data_ptr(), is64, n,
             key_out.data_ptr(), scale_out.data_ptr())
     return key_out, scale_out
@@ -919,13 +938,13 @@ def indexer_logits_fp4(q_fp8: torch.Tensor, kv_cache: torch.Tensor, weights: tor
         _fail("block_tables rows must be contiguous")
     if not (max_context_len >= 0 and bt.shape[1] * page_size >= max_context_len):
         _fail("block_tables too narrow for max_context_len")
-    dev = _check_cuda(q_fp8, kv_cache, weights, cl, bt)
+    dev = _gpu(q_fp8, kv_cache, weights, cl, bt)
     if out is None:
         out = torch.empty(B * n, max_context_len, dtype=torch.float32, device=dev)
     if not (out.dtype == torch.float32 and out.dim() == 2 and out.shape[0] == B * n
             and out.shape[1] >= max_context_len and (out.shape[1] < 2 or out.stride(1) == 1)):
         _fail("logits output must be f32 [B*n, >=max_ctx] with unit column stride")
-    _check_cuda(q_fp8, out)
+    _gpu(q_fp8, out)
     _launch(dev, "dsa_indexer_logits_fp4", q_fp8.data_ptr(), kv_cache.data_ptr(), pages, weights.data_ptr(), cl.data_ptr(),
             bt.data_ptr(), bt.stride(0), B, n, H, D, page_size, int(max_context_len), out.data_ptr(),
             _row_stride(out), int(bool(clean_logits)))
@@ -976,11 +995,8 @@ def batch_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables
         _fail("free_blocks must be contiguous int32 [F]")
     if free_head is not None and not (free_head.dtype == torch.int32 and free_head.numel() == 1):
         _fail("free_head must be int32 with one element")
-    dev = _check_cuda(cached_lens)
-    for t in (new_lens, block_tables, slot_mapping, status, free_blocks, free_head, positions, seq_lens, cu_seqlens_q,
-              cu_seqlens_k):
-        if t is not None and t.device != dev:
-            _fail(f"tensors on different devices: {t.device} vs {dev}")
+    dev = _gpu(*[t for t in (cached_lens, new_lens, block_tables, slot_mapping, status, free_blocks, free_head,
+                             positions, seq_lens, cu_seqlens_q, cu_seqlens_k) if t is not None])
     # an empty free list still means that blocks are taken from it
     free_ptr = None if free_blocks is None else (free_blocks.data_ptr() or status.data_ptr())
     _launch(dev, "dsa_batch_tables", cached_lens.data_ptr(), new_lens.data_ptr(), B, block_tables.data_ptr(),

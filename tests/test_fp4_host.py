@@ -103,7 +103,8 @@ def test_attention_and_logits_refusals(lib):
     _bad(lib, "dsa_sparse_mla_decode_fp4", args,
          [(0, P, 1), (3, P, 1), (7, P, 1), (13, P, 1), (0, ODD, 1), (3, ODD, 1), (13, ODD, 1), (1, 4, 1), (2, 580, 1),
           (4, 64 * 400 - 16, 1), (4, 64 * 400 + 8, 1), (5, 0, 1), (6, -1, 1), (9, -1, 2), (10, 24, 2), (10, 0, 2),
-          (11, 100, 2), (11, 0, 2), (9, 0, 0)])
+          (11, 100, 2), (11, 0, 2), (9, 0, 0), (12, ctypes.c_float(-1), 1), (12, ctypes.c_float(float("nan")), 1),
+          (12, ctypes.c_float(float("inf")), 1), (16, ODD, 1), (15, 4, 4)])
     args = [ONE, ONE, 8, ONE, ONE, ONE, 4, 2, 1, 64, 128, 64, 256, ONE, 256, 1, P]
     _bad(lib, "dsa_indexer_logits_fp4", args,
          [(0, P, 1), (1, P, 1), (3, P, 1), (4, P, 1), (5, P, 1), (13, P, 1), (0, ODD, 1), (1, ODD, 1), (2, -1, 1),

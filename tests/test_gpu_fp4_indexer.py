@@ -108,3 +108,48 @@ def test_blocks_of_different_size_and_nan_keys(cuda):
     assert torch.all(torch.isnan(again[:, 133]))
     keep = torch.arange(900, device=cuda) != 133
     assert torch.equal(again[:, keep], got[:, keep])
+
+
+def test_cache_past_4_gib(cuda):
+    """Pages behind 2^32 bytes of cache are written, read back and scored."""
+    pages = 2 ** 32 // (64 * 68) + 40
+    cache = torch.zeros(pages, 64 * 68, dtype=torch.uint8, device=cuda)
+    slots = torch.arange(pages * 64 - 300, pages * 64, device=cuda)
+    key = torch.randn(300, 128, device=cuda).to(torch.bfloat16)
+    ops.indexer_k_store_fp4(key, cache, slots, 64)
+    values = F.fp4_values(*F.fp4_quantize(key.float()))
+    keys, s = ops.indexer_k_load_fp4(cache, slots, 64)
+    assert torch.equal(keys.double() * s.double()[:, None], values)
+    bt = torch.arange(pages - 4, pages, device=cuda, dtype=torch.int32)[None]
+    q = (torch.randn(1, 1, 64, 128, device=cuda) * 60).to(torch.float8_e4m3fn)
+    w = torch.randn(1, 64, device=cuda)
+    got = ops.indexer_logits_fp4(q, cache, w, torch.tensor([[256]], device=cuda), bt, 256)
+    torch.cuda.synchronize()
+    want, tol = F.logits_row(q[0, 0].float(), w[0], values[300 - 256:])
+    assert torch.all((got[0].double() - want).abs() <= tol)
+
+
+@pytest.mark.parametrize("n", [1, 2])
+def test_more_entries_than_a_launch_takes(cuda, n):
+    """Past 4096 entries the batch goes in several launches; one table row serves every entry (row stride 0)."""
+    B = 4097 + 4096
+    q1, w1, cache, bt, _, values = _case([130], n, 8, cuda)
+    g = torch.Generator().manual_seed(8)
+    ctx = torch.randint(0, 131, (B, n), generator=g).to(torch.int32).to(cuda)
+    q = q1.view(torch.uint8).expand(B, n, 64, 128).contiguous()
+    got = ops.indexer_logits_fp4(q, cache, w1.repeat(B, 1), ctx, bt.expand(B, -1), 130)
+    torch.cuda.synchronize()
+    for j in range(n):
+        want, tol = F.logits_row(q1[0, j].float(), w1[j], _keys(values, bt[0], 130))
+        rows, L = got[j::n], ctx[:, j:j + 1]
+        inside = torch.arange(130, device=cuda)[None] < L
+        assert torch.all(((rows.double() - want).abs() <= tol) | ~inside)
+        assert torch.all(torch.isneginf(rows) | inside)
+
+
+def test_negative_lengths_and_wide_tables(cuda):
+    q, w, cache, bt, ctx, values = _case([200, 64, 129], 1, 9, cuda, spare=40)
+    ctx[1] = -5
+    got = ops.indexer_logits_fp4(q, cache, w, ctx.view(-1), bt, bt.shape[1] * 64)
+    torch.cuda.synchronize()
+    _check(got, q, w, bt, ctx.clamp(min=0), values, bt.shape[1] * 64)

@@ -149,3 +149,44 @@ def test_nan_rows(cuda):
         torch.cuda.synchronize()
         assert torch.all(torch.isnan(o[0])) and torch.all(torch.isnan(lse[0]))
         _check(o[1:], lse[1:], q[1:], values, idx[1:], SCALE)
+
+
+@pytest.mark.parametrize("H", [16, 32, 128])
+def test_repeated_and_unordered_slots(cuda, H):
+    """A slot listed twice counts twice; the order of a row's slots changes nothing but rounding."""
+    cache, values = _cache(40, 10, cuda)
+    q = _query(2, H, 10, cuda)
+    idx = torch.randint(0, 300, (2, 512), device=cuda).to(torch.int32)
+    o, lse = ops.sparse_mla_decode_fp4(q, cache, idx, SCALE)
+    torch.cuda.synchronize()
+    _check(o, lse, q, values, idx, SCALE)
+
+
+def test_cache_past_4_gib(cuda):
+    """Rows behind 2^32 bytes of cache are written, read back and attended over."""
+    blocks = 2 ** 32 // (65 * 400) + 70
+    cache = torch.zeros(blocks, 65, 1, 400, dtype=torch.uint8, device=cuda)[:, :64]
+    slots = torch.cat([torch.arange(96), torch.arange(blocks * 64 - 160, blocks * 64)]).to(cuda)
+    kv = torch.randn(256, 576, device=cuda).to(torch.bfloat16)
+    ops.mla_kv_store_fp4(kv, cache, slots)
+    assert torch.equal(cache[blocks - 2, 5, 0], F.mla_rows(kv[96 + 160 - 128 + 5:][:1])[0])
+    values = F.mla_values(F.mla_rows(kv))
+    assert torch.equal(ops.mla_kv_load_fp4(cache, slots).double(), values)
+    q = _query(2, 64, 11, cuda)
+    at = torch.stack([torch.randperm(256, device=cuda), torch.randperm(256, device=cuda)])
+    o, lse = ops.sparse_mla_decode_fp4(q, cache, slots[at].to(torch.int32), SCALE)
+    torch.cuda.synchronize()
+    _check(o, lse, q, values, at, SCALE)
+
+
+def test_workspace_of_the_caller(cuda):
+    """A caller's workspace is used as it is, a small or unaligned one replaced; outputs of one token from a
+    larger tensor."""
+    cache, values = _cache(40, 12, cuda)
+    q, idx = _query(3, 128, 12, cuda)[1:2], _indices(1, 2048, 2560, 12, cuda)
+    need = ops.sparse_mla_workspace_bytes(1, 128, 8)
+    for ws in (torch.empty(need, dtype=torch.uint8, device=cuda), torch.empty(need + 5, dtype=torch.uint8, device=cuda)[5:],
+               torch.empty(64, dtype=torch.uint8, device=cuda)):
+        o, lse = ops.sparse_mla_decode_fp4(q, cache, idx, SCALE, num_splits=8, workspace=ws)
+        torch.cuda.synchronize()
+        _check(o, lse, q, values, idx, SCALE)
