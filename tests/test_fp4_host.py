@@ -116,7 +116,7 @@ def test_tables_refusals(lib):
     args = [ONE, ONE, 2, ONE, 4, 4, 64, ONE, 8, P, ONE, 0, P, 0, P, 10, P, P, 0, ONE, P]
     _bad(lib, "dsa_batch_tables", args,
          [(0, P, 1), (1, P, 1), (3, P, 1), (10, P, 1), (19, P, 1), (2, -1, 1), (2, 8193, 2), (4, 3, 1), (5, -1, 1),
-          (6, 0, 1), (8, -1, 1), (15, -1, 1)])
+          (6, 0, 1), (8, -1, 1), (15, -1, 1), (8, 2 ** 31, 2), (15, 2 ** 31, 2)])
 
 
 # ------------------------------------------------------------------ refusals of the tensor adapters
