@@ -454,12 +454,20 @@ __device__ __forceinline__ void prologue_end() {
 // This wave's share of the query copies: lane l of copy i fills slot
 // 64 i + l of the staged rows. Heads past H repeat the first one (bf16 rows
 // only: are zeros), and are not written out.
-template <int kKeys>
+// (kHeads: 64, or the narrow score waves' 16 or 32.)
+template <int kHeads>
+constexpr int query_copies(int wave) {  // the first waves send one more where they do not share evenly
+  constexpr int kAll = kHeads * kQRowBytes / 1024;
+  return kAll / kMlaWaves + (wave < kAll % kMlaWaves ? 1 : 0);
+}
+template <int kKeys, int kHeads>
 __device__ __forceinline__ void issue_query(const MlaParams& P, uint8_t* smem, const MlaCtx& c, int head0) {
   const uint16_t* q = P.q + (int64_t)c.t_tok * P.q_tok_stride;
+  constexpr int kAll = kHeads * kQRowBytes / 1024, kMost = query_copies<kHeads>(0);
 #pragma unroll
-  for (int i = 0; i < kQDma / kMlaWaves; ++i) {
-    const int n = c.wave * (kQDma / kMlaWaves) + i;
+  for (int i = 0; i < kMost; ++i) {
+    if (kAll % kMlaWaves != 0 && i == kMost - 1 && c.wave >= kAll % kMlaWaves) break;
+    const int n = kAll % kMlaWaves == 0 ? c.wave * kMost + i : c.wave + i * kMlaWaves;
     const int slot = 64 * n + c.lane;
     const int r = slot / kQPieces;
     const int piece = (slot - r * kQPieces) ^ (r & 7);
@@ -1424,10 +1432,11 @@ sparse_mla_kernel(const MlaParams P) {
   // the address tables of blocks 0 and 1, then block 0's rows
   if (c.wave == kIdxWave)
     for (int j = 0; j < 4 && j < c.nblk; ++j) issue_index<kKeys>(P, smem, c, j);
-  issue_query<kKeys>(P, smem, c, hg * kMlaHeadsPerWG);
+  constexpr int kQHeads = kNarrow > 0 ? 16 * kNarrow : kMlaHeadsPerWG;
+  issue_query<kKeys, kQHeads>(P, smem, c, hg * kMlaHeadsPerWG);
   const DmaLanes dl = dma_lanes<kKeys>(c.wave, c.lane);
   if (c.wave == kIdxWave)  // its index copies landed (the query's may still be on their way)
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kQDma / kMlaWaves) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(query_copies<kQHeads>(kIdxWave)) : "memory");
   barrier();
   if (c.wave == kTabWave) {
     if (c.nblk > 0) build_addr_table<kKeys>(P, smem, c, 0);
