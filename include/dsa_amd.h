@@ -590,9 +590,10 @@ DSA_API int dsa_indexer_logits_fp4(const uint8_t* q_fp8, const uint8_t* kv_cache
  * stored as the largest). A token without a block (bits 2 and 4, or a negative
  * block number), or whose slot does not fit int32, gets slot -1. With bit 8 only
  * the first num_rows tokens are mapped and their blocks written.
- * At most 8192 requests, and 2^31 - 1 rows and free blocks. No counterpart in the reference, whose host scheduler
- * builds these (SequenceBatch block tables and slot_mapping, read by
- * dlengine/runtime/context/batch.py:10-80). */
+ * At most 8192 requests, and 2^31 - 1 rows and free blocks. The outputs must not
+ * overlap the inputs, block_tables aside. No counterpart in the reference, whose
+ * host scheduler builds these (SequenceBatch block tables and slot_mapping, read
+ * by dlengine/runtime/context/batch.py:10-80). */
 DSA_API int dsa_batch_tables(const int32_t* cached_lens, const int32_t* new_lens, int batch,
                              int32_t* block_tables, int64_t bt_stride, int bt_width,
                              int page_size, const int32_t* free_blocks, int64_t num_free,

@@ -6,12 +6,15 @@
 //   block_tables[b, old_b + i] = free[head + sum_{a<b} need_a + i]
 // Its new token j is row r = sum_{a<b} n_a + j of the batch, at position c_b + j, in
 //   slot = block_tables[b, pos / P] * P + pos % P.
-// Every workgroup takes a share of the rows and forms both prefix sums of the whole
+// Every workgroup takes 256 rows, one a thread, and forms both prefix sums of the whole
 // batch for itself in LDS (a batch is a few KB of lengths in L2), so that one launch
 // does without any exchange between workgroups: a row of a fresh page takes its block
 // from the free list, not from the table entry that another workgroup may be writing.
 // A fresh page starts with its first new token, whose row writes the table entry.
-// The call is bound by its launch and two dependent reads, not by its bytes.
+// The call is bound by its launch and three dependent reads (lengths, free list or table,
+// and the search for the row's request between them), not by its bytes: 4 requests
+// 4.1 us from a graph, 64 of two tokens 4.5, 96 with 131072 new tokens 5.1 (a store of
+// 33 keys takes 2.0).
 #include "dsa_common.h"
 #include "../../include/dsa_amd.h"
 

@@ -2,12 +2,16 @@
 //
 //   logits[b*n+j, t] = sum_h w[b*n+j, h] * relu(q[b,j,h,:] . k[t,:])
 //
-// A page of 64 keys is 4352 bytes against the 8448 of fp8 pages, 137 flop to the
-// byte of bf16 products: the pass is bound by HBM as long as the matrix and vector
-// work of a page (32 MFMAs; 64 conversions, 128 ReLU-and-weight operations) hides
-// behind the next pages' loads. The products run on bf16 MFMAs, exact with f32
-// sums: the block-scaled MFMA would take the codes as they are, but keeps only
-// ~13 bits below the largest of its products.
+// A page of 64 keys is 4352 bytes against the 8448 of fp8 pages, 240 flop to the
+// byte. The products run on bf16 MFMAs, exact with f32 sums: the block-scaled MFMA
+// would take the codes as they are, but keeps only ~13 bits below the largest of its
+// products.
+// What bounds it: 128 rows of 65536 positions take 140 us from a graph (570 MB read,
+// 34 MB written: 4.3 TB/s; 0.98 PFLOP/s). The same loop without its products takes
+// 120 us, without the ReLU and weights 127, the page loads and score stores alone 113,
+// the loads alone 87: the reads share HBM with the score stores, and the products run
+// at the clock (1.8 GHz) that their power leaves. Two query tokens (64 rows of
+// 30000: 61 us, 1.02 PFLOP/s) are bound by the products.
 //
 // Persistent kernel, one workgroup of 8 waves per CU; every wave owns one contiguous
 // range of the flattened (batch entry, page) space and no barrier after the start.
@@ -76,8 +80,8 @@ __device__ __forceinline__ void load_page4(const uint8_t* page, uint32_t lds, ui
                "global_load_lds_dwordx4 %0, %1 nt\n\tglobal_load_lds_dwordx4 %0, %1 offset:1024 nt\n\t"
                "global_load_lds_dwordx4 %0, %1 offset:2048 nt\n\tglobal_load_lds_dwordx4 %0, %1 offset:3072 nt"
                ::"v"(lane_off), "s"(page), "{m0}"(lds) : "memory");
-  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1 nt" ::"v"(lane4), "s"(page + kCodeBytes), "{m0}"(lds + kCodeBytes)
-               : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1 nt"
+               ::"v"(lane4), "s"(page + kCodeBytes), "{m0}"(lds + kCodeBytes) : "memory");
 }
 
 // max(x, 0), NaN for a NaN
@@ -94,8 +98,9 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
   // two query tokens' operands leave no registers for their head weights
   constexpr bool kWLds = NQ == 2;
   float* wl = reinterpret_cast<float*>(smem + kWaves * kBufs * kPageBytes4 + wave * kWeightBytes);
-  int32_t* prefix = reinterpret_cast<int32_t*>(smem + kWaves * (kBufs * kPageBytes4 + (kWLds ? kWeightBytes : 0)));  // [batch + 1]
-  int32_t* wsum = prefix + P.batch + 1;                                               // [kWaves]
+  int32_t* prefix =
+      reinterpret_cast<int32_t*>(smem + kWaves * (kBufs * kPageBytes4 + (kWLds ? kWeightBytes : 0)));  // [batch + 1]
+  int32_t* wsum = prefix + P.batch + 1;                                                                // [kWaves]
 
   // pages of each batch entry (the longest of its query tokens) -> exclusive prefix
   int32_t carry = 0;
@@ -161,8 +166,8 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
   auto issue = [&](int k) {
     const int page = __builtin_amdgcn_readlane(win_page, k - wb);
     const uint8_t* src = page >= 0 && page < P.num_pages ? P.kv + (int64_t)page * kPageBytes4 : g_idx4_zero_page;
-    load_page4(src, __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(ring + (k % kBufs) * kPageBytes4)),
-               lane_off, 4u * lane);
+    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(ring + (k % kBufs) * kPageBytes4);
+    load_page4(src, __builtin_amdgcn_readfirstlane(lds), lane_off, 4u * lane);
   };
 
   // the current batch entry: query operands (k-step 4c + j of head tile ht: dims 64c + 32h + 8j .. +7
@@ -197,7 +202,8 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
             }
           }
 #pragma unroll
-        for (int r = 0; r < 16 && !kWLds; ++r) w[ht][r] = P.weights[row * kHeads + 32 * ht + 8 * (r >> 2) + 4 * h_o + (r & 3)];
+        for (int r = 0; r < 16 && !kWLds; ++r)
+          w[ht][r] = P.weights[row * kHeads + 32 * ht + 8 * (r >> 2) + 4 * h_o + (r & 3)];
         __builtin_amdgcn_sched_barrier(0);
       }
       if (kWLds) wl[j * kHeads + lane] = P.weights[row * kHeads + lane];
@@ -210,9 +216,9 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
     const uint8_t* buf = ring + (k % kBufs) * kPageBytes4;
     int c32_o = c32;
     asm volatile("" : "+v"(c32_o));
-    // A unit is the eight products of one key tile, query token and head tile. The vector work, the sum of
-    // the unit before (and the next tile's conversions), is spread between its products: done in
-    // turns, one wave's products and the other's vector work covered each other only by chance.
+    // A unit is the eight products of one key tile, query token and head tile. Between its products stand
+    // the sum of the unit before and the next tile's conversions: with products and vector work in turns, the
+    // SIMD's two waves covered each other's only by chance.
     float part[NQ][2];
     v16f acc[2];
     auto read_key = [&](int tt, v4i (&raw)[2], uint32_t& sb) {
@@ -308,7 +314,8 @@ indexer_logits_fp4_kernel(const Idx4Params P) {
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
       // lane halves: {tile 0 of both, tile 1 of both}
-      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(part[j][0]), __float_as_uint(part[j][1]), false, false);
+      const auto sw =
+          __builtin_amdgcn_permlane32_swap(__float_as_uint(part[j][0]), __float_as_uint(part[j][1]), false, false);
       const float v = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
       const bool ok = t < L[j] && page >= 0 && page < P.num_pages;
       // one store a page and query token, whatever the length: the waits below count it

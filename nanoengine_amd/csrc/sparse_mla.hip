@@ -725,9 +725,12 @@ __device__ __forceinline__ uint16_t* et_block4(uint8_t* smem, int par, int dq) {
 // k-steps (dims 128c + 32g + 8i .. +7); B = the query in the same order. The shape
 // has 55% of the 32x32x16's rate, but the wave converts half the keys and takes a
 // quarter of the exponentials. A reference per wave, that is per k-step of P.V.
-// (90 tokens of 16 heads: 36.4 us on 32x32 tiles, 31.0 so; 256 tokens 61 and 54,
+// (90 tokens of 16 heads: 36.4 us on 32x32 tiles, 30.6 so; 256 tokens 61 and 54,
 // 4.1 TB/s of rows. The P.V waves' conversions, ~1600 of an iteration's ~2300 cycles,
-// set the block time then; a second block of rows in flight gains nothing.)
+// set the block time then; a second block of rows in flight gains nothing. Eight
+// waves that each take their own keys, with query and output in registers and no
+// barrier, are faster a block, 0.95 against 1.2 us, but start and merge 6 us later:
+// 34 us, and 40 against 33 for 128 tokens.)
 template <int NT>
 __device__ __forceinline__ void qk_waves4_narrow(const MlaParams& P, uint8_t* smem, const MlaCtx& c,
                                                  const DmaLanes& dl) {
@@ -741,7 +744,8 @@ __device__ __forceinline__ void qk_waves4_narrow(const MlaParams& P, uint8_t* sm
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) qn[nt][k][i] = *reinterpret_cast<const v4i*>(qrow + ((16 * (16 * k + 4 * g + i)) ^ sw));
+      for (int i = 0; i < 4; ++i)
+        qn[nt][k][i] = *reinterpret_cast<const v4i*>(qrow + ((16 * (16 * k + 4 * g + i)) ^ sw));
 #pragma unroll
     for (int i = 0; i < 2; ++i) qr[nt][i] = *reinterpret_cast<const v4i*>(qrow + ((16 * (64 + 4 * i + g)) ^ sw));
   }
@@ -828,7 +832,8 @@ __device__ __forceinline__ void qk_waves4_narrow(const MlaParams& P, uint8_t* sm
         }
         l_run[nt] += (pv[0] + pv[1]) + (pv[2] + pv[3]);
         // k-step w of P.V: lane (head, h = g % 2) holds keys 8(j/4) + 4h + j%4 in eight bf16
-        *reinterpret_cast<v2i*>(smem + kPOff + (t & 1) * 8192 + (w * 64 + 32 * (g & 1) + 16 * nt + n16) * 16 + 8 * (g >> 1)) =
+        const int p_at = (w * 64 + 32 * (g & 1) + 16 * nt + n16) * 16 + 8 * (g >> 1);
+        *reinterpret_cast<v2i*>(smem + kPOff + (t & 1) * 8192 + p_at) =
             v2i{cvt_pk_bf16(pv[0], pv[1]), cvt_pk_bf16(pv[2], pv[3])};
         if (g == 0) ref[((t & 1) * 4 + w) * 32 + 16 * nt + n16] = m_run[nt];
       }
@@ -1042,7 +1047,8 @@ __device__ __forceinline__ void pv_block4(v16f (&o)[kTiles][4], const int (&fx)[
       eq[b][u] = *reinterpret_cast<const v4i_alias*>(etl + 128 * u + 16 * ks);
     }
 #pragma unroll
-    for (int mt = 0; mt < kTiles; ++mt) pq[b][mt] = *reinterpret_cast<const v4i*>(pb + mt * 4096 + (ks * 64 + lane) * 16);
+    for (int mt = 0; mt < kTiles; ++mt)
+      pq[b][mt] = *reinterpret_cast<const v4i*>(pb + mt * 4096 + (ks * 64 + lane) * 16);
   };
   read_step(0);
 #pragma unroll
@@ -1056,8 +1062,9 @@ __device__ __forceinline__ void pv_block4(v16f (&o)[kTiles][4], const int (&fx)[
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int pe = pq[cur][mt][e];
-        pa[mt][e] = __builtin_bit_cast(int, __builtin_elementwise_sub_sat(__builtin_bit_cast(v2u16, pe),
-                                                                          __builtin_bit_cast(v2u16, fx[mt][ks * kParts / 4])));
+        const int f = fx[mt][ks * kParts / 4];
+        pa[mt][e] = __builtin_bit_cast(
+            int, __builtin_elementwise_sub_sat(__builtin_bit_cast(v2u16, pe), __builtin_bit_cast(v2u16, f)));
       }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -1653,7 +1660,8 @@ static int launch_mla(const MlaParams& P, KeyKind keys, int64_t nwg, hipStream_t
   // at most 16 heads, at most 32, more
   void (*const kernels[4][3])(MlaParams) = {
       {sparse_mla_kernel<kSlots, 1>, sparse_mla_kernel<kSlots, 1>, sparse_mla_kernel<kSlots, 2>},
-      {sparse_mla_kernel<kSlotsThenRows, 1>, sparse_mla_kernel<kSlotsThenRows, 1>, sparse_mla_kernel<kSlotsThenRows, 2>},
+      {sparse_mla_kernel<kSlotsThenRows, 1>, sparse_mla_kernel<kSlotsThenRows, 1>,
+       sparse_mla_kernel<kSlotsThenRows, 2>},
       {sparse_mla_kernel<kRows, 1>, sparse_mla_kernel<kRows, 1>, sparse_mla_kernel<kRows, 2>},
       {sparse_mla_kernel<kSlots4, 1, 1>, sparse_mla_kernel<kSlots4, 1, 2>, sparse_mla_kernel<kSlots4, 2>}};
   hipLaunchKernelGGL(kernels[keys][P.H <= 16 ? 0 : P.H <= 32 ? 1 : 2], dim3((unsigned)nwg), dim3(kMlaThreads),
@@ -1786,8 +1794,8 @@ int sparse_mla_decode_impl(const void* q, int64_t q_token_stride, int64_t q_head
     P.ws_lse = P.ws_o + (size_t)num_splits * part.rows * kMlaDv;
   }
   const int64_t nwg = whole + (items - whole) * num_splits;
-  if (int rc = launch_mla(P, fp4 ? kSlots4 : fresh ? kSlotsThenRows : kSlots, nwg, (hipStream_t)stream, "dsa_sparse_mla_decode"))
-    return rc;
+  const KeyKind keys = fp4 ? kSlots4 : fresh ? kSlotsThenRows : kSlots;
+  if (int rc = launch_mla(P, keys, nwg, (hipStream_t)stream, "dsa_sparse_mla_decode")) return rc;
   if (num_splits > 1) {
     hipLaunchKernelGGL(sparse_mla_combine_kernel, dim3((unsigned)((items - whole) * kMlaHeadsPerWG)), dim3(64), 0,
                        (hipStream_t)stream, P.ws_o, P.ws_lse, P.ws_row0, P.ws_rows, num_heads, P.whole,

@@ -825,8 +825,8 @@ def mla_kv_load_fp4(k_cache: torch.Tensor, slots: torch.Tensor, out: torch.Tenso
     if not (out.dtype == torch.bfloat16 and tuple(out.shape) == (n, MLA_D_QK) and out.stride(1) == 1):
         _fail(f"out must be bf16 [{n}, {MLA_D_QK}] with a contiguous last dim")
     _gpu(k_cache, out)
-    _launch(dev, "dsa_mla_kv_load_fp4", k_cache.data_ptr(), blk_stride, block_size, k_cache.shape[0], s.data_ptr(), is64, n,
-            out.data_ptr(), _row_stride(out))
+    _launch(dev, "dsa_mla_kv_load_fp4", k_cache.data_ptr(), blk_stride, block_size, k_cache.shape[0], s.data_ptr(),
+            is64, n, out.data_ptr(), _row_stride(out))
     return out
 
 
@@ -866,10 +866,10 @@ def sparse_mla_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, indices: torch
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need
                  or workspace.data_ptr() % 16 or workspace.get_device() != dev):
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    _launch(dev, "dsa_sparse_mla_decode_fp4", q.data_ptr(), q.stride(0) if T > 1 else 0, q.stride(1), k_cache.data_ptr(), blk_stride,
-            block_size, k_cache.shape[0], indices.data_ptr(), indices.stride(0), T, H, topk, float(sm_scale),
-            out.data_ptr(), lse.data_ptr(), int(num_splits), workspace.data_ptr() if need else None,
-            workspace.numel() * workspace.element_size() if need else 0)
+    _launch(dev, "dsa_sparse_mla_decode_fp4", q.data_ptr(), q.stride(0) if T > 1 else 0, q.stride(1),
+            k_cache.data_ptr(), blk_stride, block_size, k_cache.shape[0], indices.data_ptr(), indices.stride(0), T, H,
+            topk, float(sm_scale), out.data_ptr(), lse.data_ptr(), int(num_splits),
+            workspace.data_ptr() if need else None, workspace.numel() * workspace.element_size() if need else 0)
     return out, lse
 
 
@@ -945,8 +945,8 @@ def indexer_logits_fp4(q_fp8: torch.Tensor, kv_cache: torch.Tensor, weights: tor
             and out.shape[1] >= max_context_len and (out.shape[1] < 2 or out.stride(1) == 1)):
         _fail("logits output must be f32 [B*n, >=max_ctx] with unit column stride")
     _gpu(q_fp8, out)
-    _launch(dev, "dsa_indexer_logits_fp4", q_fp8.data_ptr(), kv_cache.data_ptr(), pages, weights.data_ptr(), cl.data_ptr(),
-            bt.data_ptr(), bt.stride(0), B, n, H, D, page_size, int(max_context_len), out.data_ptr(),
+    _launch(dev, "dsa_indexer_logits_fp4", q_fp8.data_ptr(), kv_cache.data_ptr(), pages, weights.data_ptr(),
+            cl.data_ptr(), bt.data_ptr(), bt.stride(0), B, n, H, D, page_size, int(max_context_len), out.data_ptr(),
             _row_stride(out), int(bool(clean_logits)))
     return out
 
