@@ -754,8 +754,10 @@ def _gpu(*tensors: torch.Tensor) -> int:
     device object per tensor is most of a small call's checks)."""
     index = tensors[0].get_device()
     for t in tensors:
-        if index < 0 or t.get_device() != index:
-            _check_cuda(*tensors)
+        if t.get_device() != index:
+            index = -1
+    if index < 0:
+        _check_cuda(*tensors)
     return index
 
 
@@ -773,16 +775,17 @@ def _launch(index: int, name: str, *args) -> None:
 def mla_fp4_geometry(k_cache: torch.Tensor) -> tuple[int, int]:
     """(block stride in bytes, rows per block) of a 4-bit MLA cache view
     [num_blocks, block_size, (1,) 400] whose block stride may include a padding row."""
-    if not (k_cache.dtype == torch.uint8 and k_cache.dim() in (3, 4)
-            and k_cache.shape[-1] == MLA_FP4_ROW_BYTES and k_cache.stride(-1) == 1):
+    shape, stride = k_cache.shape, k_cache.stride()  # (asked for once: a call's checks are most of its time)
+    if not (len(shape) in (3, 4) and shape[-1] == MLA_FP4_ROW_BYTES and stride[-1] == 1
+            and k_cache.dtype == torch.uint8):
         _fail(f"k_cache must be uint8 [blocks, block_size, (1,) {MLA_FP4_ROW_BYTES}] with contiguous rows, "
-              f"got {k_cache.dtype} {tuple(k_cache.shape)}")
-    if k_cache.dim() == 4 and k_cache.shape[2] != 1:
+              f"got {k_cache.dtype} {tuple(shape)}")
+    if len(shape) == 4 and shape[2] != 1:
         _fail("MLA cache has one KV head")
-    block_size = k_cache.shape[1]
-    if block_size > 1 and k_cache.stride(1) != MLA_FP4_ROW_BYTES:
+    block_size = shape[1]
+    if block_size > 1 and stride[1] != MLA_FP4_ROW_BYTES:
         _fail(f"rows inside a block must be {MLA_FP4_ROW_BYTES} B apart")
-    return (k_cache.stride(0) if k_cache.shape[0] > 1 else block_size * MLA_FP4_ROW_BYTES), block_size
+    return (stride[0] if shape[0] > 1 else block_size * MLA_FP4_ROW_BYTES), block_size
 
 
 def _fp4_pages(cache: torch.Tensor, page_size: int) -> int:
@@ -802,14 +805,15 @@ def _row_stride(t: torch.Tensor) -> int:
 def mla_kv_store_fp4(kv: torch.Tensor, k_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
     """Quantise kv [N, (1,) 576] bf16 into the 4-bit MLA cache [blocks, block_size, (1,) 400] at
     slot_mapping; slots that are negative or past the cache are skipped (see dsa_mla_kv_store_fp4)."""
-    if not (kv.dim() in (2, 3) and kv.dtype == torch.bfloat16 and kv.shape[-1] == MLA_D_QK and kv.stride(-1) == 1
-            and (kv.dim() == 2 or kv.shape[1] == 1)):
+    shape, stride = kv.shape, kv.stride()
+    if not (len(shape) in (2, 3) and shape[-1] == MLA_D_QK and stride[-1] == 1 and kv.dtype == torch.bfloat16
+            and (len(shape) == 2 or shape[1] == 1)):
         _fail(f"kv must be bf16 [N, (1,) {MLA_D_QK}] with a contiguous last dim")
     blk_stride, block_size = mla_fp4_geometry(k_cache)
-    n = kv.shape[0]
+    n = shape[0]
     slots, is64 = _slots(slot_mapping, n)
     dev = _gpu(kv, k_cache, slots)
-    _launch(dev, "dsa_mla_kv_store_fp4", kv.data_ptr(), kv.stride(0) if n > 1 else MLA_D_QK, slots.data_ptr(), is64, n,
+    _launch(dev, "dsa_mla_kv_store_fp4", kv.data_ptr(), stride[0] if n > 1 else MLA_D_QK, slots.data_ptr(), is64, n,
             k_cache.data_ptr(), blk_stride, block_size, k_cache.shape[0])
 
 
@@ -821,10 +825,11 @@ def mla_kv_load_fp4(k_cache: torch.Tensor, slots: torch.Tensor, out: torch.Tenso
     n = s.shape[0]
     dev = _gpu(k_cache, s)
     if out is None:
-        out = torch.empty(n, MLA_D_QK, dtype=torch.bfloat16, device=dev)
-    if not (out.dtype == torch.bfloat16 and tuple(out.shape) == (n, MLA_D_QK) and out.stride(1) == 1):
-        _fail(f"out must be bf16 [{n}, {MLA_D_QK}] with a contiguous last dim")
-    _gpu(k_cache, out)
+        out = k_cache.new_empty((n, MLA_D_QK), dtype=torch.bfloat16)
+    else:
+        if not (out.dtype == torch.bfloat16 and tuple(out.shape) == (n, MLA_D_QK) and out.stride(1) == 1):
+            _fail(f"out must be bf16 [{n}, {MLA_D_QK}] with a contiguous last dim")
+        _gpu(k_cache, out)
     _launch(dev, "dsa_mla_kv_load_fp4", k_cache.data_ptr(), blk_stride, block_size, k_cache.shape[0], s.data_ptr(),
             is64, n, out.data_ptr(), _row_stride(out))
     return out
@@ -895,13 +900,13 @@ def indexer_k_load_fp4(cache: torch.Tensor, slots: torch.Tensor, page_size: int,
     n = s.shape[0]
     dev = _gpu(cache, s)
     if key_out is None:
-        key_out = torch.empty(n, INDEXER_HEAD_DIM, dtype=torch.float8_e4m3fn, device=dev)
-    if scale_out is None:
-        scale_out = torch.empty(n, dtype=torch.float32, device=dev)
-    if not (key_out.dtype in (torch.float8_e4m3fn, torch.uint8) and tuple(key_out.shape) == (n, INDEXER_HEAD_DIM)
-            and key_out.is_contiguous()):
+        key_out = cache.new_empty((n, INDEXER_HEAD_DIM), dtype=torch.float8_e4m3fn)
+    elif not (key_out.dtype in (torch.float8_e4m3fn, torch.uint8) and tuple(key_out.shape) == (n, INDEXER_HEAD_DIM)
+              and key_out.is_contiguous()):
         _fail(f"key_out must be contiguous fp8 [{n}, 128]")
-    if not (scale_out.dtype == torch.float32 and scale_out.numel() == n and scale_out.is_contiguous()):
+    if scale_out is None:
+        scale_out = cache.new_empty((n,), dtype=torch.float32)
+    elif not (scale_out.dtype == torch.float32 and scale_out.numel() == n and scale_out.is_contiguous()):
         _fail(f"scale_out must be contiguous f32 [{n}]")
     _gpu(cache, key_out, scale_out)
     _launch(dev, "dsa_indexer_k_load_fp4", cache.data_ptr(), int(page_size), pages, s.data_ptr(), is64, n,
@@ -952,13 +957,17 @@ def indexer_logits_fp4(q_fp8: torch.Tensor, kv_cache: torch.Tensor, weights: tor
 
 
 # --------------------------------------------------------------------------- batch tables
-def _int_out(t: torch.Tensor | None, n: int, name: str, dtypes=(torch.int32, torch.int64)) -> int:
+_INTS = (torch.int32, torch.int64)
+
+
+def _int_out(t: torch.Tensor | None, shape: tuple[int], name: str, dtypes=_INTS) -> int:
     """1 when the optional output is int64."""
     if t is None:
         return 0
-    if not (t.dtype in dtypes and t.dim() == 1 and t.numel() == n and t.is_contiguous()):
-        _fail(f"{name} must be contiguous {' or '.join(str(d).replace('torch.', '') for d in dtypes)} [{n}]")
-    return int(t.dtype == torch.int64)
+    dtype = t.dtype
+    if dtype not in dtypes or t.shape != shape or not t.is_contiguous():
+        _fail(f"{name} must be contiguous {' or '.join(str(d).replace('torch.', '') for d in dtypes)} [{shape[0]}]")
+    return 1 if dtype is torch.int64 else 0
 
 
 def batch_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor, page_size: int,
@@ -969,38 +978,45 @@ def batch_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables
     """Extend a batch's block tables and map its new tokens to cache slots, on the device, from each
     request's cached and new token counts [B] int32 (see dsa_batch_tables for every output and for the
     fault bits of ``status`` [4] int64, which the caller reads when it next synchronises)."""
-    if not (cached_lens.dim() == 1 and cached_lens.dtype == torch.int32 and cached_lens.is_contiguous()
-            and new_lens.shape == cached_lens.shape and new_lens.dtype == torch.int32 and new_lens.is_contiguous()):
+    i32 = torch.int32
+    lens = cached_lens.shape
+    if not (len(lens) == 1 and new_lens.shape == lens and cached_lens.dtype == i32 and new_lens.dtype == i32
+            and cached_lens.is_contiguous() and new_lens.is_contiguous()):
         _fail("cached_lens and new_lens must be contiguous int32 [B]")
-    B = cached_lens.shape[0]
-    if not (block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.dtype == torch.int32
-            and (block_tables.stride(1) == 1 or block_tables.shape[1] < 2)):
+    B = lens[0]
+    shape, stride = block_tables.shape, block_tables.stride()
+    if not (len(shape) == 2 and shape[0] == B and block_tables.dtype == i32 and (stride[1] == 1 or shape[1] < 2)):
         _fail("block_tables must be int32 [B, M] with unit column stride")
-    if B > 1 and block_tables.stride(0) < block_tables.shape[1]:
+    width = shape[1]
+    if B > 1 and stride[0] < width:
         _fail("block_tables rows must not overlap")
     if page_size <= 0:
         raise ValueError("page_size must be positive")
-    rows = slot_mapping.shape[0] if slot_mapping.dim() == 1 else -1
+    rows = tuple(slot_mapping.shape) if slot_mapping.dim() == 1 else (-1,)
     s64 = _int_out(slot_mapping, rows, "slot_mapping")
     p64 = _int_out(positions, rows, "positions")
-    _int_out(seq_lens, rows, "seq_lens", (torch.int32,))
-    c64 = _int_out(cu_seqlens_q, B + 1, "cu_seqlens_q")
-    k64 = _int_out(cu_seqlens_k, B + 1, "cu_seqlens_k")
-    if cu_seqlens_q is not None and cu_seqlens_k is not None and c64 != k64:
+    _int_out(seq_lens, rows, "seq_lens", (i32,))
+    c64 = _int_out(cu_seqlens_q, (B + 1,), "cu_seqlens_q")
+    k64 = _int_out(cu_seqlens_k, (B + 1,), "cu_seqlens_k")
+    if c64 != k64 and cu_seqlens_q is not None and cu_seqlens_k is not None:
         _fail("cu_seqlens_q and cu_seqlens_k must share one dtype")
     if not (status.dtype == torch.int64 and status.numel() == 4 and status.is_contiguous()):
         _fail("status must be contiguous int64 [4]")
-    if free_blocks is not None and not (free_blocks.dim() == 1 and free_blocks.dtype == torch.int32
-                                        and free_blocks.is_contiguous()):
-        _fail("free_blocks must be contiguous int32 [F]")
-    if free_head is not None and not (free_head.dtype == torch.int32 and free_head.numel() == 1):
-        _fail("free_head must be int32 with one element")
-    dev = _gpu(*[t for t in (cached_lens, new_lens, block_tables, slot_mapping, status, free_blocks, free_head,
-                             positions, seq_lens, cu_seqlens_q, cu_seqlens_k) if t is not None])
-    # an empty free list still means that blocks are taken from it
-    free_ptr = None if free_blocks is None else (free_blocks.data_ptr() or status.data_ptr())
+    tensors = [cached_lens, new_lens, block_tables, slot_mapping, status]
+    tensors += [t for t in (positions, seq_lens, cu_seqlens_q, cu_seqlens_k) if t is not None]
+    free_ptr, num_free = None, 0
+    if free_blocks is not None:
+        if not (free_blocks.dim() == 1 and free_blocks.dtype == i32 and free_blocks.is_contiguous()):
+            _fail("free_blocks must be contiguous int32 [F]")
+        # an empty free list still means that blocks are taken from it
+        free_ptr, num_free = free_blocks.data_ptr() or status.data_ptr(), free_blocks.shape[0]
+        tensors.append(free_blocks)
+    if free_head is not None:
+        if not (free_head.dtype == i32 and free_head.numel() == 1):
+            _fail("free_head must be int32 with one element")
+        tensors.append(free_head)
+    dev = _gpu(*tensors)
     _launch(dev, "dsa_batch_tables", cached_lens.data_ptr(), new_lens.data_ptr(), B, block_tables.data_ptr(),
-            _row_stride(block_tables), block_tables.shape[1], int(page_size), free_ptr,
-            0 if free_blocks is None else free_blocks.shape[0], _ptr(free_head), slot_mapping.data_ptr(), s64,
-            _ptr(positions), p64, _ptr(seq_lens), rows, _ptr(cu_seqlens_q), _ptr(cu_seqlens_k), c64 or k64,
-            status.data_ptr())
+            stride[0] if B > 1 else width, width, int(page_size), free_ptr, num_free, _ptr(free_head),
+            slot_mapping.data_ptr(), s64, _ptr(positions), p64, _ptr(seq_lens), rows[0], _ptr(cu_seqlens_q),
+            _ptr(cu_seqlens_k), c64 or k64, status.data_ptr())
