@@ -77,9 +77,9 @@ struct Idx4Params {
 // A page into LDS at `lds` (wave-uniform). The immediate offset moves both addresses.
 __device__ __forceinline__ void load_page4(const uint8_t* page, uint32_t lds, uint32_t lane_off, uint32_t lane4) {
   asm volatile("s_waitcnt lgkmcnt(0)\n\t"
-               "global_load_lds_dwordx4 %0, %1 nt\n\tglobal_load_lds_dwordx4 %0, %1 offset:1024 nt\n\t"
-               "global_load_lds_dwordx4 %0, %1 offset:2048 nt\n\tglobal_load_lds_dwordx4 %0, %1 offset:3072 nt"
-               ::"v"(lane_off), "s"(page), "{m0}"(lds) : "memory");
+               "global_load_lds_dwordx4 %0, %1 nt\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3 nt\n\t"
+               "global_load_lds_dwordx4 %0, %1 offset:%4 nt\n\tglobal_load_lds_dwordx4 %0, %1 offset:%5 nt"
+               ::"v"(lane_off), "s"(page), "{m0}"(lds), "n"(1024), "n"(2 * 1024), "n"(3 * 1024) : "memory");
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1 nt"
                ::"v"(lane4), "s"(page + kCodeBytes), "{m0}"(lds + kCodeBytes) : "memory");
 }
