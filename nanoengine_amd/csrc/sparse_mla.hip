@@ -1463,21 +1463,16 @@ sparse_mla_kernel(const MlaParams P) {
   } else pv_waves<kKeys, kTiles, kNarrow>(P, smem, c, dl, split);
 }
 
-// One wave per (split item, head): merge the split partials. Bound by the
+// One wave per (token, head) row with partials: merge them. Bound by the
 // latency of its loads, so those of up to 8 splits go out together, right
 // after the splits' LSEs (one per lane) and before anything waits for either
 // (3.9 us for 4 tokens of 128 heads in 8 splits; one split after another, the
 // LSEs first: 5.5).
 __global__ void __launch_bounds__(64)
 sparse_mla_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_lse, int64_t ws_row0,
-                          int64_t ws_rows, int H, int whole, int head_groups, int splits, uint16_t* __restrict__ out,
-                          float* __restrict__ lse_out) {
-  const int item = whole + (int)blockIdx.x / kMlaHeadsPerWG;
-  const int head = item % head_groups * kMlaHeadsPerWG + (int)blockIdx.x % kMlaHeadsPerWG;
-  if (head >= H) return;
+                          int64_t ws_rows, int splits, uint16_t* __restrict__ out, float* __restrict__ lse_out) {
   const int lane = threadIdx.x;
-  const int64_t th = (int64_t)(item / head_groups) * H + head;
-  const int64_t part = th - ws_row0, stride = ws_rows;
+  const int64_t part = blockIdx.x, th = ws_row0 + part, stride = ws_rows;
   constexpr int kGroup = 8;
   const float* src = ws_o + part * kMlaDv + lane * 8;
   auto load_lse = [&](int s0) {  // split s0 + lane
@@ -1797,9 +1792,8 @@ int sparse_mla_decode_impl(const void* q, int64_t q_token_stride, int64_t q_head
   const KeyKind keys = fp4 ? kSlots4 : fresh ? kSlotsThenRows : kSlots;
   if (int rc = launch_mla(P, keys, nwg, (hipStream_t)stream, "dsa_sparse_mla_decode")) return rc;
   if (num_splits > 1) {
-    hipLaunchKernelGGL(sparse_mla_combine_kernel, dim3((unsigned)((items - whole) * kMlaHeadsPerWG)), dim3(64), 0,
-                       (hipStream_t)stream, P.ws_o, P.ws_lse, P.ws_row0, P.ws_rows, num_heads, P.whole,
-                       P.head_groups, num_splits, P.out, lse);
+    hipLaunchKernelGGL(sparse_mla_combine_kernel, dim3((unsigned)part.rows), dim3(64), 0, (hipStream_t)stream, P.ws_o,
+                       P.ws_lse, P.ws_row0, P.ws_rows, num_splits, P.out, lse);
     return check_launch("dsa_sparse_mla_decode(combine)");
   }
   return kOk;
