@@ -1324,7 +1324,9 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
     const int h_half = hg_base + 32 * mt;
     if (h_half >= P.H) break;
     const int head = h_half + c32;
-    const bool head_ok = head < P.H;
+    // one tile of 16 heads fills half of the 32: the other half's rows are the next group's
+    const int h_end = kNarrow == 1 ? min(P.H, h_half + 16) : P.H;
+    const bool head_ok = head < h_end;
     // Through this wave's LDS staging (the row and P buffers are free), so that
     // the stores are whole 16-byte pieces: a head's 128 dims are 256
     // (partials: 512) contiguous bytes, where a lane holds one dim of 16 heads.
@@ -1347,7 +1349,7 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
       for (int i = 0; i < 8; ++i) {
         const int hr = 4 * i + (lane >> 4);
         const v4i_alias v = *reinterpret_cast<const v4i_alias*>(st + hr * kStageRow16 + 16 * (lane & 15));
-        if (h_half + hr < P.H)
+        if (h_half + hr < h_end)
           *reinterpret_cast<v4i_alias*>(P.out + ((int64_t)c.t_tok * P.H + h_half + hr) * kMlaDv + 128 * dq +
                                         8 * (lane & 15)) = v;
       }
@@ -1375,7 +1377,7 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
       for (int i = 0; i < 16; ++i) {
         const int hr = 2 * i + h;
         const v4i_alias v = *reinterpret_cast<const v4i_alias*>(st + hr * kStageRow32 + 16 * c32);
-        if (h_half + hr < P.H)
+        if (h_half + hr < h_end)
           *reinterpret_cast<v4i_alias*>(P.ws_o + (row0 + hr) * kMlaDv + 128 * dq + 4 * c32) = v;
       }
       if (dq == 0 && h == 0 && head_ok) P.ws_lse[row0 + c32] = lse;
@@ -1388,7 +1390,7 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
 // tensor-parallel rank's 16) the second tile would be padding: its score waves
 // idle and its P.V products are left out. (As a run-time condition this cost
 // the 64-head kernel 5%: the branches stop the P.V loop's read-ahead.)
-// kNarrow: 4-bit rows and at most 32 heads, as that many tiles of 16.
+// kNarrow: 4-bit rows and head groups of at most 32, as that many tiles of 16.
 template <int kKeys, int kTiles, int kNarrow = 0>
 __global__ void __launch_bounds__(kMlaThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 sparse_mla_kernel(const MlaParams P) {
@@ -1431,7 +1433,8 @@ sparse_mla_kernel(const MlaParams P) {
     c.ncached = 0;
     c.nblk = P.topk / kFreshKeys;
   }
-  c.h_half = hg * kMlaHeadsPerWG + c.hp * 32;
+  constexpr int kGroup = kNarrow > 0 ? 16 * kNarrow : kMlaHeadsPerWG;  // heads of a head group
+  c.h_half = hg * kGroup + c.hp * 32;
   c.head = c.h_half + c.c32;
   c.head_ok = c.head < P.H;
 
@@ -1439,11 +1442,10 @@ sparse_mla_kernel(const MlaParams P) {
   // the address tables of blocks 0 and 1, then block 0's rows
   if (c.wave == kIdxWave)
     for (int j = 0; j < 4 && j < c.nblk; ++j) issue_index<kKeys>(P, smem, c, j);
-  constexpr int kQHeads = kNarrow > 0 ? 16 * kNarrow : kMlaHeadsPerWG;
-  issue_query<kKeys, kQHeads>(P, smem, c, hg * kMlaHeadsPerWG);
+  issue_query<kKeys, kGroup>(P, smem, c, hg * kGroup);
   const DmaLanes dl = dma_lanes<kKeys>(c.wave, c.lane);
   if (c.wave == kIdxWave)  // its index copies landed (the query's may still be on their way)
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(query_copies<kQHeads>(kIdxWave)) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(query_copies<kGroup>(kIdxWave)) : "memory");
   barrier();
   if (c.wave == kTabWave) {
     if (c.nblk > 0) build_addr_table<kKeys>(P, smem, c, 0);
@@ -1638,7 +1640,8 @@ int dsa_sparse_mla_decode_fp4(const void* q, int64_t q_token_stride, int64_t q_h
 
 namespace dsa {
 
-static int launch_mla(const MlaParams& P, KeyKind keys, int64_t nwg, hipStream_t stream, const char* what) {
+static int launch_mla(const MlaParams& P, KeyKind keys, int64_t nwg, hipStream_t stream, const char* what,
+                      int group = kMlaHeadsPerWG) {
   static int smem_status = -1;
   if (smem_status < 0) {
     smem_status = 0;
@@ -1652,14 +1655,15 @@ static int launch_mla(const MlaParams& P, KeyKind keys, int64_t nwg, hipStream_t
   }
   if (smem_status) return set_error(kLaunchFailed, "sparse_mla: cannot reserve %zu B of LDS", kRowsSmemBytes);
   if (nwg > INT32_MAX) return set_error(kInvalidArgument, "%s: grid too large", what);
-  // at most 16 heads, at most 32, more
   void (*const kernels[4][3])(MlaParams) = {
       {sparse_mla_kernel<kSlots, 1>, sparse_mla_kernel<kSlots, 1>, sparse_mla_kernel<kSlots, 2>},
       {sparse_mla_kernel<kSlotsThenRows, 1>, sparse_mla_kernel<kSlotsThenRows, 1>,
        sparse_mla_kernel<kSlotsThenRows, 2>},
       {sparse_mla_kernel<kRows, 1>, sparse_mla_kernel<kRows, 1>, sparse_mla_kernel<kRows, 2>},
       {sparse_mla_kernel<kSlots4, 1, 1>, sparse_mla_kernel<kSlots4, 1, 2>, sparse_mla_kernel<kSlots4, 2>}};
-  hipLaunchKernelGGL(kernels[keys][P.H <= 16 ? 0 : P.H <= 32 ? 1 : 2], dim3((unsigned)nwg), dim3(kMlaThreads),
+  // head groups of 16, of 32 (fewer heads than a group are one too), of 64
+  const int heads = std::min(P.H, group);
+  hipLaunchKernelGGL(kernels[keys][heads <= 16 ? 0 : heads <= 32 ? 1 : 2], dim3((unsigned)nwg), dim3(kMlaThreads),
                      keys == kRows ? kRowsSmemBytes : kMlaSmemBytes, stream, P);
   return check_launch(what);
 }
@@ -1788,9 +1792,25 @@ int sparse_mla_decode_impl(const void* q, int64_t q_token_stride, int64_t q_head
     P.ws_o = static_cast<float*>(workspace);
     P.ws_lse = P.ws_o + (size_t)num_splits * part.rows * kMlaDv;
   }
-  const int64_t nwg = whole + (items - whole) * num_splits;
+  int64_t nwg = whole + (items - whole) * num_splits;
+  // 4-bit rows, and a launch that fills no more than a quarter or a half of the CUs: head groups of
+  // 16 or 32. A workgroup's blocks take 1.3 or 1.2 us instead of 2.4, for gathering each row two
+  // or four times as often (from graphs: 4 tokens of 128 heads 22.8 us in groups of 64,
+  // 20.0 of 32, 19.3 of 16; 8 tokens 28.3 and 25.4; one token 20.1, 16.5 and 15.2). The
+  // partials lie where they did.
+  int group = kMlaHeadsPerWG;
+  for (const int g : {16, 32}) {
+    const int64_t n = (int64_t)num_tokens * ((num_heads + g - 1) / g) * num_splits;
+    if (fp4 && whole == 0 && n <= current_cus()) {
+      group = g;
+      P.head_groups = (num_heads + g - 1) / g;
+      nwg = n;
+      break;
+    }
+  }
   const KeyKind keys = fp4 ? kSlots4 : fresh ? kSlotsThenRows : kSlots;
-  if (int rc = launch_mla(P, keys, nwg, (hipStream_t)stream, "dsa_sparse_mla_decode")) return rc;
+  if (int rc = launch_mla(P, keys, nwg, (hipStream_t)stream, "dsa_sparse_mla_decode", group))
+    return rc;
   if (num_splits > 1) {
     hipLaunchKernelGGL(sparse_mla_combine_kernel, dim3((unsigned)part.rows), dim3(64), 0, (hipStream_t)stream, P.ws_o,
                        P.ws_lse, P.ws_row0, P.ws_rows, num_splits, P.out, lse);

@@ -190,3 +190,69 @@ def test_workspace_of_the_caller(cuda):
         o, lse = ops.sparse_mla_decode_fp4(q, cache, idx, SCALE, num_splits=8, workspace=ws)
         torch.cuda.synchronize()
         _check(o, lse, q, values, idx, SCALE)
+
+
+def _group_batch(H, group):
+    """The largest batch that is taken, unsplit, in head groups of 16 (group 0) or 32 (1); one in groups of 64 (2)."""
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    return (cus // -(-H // 16), cus // -(-H // 32), cus // -(-H // 32) + 1)[group]
+
+
+@pytest.mark.parametrize("group", [0, 1, 2])
+@pytest.mark.parametrize("H", [128, 112, 48])
+def test_masks_in_every_head_group(cuda, group, H):
+    """The rows of the mask and NaN tests at both ends of a batch of either head group, no output outside
+    the batch touched."""
+    T = _group_batch(H, group)
+    print(f"mla fp4 head groups T={T} H={H}", flush=True)
+    cache, values = _cache(40, 13, cuda)
+    q, idx = _query(T, H, 13, cuda), _indices(T, 512, 2559, 13, cuda)
+    for at in (0, T - 7):
+        idx[at] = -1                                # nothing
+        idx[at + 1, 1:] = -1                        # one key, the first
+        idx[at + 2, :511] = -1                      # one key, the last
+        idx[at + 3, :32] = -1                       # no key in the first half of the first block
+        idx[at + 4, 40:] = 10 ** 6                  # stale slots past the cache
+        idx[at + 5, ::2] = -5
+        idx[at + 6, 77] = 2559
+    cache[39, 63, 0, 256 + 15] = 255                # slot 2559: a NaN row, selected by tokens 6 and T - 1
+    outs = torch.full((T + 2, H, 512), 7.0, dtype=torch.bfloat16, device=cuda)
+    lses = torch.full((T + 2, H), 7.0, device=cuda)
+    for splits in (1, 2):
+        o, lse = ops.sparse_mla_decode_fp4(q, cache, idx, SCALE, out=outs[1:-1], lse=lses[1:-1], num_splits=splits)
+        torch.cuda.synchronize()
+        assert torch.all(outs[::T + 1] == 7) and torch.all(lses[::T + 1] == 7)
+        for t in (6, T - 1):
+            assert torch.all(torch.isnan(o[t])) and torch.all(torch.isnan(lse[t]))
+        rest = [t for t in range(T) if t not in (6, T - 1)]
+        _check(o[rest], lse[rest], q[rest], values, idx[rest], SCALE)
+
+
+@pytest.mark.parametrize("group", [0, 1, 2])
+@pytest.mark.parametrize("order", ["rising", "falling"])
+def test_far_apart_scores_in_every_head_group(cuda, group, order):
+    T, H, K = _group_batch(128, group), 128, 512
+    cache, values = _cache(40, 14, cuda, spread=0.5)
+    q, idx = _query(T, H, 14, cuda), _indices(T, K, 2560, 14, cuda)
+    s = (values[idx.long()] @ q[:, 0].double()[..., None]).squeeze(-1)
+    by = s.argsort(dim=1, descending=order == "falling")
+    if order == "falling":
+        by = torch.stack([by[:, :K // 2].view(T, -1, 32), by[:, K // 2:].flip(1).view(T, -1, 32)], dim=2).view(T, K)
+    idx = idx.gather(1, by)
+    o, lse = ops.sparse_mla_decode_fp4(q, cache, idx, 1.0, num_splits=1)
+    torch.cuda.synchronize()
+    _check(o, lse, q, values, idx, 1.0)
+
+
+@pytest.mark.parametrize("group", [0, 1, 2])
+def test_scale_bytes_in_every_head_group(cuda, group):
+    g = torch.Generator(device=cuda).manual_seed(15)
+    kv = torch.randn(2560, 576, generator=g, device=cuda)
+    kv[:, :512] *= torch.exp2(torch.randint(-20, 6, (2560, 16), generator=g, device=cuda).float()).repeat_interleave(32, 1)
+    kv[::7, :512] = 0
+    rows = F.mla_rows(kv.to(torch.bfloat16))
+    T = _group_batch(128, group)
+    q, idx = _query(T, 128, 15, cuda), _indices(T, 512, 2560, 15, cuda, 0.05)
+    o, lse = ops.sparse_mla_decode_fp4(q, rows.view(40, 64, 400), idx, 0.002, num_splits=1)
+    torch.cuda.synchronize()
+    _check(o, lse, q, F.mla_values(rows), idx, 0.002)
