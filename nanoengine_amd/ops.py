@@ -841,40 +841,45 @@ def sparse_mla_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, indices: torch
                           workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``sparse_mla_decode`` over the 4-bit MLA cache: q [T,H,576] bf16, k_cache [blocks, block_size,
     (1,) 400] uint8, indices [T,topk] int32 physical slots -> (o [T,H,512] bf16, lse [T,H] f32)."""
-    if not (q.dim() == 3 and q.shape[2] == MLA_D_QK and q.dtype == torch.bfloat16 and q.stride(2) == 1):
+    shape, stride = q.shape, q.stride()
+    if not (len(shape) == 3 and shape[2] == MLA_D_QK and stride[2] == 1 and q.dtype == torch.bfloat16):
         _fail(f"q must be bf16 [T, H, {MLA_D_QK}] with a contiguous last dim")
-    T, H, _ = q.shape
-    if not (indices.dim() == 2 and indices.shape[0] == T and indices.dtype == torch.int32
-            and indices.stride(1) == 1):
+    T, H, _ = shape
+    ishape, istride = indices.shape, indices.stride()
+    if not (len(ishape) == 2 and ishape[0] == T and istride[1] == 1 and indices.dtype == torch.int32):
         _fail("indices must be int32 [T, topk] with unit column stride")
-    topk = indices.shape[1]
+    topk = ishape[1]
     blk_stride, block_size = mla_fp4_geometry(k_cache)
     dev = _gpu(q, k_cache, indices)
     if out is None:
-        out = torch.empty(T, H, MLA_D_V, dtype=torch.bfloat16, device=dev)
+        out = q.new_empty((T, H, MLA_D_V))
+    else:
+        if not (out.dtype == torch.bfloat16 and tuple(out.shape) == (T, H, MLA_D_V) and out.is_contiguous()):
+            _fail("out must be contiguous bf16 [T, H, 512]")
+        _gpu(q, out)
     if lse is None:
-        lse = torch.empty(T, H, dtype=torch.float32, device=dev)
-    if not (out.dtype == torch.bfloat16 and tuple(out.shape) == (T, H, MLA_D_V) and out.is_contiguous()):
-        _fail("out must be contiguous bf16 [T, H, 512]")
-    if not (lse.dtype == torch.float32 and tuple(lse.shape) == (T, H) and lse.is_contiguous()):
-        _fail("lse must be contiguous f32 [T, H]")
-    _gpu(q, out, lse)
+        lse = q.new_empty((T, H), dtype=torch.float32)
+    else:
+        if not (lse.dtype == torch.float32 and tuple(lse.shape) == (T, H) and lse.is_contiguous()):
+            _fail("lse must be contiguous f32 [T, H]")
+        _gpu(q, lse)
     if num_splits is None:
         num_splits = sparse_mla_num_splits(T, H, topk, dev)
-    need = 0
+    need, ws_ptr, ws_bytes = 0, None, 0
     if num_splits > 1:
         if dev == _CURRENT_DEVICE():
             need = sparse_mla_workspace_bytes(T, H, num_splits)
         else:  # the size goes by the current device's CUs
             with torch.cuda.device(dev):
                 need = sparse_mla_workspace_bytes(T, H, num_splits)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need
-                 or workspace.data_ptr() % 16 or workspace.get_device() != dev):
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    _launch(dev, "dsa_sparse_mla_decode_fp4", q.data_ptr(), q.stride(0) if T > 1 else 0, q.stride(1),
-            k_cache.data_ptr(), blk_stride, block_size, k_cache.shape[0], indices.data_ptr(), indices.stride(0), T, H,
-            topk, float(sm_scale), out.data_ptr(), lse.data_ptr(), int(num_splits),
-            workspace.data_ptr() if need else None, workspace.numel() * workspace.element_size() if need else 0)
+    if need:
+        if (workspace is None or workspace.numel() * workspace.element_size() < need
+                or workspace.data_ptr() % 16 or workspace.get_device() != dev):
+            workspace = k_cache.new_empty((need,))
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _launch(dev, "dsa_sparse_mla_decode_fp4", q.data_ptr(), stride[0] if T > 1 else 0, stride[1],
+            k_cache.data_ptr(), blk_stride, block_size, k_cache.shape[0], indices.data_ptr(), istride[0], T, H, topk,
+            float(sm_scale), out.data_ptr(), lse.data_ptr(), int(num_splits), ws_ptr, ws_bytes)
     return out, lse
 
 
@@ -920,39 +925,45 @@ def indexer_logits_fp4(q_fp8: torch.Tensor, kv_cache: torch.Tensor, weights: tor
     """Indexer logits [B*n, max_context_len] f32 over the 4-bit pages [num_pages, 64*68] (see
     dsa_indexer_logits_fp4). With ``clean_logits`` the positions past each row's length are -inf; without
     it only those up to the end of its last page are written."""
-    if not (q_fp8.dim() == 4 and q_fp8.dtype in (torch.float8_e4m3fn, torch.uint8) and q_fp8.is_contiguous()):
-        _fail(f"q_fp8 must be contiguous fp8 [B, next_n, H, D], got {q_fp8.dtype} {tuple(q_fp8.shape)}")
-    B, n, H, D = q_fp8.shape
+    shape = q_fp8.shape
+    if not (len(shape) == 4 and q_fp8.dtype in (torch.float8_e4m3fn, torch.uint8) and q_fp8.is_contiguous()):
+        _fail(f"q_fp8 must be contiguous fp8 [B, next_n, H, D], got {q_fp8.dtype} {tuple(shape)}")
+    B, n, H, D = shape
+    rows = B * n
     pages = kv_cache.shape[0]
     page_bytes = kv_cache.numel() // max(pages, 1)
     page_size = page_bytes // INDEXER_FP4_ROW_BYTES if pages else 64
-    if not (kv_cache.dtype == torch.uint8 and kv_cache.is_contiguous()
-            and page_bytes % INDEXER_FP4_ROW_BYTES == 0):
+    if not (kv_cache.dtype == torch.uint8 and page_bytes % INDEXER_FP4_ROW_BYTES == 0 and kv_cache.is_contiguous()):
         _fail(f"kv_cache must be contiguous uint8 [pages, page_size*{INDEXER_FP4_ROW_BYTES}], "
               f"got {kv_cache.dtype} {tuple(kv_cache.shape)}")
-    if not (weights.dtype == torch.float32 and tuple(weights.shape) == (B * n, H)):
-        _fail(f"weights must be f32 [{B * n}, {H}], got {weights.dtype} {tuple(weights.shape)}")
+    if not (weights.dtype == torch.float32 and weights.shape == (rows, H)):
+        _fail(f"weights must be f32 [{rows}, {H}], got {weights.dtype} {tuple(weights.shape)}")
     weights = weights.contiguous()
-    if not (context_lens.numel() == B * n):
+    if context_lens.numel() != rows:
         _fail(f"context_lens must be [B, next_n]={B, n}, got {tuple(context_lens.shape)}")
     cl = context_lens.to(torch.int32).contiguous()
-    if not (block_tables.dim() == 2 and block_tables.shape[0] == B):
-        _fail("block_tables must be [B, M]")
     bt = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
-    if not (bt.stride(1) == 1):
+    bt_shape, bt_stride = bt.shape, bt.stride()
+    if not (len(bt_shape) == 2 and bt_shape[0] == B):
+        _fail("block_tables must be [B, M]")
+    if bt_stride[1] != 1:
         _fail("block_tables rows must be contiguous")
-    if not (max_context_len >= 0 and bt.shape[1] * page_size >= max_context_len):
+    if not (max_context_len >= 0 and bt_shape[1] * page_size >= max_context_len):
         _fail("block_tables too narrow for max_context_len")
     dev = _gpu(q_fp8, kv_cache, weights, cl, bt)
     if out is None:
-        out = torch.empty(B * n, max_context_len, dtype=torch.float32, device=dev)
-    if not (out.dtype == torch.float32 and out.dim() == 2 and out.shape[0] == B * n
-            and out.shape[1] >= max_context_len and (out.shape[1] < 2 or out.stride(1) == 1)):
-        _fail("logits output must be f32 [B*n, >=max_ctx] with unit column stride")
-    _gpu(q_fp8, out)
+        out = weights.new_empty((rows, max_context_len))
+        out_stride = max_context_len
+    else:
+        o_shape = out.shape
+        if not (out.dtype == torch.float32 and len(o_shape) == 2 and o_shape[0] == rows
+                and o_shape[1] >= max_context_len and (o_shape[1] < 2 or out.stride(1) == 1)):
+            _fail("logits output must be f32 [B*n, >=max_ctx] with unit column stride")
+        _gpu(q_fp8, out)
+        out_stride = _row_stride(out)
     _launch(dev, "dsa_indexer_logits_fp4", q_fp8.data_ptr(), kv_cache.data_ptr(), pages, weights.data_ptr(),
-            cl.data_ptr(), bt.data_ptr(), bt.stride(0), B, n, H, D, page_size, int(max_context_len), out.data_ptr(),
-            _row_stride(out), int(bool(clean_logits)))
+            cl.data_ptr(), bt.data_ptr(), bt_stride[0], B, n, H, D, page_size, int(max_context_len), out.data_ptr(),
+            out_stride, int(bool(clean_logits)))
     return out
 
 
