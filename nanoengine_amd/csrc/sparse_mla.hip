@@ -58,8 +58,9 @@
 // exponent, subtracted with saturation. Either way every converted value is the bf16
 // the row stands for. The row is 61% of the fp8 one and the time the same (128
 // tokens of 128 heads, 2048 keys: 77 us from a graph, 1.84 TB/s, 0.95 PFLOP/s): the
-// block time follows the SIMDs' instructions, not the bytes. With at most 32 heads
-// the score waves take 16 keys each on 16x16x32 products (qk_waves4_narrow).
+// block time follows the SIMDs' instructions, not the bytes. With at most 32 heads,
+// or in head groups of at most 32 where a batch leaves CUs idle, the score waves take
+// 16 keys each on 16x16x32 products (qk_waves4_narrow).
 // Splits over the key list (the items of the last, partial round of the CUs)
 // write normalised partial outputs and LSEs to a caller-provided workspace; a
 // combine kernel merges them with the LSE rule of merge_attention_states.
@@ -718,14 +719,14 @@ __device__ __forceinline__ uint16_t* et_block4(uint8_t* smem, int par, int dq) {
 }
 
 // QK waves over 4-bit rows for at most 32 heads (a tensor-parallel rank's 16 or
-// 32; NT tiles of 16 heads): with 32-head tiles half of these waves would idle and
+// 32, or a small batch's head group; NT tiles of 16 heads): with 32-head tiles half of these waves would idle and
 // the others set the block time. Each of the four waves owns 16 keys of a block, over
 // all dims, as 18 v_mfma_f32_16x16x32_bf16 a head tile: A = the keys, lane (n16, g)
 // reading 16 bytes of key n16, its 32-dim blocks 4c + g with one scale each, for four
 // k-steps (dims 128c + 32g + 8i .. +7); B = the query in the same order. The shape
 // has 55% of the 32x32x16's rate, but the wave converts half the keys and takes a
 // quarter of the exponentials. A reference per wave, that is per k-step of P.V.
-// (90 tokens of 16 heads: 36.4 us on 32x32 tiles, 30.6 so; 256 tokens 61 and 54,
+// (90 tokens of 16 heads: 36.4 us on 32x32 tiles, 30.2 so; 256 tokens 61 and 53.5,
 // 4.1 TB/s of rows. The P.V waves' conversions, ~1600 of an iteration's ~2300 cycles,
 // set the block time then; a second block of rows in flight gains nothing. Eight
 // waves that each take their own keys, with query and output in registers and no
