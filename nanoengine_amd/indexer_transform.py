@@ -19,5 +19,4 @@ def indexer_k_transform_store_fp8(key: torch.Tensor, weight: torch.Tensor, bias:
     """Fuse the complete decode-time Indexer K transform and cache store."""
     if key.dtype != torch.bfloat16 or key.ndim != 2 or key.shape[1] != 128:
         raise ValueError("fused Indexer K path requires a bfloat16 [T, 128] key")
-    ops.indexer_k_transform_store(key, weight, bias, eps, positions, cos_sin_cache, cache.view(-1), slot_mapping,
-                                  page_size)
+    ops.indexer_k_transform_store(key, weight, bias, eps, positions, cos_sin_cache, cache, slot_mapping, page_size)

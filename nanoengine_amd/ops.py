@@ -427,6 +427,19 @@ def _slots(slot_mapping: torch.Tensor, n: int) -> tuple[torch.Tensor, int]:
     return s, int(s.dtype == torch.int64)
 
 
+def _key_pages(cache: torch.Tensor, page_size: int, row_bytes: int) -> int:
+    """Pages of a contiguous indexer key cache of ``row_bytes`` a key. fp8 and 4-bit pages are both uint8, and
+    the fp8 writers know no page count: in a 4-bit cache they would write past its end. So the last dimension of
+    a cache with more than one must be a page's bytes, whole pages', or a key's; a flat cache holds what its
+    caller says."""
+    page_bytes, width = int(page_size) * row_bytes, cache.shape[-1] if cache.dim() else 0
+    if not (page_bytes > 0 and cache.dtype == torch.uint8 and cache.is_contiguous()
+            and (width % page_bytes == 0 or width == row_bytes) and cache.numel() % page_bytes == 0):
+        _fail(f"cache must be contiguous uint8 pages of page_size*{row_bytes} bytes, got {cache.dtype} "
+              f"{tuple(cache.shape)} for page_size {page_size}")
+    return cache.numel() // page_bytes
+
+
 def mla_kv_store(kv: torch.Tensor, k_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
     """Quantise kv [N, (1,) 576] bf16 into the fp8 MLA cache at slot_mapping (see dsa_mla_kv_store)."""
     kv2 = kv.reshape(kv.shape[0], -1)
@@ -444,9 +457,7 @@ def indexer_k_store(key: torch.Tensor, cache: torch.Tensor, slot_mapping: torch.
     if not (key.dim() == 2 and key.shape[1] == INDEXER_HEAD_DIM and key.dtype == torch.bfloat16
             and key.stride(1) == 1):
         _fail("key must be bf16 [N, 128] with a contiguous last dim")
-    if not (cache.dtype == torch.uint8 and cache.is_contiguous()
-            and cache.numel() % (page_size * INDEXER_ROW_BYTES) == 0):
-        _fail("cache must be contiguous uint8 pages")
+    _key_pages(cache, page_size, INDEXER_ROW_BYTES)
     slots, is64 = _slots(slot_mapping, key.shape[0])
     dev = _check_cuda(key, cache, slots)
     _lib.call("dsa_indexer_k_store", key.data_ptr(), key.stride(0), slots.data_ptr(), is64, key.shape[0],
@@ -508,9 +519,7 @@ def indexer_k_transform_store(key: torch.Tensor, ln_weight: torch.Tensor, ln_bia
     lb = ln_bias.to(torch.float32).contiguous()
     if not (lw.numel() == INDEXER_HEAD_DIM and lb.numel() == INDEXER_HEAD_DIM):
         _fail("LayerNorm weight/bias must have 128 entries")
-    if not (cache.dtype == torch.uint8 and cache.is_contiguous()
-            and cache.numel() % (page_size * INDEXER_ROW_BYTES) == 0):
-        _fail("cache must be contiguous uint8 pages")
+    _key_pages(cache, page_size, INDEXER_ROW_BYTES)
     cs = _rope_cache(cos_sin_cache)
     pos, pos64 = _positions(positions, key.shape[0])
     slots, is64 = _slots(slot_mapping, key.shape[0])
@@ -788,15 +797,6 @@ def mla_fp4_geometry(k_cache: torch.Tensor) -> tuple[int, int]:
     return (stride[0] if shape[0] > 1 else block_size * MLA_FP4_ROW_BYTES), block_size
 
 
-def _fp4_pages(cache: torch.Tensor, page_size: int) -> int:
-    """Pages of a contiguous 4-bit indexer cache."""
-    page_bytes = int(page_size) * INDEXER_FP4_ROW_BYTES
-    if not (page_bytes > 0 and cache.dtype == torch.uint8 and cache.is_contiguous()
-            and cache.numel() % page_bytes == 0):
-        _fail(f"cache must be contiguous uint8 pages of page_size*{INDEXER_FP4_ROW_BYTES} bytes")
-    return cache.numel() // page_bytes
-
-
 def _row_stride(t: torch.Tensor) -> int:
     """Row stride of a 2-D tensor (torch leaves that of a single row free)."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -889,7 +889,7 @@ def indexer_k_store_fp4(key: torch.Tensor, cache: torch.Tensor, slot_mapping: to
     if not (key.dim() == 2 and key.shape[1] == INDEXER_HEAD_DIM and key.dtype == torch.bfloat16
             and key.stride(1) == 1):
         _fail("key must be bf16 [N, 128] with a contiguous last dim")
-    pages = _fp4_pages(cache, page_size)
+    pages = _key_pages(cache, page_size, INDEXER_FP4_ROW_BYTES)
     slots, is64 = _slots(slot_mapping, key.shape[0])
     dev = _gpu(key, cache, slots)
     _launch(dev, "dsa_indexer_k_store_fp4", key.data_ptr(), _row_stride(key), slots.data_ptr(), is64, key.shape[0],
@@ -900,7 +900,7 @@ def indexer_k_load_fp4(cache: torch.Tensor, slots: torch.Tensor, page_size: int,
                        scale_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The 4-bit indexer keys at slots [N] as (fp8 keys [N, 128] float8_e4m3fn, scales [N] f32), the
     operands of ``mqa_logits`` and ``mqa_topk`` (see dsa_indexer_k_load_fp4)."""
-    pages = _fp4_pages(cache, page_size)
+    pages = _key_pages(cache, page_size, INDEXER_FP4_ROW_BYTES)
     s, is64 = _slots(slots, 0)
     n = s.shape[0]
     dev = _gpu(cache, s)
