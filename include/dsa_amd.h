@@ -523,7 +523,9 @@ DSA_API int dsa_mla_kv_load_fp4(const uint8_t* kv_cache, int64_t kv_block_stride
 /* Sparse MLA decode over the 4-bit MLA cache (counterpart of
  * dsa_sparse_mla_decode: same arguments, outputs, split counts and workspace;
  * rows of 400 bytes, sm_scale finite and not negative, the workspace 16-byte
- * aligned). A head whose valid keys hold a NaN gets NaN outputs. */
+ * aligned). A head with a score of NaN or +inf among its valid keys gets NaN
+ * outputs; keys that score -inf weigh nothing, and a head with no other keys
+ * gets zeros and an LSE of -inf, as one without valid keys. */
 DSA_API int dsa_sparse_mla_decode_fp4(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                       const uint8_t* kv_cache, int64_t kv_block_stride_bytes,
                                       int kv_block_size, int64_t kv_num_blocks,

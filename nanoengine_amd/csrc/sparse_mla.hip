@@ -646,9 +646,9 @@ __device__ __forceinline__ void qk_waves(const MlaParams& P, uint8_t* smem, cons
       // lazy reference: it moves (to an integer) only when a block exceeds it by 2^8
       const bool need = mblk > m_run + kRescaleThreshold;
       if (__ballot(need)) {
-        const float m_new = need ? ceilf(mblk) : m_run;
-        l_run *= __builtin_amdgcn_exp2f(m_run - m_new);  // a power of two (0 from -inf)
-        m_run = m_new;
+        // a power of two, 0 from -inf (a head whose scores are all -inf so far stays there: no -inf - -inf)
+        l_run *= need ? __builtin_amdgcn_exp2f(m_run - ceilf(mblk)) : 1.f;
+        m_run = need ? ceilf(mblk) : m_run;
       }
       const float m_use = m_run == -__builtin_inff() ? 0.f : m_run;
       float pv[16];
@@ -818,9 +818,9 @@ __device__ __forceinline__ void qk_waves4_narrow(const MlaParams& P, uint8_t* sm
         m_max[nt] = fmaxf(m_max[nt], mblk);
         const bool need = mblk > m_run[nt] + kRescaleThreshold;
         if (__ballot(need)) {
-          const float m_new = need ? ceilf(mblk) : m_run[nt];
-          l_run[nt] *= __builtin_amdgcn_exp2f(m_run[nt] - m_new);  // a power of two (0 from -inf)
-          m_run[nt] = m_new;
+          // a power of two, 0 from -inf (as in qk_waves)
+          l_run[nt] *= need ? __builtin_amdgcn_exp2f(m_run[nt] - ceilf(mblk)) : 1.f;
+          m_run[nt] = need ? ceilf(mblk) : m_run[nt];
         }
         const float m_use = m_run[nt] == -__builtin_inff() ? 0.f : m_run[nt];
         float pv[4];
