@@ -55,10 +55,14 @@ class BatchTables:
 
     def context_fields(self, num_tokens_per_seq: int = 1) -> dict:
         """The fields of ``mla_backend.BatchContext`` for a decode step of ``num_tokens_per_seq`` new tokens a
-        request: tables, slot mapping, and each request's length after the step (0 for the requests that pad
-        the batch; those have no new tokens and come last)."""
-        if self.num_rows < self.batch * num_tokens_per_seq:
-            raise ValueError(f"{self.num_rows} rows cannot hold {num_tokens_per_seq} tokens of {self.batch} requests")
-        last = self.seq_lens[: self.batch * num_tokens_per_seq].view(self.batch, num_tokens_per_seq)[:, -1]
-        return {"is_prefill": False, "context_lens": last.unsqueeze(0), "block_tables": self.block_tables.unsqueeze(0),
-                "slot_mapping": self.slot_mapping, "num_tokens_per_seq": num_tokens_per_seq}
+        request: tables, slot mapping and lengths. ``context_lens`` is [1, batch] for one new token, each request's
+        length after the step, and [1, batch, num_tokens_per_seq] for more, each query token's own. Requests that
+        pad the batch have no new tokens and come last; their lengths are 0. (A final length alone would not do
+        for several tokens: its expansion to one length a token starts at 1.)"""
+        n = num_tokens_per_seq
+        if self.num_rows < self.batch * n:
+            raise ValueError(f"{self.num_rows} rows cannot hold {n} tokens of {self.batch} requests")
+        lens = self.seq_lens[: self.batch * n]
+        return {"is_prefill": False, "context_lens": (lens if n == 1 else lens.view(self.batch, n)).unsqueeze(0),
+                "block_tables": self.block_tables.unsqueeze(0), "slot_mapping": self.slot_mapping,
+                "num_tokens_per_seq": n}

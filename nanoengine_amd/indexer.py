@@ -120,7 +120,8 @@ def indexer_decode_topk(q_fp8: torch.Tensor, weights: torch.Tensor, kv_cache_buf
     q_fp8 [num_tokens, 64, 128] (num_tokens = batch * next_n); weights
     [num_tokens, 64] f32; kv_cache_buf [num_pages, page_size * 132] uint8, or
     [num_pages, page_size * 68] of 4-bit keys;
-    context_lens [batch] int (length after the last query token); block_tables
+    context_lens [batch] int (length after the last query token), or
+    [batch, next_n] of each query token's own (0: selects nothing); block_tables
     [batch, M] int32. Returns logical top-k positions [num_tokens, index_topk]
     int32 (ascending, -1 padded), or (logical, physical) when ``translate_topk``.
     Selection always runs on the exact HIP top-k, at every context length.

@@ -27,7 +27,7 @@ class BatchContext:
     BatchContext; names and meaning unchanged)."""
     is_prefill: bool = False
     is_dummy: bool = False
-    context_lens: torch.Tensor | None = None     # [1, B] int32
+    context_lens: torch.Tensor | None = None     # [1, B] int32, or [1, B, num_tokens_per_seq] per query token
     block_tables: torch.Tensor | None = None     # [1, B, M] int32
     slot_mapping: torch.Tensor | None = None     # [T] slots of the new tokens
     num_tokens_per_seq: int = 1

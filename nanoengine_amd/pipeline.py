@@ -77,9 +77,10 @@ class DsaDecodeStep:
         return self.workspace
 
     def expand_lens(self, context_lens: torch.Tensor) -> torch.Tensor:
-        """Per-query causal lengths, flattened [batch*next_n] int32."""
+        """Per-query causal lengths, flattened [batch*next_n] int32, of final ones [batch] or per-query ones
+        [batch, next_n]."""
         n = self.next_n
-        if n == 1:
+        if n == 1 or (context_lens.dim() == 2 and context_lens.shape[1] == n):
             return context_lens.to(torch.int32).reshape(-1).contiguous()
         offs = torch.arange(n - 1, -1, -1, dtype=torch.int32, device=context_lens.device)
         return (context_lens.to(torch.int32)[:, None] - offs).clamp_min(1).reshape(-1).contiguous()
