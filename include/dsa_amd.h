@@ -587,11 +587,13 @@ DSA_API int dsa_indexer_logits_fp4(const uint8_t* q_fp8, const uint8_t* kv_cache
  *                c_b + n_b (either may be NULL)
  *   status       [4] int64: {fault bits, new tokens, blocks taken, longest c_b + n_b}
  * Fault bits: 1 a length is negative or c_b + n_b passes int32 (that request is
- * taken as empty); 2 a request has more pages than bt_width; 4 the free list is too
+ * taken as empty); 2 a request with new tokens has more pages than bt_width; 4 the free list is too
  * short; 8 more new tokens than num_rows; 16 a prefix sum does not fit int32 (it is
  * stored as the largest). A token without a block (bits 2 and 4, or a negative
- * block number), or whose slot does not fit int32, gets slot -1. With bit 8 only
- * the first num_rows tokens are mapped and their blocks written.
+ * block number), or whose slot does not fit int32, gets slot -1; a negative block
+ * number and a slot past int32 set no bit, and such a token counts in seq_lens
+ * all the same: it shows as a row with slots[r] < 0 and seq_lens[r] > 0. With bit 8
+ * only the first num_rows tokens are mapped and their blocks written.
  * At most 8192 requests, and 2^31 - 1 rows and free blocks. The outputs must not
  * overlap the inputs, block_tables aside. No counterpart in the reference, whose
  * host scheduler builds these (SequenceBatch block tables and slot_mapping, read

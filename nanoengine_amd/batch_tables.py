@@ -47,10 +47,16 @@ class BatchTables:
 
     def check(self) -> tuple[int, int, int]:
         """Read the last plan's status (synchronises): (new tokens, blocks taken, longest request), or
-        RuntimeError naming its faults."""
-        faults, tokens, taken, longest = self.status.tolist()
-        if faults:
-            raise RuntimeError("batch tables: " + "; ".join(m for bit, m in _FAULTS.items() if faults & bit))
+        RuntimeError naming its faults. A new token without a cache slot is one too: it counts in the lengths,
+        but its row is not written."""
+        lost = ((self.slot_mapping < 0) & (self.seq_lens > 0)).sum()
+        faults, tokens, taken, longest, lost = torch.cat([self.status, lost.view(1)]).tolist()
+        what = [m for bit, m in _FAULTS.items() if faults & bit]
+        if lost and not what:
+            what.append(f"{lost} new tokens have no cache slot (a negative block number, or a slot that passes "
+                        f"{str(self.slot_mapping.dtype).replace('torch.', '')})")
+        if what:
+            raise RuntimeError("batch tables: " + "; ".join(what))
         return tokens, taken, longest
 
     def context_fields(self, num_tokens_per_seq: int = 1) -> dict:

@@ -988,7 +988,8 @@ def batch_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables
                  cu_seqlens_k: torch.Tensor | None = None) -> None:
     """Extend a batch's block tables and map its new tokens to cache slots, on the device, from each
     request's cached and new token counts [B] int32 (see dsa_batch_tables for every output and for the
-    fault bits of ``status`` [4] int64, which the caller reads when it next synchronises)."""
+    fault bits of ``status`` [4] int64, which the caller reads when it next synchronises). Clean bits do not say
+    that every token has a slot: see there, and ``BatchTables.check``, which looks."""
     i32 = torch.int32
     lens = cached_lens.shape
     if not (len(lens) == 1 and new_lens.shape == lens and cached_lens.dtype == i32 and new_lens.dtype == i32
