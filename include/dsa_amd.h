@@ -489,7 +489,9 @@ DSA_API int dsa_sparse_mla_prefill(const void* q, int64_t q_token_stride, int64_
 /* ---- 4-bit caches ------------------------------------------------------------
  * Blocks of 32 elements: e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign bit;
  * element 2i in the low nibble of byte i) with one UE8M0 scale byte a block,
- * value = code * 2^(byte - 127), byte 255 = a block of NaN.
+ * value = code * 2^(byte - 127), byte 255 = a block of NaN. Any byte is read as it
+ * is; bytes 253 and 254 give values of 2^128 and more (codes from 4 and from 2 on),
+ * which the bf16 reader, the attention and the logits take as infinities.
  *   MLA row, 400 bytes:   [256 B codes of the 512 nope dims][16 scale bytes]
  *                         [64 x bf16 rope]
  *   indexer page, page_size x 68 bytes: [page_size x 64 B codes of 128 dims]
@@ -512,7 +514,7 @@ DSA_API int dsa_mla_kv_store_fp4(const void* kv, int64_t kv_row_stride, const vo
                                  int64_t kv_block_stride_bytes, int kv_block_size,
                                  int64_t kv_num_blocks, void* stream);
 
-/* The rows at `slots` as bf16 [num_tokens, 576] (exact), row stride
+/* The rows at `slots` as bf16 [num_tokens, 576] (exact up to scale byte 252), row stride
  * out_row_stride elements: the keys of a prefill over cached tokens, for
  * dsa_sparse_mla_prefill (counterpart of the cached part of dsa_mla_prefill_kv). */
 DSA_API int dsa_mla_kv_load_fp4(const uint8_t* kv_cache, int64_t kv_block_stride_bytes,

@@ -3,14 +3,16 @@
 // A block is 32 consecutive elements: 16 bytes of e2m1 codes (element 2i in the
 // low nibble of byte i; codes 0..7 are 0, .5, 1, 1.5, 2, 3, 4, 6, bit 3 the sign)
 // and one UE8M0 scale byte. value = code * 2^(byte - 127); byte 255 makes the
-// whole block NaN. Every value is a bf16 value (two significant bits times a
-// power of two).
+// whole block NaN. Up to byte 252, the largest that the writers store, every value is a
+// bf16 value (two significant bits times a power of two, subnormal ones
+// included); at bytes 253 and 254 the codes from 4 and from 2 on are 2^128 and
+// more, which bf16 holds as infinities.
 //   MLA row (400 B)     : [256 B codes of 512 dims][16 scale bytes][64 bf16 rope]
 //   indexer page (4352 B): [64 keys x 64 B codes of 128 dims][64 x 4 scale bytes]
 // Rounding: the scale is the smallest 2^k with amax <= 6 * 2^k, so that no finite
 // element is cut off at the largest code (k is kept in [-40, 125]: below, blocks
 // that no attention could tell from zero; above, 6 * 2^k would not be finite). An
-// element is off by at most 2^(k-1), half the step between the largest codes' 4 and
+// element is off by at most 2^k, half the step between the largest codes' 4 and
 // 6, ties going to the even code; an infinity becomes the largest code.
 #pragma once
 
