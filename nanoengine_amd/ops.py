@@ -432,12 +432,13 @@ def _key_pages(cache: torch.Tensor, page_size: int, row_bytes: int) -> int:
     the fp8 writers know no page count: in a 4-bit cache they would write past its end. So the last dimension of
     a cache with more than one must be a page's bytes, whole pages', or a key's; a flat cache holds what its
     caller says."""
-    page_bytes, width = int(page_size) * row_bytes, cache.shape[-1] if cache.dim() else 0
+    page_bytes, shape, total = int(page_size) * row_bytes, cache.shape, cache.numel()
+    width = shape[-1] if shape else 1
     if not (page_bytes > 0 and cache.dtype == torch.uint8 and cache.is_contiguous()
-            and (width % page_bytes == 0 or width == row_bytes) and cache.numel() % page_bytes == 0):
+            and (width % page_bytes == 0 or (width == row_bytes and total % page_bytes == 0))):
         _fail(f"cache must be contiguous uint8 pages of page_size*{row_bytes} bytes, got {cache.dtype} "
-              f"{tuple(cache.shape)} for page_size {page_size}")
-    return cache.numel() // page_bytes
+              f"{tuple(shape)} for page_size {page_size}")
+    return total // page_bytes
 
 
 def mla_kv_store(kv: torch.Tensor, k_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:

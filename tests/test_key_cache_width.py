@@ -72,3 +72,9 @@ def test_the_formats_own_shapes_are_taken(calls, row):
         for call in calls:
             with pytest.raises(RuntimeError, match="GPU only"):
                 call(torch.zeros(shape, dtype=U8))
+
+
+@pytest.mark.parametrize("call", FP8 + FP4)
+def test_a_cache_without_dimensions_is_refused(call):
+    with pytest.raises(RuntimeError, match="pages of page_size"):
+        call(torch.zeros((), dtype=U8))
