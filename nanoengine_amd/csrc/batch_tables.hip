@@ -13,8 +13,8 @@
 // A fresh page starts with its first new token, whose row writes the table entry.
 // The call is bound by its launch and three dependent reads (lengths, free list or table,
 // and the search for the row's request between them), not by its bytes: 4 requests
-// 4.1 us from a graph, 64 of two tokens 4.5, 96 with 131072 new tokens 5.1 (a store of
-// 33 keys takes 2.0).
+// 4.1 us from a graph, 64 of two tokens 4.5, 96 with 131072 new tokens 5.1 (33 keys
+// stored and read back, two launches: 3.9).
 #include "dsa_common.h"
 #include "../../include/dsa_amd.h"
 

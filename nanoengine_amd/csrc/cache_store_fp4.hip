@@ -5,7 +5,7 @@
 // codes are one 4-byte store. An MLA row is one wave (64 lanes x 8 dims), an indexer
 // key 16 lanes, four keys to a wave. What bounds both directions is the launch for a
 // decode batch and the bytes for a prefill chunk: 128 MLA rows stored in 2.9 us and read
-// back in 2.7, 8192 in 5.0 and 4.8 (12.7 MB each way, 2.6 TB/s with the launch in it);
+// back in 2.7, 8192 in 5.2 and 4.9 (12.7 MB each way, 2.5 TB/s with the launch in it);
 // 33 indexer keys 2.0 and 1.9 us, 8192 of them 2.9 and 2.9 (2.7 MB).
 #include "dsa_common.h"
 #include "fp4.h"

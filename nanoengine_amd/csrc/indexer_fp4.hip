@@ -6,12 +6,13 @@
 // byte. The products run on bf16 MFMAs, exact with f32 sums: the block-scaled MFMA
 // would take the codes as they are, but keeps only ~13 bits below the largest of its
 // products.
-// What bounds it: 128 rows of 65536 positions take 140 us from a graph (570 MB read,
-// 34 MB written: 4.3 TB/s; 0.98 PFLOP/s). The same loop without its products takes
-// 120 us, without the ReLU and weights 127, the page loads and score stores alone 113,
-// the loads alone 87: the reads share HBM with the score stores, and the products run
-// at the clock (1.8 GHz) that their power leaves. Two query tokens (64 rows of
-// 30000: 61 us, 1.02 PFLOP/s) are bound by the products.
+// What bounds it: 128 rows of 65536 positions take 140 to 148 us from a graph, by the
+// card (570 MB read, 34 MB written: 4.2 TB/s; 0.95 PFLOP/s at 144). Where they took 140, the
+// same loop without its products took 120 us, without the ReLU and weights 127, the
+// page loads and score stores alone 113, the loads alone 87: the reads share HBM with
+// the score stores, and the products run at the clock (1.8 GHz) that their power
+// leaves. Two query tokens (64 rows of 30000: 63 us, 0.99 PFLOP/s) are bound by the
+// products.
 //
 // Persistent kernel, one workgroup of 8 waves per CU; every wave owns one contiguous
 // range of the flattened (batch entry, page) space and no barrier after the start.

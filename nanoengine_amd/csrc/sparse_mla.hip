@@ -56,11 +56,17 @@
 // A PV wave's 128 dims have four scales a key instead of one, so P carries none: the
 // codes are converted with their scales (pv_block4), and P needs only its reference's
 // exponent, subtracted with saturation. Either way every converted value is the bf16
-// the row stands for. The row is 61% of the fp8 one and the time the same (128
-// tokens of 128 heads, 2048 keys: 77 us from a graph, 1.84 TB/s, 0.95 PFLOP/s): the
-// block time follows the SIMDs' instructions, not the bytes. With at most 32 heads,
-// or in head groups of at most 32 where a batch leaves CUs idle, the score waves take
-// 16 keys each on 16x16x32 products (qk_waves4_narrow).
+// the row stands for. P is rounded to bf16 for its product, as over fp8 rows, and the
+// sum that divides the output is not: that costs about as much as the output's own last
+// rounding (off the exact result by 0.0021 to 0.0023 of its size, where f32
+// probabilities leave 0.0017), and more bits of P would cost a second set of products.
+// The row is 61% of the fp8 one and the time the same (128 tokens of 128 heads, 2048
+// keys: 78 us from a graph, 1.8 TB/s, 0.93 PFLOP/s): the block time follows the SIMDs'
+// instructions, not the bytes. (Each of a SIMD's two waves issues in 38% of its
+// cycles and waits for the port in 27; the matrix cores are busy in 44% of the
+// cycles of a busy CU.) With at most 32 heads, or in head groups of at most 32 where a
+// batch leaves CUs idle, the score waves take 16 keys each on 16x16x32 products
+// (qk_waves4_narrow).
 // Splits over the key list (the items of the last, partial round of the CUs)
 // write normalised partial outputs and LSEs to a caller-provided workspace; a
 // combine kernel merges them with the LSE rule of merge_attention_states.
@@ -726,12 +732,13 @@ __device__ __forceinline__ uint16_t* et_block4(uint8_t* smem, int par, int dq) {
 // k-steps (dims 128c + 32g + 8i .. +7); B = the query in the same order. The shape
 // has 55% of the 32x32x16's rate, but the wave converts half the keys and takes a
 // quarter of the exponentials. A reference per wave, that is per k-step of P.V.
-// (90 tokens of 16 heads: 36.4 us on 32x32 tiles, 30.2 so; 256 tokens 61 and 53.5,
-// 4.1 TB/s of rows. The P.V waves' conversions, ~1600 of an iteration's ~2300 cycles,
-// set the block time then; a second block of rows in flight gains nothing. Eight
-// waves that each take their own keys, with query and output in registers and no
-// barrier, are faster a block, 0.95 against 1.2 us, but start and merge 6 us later:
-// 34 us, and 40 against 33 for 128 tokens.)
+// (90 tokens of 16 heads: 36.4 us on 32x32 tiles, 30.3 so; 256 tokens 61 and 55,
+// 4.0 TB/s of rows. The 90 tokens' waves issue in 39% of their cycles, wait for the
+// port in 18 and for data in 44, the matrix cores are busy in 21: the chain of reads,
+// conversions and products inside a block sets its time, and a second block of rows
+// in flight gains nothing. Eight waves that each take their own keys, with query and
+// output in registers and no barrier, are faster a block, 0.95 against 1.2 us, but
+// start and merge 6 us later: 34 us, and 40 against 33 for 128 tokens.)
 template <int NT>
 __device__ __forceinline__ void qk_waves4_narrow(const MlaParams& P, uint8_t* smem, const MlaCtx& c,
                                                  const DmaLanes& dl) {
