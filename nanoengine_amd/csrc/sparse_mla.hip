@@ -996,7 +996,9 @@ __device__ __forceinline__ void qk_waves_rows(const MlaParams& P, uint8_t* smem,
       const bool need = mblk > m_run + kRescaleThreshold;
       if (__ballot(need)) {
         const float m_new = need ? mblk : m_run;
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);  // 0 from -inf
+        // 0 from -inf; 1 for a head that stays, also at -inf (the difference is of the reference as it is rounded:
+        // written with mblk it would become an FMA of the scores)
+        const float alpha = m_new == m_run ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
         l_run[0] *= alpha;
         l_run[1] *= alpha;
         m_run = m_new;
@@ -1180,8 +1182,7 @@ __device__ __forceinline__ void pv_waves(const MlaParams& P, uint8_t* smem, cons
         }
         const bool up = mn > R[mt];
         if (__ballot(up)) {
-          // 0 from -inf (a head of bf16 rows that stays at -inf has NaN sums already)
-          const float alpha = up || kKeys == kRows ? __builtin_amdgcn_exp2f(R[mt] - mn) : 1.f;
+          const float alpha = up ? __builtin_amdgcn_exp2f(R[mt] - mn) : 1.f;  // 0 from -inf
           R[mt] = up ? mn : R[mt];
           int hb = 4 * h;
           asm volatile("" : "+v"(hb));
