@@ -175,7 +175,13 @@ def _scale_of(amax, kind):
         return s, s
     m, e = torch.frexp(s)  # s = m * 2^e, m in [0.5, 1): the smallest power of two that is not below it
     byte = e + 127 - (m == 0.5).to(e.dtype)
-    return torch.ldexp(torch.ones_like(s), byte - 127), byte.to(torch.uint8).view(E8M0)
+    held = byte.to(torch.uint8).view(E8M0)
+    return _values(held), held
+
+
+def _values(scales):
+    """The float32 numbers that scales stand for (an exponent's bits: exp2 is not exact on every device)."""
+    return scales if scales.dtype == torch.float32 else (scales.view(torch.uint8).to(torch.int32) << 23).view(torch.float32)
 
 
 def _to_fp8(y, kind):
@@ -216,10 +222,6 @@ def _run_quant(st):
         from nanoengine_amd import ops
         return ops.act_quant(st["x"], st["codes"], st["scales"])
     return _to_fp8(st["x"].float(), _kind(st["scales"]))
-
-
-def _values(scales):
-    return scales if scales.dtype == torch.float32 else torch.exp2(scales.view(torch.uint8).float() - 127.0)
 
 
 def _run_gemm(st):
@@ -272,8 +274,9 @@ def _coded64(y, scale):
     top = torch.zeros(T, n, dtype=torch.float64, device=y.device)
     top.scatter_reduce_(1, (torch.arange(D, device=y.device) // BLOCK).expand(T, D), y.abs(), "amax")
     s = top.clamp(min=2.0 ** -40) / 448.0
-    if scale == "e8m0":
-        s = torch.exp2(torch.ceil(torch.log2(s)))
+    if scale == "e8m0":  # the power of two below it, doubled unless it is that one
+        whole = (s.view(torch.int64) >> 52 << 52).view(torch.float64)
+        s = torch.where(whole == s, s, 2.0 * whole)
     return y / s[:, torch.arange(D, device=y.device) // BLOCK], s
 
 
@@ -293,8 +296,8 @@ def exact(case, seed):
     if kind == "gemm":
         out = torch.zeros(case["tokens"], case["n"], dtype=torch.float64, device=DEV)
         rows = torch.arange(case["n"], device=DEV) // BLOCK
-        sa, sb = (s.double() if s.dtype == torch.float32 else torch.pow(2.0, s.view(torch.uint8).double() - 127.0)
-                  for s in (st["sa"], st["sb"]))
+        sa, sb = (s.double() if s.dtype == torch.float32 else
+                  ((s.view(torch.uint8).long() + (1023 - 127)) << 52).view(torch.float64) for s in (st["sa"], st["sb"]))
         for at in range(_ceil(case["k"], BLOCK)):  # block by block: products of codes, then both scales
             cut = slice(at * BLOCK, (at + 1) * BLOCK)
             out += (st["a"][:, cut].double() @ st["b"][:, cut].double().T) * sa[:, at, None] * sb[rows, at]
