@@ -608,6 +608,83 @@ DSA_API int dsa_batch_tables(const int32_t* cached_lens, const int32_t* new_lens
                              int64_t num_rows, void* cu_seqlens_q, void* cu_seqlens_k,
                              int cu_is_64, int64_t* status, void* stream);
 
+/* ---- the steps around the attention -------------------------------------------
+ * From hidden states to the indexer's and the attention's inputs, and from the
+ * attention's output on. fp8 activations carry one scale per 128 elements of a row,
+ * fp8 weights one per 128 x 128 block; the last block of a row may be short.
+ * scale_kind:
+ *   0  float32: s = max(amax, 2^-40) / 448
+ *   1  e8m0: the byte of the smallest power of two 2^(byte - 127) >= that (at most 254)
+ * value = code * s. A NaN gets the NaN code, an infinity too (its block's scale is then
+ * infinite, or byte 254). The reference runs these steps in third-party kernels
+ * outside the paths cited above. */
+
+/* Root-mean-square norm of rows, with the residual's addition and an fp8 output.
+ *   x            [rows, dim] bf16, row stride x_stride elements
+ *   residual     [rows, dim] bf16, or NULL
+ *   residual_out [rows, dim] bf16, or NULL: h = bf16(x + residual); may be residual or x
+ *   weight       [dim] bf16, or f32 when weight_is_f32
+ *   out          [rows, dim] bf16, or NULL: y = h * (mean(h^2) + eps)^-1/2 * weight, rounded
+ *                once from f32 (h = x without a residual); may be x
+ *   codes        [rows, dim] e4m3fn, row stride code_stride bytes, or NULL; rounded from the
+ *                same f32 y
+ *   scales       [rows, ceil(dim / 128)] of scale_kind, row stride scale_stride elements
+ *                (NULL exactly when codes is)
+ * One of out and codes at least. 1 <= dim <= 32768; rows that are 16-byte aligned (codes
+ * 8-byte) and a dim that is a multiple of 8 take wide loads, others narrow ones. Apart from
+ * the pairs named, outputs must not overlap inputs. */
+DSA_API int dsa_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                         void* residual_out, int64_t residual_out_stride, const void* weight,
+                         int weight_is_f32, float eps, int64_t rows, int dim, void* out, int64_t out_stride,
+                         uint8_t* codes, int64_t code_stride, void* scales, int64_t scale_stride,
+                         int scale_kind, void* stream);
+
+/* The fp8 rounding alone: x [rows, dim] bf16 to codes and scales as in dsa_rms_norm
+ * (any dim), such as the attention's output before the output projection. */
+DSA_API int dsa_act_quant(const void* x, int64_t x_stride, int64_t rows, int dim, uint8_t* codes,
+                          int64_t code_stride, void* scales, int64_t scale_stride, int scale_kind,
+                          void* stream);
+
+/* Workspace bytes dsa_fp8_gemm needs for this shape on the current device (0: none). */
+DSA_API size_t dsa_fp8_gemm_workspace_bytes(int m, int n, int k);
+
+/* Product of block-scaled fp8 matrices:
+ *   out[i, j] = sum_kb a_scale[i, kb] b_scale[j / 128, kb] sum_{t in block kb} a[i, t] b[j, t]
+ *   a        [m, k] e4m3fn, row stride a_stride bytes;  a_scale [m, ceil(k / 128)]
+ *   b        [n, k] e4m3fn, row stride b_stride bytes;  b_scale [ceil(n / 128), ceil(k / 128)]
+ *   out      [m, n] bf16, or f32 when out_is_f32, row stride out_stride elements
+ * Scales are of scale_kind, their strides in elements; float32 ones may be any numbers, byte
+ * 255 of an e8m0 one is NaN. k a multiple of 16; a and b rows 16-byte aligned.
+ * Products of 64 neighbouring k are summed by the matrix instruction, which drops what lies
+ * more than 13 bits below the largest of them; those sums are added in f32. A NaN code or
+ * scale gives NaN in the rows or columns that it belongs to.
+ * workspace: dsa_fp8_gemm_workspace_bytes, 16-byte aligned (NULL where that is 0); calls that
+ * share one must be ordered. The result does not depend on what it held. Stands beside dsa_mqa_logits as the
+ * second of DeepGEMM's fp8 products (its fp8_gemm_nt). */
+DSA_API int dsa_fp8_gemm(const uint8_t* a, int64_t a_stride, const void* a_scale, int64_t a_scale_stride,
+                         const uint8_t* b, int64_t b_stride, const void* b_scale, int64_t b_scale_stride,
+                         int scale_kind, int m, int n, int k, void* out, int64_t out_stride,
+                         int out_is_f32, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary positions of query heads and of key heads, in one launch.
+ *   q        [num_tokens, q_heads, rot_dim] bf16: the rotated part of each head (strides of
+ *            token and head in elements, dims contiguous);  q_out likewise, may be q
+ *   k, k_out [num_tokens, k_heads, rot_dim] likewise (k_heads 0: none)
+ *   cos_sin_cache [cache_positions, rot_dim] f32 = [cos of rot_dim / 2 | sin] per position
+ *   positions [num_tokens] int32, or int64 when pos_is_64, clamped to the cache
+ * Pair p of a head is dims (2p, 2p + 1) when interleaved, else (p, p + rot_dim / 2), and
+ * (a, b) becomes (a cos - b sin, b cos + a sin); out_interleaved says the same of the output.
+ * f32, rounded once. rot_dim even, at most 512; a multiple of 8 with 16-byte aligned rows
+ * takes wide loads. An output is its input, with the same strides, or does not overlap it.
+ * Beside dsa_indexer_q_prologue, whose rotation is fused for the indexer's own heads. */
+DSA_API int dsa_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads, void* q_out,
+                     int64_t q_out_token_stride, int64_t q_out_head_stride, const void* k,
+                     int64_t k_token_stride, int64_t k_head_stride, int k_heads, void* k_out,
+                     int64_t k_out_token_stride, int64_t k_out_head_stride, int64_t num_tokens,
+                     int rot_dim, const float* cos_sin_cache, int64_t cache_positions,
+                     const void* positions, int pos_is_64, int interleaved, int out_interleaved,
+                     void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

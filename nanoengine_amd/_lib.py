@@ -71,6 +71,14 @@ SIGNATURES = {
     "dsa_indexer_k_load_fp4": (c_int, [_P, c_int, c_int64, _P, c_int, c_int, _P, _P, _P]),
     "dsa_indexer_logits_fp4": (c_int, [_P, _P, c_int64, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int,
                                        c_int64, _P, c_int64, c_int, _P]),
+    "dsa_rms_norm": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int, c_float, c_int64, c_int, _P, c_int64,
+                             _P, c_int64, _P, c_int64, c_int, _P]),
+    "dsa_act_quant": (c_int, [_P, c_int64, c_int64, c_int, _P, c_int64, _P, c_int64, c_int, _P]),
+    "dsa_fp8_gemm_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "dsa_fp8_gemm": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int, c_int, c_int, c_int, _P,
+                             c_int64, c_int, _P, c_size_t, _P]),
+    "dsa_rope": (c_int, [_P, c_int64, c_int64, c_int, _P, c_int64, c_int64, _P, c_int64, c_int64, c_int, _P, c_int64,
+                         c_int64, c_int64, c_int, _P, c_int64, _P, c_int, c_int, c_int, _P]),
 }
 
 _lib = None

@@ -19,7 +19,8 @@ MICROBENCH_SRC = "microbench.hip"
 MICROBENCH_LIB = PKG_DIR / "libdsa_microbench.so"
 SOURCES = ["capi.hip", "topk.hip", "indexer.hip", "sparse_mla.hip", "cache_store.hip",
            "indexer_prologue.hip", "prefill_logits.hip", "sparse_mla_prefill.hip",
-           "prefill_topk.hip", "cache_store_fp4.hip", "indexer_fp4.hip", "batch_tables.hip"]
+           "prefill_topk.hip", "cache_store_fp4.hip", "indexer_fp4.hip", "batch_tables.hip",
+           "norm_quant.hip", "rope.hip", "fp8_gemm.hip"]
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -51,6 +52,9 @@ PER_FILE_FLAGS = {
     "cache_store_fp4.hip": [],
     "indexer_fp4.hip": VGPR_FORM,
     "batch_tables.hip": [],
+    "norm_quant.hip": [],
+    "rope.hip": [],
+    "fp8_gemm.hip": [],
 }
 
 

@@ -1,0 +1,198 @@
+// Rotary positions of query heads and of the shared key, for gfx950.
+//
+//   (u, v) = (a cos - b sin, b cos + a sin)
+// for the rot / 2 pairs (a, b) of a head at its token's position; pair p turns by the
+// table's angle p. Pairs lie beside each other (2p, 2p + 1) or in halves (p, p + rot / 2),
+// in the input and in the output each: a layout can change on the way. The output may be the
+// input (a row belongs to lanes of one wave, which hold all of it before they write) or
+// another tensor, such as the tail of the rows that the attention reads.
+//
+// A lane takes four pairs of a token and goes through kHeads heads with one read of their
+// cosines and sines. f32 arithmetic, one rounding to bf16.
+#include "dsa_common.h"
+#include "../../include/dsa_amd.h"
+
+namespace dsa {
+namespace {
+
+constexpr int kRopeThreads = 256;
+constexpr int kMaxRot = 512;  // a row within one wave
+
+struct RopeParams {
+  const uint16_t* x[2];  // queries, keys (may be null: no heads)
+  uint16_t* out[2];
+  int64_t x_token[2], x_head[2], out_token[2], out_head[2];
+  int heads[2];
+  int64_t tokens;
+  int rot;
+  const float* table;
+  int64_t table_rows;
+  const void* positions;
+  int wide;
+  int lanes;       // a row's lanes: a power of two, four pairs each
+  int lane_shift;
+  int groups;      // groups of heads of a token: queries' ones, then the keys'
+  int q_groups;
+};
+
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float lo_f32(int v) { return __uint_as_float((uint32_t)v << 16); }
+__device__ __forceinline__ float hi_f32(int v) { return __uint_as_float((uint32_t)v & 0xffff0000u); }
+__device__ __forceinline__ int pack2(float a, float b) {
+  return __builtin_bit_cast(int, (v2bf){(__bf16)a, (__bf16)b});
+}
+
+// Pairs p .. p + 3 of a row (half = rot / 2 pairs). VEC: rot a multiple of eight, rows 16-byte aligned.
+template <bool PAIRS, bool VEC>
+__device__ __forceinline__ void load_pairs(const uint16_t* row, int p, int half, float* a, float* b) {
+  if (VEC) {
+    if (p >= half) return;
+    if (PAIRS) {
+      const v4i v = *reinterpret_cast<const v4i*>(row + 2 * p);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a[j] = lo_f32(v[j]), b[j] = hi_f32(v[j]);
+    } else {
+      const v2i u = *reinterpret_cast<const v2i*>(row + p), w = *reinterpret_cast<const v2i*>(row + half + p);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        a[2 * j] = lo_f32(u[j]), a[2 * j + 1] = hi_f32(u[j]);
+        b[2 * j] = lo_f32(w[j]), b[2 * j + 1] = hi_f32(w[j]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (p + j < half) {
+        a[j] = bf16_to_f32(row[PAIRS ? 2 * (p + j) : p + j]);
+        b[j] = bf16_to_f32(row[PAIRS ? 2 * (p + j) + 1 : half + p + j]);
+      }
+  }
+}
+
+template <bool PAIRS, bool VEC>
+__device__ __forceinline__ void store_pairs(uint16_t* row, int p, int half, const float* u, const float* v) {
+  if (VEC) {
+    if (p >= half) return;
+    if (PAIRS) {
+      *reinterpret_cast<v4i*>(row + 2 * p) =
+          (v4i){pack2(u[0], v[0]), pack2(u[1], v[1]), pack2(u[2], v[2]), pack2(u[3], v[3])};
+    } else {
+      *reinterpret_cast<v2i*>(row + p) = (v2i){pack2(u[0], u[1]), pack2(u[2], u[3])};
+      *reinterpret_cast<v2i*>(row + half + p) = (v2i){pack2(v[0], v[1]), pack2(v[2], v[3])};
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (p + j < half) {
+        const int w = pack2(u[j], v[j]);
+        row[PAIRS ? 2 * (p + j) : p + j] = (uint16_t)w;
+        row[PAIRS ? 2 * (p + j) + 1 : half + p + j] = (uint16_t)((uint32_t)w >> 16);
+      }
+  }
+}
+
+template <bool PAIRS, bool OUT_PAIRS, bool VEC, int HEADS>
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams P) {
+  const int64_t at = ((int64_t)blockIdx.x * kRopeThreads + threadIdx.x) >> P.lane_shift;
+  const int64_t token = at / P.groups;
+  if (token >= P.tokens) return;  // a row's lanes together
+  int g = (int)(at - token * P.groups);
+  const int which = g >= P.q_groups;
+  if (which) g -= P.q_groups;
+  const int half = P.rot >> 1, p = 4 * (threadIdx.x & (P.lanes - 1));
+  const int heads = P.heads[which];
+  const uint16_t* x = P.x[which] + token * P.x_token[which];
+  uint16_t* out = P.out[which] + token * P.out_token[which];
+
+  float a[HEADS][4], b[HEADS][4], cos[4], sin[4];
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i) {
+    const int h = g * HEADS + i;
+    if (h < heads) load_pairs<PAIRS, VEC>(x + h * P.x_head[which], p, half, a[i], b[i]);
+  }
+  int64_t pos = P.wide ? static_cast<const int64_t*>(P.positions)[token]
+                       : (int64_t)static_cast<const int32_t*>(P.positions)[token];
+  pos = pos < 0 ? 0 : pos >= P.table_rows ? P.table_rows - 1 : pos;
+  const float* row = P.table + pos * P.rot;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int i = VEC ? (p < half ? p + j : j) : p + j < half ? p + j : 0;
+    cos[j] = row[i];
+    sin[j] = row[half + i];
+  }
+  asm volatile("" ::: "memory");  // where the output is the input: rows are read before they are written
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i) {
+    const int h = g * HEADS + i;
+    if (h >= heads) break;
+    float u[4], v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u[j] = a[i][j] * cos[j] - b[i][j] * sin[j];
+      v[j] = b[i][j] * cos[j] + a[i][j] * sin[j];
+    }
+    store_pairs<OUT_PAIRS, VEC>(out + h * P.out_head[which], p, half, u, v);
+  }
+}
+
+template <int HEADS>
+void launch_rope(RopeParams P, bool pairs, bool out_pairs, bool vec, hipStream_t st) {
+  P.q_groups = (P.heads[0] + HEADS - 1) / HEADS;
+  P.groups = P.q_groups + (P.heads[1] + HEADS - 1) / HEADS;
+  const int64_t threads = P.tokens * P.groups * P.lanes;
+  const dim3 grid((unsigned)((threads + kRopeThreads - 1) / kRopeThreads)), block(kRopeThreads);
+#define DSA_ROPE(A, B, V) hipLaunchKernelGGL((rope_kernel<A, B, V, HEADS>), grid, block, 0, st, P)
+  if (pairs && out_pairs) { if (vec) DSA_ROPE(true, true, true); else DSA_ROPE(true, true, false); }
+  else if (pairs) { if (vec) DSA_ROPE(true, false, true); else DSA_ROPE(true, false, false); }
+  else if (out_pairs) { if (vec) DSA_ROPE(false, true, true); else DSA_ROPE(false, true, false); }
+  else { if (vec) DSA_ROPE(false, false, true); else DSA_ROPE(false, false, false); }
+#undef DSA_ROPE
+}
+
+bool rope_aligned(const void* p, int64_t token, int64_t head) {
+  return !p || (!(reinterpret_cast<uintptr_t>(p) & 15) && !(token & 7) && !(head & 7));
+}
+
+}  // namespace
+}  // namespace dsa
+
+extern "C" int dsa_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads, void* q_out,
+                        int64_t q_out_token_stride, int64_t q_out_head_stride, const void* k, int64_t k_token_stride,
+                        int64_t k_head_stride, int k_heads, void* k_out, int64_t k_out_token_stride,
+                        int64_t k_out_head_stride, int64_t num_tokens, int rot_dim, const float* cos_sin_cache,
+                        int64_t cache_positions, const void* positions, int pos_is_64, int interleaved,
+                        int out_interleaved, void* stream) {
+  using namespace dsa;
+  if (num_tokens < 0 || num_tokens > INT32_MAX || q_heads < 0 || k_heads < 0 || q_heads > 65536 || k_heads > 65536)
+    return set_error(kInvalidArgument, "dsa_rope: bad sizes");
+  if (rot_dim < 2 || (rot_dim & 1)) return set_error(kInvalidArgument, "dsa_rope: rot_dim %d must be even", rot_dim);
+  if (rot_dim > kMaxRot) return set_error(kUnsupported, "dsa_rope: rot_dim %d (at most %d)", rot_dim, kMaxRot);
+  if (num_tokens == 0 || q_heads + k_heads == 0) return kOk;
+  if ((q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)) || !cos_sin_cache || !positions)
+    return set_error(kInvalidArgument, "dsa_rope: null pointer");
+  if (cache_positions < 1) return set_error(kInvalidArgument, "dsa_rope: empty cos_sin_cache");
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k) |
+        reinterpret_cast<uintptr_t>(k_out)) & 1) ||
+      (reinterpret_cast<uintptr_t>(cos_sin_cache) & 3) || (reinterpret_cast<uintptr_t>(positions) & (pos_is_64 ? 7 : 3)))
+    return set_error(kInvalidArgument, "dsa_rope: pointers must be aligned to their elements");
+  int lanes = 1, shift = 0;
+  while (lanes * 8 < rot_dim) lanes <<= 1, ++shift;
+  RopeParams P = {{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k)},
+                  {static_cast<uint16_t*>(q_out), static_cast<uint16_t*>(k_out)},
+                  {q_token_stride, k_token_stride},
+                  {q_head_stride, k_head_stride},
+                  {q_out_token_stride, k_out_token_stride},
+                  {q_out_head_stride, k_out_head_stride},
+                  {q_heads, k_heads},
+                  num_tokens, rot_dim, cos_sin_cache, cache_positions, positions, pos_is_64, lanes, shift, 0, 0};
+  const bool vec = rot_dim % 8 == 0 && rope_aligned(q_heads ? q : nullptr, q_token_stride, q_head_stride) &&
+                   rope_aligned(q_heads ? q_out : nullptr, q_out_token_stride, q_out_head_stride) &&
+                   rope_aligned(k_heads ? k : nullptr, k_token_stride, k_head_stride) &&
+                   rope_aligned(k_heads ? k_out : nullptr, k_out_token_stride, k_out_head_stride);
+  if (num_tokens * (q_heads + k_heads + 2) * lanes / kRopeThreads > INT32_MAX - 1)
+    return set_error(kUnsupported, "dsa_rope: more than 2^31 workgroups");
+  launch_rope<1>(P, interleaved, out_interleaved, vec, (hipStream_t)stream);
+  return check_launch("dsa_rope");
+}

@@ -1033,3 +1033,201 @@ def batch_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables
             stride[0] if B > 1 else width, width, int(page_size), free_ptr, num_free, _ptr(free_head),
             slot_mapping.data_ptr(), s64, _ptr(positions), p64, _ptr(seq_lens), rows[0], _ptr(cu_seqlens_q),
             _ptr(cu_seqlens_k), c64 or k64, status.data_ptr())
+
+
+# --------------------------------------------------------------------------- around the attention
+FP8_BLOCK = 128
+_FP8_TYPES = (torch.float8_e4m3fn, torch.uint8)
+# scales of fp8 blocks: float32, or powers of two as their exponent byte (uint8: the same bytes)
+_SCALE_KINDS = {torch.float32: 0, torch.float8_e8m0fnu: 1, torch.uint8: 1}
+
+
+def _rows2d(t: torch.Tensor, name: str, dtypes, shape=None) -> int:
+    """Row stride of a 2-D tensor with a contiguous last dim, of this shape where one is given."""
+    s, st = t.shape, t.stride()
+    if not (len(s) == 2 and t.dtype in dtypes and (st[1] == 1 or s[1] == 1) and (shape is None or s == shape)):
+        want = "2-D" if shape is None else str(list(shape))
+        _fail(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)} {want} with a contiguous "
+              f"last dim, got {t.dtype} {tuple(s)}")
+    return st[0] if s[0] > 1 else s[1]
+
+
+_BF16 = (torch.bfloat16,)
+
+
+def _coded(rows: int, dim: int, codes: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, int]:
+    """(row stride of the codes, of the scales, scale kind) of fp8 rows with a scale per 128 elements."""
+    code_stride = _rows2d(codes, "codes", _FP8_TYPES, (rows, dim))
+    kind = _SCALE_KINDS.get(scales.dtype)
+    if kind is None:
+        _fail(f"scales must be float32 or float8_e8m0fnu, got {scales.dtype}")
+    return code_stride, _rows2d(scales, "scales", _SCALE_KINDS, (rows, -(-dim // FP8_BLOCK))), kind
+
+
+def _norm(x, weight, eps, out, residual, residual_out, codes, scales) -> None:
+    stride = _rows2d(x, "x", _BF16)
+    shape = x.shape
+    rows, dim = shape
+    if not (weight.dim() == 1 and weight.shape[0] == dim and weight.dtype in (torch.bfloat16, torch.float32)
+            and weight.is_contiguous()):
+        _fail(f"weight must be contiguous bfloat16 or float32 [{dim}]")
+    tensors = [x, weight]
+    res_stride = sum_stride = out_stride = code_stride = scale_stride = kind = 0
+    if residual is not None:
+        res_stride = _rows2d(residual, "residual", _BF16, shape)
+        tensors.append(residual)
+    if residual_out is not None:
+        if residual is None:
+            _fail("residual_out needs a residual")
+        sum_stride = _rows2d(residual_out, "residual_out", _BF16, shape)
+        tensors.append(residual_out)
+    if out is not None:
+        out_stride = _rows2d(out, "out", _BF16, shape)
+        tensors.append(out)
+    if codes is not None:
+        code_stride, scale_stride, kind = _coded(rows, dim, codes, scales)
+        tensors += (codes, scales)
+    _launch(_gpu(*tensors), "dsa_rms_norm", x.data_ptr(), stride, _ptr(residual), res_stride, _ptr(residual_out),
+            sum_stride, weight.data_ptr(), int(weight.dtype is torch.float32), float(eps), rows, dim, _ptr(out),
+            out_stride, _ptr(codes), code_stride, _ptr(scales), scale_stride, kind)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, out: torch.Tensor | None = None, *,
+             residual: torch.Tensor | None = None, residual_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Root-mean-square norm of x [T, D] bf16 (row stride free) by weight [D] (bf16 or f32). With a ``residual``
+    [T, D] bf16 the norm is that of bf16(x + residual), which ``residual_out`` receives when given (the residual
+    itself: in place). Returns out [T, D] bf16 (see dsa_rms_norm)."""
+    if out is None:
+        out = x.new_empty(x.shape)
+    _norm(x, weight, eps, out, residual, residual_out, None, None)
+    return out
+
+
+def _new_codes(x: torch.Tensor, codes, scales, scale_dtype):
+    if x.dim() != 2:
+        _fail(f"x must be bfloat16 2-D, got {x.dtype} {tuple(x.shape)}")
+    if codes is None:
+        codes = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    if scales is None:
+        scales = x.new_empty((x.shape[0], -(-x.shape[1] // FP8_BLOCK)), dtype=scale_dtype)
+    return codes, scales
+
+
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, codes: torch.Tensor | None = None,
+                   scales: torch.Tensor | None = None, *, out: torch.Tensor | None = None,
+                   residual: torch.Tensor | None = None, residual_out: torch.Tensor | None = None,
+                   scale_dtype: torch.dtype = torch.float8_e8m0fnu) -> tuple[torch.Tensor, torch.Tensor]:
+    """``rms_norm`` rounded to fp8 by blocks of 128: codes [T, D] float8_e4m3fn and scales [T, ceil(D / 128)],
+    float32 (amax / 448) or float8_e8m0fnu (the power of two above), the operands of ``fp8_gemm``. ``out`` receives
+    the bf16 norm too when given. ``scale_dtype`` is that of scales that are not given (see dsa_rms_norm)."""
+    codes, scales = _new_codes(x, codes, scales, scale_dtype)
+    _norm(x, weight, eps, out, residual, residual_out, codes, scales)
+    return codes, scales
+
+
+def act_quant(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None, *,
+              scale_dtype: torch.dtype = torch.float8_e8m0fnu) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [T, D] bf16 (row stride free) rounded to fp8 by blocks of 128, as in ``rms_norm_quant`` (see dsa_act_quant)."""
+    codes, scales = _new_codes(x, codes, scales, scale_dtype)
+    stride = _rows2d(x, "x", _BF16)
+    rows, dim = x.shape
+    code_stride, scale_stride, kind = _coded(rows, dim, codes, scales)
+    _launch(_gpu(x, codes, scales), "dsa_act_quant", x.data_ptr(), stride, rows, dim, codes.data_ptr(), code_stride,
+            scales.data_ptr(), scale_stride, kind)
+    return codes, scales
+
+
+def fp8_gemm_workspace_bytes(m: int, n: int, k: int) -> int:
+    return int(_lib.load().dsa_fp8_gemm_workspace_bytes(int(m), int(n), int(k)))
+
+
+def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+             out: torch.Tensor | None = None, *, out_dtype: torch.dtype = torch.bfloat16,
+             workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """out [M, N] = a @ b.T of block-scaled fp8 matrices: a [M, K] with a_scale [M, ceil(K / 128)], b [N, K] with
+    b_scale [ceil(N / 128), ceil(K / 128)], both scales float32 or both float8_e8m0fnu (uint8: the same bytes). out
+    is bf16 or float32 (``out_dtype`` when it is not given). K a multiple of 16 (see dsa_fp8_gemm)."""
+    a_stride, b_stride = _rows2d(a, "a", _FP8_TYPES), _rows2d(b, "b", _FP8_TYPES)
+    (M, K), (N, Kb) = a.shape, b.shape
+    if K != Kb:
+        _fail(f"a and b must share K, got {K} and {Kb}")
+    kind = _SCALE_KINDS.get(a_scale.dtype)
+    if kind is None or kind != _SCALE_KINDS.get(b_scale.dtype):
+        _fail(f"a_scale and b_scale must both be float32 or both float8_e8m0fnu, got {a_scale.dtype} and {b_scale.dtype}")
+    blocks = -(-K // FP8_BLOCK)
+    sa_stride = _rows2d(a_scale, "a_scale", _SCALE_KINDS, (M, blocks))
+    sb_stride = _rows2d(b_scale, "b_scale", _SCALE_KINDS, (-(-N // FP8_BLOCK), blocks))
+    dev = _gpu(a, a_scale, b, b_scale)
+    if out is None:
+        if out_dtype not in (torch.bfloat16, torch.float32):
+            _fail(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
+        out = a.new_empty((M, N), dtype=out_dtype)
+        out_stride = N
+    else:
+        out_stride = _rows2d(out, "out", (torch.bfloat16, torch.float32), (M, N))
+        _gpu(a, out)
+    if dev == _CURRENT_DEVICE():
+        need = (_lib._lib or _lib.load()).dsa_fp8_gemm_workspace_bytes(M, N, K)
+    else:  # the size goes by the current device's CUs
+        with torch.cuda.device(dev):
+            need = fp8_gemm_workspace_bytes(M, N, K)
+    ws_ptr, ws_bytes = None, 0
+    if need:
+        if (workspace is None or workspace.numel() * workspace.element_size() < need or workspace.data_ptr() % 16
+                or workspace.get_device() != dev):
+            workspace = a.new_empty((need,), dtype=torch.uint8)
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _launch(dev, "dsa_fp8_gemm", a.data_ptr(), a_stride, a_scale.data_ptr(), sa_stride, b.data_ptr(), b_stride,
+            b_scale.data_ptr(), sb_stride, kind, M, N, K, out.data_ptr(), out_stride, int(out.dtype is torch.float32),
+            ws_ptr, ws_bytes)
+    return out
+
+
+def _heads3d(t: torch.Tensor, name: str, shape=None) -> tuple[int, int]:
+    """(token stride, head stride) of a bf16 tensor [T, H, rot] with a contiguous last dim."""
+    s, st = t.shape, t.stride()
+    if not (len(s) == 3 and t.dtype is torch.bfloat16 and (st[2] == 1 or s[2] == 1) and (shape is None or s == shape)):
+        want = "[T, H, rot_dim]" if shape is None else str(list(shape))
+        _fail(f"{name} must be bfloat16 {want} with a contiguous last dim, got {t.dtype} {tuple(s)}")
+    # torch leaves the stride of a single head or token free
+    head = st[1] if s[1] > 1 else s[2]
+    return (st[0] if s[0] > 1 else s[1] * head), head
+
+
+def rope(q: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor, out: torch.Tensor | None = None, *,
+         k: torch.Tensor | None = None, k_out: torch.Tensor | None = None, interleaved: bool = True,
+         out_interleaved: bool | None = None):
+    """Rotary positions of q [T, H, rot_dim] bf16, the rotated part of each head (token and head strides free: a
+    slice of wider heads), and of k [T, Hk, rot_dim] in the same launch. cos_sin_cache [max_pos, rot_dim] f32 =
+    [cos | sin] (``rotary.cos_sin_cache``); positions [T] int32 or int64, clamped to it. Pairs lie beside each
+    other (``interleaved``) or in halves, in the output as in the input unless ``out_interleaved`` says
+    otherwise. ``out`` and ``k_out`` default to q and k (in place). Returns out, or (out, k_out) (see dsa_rope)."""
+    q_t, q_h = _heads3d(q, "q")
+    T, H, rot = q.shape
+    if out is None or out is q:
+        out, o_t, o_h = q, q_t, q_h
+    else:
+        o_t, o_h = _heads3d(out, "out", q.shape)
+    table = cos_sin_cache if cos_sin_cache.dim() == 2 else cos_sin_cache.reshape(cos_sin_cache.shape[0], -1)
+    if not (table.shape[1] == rot and table.dtype is torch.float32 and table.is_contiguous()):
+        _fail(f"cos_sin_cache must be contiguous float32 [max_pos, {rot}], got {table.dtype} {tuple(cos_sin_cache.shape)}")
+    pos, wide = _positions(positions, T)
+    tensors = [q, out, table, pos]
+    k_args = (None, 0, 0, 0, None, 0, 0)
+    if k is not None:
+        k_t, k_h = _heads3d(k, "k")
+        Hk = k.shape[1]
+        if k.shape != (T, Hk, rot):
+            _fail(f"k must be bfloat16 [{T}, Hk, {rot}], got {tuple(k.shape)}")
+        if k_out is None or k_out is k:
+            k_out, ko_t, ko_h = k, k_t, k_h
+        else:
+            ko_t, ko_h = _heads3d(k_out, "k_out", k.shape)
+        tensors += (k, k_out)
+        k_args = (k.data_ptr(), k_t, k_h, Hk, k_out.data_ptr(), ko_t, ko_h)
+    elif k_out is not None:
+        _fail("k_out needs k")
+    _launch(_gpu(*tensors), "dsa_rope", q.data_ptr(), q_t, q_h, H, out.data_ptr(), o_t, o_h, *k_args, T, rot,
+            table.data_ptr(), table.shape[0], pos.data_ptr(), wide, int(bool(interleaved)),
+            int(bool(interleaved if out_interleaved is None else out_interleaved)))
+    return out if k is None else (out, k_out)
