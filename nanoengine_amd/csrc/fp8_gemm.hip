@@ -36,14 +36,23 @@ struct GemmParams {
   int64_t out_stride;
 };
 
-// What rows' pieces past the end of K are read from.
-__device__ __align__(16) const uint8_t g_gemm_zero[16] = {};
-
-__device__ __forceinline__ void dma16(const void* g, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+// 16 bytes a lane from base + offset into LDS at lds + 16 * lane, without registers; the kernel
+// waits for them itself (vmcnt).
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base),
+               "{m0}"(__builtin_amdgcn_readfirstlane(lds))
                : "memory");
 }
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)reinterpret_cast<uintptr_t>(p); }
+
+// All of this wave's loads and LDS accesses are done, then all waves' are. (The wait is a builtin:
+// the compiler's own counting of what is under way starts anew behind it.)
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 enum OutKind : int { kOutBf16 = 0, kOutF32 = 1 };
 
@@ -74,16 +83,55 @@ __device__ __forceinline__ void store4(void* out, int64_t at, bool whole, int le
   }
 }
 
+// Bytes of a tile's activation scales that lie in LDS at a time, two such chunks: 32 e8m0 or
+// 8 f32 blocks of each row. Rows are 36 bytes apart, so that 32 rows' reads of one block fall
+// on different banks.
+constexpr int kMaxStride = 1 << 23;  // a tile's offsets are 32-bit
+constexpr int kScaleChunk = 32, kScaleRow = 36;
+
+template <int BM, int BN>
+constexpr int gemm_smem() {
+  return 2 * (BM + BN) * kBlock + 2 * BM * kScaleRow;
+}
+
+// 16 bytes of scales from element i of a row of n, at any address.
+template <int KIND>
+__device__ __forceinline__ v4i load_scale_piece(const void* row, int i, int n) {
+  constexpr int kSize = KIND == kScaleF32 ? 4 : 1;
+  const uint8_t* p = static_cast<const uint8_t*>(row) + (int64_t)i * kSize;
+  v4i v = {0, 0, 0, 0};
+  if (i + 16 / kSize <= n) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (KIND == kScaleF32) {
+        if (i + j < n) v[j] = reinterpret_cast<const int*>(p)[j];
+      } else {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (i + 4 * j + b < n) v[j] |= (int)((uint32_t)p[4 * j + b] << (8 * b));
+      }
+  }
+  return v;
+}
+
 // A tile of BM activation rows and BN weight rows; a wave takes WM x WN of it.
+//
+// Operands are read from LDS a few products ahead of those that run. Where the reads
+// of block s end and those of block s + 1 begin, the waves meet, once a block: all have read block
+// s by then, and block s + 1 has landed; block s + 2 is sent for in block s's place.
 template <int BM, int BN, int WM, int WN, int KIND, int OUT>
-__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) fp8_gemm_kernel(const GemmParams P) {
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) __attribute__((amdgpu_waves_per_eu(2)))
+fp8_gemm_kernel(const GemmParams P) {
   constexpr int kWaves = (BM / WM) * (BN / WN);
   constexpr int kMt = WM / 32, kNt = WN / 32;
   constexpr int kStage = (BM + BN) * kBlock;
-  constexpr int kLoads = (BM + BN) / 8;            // instructions of a stage: eight rows each
-  constexpr int kPer = (kLoads + kWaves - 1) / kWaves;
-  static_assert(kLoads % kWaves == 0 && BM % 8 == 0, "rows dealt out evenly");
+  constexpr int kPerA = BM / 8 / kWaves, kPerB = BN / 8 / kWaves;  // instructions of a stage: eight rows each
+  constexpr int kScales = KIND == kScaleF32 ? kScaleChunk / 4 : kScaleChunk;
+  static_assert(kPerA * kWaves * 8 == BM && kPerB * kWaves * 8 == BN, "rows dealt out evenly");
   static_assert(kBlock % WN == 0, "one weight scale a wave");
+  static_assert(2 * BM <= kWaves * 64, "a piece of a scale chunk a thread");
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = blockIdx.x % (P.mtiles * P.ntiles), split = blockIdx.x / (P.mtiles * P.ntiles);
@@ -92,111 +140,179 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) fp8_gemm_kernel(co
   const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
   const int c32 = lane & 31, half = lane >> 5;
 
-  // this lane's pieces of a stage; rows past the matrix repeat its last one
-  const uint8_t* src[kPer];
+  // this lane's pieces of a stage, from the tile's first row on; rows past the matrix repeat its last one
+  uint32_t off_a[kPerA], off_b[kPerB];
   const int piece = (lane & 7) ^ (lane >> 3);
+  auto offset = [&](int i, int last, int64_t stride) {
+    uint32_t v = (uint32_t)min(8 * (wave + i * kWaves) + (lane >> 3), last) * (uint32_t)stride + 16 * piece;
+    asm volatile("" : "+v"(v));  // (one register, not the pair of a 64-bit product)
+    return v;
+  };
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int row = 8 * (wave + i * kWaves) + (lane >> 3);
-    src[i] = row < BM ? P.a + (int64_t)min(m0 + row, P.m - 1) * P.a_stride
-                      : P.b + (int64_t)min(n0 + row - BM, P.n - 1) * P.b_stride;
-    src[i] += 16 * piece;
-  }
+  for (int i = 0; i < kPerA; ++i) off_a[i] = offset(i, P.m - 1 - m0, P.a_stride);
+#pragma unroll
+  for (int i = 0; i < kPerB; ++i) off_b[i] = offset(i, P.n - 1 - n0, P.b_stride);
+  const uint8_t* tile_a = P.a + (int64_t)m0 * P.a_stride;
+  const uint8_t* tile_b = P.b + (int64_t)n0 * P.b_stride;
   auto issue = [&](int kb, int buf) {
     const uint32_t dst = lds_addr(smem) + buf * kStage + wave * 1024;
-    const bool there = kb * kBlock + 16 * piece < P.k;
+    const uint8_t *pa = tile_a + (int64_t)kb * kBlock, *pb = tile_b + (int64_t)kb * kBlock;
+    auto copy = [&] {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      dma16(there ? src[i] + (int64_t)kb * kBlock : g_gemm_zero, dst + i * kWaves * 1024);
+      for (int i = 0; i < kPerA; ++i) dma16(pa, off_a[i], dst + i * kWaves * 1024);
+#pragma unroll
+      for (int i = 0; i < kPerB; ++i) dma16(pb, off_b[i], dst + BM * kBlock + i * kWaves * 1024);
+    };
+    if ((kb + 1) * kBlock <= P.k) {
+      copy();
+    } else if (kb * kBlock + 16 * piece < P.k) {
+      copy();
+    } else {  // past the end of K: zeros
+      uint8_t* z = smem + buf * kStage + wave * 1024 + lane * 16;
+#pragma unroll
+      for (int i = 0; i < kPerA + kPerB; ++i) *reinterpret_cast<v4i*>(z + i * kWaves * 1024) = (v4i){0, 0, 0, 0};
+    }
   };
 
-  int64_t sa_at[kMt];
+  // activation scales: thread 2 r + h brings half h of a chunk of row r. (Its addresses are made anew from an
+  // opaque copy of the thread's number: kept in registers they would be spilled.)
+  uint8_t* scale_lds = smem + 2 * kStage;
+  const bool brings = 2 * BM == kWaves * 64 || (int)threadIdx.x < 2 * BM;
+  auto load_chunk = [&](int kb) {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    const int64_t row = (int64_t)min(m0 + t / 2, P.m - 1) * P.sa_stride;
+    return load_scale_piece<KIND>(KIND == kScaleF32 ? (const void*)(static_cast<const uint32_t*>(P.sa) + row)
+                                                    : (const void*)(static_cast<const uint8_t*>(P.sa) + row),
+                                  kb + (t & 1) * (kScales / 2), P.kblocks);
+  };
+  auto keep_chunk = [&](v4i v, int c) {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    uint32_t* d = reinterpret_cast<uint32_t*>(scale_lds + c * BM * kScaleRow + (t / 2) * kScaleRow + (t & 1) * 16);
 #pragma unroll
-  for (int i = 0; i < kMt; ++i) sa_at[i] = (int64_t)min(m0 + wm + 32 * i + c32, P.m - 1) * P.sa_stride;
+    for (int j = 0; j < 4; ++j) d[j] = (uint32_t)v[j];
+  };
+  // the scale of this lane's row in activation tile j at block kb
+  auto row_scale = [&](int step, int j) -> uint32_t {
+    const uint8_t* p = scale_lds + ((step / kScales) & 1) * BM * kScaleRow + (wm + 32 * j + c32) * kScaleRow;
+    return KIND == kScaleF32 ? reinterpret_cast<const uint32_t*>(p)[step % kScales] : (uint32_t)p[step % kScales];
+  };
+  // the wave's one weight scale of a block, read two blocks ahead
   const int64_t sb_at = (int64_t)min((n0 + wn) / kBlock, (P.n - 1) / kBlock) * P.sb_stride;
-  uint32_t sa[kMt], sb;
-  auto load_scales = [&](int kb) {
-#pragma unroll
-    for (int i = 0; i < kMt; ++i) sa[i] = load_scale<KIND>(P.sa, sa_at[i] + kb);
-    sb = load_scale<KIND>(P.sb, sb_at + kb);
-  };
 
-  v16f acc[kNt][kMt];
+  v16f acc[kNt][kMt], part[kNt][kMt];
 #pragma unroll
   for (int i = 0; i < kNt; ++i)
 #pragma unroll
     for (int j = 0; j < kMt; ++j) acc[i][j] = (v16f){};
 
-  // offsets of this lane's two 16-byte pieces of each 64-deep half of a row
-  uint32_t off[2][2];
-#pragma unroll
-  for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) off[ks][j] = c32 * kBlock + 16 * ((4 * ks + 2 * half + j) ^ (lane & 7));
+  // this lane's two 16-byte pieces of half h of a row: at0 ^ 64 h and that ^ 16
+  const uint32_t at0 = c32 * kBlock + 16 * ((2 * half) ^ (lane & 7));
+  auto operand = [&](int buf, int row, int h) {
+    const uint8_t* rows = smem + (buf * kStage + row * kBlock);
+    const v4i x = *reinterpret_cast<const v4i*>(rows + (at0 ^ (64 * h))), y = *reinterpret_cast<const v4i*>(rows + (at0 ^ (64 * h + 16)));
+    return (v8i){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  };
+  // A step's groups: half h of activation tile j times all weight tiles. Group g's activations lie in
+  // slot g % kSlots and are read kAhead groups before; weights a half before.
+  constexpr int kGroups = 2 * kMt, kAhead = kMt == 4 ? 3 : kMt, kSlots = kMt == 4 ? 4 : kGroups;
+  v8i fa[kSlots], fb[2][kNt];
+  // scales of this block, and of the next ones; those of four tiles are replaced one by one behind their last use
+  constexpr bool kEach = kAhead < kMt;
+  uint32_t ca[kMt], na[kMt], cb, cb1, cb2;
 
-  if (kb0 < kb1) {
-    load_scales(kb0);
+  const int steps = kb1 - kb0;
+  if (steps > 0) {
     issue(kb0, 0);
+    if (brings) keep_chunk(load_chunk(kb0), 0);
+    cb = load_scale<KIND>(P.sb, sb_at + kb0);
+    cb1 = load_scale<KIND>(P.sb, sb_at + min(kb0 + 1, kb1 - 1));
+    cb = __builtin_amdgcn_readfirstlane(cb);
+    cb1 = __builtin_amdgcn_readfirstlane(cb1);
+    meet();
+    if (steps > 1) issue(kb0 + 1, 1);
+#pragma unroll
+    for (int i = 0; i < kNt; ++i) fb[0][i] = operand(0, BM + wn + 32 * i, 0);
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) fa[g % kSlots] = operand(0, wm + 32 * (g % kMt), g / kMt);
+#pragma unroll
+    for (int j = 0; j < kMt; ++j) ca[j] = row_scale(0, j);
   }
-  for (int kb = kb0; kb < kb1; ++kb) {
-    const int buf = (kb - kb0) & 1;
-    // this wave's share of the block has landed and its reads of the other buffer are done; past
-    // the barrier so are the others'
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    uint32_t ca[kMt], cb;  // this block's scales, read one block ahead
+  // What the epilogue needs is loaded, and waited for, before the loop: with a scalar load under way the
+  // compiler would wait for every LDS read at each step's first product.
+  void* out = P.out;
+  int64_t out_stride = P.out_stride;
+  asm volatile("" : "+s"(out), "+s"(out_stride));
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  for (int s = 0; s < steps; ++s) {
+    const int buf = s & 1;
+    const bool chunk = s % kScales == 0 && s + kScales < steps;
+    v4i next_chunk;
 #pragma unroll
-    for (int i = 0; i < kMt; ++i) {
-      asm volatile("" : "+v"(sa[i]));
-      ca[i] = sa[i];
-    }
-    asm volatile("" : "+v"(sb));
-    cb = sb;
-    if (kb + 1 < kb1) {
-      load_scales(kb + 1);
-      issue(kb + 1, buf ^ 1);
-    }
-    const uint8_t* at = smem + buf * kStage + wm * kBlock;
-    const uint8_t* bt = smem + buf * kStage + (BM + wn) * kBlock;
-    auto operand = [&](const uint8_t* base, int ks) {
-      const v4i x = *reinterpret_cast<const v4i*>(base + off[ks][0]), y = *reinterpret_cast<const v4i*>(base + off[ks][1]);
-      return (v8i){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-    };
-    v8i fa[kMt][2], fb[kNt][2];
+    for (int g = 0; g < kGroups; ++g) {
+      const int h = g / kMt, j = g % kMt;
+      if (g == 0) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
+        for (int i = 0; i < kNt; ++i) fb[1][i] = operand(buf, BM + wn + 32 * i, 1);
+        if (chunk && brings) next_chunk = load_chunk(kb0 + s + kScales);
+        cb2 = load_scale<KIND>(P.sb, sb_at + min(kb0 + s + 2, kb1 - 1));
+      }
+      if (g == kGroups - kAhead) {
+        // this wave has read all of the block, and its share of the next has landed; past the barrier
+        // that holds for all (behind the last block nothing has been sent: what is read then is not used).
+        // The products before it stay before it: without a use there the compiler moves them past the branches.
 #pragma unroll
-      for (int i = 0; i < kNt; ++i) fb[i][ks] = operand(bt + i * 32 * kBlock, ks);
+        for (int i = 0; i < kNt; ++i)
 #pragma unroll
-      for (int j = 0; j < kMt; ++j) fa[j][ks] = operand(at + j * 32 * kBlock, ks);
-    }
-    if (KIND == kScaleE8M0) {
+          for (int t = 0; t < kMt; ++t) {
+            if (KIND == kScaleE8M0) asm volatile("" : "+v"(acc[i][t]));
+            else asm volatile("" : "+v"(part[i][t]));
+          }
+        meet();
+        cb2 = __builtin_amdgcn_readfirstlane(cb2);
+        if (chunk && brings) keep_chunk(next_chunk, ((s / kScales) & 1) ^ 1);
+        if (s + 2 < steps) issue(kb0 + s + 2, buf);
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
+        for (int i = 0; i < kNt; ++i) fb[0][i] = operand(buf ^ 1, BM + wn + 32 * i, 0);
+        if (!kEach) {
 #pragma unroll
-        for (int j = 0; j < kMt; ++j)
-#pragma unroll
-          for (int i = 0; i < kNt; ++i)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[i][ks], fa[j][ks], acc[i][j], 0, 0, 0, cb, 0,
-                                                                        ca[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kMt; ++j) {
-        const float s = __uint_as_float(ca[j]) * __uint_as_float(cb);
-#pragma unroll
-        for (int i = 0; i < kNt; ++i) {
-          v16f part = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[i][0], fa[j][0], (v16f){}, 0, 0, 0, 127, 0, 127);
-          part = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[i][1], fa[j][1], part, 0, 0, 0, 127, 0, 127);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] += part[r] * s;
+          for (int t = 0; t < kMt; ++t) na[t] = row_scale(s + 1, t);
         }
       }
+      if (kEach && g >= kGroups - kAhead) ca[g - (kGroups - kAhead)] = row_scale(s + 1, g - (kGroups - kAhead));
+      if (kEach && g == 0) ca[kMt - 1] = row_scale(s, kMt - 1);
+      const int t = g + kAhead;
+      fa[t % kSlots] = t < kGroups ? operand(buf, wm + 32 * (t % kMt), t / kMt) : operand(buf ^ 1, wm + 32 * (t % kMt), 0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kNt; ++i) {
+        if (KIND == kScaleE8M0)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h][i], fa[g % kSlots], acc[i][j], 0, 0, 0, cb, 0, ca[j]);
+        else
+          part[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h][i], fa[g % kSlots], h ? part[i][j] : (v16f){}, 0, 0,
+                                                                       0, 127, 0, 127);
+      }
+      if (KIND == kScaleF32 && h == 1) {
+        const float f = __uint_as_float(ca[j]) * __uint_as_float(cb);
+#pragma unroll
+        for (int i = 0; i < kNt; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] += part[i][j][r] * f;
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    if (!kEach) {
+#pragma unroll
+      for (int j = 0; j < kMt; ++j) ca[j] = na[j];
+    }
+    cb = cb1;
+    cb1 = cb2;
   }
 
   // lane (c32, half): row c32 of an activation tile, columns 8g + 4 half .. + 3 of a weight tile
-  void* out = P.out;
-  if (P.splits > 1) out = static_cast<float*>(P.out) + (int64_t)split * P.m * P.n;
-  const bool aligned = !((reinterpret_cast<uintptr_t>(out) & (OUT == kOutBf16 ? 7 : 15)) | (P.out_stride & 3));
+  if (P.splits > 1) out = static_cast<float*>(out) + (int64_t)split * P.m * P.n;
+  const bool aligned = !((reinterpret_cast<uintptr_t>(out) & (OUT == kOutBf16 ? 7 : 15)) | (out_stride & 3));
 #pragma unroll
   for (int j = 0; j < kMt; ++j) {
     const int m = m0 + wm + 32 * j + c32;
@@ -207,7 +323,7 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) fp8_gemm_kernel(co
       for (int g = 0; g < 4; ++g) {
         const int n = n0 + wn + 32 * i + 8 * g + 4 * half;
         const float v[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        if (n < P.n) store4<OUT>(out, (int64_t)m * P.out_stride + n, aligned && n + 4 <= P.n, P.n - n, v);
+        if (n < P.n) store4<OUT>(out, (int64_t)m * out_stride + n, aligned && n + 4 <= P.n, P.n - n, v);
       }
   }
 }
@@ -266,7 +382,7 @@ int device_cus() {
 
 template <int BM, int BN, int WM, int WN, int KIND, int OUT>
 int launch_tile(GemmParams P, hipStream_t st) {
-  constexpr int kSmem = 2 * (BM + BN) * kBlock;
+  constexpr int kSmem = gemm_smem<BM, BN>();
   auto kern = fp8_gemm_kernel<BM, BN, WM, WN, KIND, OUT>;
   if (kSmem > 64 * 1024) {
     const hipError_t e =
@@ -283,7 +399,8 @@ int launch_tile(GemmParams P, hipStream_t st) {
 
 template <int KIND, int OUT>
 int launch_plan(const Plan& p, const GemmParams& P, hipStream_t st) {
-  if (p.bm == 256) return launch_tile<256, 256, 128, 64, KIND, OUT>(P, st);
+  // f32 scales take a second set of accumulators: narrower tiles
+  if (p.bm == 256) return KIND == kScaleE8M0 ? launch_tile<256, 256, 128, 64, kScaleE8M0, OUT>(P, st) : launch_tile<256, 128, 64, 64, kScaleF32, OUT>(P, st);
   if (p.bm == 128) return launch_tile<128, 128, 64, 64, KIND, OUT>(P, st);
   if (p.bm == 64) return launch_tile<64, 128, 64, 32, KIND, OUT>(P, st);
   return launch_tile<32, 64, 32, 32, KIND, OUT>(P, st);
@@ -318,6 +435,8 @@ int dsa_fp8_gemm(const uint8_t* a, int64_t a_stride, const void* a_scale, int64_
     return set_error(kInvalidArgument, "dsa_fp8_gemm: rows overlap");
   if (((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) || ((a_stride | b_stride) & 15))
     return set_error(kInvalidArgument, "dsa_fp8_gemm: rows of a and b must be 16-byte aligned");
+  if ((m > 1 && a_stride > kMaxStride) || (n > 1 && b_stride > kMaxStride))
+    return set_error(kUnsupported, "dsa_fp8_gemm: rows more than %d bytes apart", kMaxStride);
   if ((scale_kind == kScaleF32 && ((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(b_scale)) & 3)) ||
       (reinterpret_cast<uintptr_t>(out) & (out_is_f32 ? 3 : 1)))
     return set_error(kInvalidArgument, "dsa_fp8_gemm: pointers must be aligned to their elements");
@@ -327,7 +446,7 @@ int dsa_fp8_gemm(const uint8_t* a, int64_t a_stride, const void* a_scale, int64_
     return set_error(kWorkspaceTooSmall, "dsa_fp8_gemm: workspace %zu bytes, %zu needed", workspace_bytes, need);
   if (need && (reinterpret_cast<uintptr_t>(workspace) & 15))
     return set_error(kInvalidArgument, "dsa_fp8_gemm: the workspace must be 16-byte aligned");
-  GemmParams P = {a, b, a_stride, b_stride, a_scale, b_scale, a_scale_stride, b_scale_stride, m, n, k, kblocks,
+  GemmParams P = {a, b, m > 1 ? a_stride : k, n > 1 ? b_stride : k, a_scale, b_scale, a_scale_stride, b_scale_stride, m, n, k, kblocks,
                   0, 0, p.splits, out, out_stride};
   const hipStream_t st = (hipStream_t)stream;
   if (p.splits > 1) {
