@@ -9,8 +9,8 @@
 // a lane ends up with one activation row's results for four neighbouring columns at a time.
 // A workgroup's tiles of a and b go straight from HBM into LDS, a block of 128 deep, two
 // buffers deep: while one is multiplied the next is on its way. A row's eight 16-byte pieces
-// are stored in the order piece ^ (row & 7): eight rows' reads of one piece fall on
-// different banks.
+// are stored in the order piece ^ (row / 2 % 8): 16 rows' reads of one piece fall on different banks
+// (rows are half the banks' span apart; with row % 8 two of 16 met on each bank).
 #include <algorithm>
 
 #include "dsa_common.h"
@@ -36,20 +36,22 @@ struct GemmParams {
   int64_t out_stride;
 };
 
-// 16 bytes a lane from base + offset into LDS at lds + 16 * lane, without registers; the kernel
-// waits for them itself (vmcnt).
-__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base),
-               "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+// 16 bytes from base + offset into LDS at lds + 16 * lane, for the lanes in `mask`, without registers; the
+// kernel waits for them itself (vmcnt). To be called with every lane active.
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t offset, uint32_t lds, uint64_t mask) {
+  asm volatile("s_mov_b64 exec, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1" ::"v"(offset),
+               "s"(base), "s"(mask), "{m0}"(__builtin_amdgcn_readfirstlane(lds))
                : "memory");
 }
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)reinterpret_cast<uintptr_t>(p); }
 
-// All of this wave's loads and LDS accesses are done, then all waves' are. (The wait is a builtin:
+// All of this wave's loads but the last LEFT and its LDS accesses are done, then all waves' are. (The wait is a builtin:
 // the compiler's own counting of what is under way starts anew behind it.)
+template <int LEFT>
 __device__ __forceinline__ void meet() {
+  static_assert(LEFT < 16, "low bits of the count");
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0);
+  __builtin_amdgcn_s_waitcnt(LEFT);
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -130,6 +132,7 @@ fp8_gemm_kernel(const GemmParams P) {
   constexpr int kPerA = BM / 8 / kWaves, kPerB = BN / 8 / kWaves;  // instructions of a stage: eight rows each
   constexpr int kScales = KIND == kScaleF32 ? kScaleChunk / 4 : kScaleChunk;
   static_assert(kPerA * kWaves * 8 == BM && kPerB * kWaves * 8 == BN, "rows dealt out evenly");
+  static_assert(kWaves % 2 == 0, "a wave's rows of a stage have one order of pieces");
   static_assert(kBlock % WN == 0, "one weight scale a wave");
   static_assert(2 * BM <= kWaves * 64, "a piece of a scale chunk a thread");
   extern __shared__ __align__(16) uint8_t smem[];
@@ -142,7 +145,7 @@ fp8_gemm_kernel(const GemmParams P) {
 
   // this lane's pieces of a stage, from the tile's first row on; rows past the matrix repeat its last one
   uint32_t off_a[kPerA], off_b[kPerB];
-  const int piece = (lane & 7) ^ (lane >> 3);
+  const int piece = (lane & 7) ^ (4 * (wave & 1) + (lane >> 4));
   auto offset = [&](int i, int last, int64_t stride) {
     uint32_t v = (uint32_t)min(8 * (wave + i * kWaves) + (lane >> 3), last) * (uint32_t)stride + 16 * piece;
     asm volatile("" : "+v"(v));  // (one register, not the pair of a 64-bit product)
@@ -154,24 +157,32 @@ fp8_gemm_kernel(const GemmParams P) {
   for (int i = 0; i < kPerB; ++i) off_b[i] = offset(i, P.n - 1 - n0, P.b_stride);
   const uint8_t* tile_a = P.a + (int64_t)m0 * P.a_stride;
   const uint8_t* tile_b = P.b + (int64_t)n0 * P.b_stride;
-  auto issue = [&](int kb, int buf) {
-    const uint32_t dst = lds_addr(smem) + buf * kStage + wave * 1024;
-    const uint8_t *pa = tile_a + (int64_t)kb * kBlock, *pb = tile_b + (int64_t)kb * kBlock;
-    auto copy = [&] {
-#pragma unroll
-      for (int i = 0; i < kPerA; ++i) dma16(pa, off_a[i], dst + i * kWaves * 1024);
-#pragma unroll
-      for (int i = 0; i < kPerB; ++i) dma16(pb, off_b[i], dst + BM * kBlock + i * kWaves * 1024);
-    };
-    if ((kb + 1) * kBlock <= P.k) {
-      copy();
-    } else if (kb * kBlock + 16 * piece < P.k) {
-      copy();
-    } else {  // past the end of K: zeros
+  // the lanes of a copy of block kb whose pieces lie inside K
+  auto lanes_of = [&](int kb) -> uint64_t {
+    return (kb + 1) * kBlock <= P.k ? ~0ull : __builtin_amdgcn_ballot_w64(kb * kBlock + 16 * piece < P.k);
+  };
+  const uint32_t dst0 = lds_addr(smem) + wave * 1024;
+  auto issue_a = [&](int kb, int buf, int i, uint64_t mask) {
+    dma16(tile_a + (int64_t)kb * kBlock, off_a[i], dst0 + buf * kStage + i * kWaves * 1024, mask);
+  };
+  auto issue_b = [&](int kb, int buf, int i, uint64_t mask) {
+    dma16(tile_b + (int64_t)kb * kBlock, off_b[i], dst0 + buf * kStage + BM * kBlock + i * kWaves * 1024, mask);
+  };
+  // zeros where a block lies past the end of K
+  auto clear_tail = [&](int kb, int buf) {
+    if (kb * kBlock + 16 * piece >= P.k) {
       uint8_t* z = smem + buf * kStage + wave * 1024 + lane * 16;
 #pragma unroll
       for (int i = 0; i < kPerA + kPerB; ++i) *reinterpret_cast<v4i*>(z + i * kWaves * 1024) = (v4i){0, 0, 0, 0};
     }
+  };
+  auto issue = [&](int kb, int buf) {
+    const uint64_t mask = lanes_of(kb);
+#pragma unroll
+    for (int i = 0; i < kPerA; ++i) issue_a(kb, buf, i, mask);
+#pragma unroll
+    for (int i = 0; i < kPerB; ++i) issue_b(kb, buf, i, mask);
+    if (mask != ~0ull) clear_tail(kb, buf);
   };
 
   // activation scales: thread 2 r + h brings half h of a chunk of row r. (Its addresses are made anew from an
@@ -198,8 +209,9 @@ fp8_gemm_kernel(const GemmParams P) {
     const uint8_t* p = scale_lds + ((step / kScales) & 1) * BM * kScaleRow + (wm + 32 * j + c32) * kScaleRow;
     return KIND == kScaleF32 ? reinterpret_cast<const uint32_t*>(p)[step % kScales] : (uint32_t)p[step % kScales];
   };
-  // the wave's one weight scale of a block, read two blocks ahead
+  // a chunk of the wave's one weight scale a block, a lane each
   const int64_t sb_at = (int64_t)min((n0 + wn) / kBlock, (P.n - 1) / kBlock) * P.sb_stride;
+  auto load_weight_scales = [&](int kb) { return load_scale<KIND>(P.sb, sb_at + min(kb + lane % kScales, P.kblocks - 1)); };
 
   v16f acc[kNt][kMt], part[kNt][kMt];
 #pragma unroll
@@ -208,7 +220,7 @@ fp8_gemm_kernel(const GemmParams P) {
     for (int j = 0; j < kMt; ++j) acc[i][j] = (v16f){};
 
   // this lane's two 16-byte pieces of half h of a row: at0 ^ 64 h and that ^ 16
-  const uint32_t at0 = c32 * kBlock + 16 * ((2 * half) ^ (lane & 7));
+  const uint32_t at0 = c32 * kBlock + 16 * ((2 * half) ^ ((lane >> 1) & 7));
   auto operand = [&](int buf, int row, int h) {
     const uint8_t* rows = smem + (buf * kStage + row * kBlock);
     const v4i x = *reinterpret_cast<const v4i*>(rows + (at0 ^ (64 * h))), y = *reinterpret_cast<const v4i*>(rows + (at0 ^ (64 * h + 16)));
@@ -220,17 +232,16 @@ fp8_gemm_kernel(const GemmParams P) {
   v8i fa[kSlots], fb[2][kNt];
   // scales of this block, and of the next ones; those of four tiles are replaced one by one behind their last use
   constexpr bool kEach = kAhead < kMt;
-  uint32_t ca[kMt], na[kMt], cb, cb1, cb2;
+  constexpr bool kSpread = kMt == 4;  // copies sent between the products
+  uint32_t ca[kMt], na[kMt], cb, sb = 0, sb_next = 0;
 
   const int steps = kb1 - kb0;
   if (steps > 0) {
     issue(kb0, 0);
     if (brings) keep_chunk(load_chunk(kb0), 0);
-    cb = load_scale<KIND>(P.sb, sb_at + kb0);
-    cb1 = load_scale<KIND>(P.sb, sb_at + min(kb0 + 1, kb1 - 1));
-    cb = __builtin_amdgcn_readfirstlane(cb);
-    cb1 = __builtin_amdgcn_readfirstlane(cb1);
-    meet();
+    sb = load_weight_scales(kb0);
+    asm volatile("" : "+v"(sb));
+    meet<0>();
     if (steps > 1) issue(kb0 + 1, 1);
 #pragma unroll
     for (int i = 0; i < kNt; ++i) fb[0][i] = operand(0, BM + wn + 32 * i, 0);
@@ -245,18 +256,28 @@ fp8_gemm_kernel(const GemmParams P) {
   int64_t out_stride = P.out_stride;
   asm volatile("" : "+s"(out), "+s"(out_stride));
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+  v4i next_chunk = {0, 0, 0, 0};
   for (int s = 0; s < steps; ++s) {
     const int buf = s & 1;
-    const bool chunk = s % kScales == 0 && s + kScales < steps;
-    v4i next_chunk;
+    const bool more = s + 2 < steps;
+    const uint64_t mask = more ? lanes_of(kb0 + s + 2) : 0ull;
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const int h = g / kMt, j = g % kMt;
       if (g == 0) {
 #pragma unroll
         for (int i = 0; i < kNt; ++i) fb[1][i] = operand(buf, BM + wn + 32 * i, 1);
-        if (chunk && brings) next_chunk = load_chunk(kb0 + s + kScales);
-        cb2 = load_scale<KIND>(P.sb, sb_at + min(kb0 + s + 2, kb1 - 1));
+        cb = __builtin_amdgcn_readlane(sb, s % kScales);
+      }
+      if (kSpread && g == 2) {
+        // every wave has read the block's weights (behind them two reads are under way): those of block
+        // s + 2 take their place
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(2)\n\ts_barrier" ::: "memory");
+      }
+      if (kSpread && (g == 2 || g == 3)) {
+#pragma unroll
+        for (int i = (g - 2) * kPerB / 2; i < (g - 1) * kPerB / 2; ++i) issue_b(kb0 + s + 2, buf, i, mask);
       }
       if (g == kGroups - kAhead) {
         // this wave has read all of the block, and its share of the next has landed; past the barrier
@@ -269,16 +290,38 @@ fp8_gemm_kernel(const GemmParams P) {
             if (KIND == kScaleE8M0) asm volatile("" : "+v"(acc[i][t]));
             else asm volatile("" : "+v"(part[i][t]));
           }
-        meet();
-        cb2 = __builtin_amdgcn_readfirstlane(cb2);
-        if (chunk && brings) keep_chunk(next_chunk, ((s / kScales) & 1) ^ 1);
-        if (s + 2 < steps) issue(kb0 + s + 2, buf);
+        if (kSpread && more) meet<kPerB>();  // all but the weights of block s + 2
+        else meet<0>();
+        // the next chunk of scales: sent for at a chunk's first step, kept at its second
+        if (s % kScales == 1) {
+          asm volatile("" : "+v"(sb_next), "+v"(next_chunk));
+          if (brings) keep_chunk(next_chunk, ((s / kScales) & 1) ^ 1);
+        }
+        if (s % kScales == kScales - 1) {
+          sb = sb_next;
+          asm volatile("" : "+v"(sb));  // (a branch: as a select it would wait for loads at every step)
+        }
+        if (s % kScales == 0 && s + kScales < steps) {
+          sb_next = load_weight_scales(kb0 + s + kScales);
+          if (brings) next_chunk = load_chunk(kb0 + s + kScales);
+        }
+        if (more && mask != ~0ull) clear_tail(kb0 + s + 2, buf);
+        if (!kSpread && more) {
+#pragma unroll
+          for (int i = 0; i < kPerA; ++i) issue_a(kb0 + s + 2, buf, i, mask);
+#pragma unroll
+          for (int i = 0; i < kPerB; ++i) issue_b(kb0 + s + 2, buf, i, mask);
+        }
 #pragma unroll
         for (int i = 0; i < kNt; ++i) fb[0][i] = operand(buf ^ 1, BM + wn + 32 * i, 0);
         if (!kEach) {
 #pragma unroll
           for (int t = 0; t < kMt; ++t) na[t] = row_scale(s + 1, t);
         }
+      }
+      if (kSpread && g >= kGroups - 2) {
+#pragma unroll
+        for (int i = (g - kGroups + 2) * kPerA / 2; i < (g - kGroups + 3) * kPerA / 2; ++i) issue_a(kb0 + s + 2, buf, i, mask);
       }
       if (kEach && g >= kGroups - kAhead) ca[g - (kGroups - kAhead)] = row_scale(s + 1, g - (kGroups - kAhead));
       if (kEach && g == 0) ca[kMt - 1] = row_scale(s, kMt - 1);
@@ -306,8 +349,6 @@ fp8_gemm_kernel(const GemmParams P) {
 #pragma unroll
       for (int j = 0; j < kMt; ++j) ca[j] = na[j];
     }
-    cb = cb1;
-    cb1 = cb2;
   }
 
   // lane (c32, half): row c32 of an activation tile, columns 8g + 4 half .. + 3 of a weight tile
