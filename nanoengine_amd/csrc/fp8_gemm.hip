@@ -124,7 +124,7 @@ __device__ __forceinline__ v4i load_scale_piece(const void* row, int i, int n) {
 // of block s end and those of block s + 1 begin, the waves meet, once a block: all have read block
 // s by then, and block s + 1 has landed; block s + 2 is sent for in block s's place.
 template <int BM, int BN, int WM, int WN, int KIND, int OUT>
-__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) __attribute__((amdgpu_waves_per_eu(WM * WN > 128 * 64 ? 1 : 2)))
 fp8_gemm_kernel(const GemmParams P) {
   constexpr int kWaves = (BM / WM) * (BN / WN);
   constexpr int kMt = WM / 32, kNt = WN / 32;
@@ -134,7 +134,8 @@ fp8_gemm_kernel(const GemmParams P) {
   static_assert(kPerA * kWaves * 8 == BM && kPerB * kWaves * 8 == BN, "rows dealt out evenly");
   static_assert(kWaves % 2 == 0, "a wave's rows of a stage have one order of pieces");
   static_assert(kBlock % WN == 0, "one weight scale a wave");
-  static_assert(2 * BM <= kWaves * 64, "a piece of a scale chunk a thread");
+  constexpr int kThreads = kWaves * 64, kPieces = (2 * BM + kThreads - 1) / kThreads;  // of a scale chunk, a thread
+  static_assert(2 * BM % (kPieces * 64) == 0, "whole waves bring scales");
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = blockIdx.x % (P.mtiles * P.ntiles), split = blockIdx.x / (P.mtiles * P.ntiles);
@@ -185,24 +186,35 @@ fp8_gemm_kernel(const GemmParams P) {
     if (mask != ~0ull) clear_tail(kb, buf);
   };
 
-  // activation scales: thread 2 r + h brings half h of a chunk of row r. (Its addresses are made anew from an
+  // activation scales: thread t brings half t % 2 of a chunk of row t / 2. (Its addresses are made anew from an
   // opaque copy of the thread's number: kept in registers they would be spilled.)
   uint8_t* scale_lds = smem + 2 * kStage;
-  const bool brings = 2 * BM == kWaves * 64 || (int)threadIdx.x < 2 * BM;
-  auto load_chunk = [&](int kb) {
-    int t = threadIdx.x;
-    asm volatile("" : "+v"(t));
-    const int64_t row = (int64_t)min(m0 + t / 2, P.m - 1) * P.sa_stride;
-    return load_scale_piece<KIND>(KIND == kScaleF32 ? (const void*)(static_cast<const uint32_t*>(P.sa) + row)
-                                                    : (const void*)(static_cast<const uint8_t*>(P.sa) + row),
-                                  kb + (t & 1) * (kScales / 2), P.kblocks);
+  const bool brings = kPieces * kThreads == 2 * BM || (int)threadIdx.x < 2 * BM;
+  struct Chunk {
+    v4i v[kPieces];
   };
-  auto keep_chunk = [&](v4i v, int c) {
-    int t = threadIdx.x;
-    asm volatile("" : "+v"(t));
-    uint32_t* d = reinterpret_cast<uint32_t*>(scale_lds + c * BM * kScaleRow + (t / 2) * kScaleRow + (t & 1) * 16);
+  auto load_chunk = [&](int kb) {
+    Chunk c;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) d[j] = (uint32_t)v[j];
+    for (int i = 0; i < kPieces; ++i) {
+      int t = threadIdx.x + i * kThreads;
+      asm volatile("" : "+v"(t));
+      const int64_t row = (int64_t)min(m0 + t / 2, P.m - 1) * P.sa_stride;
+      c.v[i] = load_scale_piece<KIND>(KIND == kScaleF32 ? (const void*)(static_cast<const uint32_t*>(P.sa) + row)
+                                                        : (const void*)(static_cast<const uint8_t*>(P.sa) + row),
+                                      kb + (t & 1) * (kScales / 2), P.kblocks);
+    }
+    return c;
+  };
+  auto keep_chunk = [&](const Chunk& c, int which) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      int t = threadIdx.x + i * kThreads;
+      asm volatile("" : "+v"(t));
+      uint32_t* d = reinterpret_cast<uint32_t*>(scale_lds + which * BM * kScaleRow + (t / 2) * kScaleRow + (t & 1) * 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] = (uint32_t)c.v[i][j];
+    }
   };
   // the scale of this lane's row in activation tile j at block kb
   auto row_scale = [&](int step, int j) -> uint32_t {
@@ -256,85 +268,86 @@ fp8_gemm_kernel(const GemmParams P) {
   int64_t out_stride = P.out_stride;
   asm volatile("" : "+s"(out), "+s"(out_stride));
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-  v4i next_chunk = {0, 0, 0, 0};
+  Chunk next_chunk = {};
   for (int s = 0; s < steps; ++s) {
     const int buf = s & 1;
     const bool more = s + 2 < steps;
     const uint64_t mask = more ? lanes_of(kb0 + s + 2) : 0ull;
+    cb = __builtin_amdgcn_readlane(sb, s % kScales);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      const int h = g / kMt, j = g % kMt;
-      if (g == 0) {
+      const int h = g / kMt, j = g % kMt, t = g + kAhead;
 #pragma unroll
-        for (int i = 0; i < kNt; ++i) fb[1][i] = operand(buf, BM + wn + 32 * i, 1);
-        cb = __builtin_amdgcn_readlane(sb, s % kScales);
-      }
-      if (kSpread && g == 2) {
-        // every wave has read the block's weights (behind them two reads are under way): those of block
-        // s + 2 take their place
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt lgkmcnt(2)\n\ts_barrier" ::: "memory");
-      }
-      if (kSpread && (g == 2 || g == 3)) {
+      for (int i = 0; i < kNt; ++i) {  // one product, and what is sent for meanwhile
+        if (kSpread && g == 2 && i == 0) {
+          // every wave has read the block's weights: those of block s + 2 take their place
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+        if (g == kGroups - kAhead && i == 0) {
+          // this wave has read all of the block, and its share of the next has landed; past the barrier
+          // that holds for all (behind the last block nothing has been sent: what is read then is not used).
+          // The products before it stay before it: without a use there the compiler moves them past the branches.
 #pragma unroll
-        for (int i = (g - 2) * kPerB / 2; i < (g - 1) * kPerB / 2; ++i) issue_b(kb0 + s + 2, buf, i, mask);
-      }
-      if (g == kGroups - kAhead) {
-        // this wave has read all of the block, and its share of the next has landed; past the barrier
-        // that holds for all (behind the last block nothing has been sent: what is read then is not used).
-        // The products before it stay before it: without a use there the compiler moves them past the branches.
+          for (int x = 0; x < kNt; ++x)
 #pragma unroll
-        for (int i = 0; i < kNt; ++i)
+            for (int y = 0; y < kMt; ++y) {
+              if (WM * WN > 128 * 64) asm volatile("" : "+a"(acc[x][y]));
+              else if (KIND == kScaleE8M0) asm volatile("" : "+v"(acc[x][y]));
+              else asm volatile("" : "+v"(part[x][y]));
+            }
+          if (kSpread && more) meet<kPerB>();  // all but the weights of block s + 2
+          else meet<0>();
+          // the next chunk of scales: sent for at a chunk's first step, kept at its second
+          if (s % kScales == 1) {
+            asm volatile("" : "+v"(sb_next));
 #pragma unroll
-          for (int t = 0; t < kMt; ++t) {
-            if (KIND == kScaleE8M0) asm volatile("" : "+v"(acc[i][t]));
-            else asm volatile("" : "+v"(part[i][t]));
+            for (int x = 0; x < kPieces; ++x) asm volatile("" : "+v"(next_chunk.v[x]));
+            if (brings) keep_chunk(next_chunk, ((s / kScales) & 1) ^ 1);
           }
-        if (kSpread && more) meet<kPerB>();  // all but the weights of block s + 2
-        else meet<0>();
-        // the next chunk of scales: sent for at a chunk's first step, kept at its second
-        if (s % kScales == 1) {
-          asm volatile("" : "+v"(sb_next), "+v"(next_chunk));
-          if (brings) keep_chunk(next_chunk, ((s / kScales) & 1) ^ 1);
+          if (s % kScales == kScales - 1) {
+            sb = sb_next;
+            asm volatile("" : "+v"(sb));  // (a branch: as a select it would wait for loads at every step)
+          }
+          if (s % kScales == 0 && s + kScales < steps) {
+            sb_next = load_weight_scales(kb0 + s + kScales);
+            if (brings) next_chunk = load_chunk(kb0 + s + kScales);
+          }
+          if (more && mask != ~0ull) clear_tail(kb0 + s + 2, buf);
+          if (!kSpread && more) {
+#pragma unroll
+            for (int x = 0; x < kPerA; ++x) issue_a(kb0 + s + 2, buf, x, mask);
+#pragma unroll
+            for (int x = 0; x < kPerB; ++x) issue_b(kb0 + s + 2, buf, x, mask);
+          }
+          if (!kEach) {
+#pragma unroll
+            for (int x = 0; x < kMt; ++x) na[x] = row_scale(s + 1, x);
+          }
         }
-        if (s % kScales == kScales - 1) {
-          sb = sb_next;
-          asm volatile("" : "+v"(sb));  // (a branch: as a select it would wait for loads at every step)
+        if (kSpread && g / 2 == 1) {
+          constexpr int kNow = kPerB / (2 * kNt);
+#pragma unroll
+          for (int x = 0; x < kNow; ++x) issue_b(kb0 + s + 2, buf, ((g - 2) * kNt + i) * kNow + x, mask);
         }
-        if (s % kScales == 0 && s + kScales < steps) {
-          sb_next = load_weight_scales(kb0 + s + kScales);
-          if (brings) next_chunk = load_chunk(kb0 + s + kScales);
+        if (kSpread && g >= kGroups - 2) {
+          constexpr int kNow = kPerA / (2 * kNt);
+#pragma unroll
+          for (int x = 0; x < kNow; ++x) issue_a(kb0 + s + 2, buf, ((g - kGroups + 2) * kNt + i) * kNow + x, mask);
         }
-        if (more && mask != ~0ull) clear_tail(kb0 + s + 2, buf);
-        if (!kSpread && more) {
-#pragma unroll
-          for (int i = 0; i < kPerA; ++i) issue_a(kb0 + s + 2, buf, i, mask);
-#pragma unroll
-          for (int i = 0; i < kPerB; ++i) issue_b(kb0 + s + 2, buf, i, mask);
+        if (g == 0) fb[1][i] = operand(buf, BM + wn + 32 * i, 1);
+        if (g == kGroups - kAhead) fb[0][i] = operand(buf ^ 1, BM + wn + 32 * i, 0);
+        if (i == 0) {
+          if (kEach && g >= kGroups - kAhead) ca[g - (kGroups - kAhead)] = row_scale(s + 1, g - (kGroups - kAhead));
+          if (kEach && g == 0) ca[kMt - 1] = row_scale(s, kMt - 1);
+          fa[t % kSlots] = t < kGroups ? operand(buf, wm + 32 * (t % kMt), t / kMt) : operand(buf ^ 1, wm + 32 * (t % kMt), 0);
         }
-#pragma unroll
-        for (int i = 0; i < kNt; ++i) fb[0][i] = operand(buf ^ 1, BM + wn + 32 * i, 0);
-        if (!kEach) {
-#pragma unroll
-          for (int t = 0; t < kMt; ++t) na[t] = row_scale(s + 1, t);
-        }
-      }
-      if (kSpread && g >= kGroups - 2) {
-#pragma unroll
-        for (int i = (g - kGroups + 2) * kPerA / 2; i < (g - kGroups + 3) * kPerA / 2; ++i) issue_a(kb0 + s + 2, buf, i, mask);
-      }
-      if (kEach && g >= kGroups - kAhead) ca[g - (kGroups - kAhead)] = row_scale(s + 1, g - (kGroups - kAhead));
-      if (kEach && g == 0) ca[kMt - 1] = row_scale(s, kMt - 1);
-      const int t = g + kAhead;
-      fa[t % kSlots] = t < kGroups ? operand(buf, wm + 32 * (t % kMt), t / kMt) : operand(buf ^ 1, wm + 32 * (t % kMt), 0);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < kNt; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
         if (KIND == kScaleE8M0)
           acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h][i], fa[g % kSlots], acc[i][j], 0, 0, 0, cb, 0, ca[j]);
         else
           part[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h][i], fa[g % kSlots], h ? part[i][j] : (v16f){}, 0, 0,
                                                                        0, 127, 0, 127);
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (KIND == kScaleF32 && h == 1) {
         const float f = __uint_as_float(ca[j]) * __uint_as_float(cb);
@@ -342,8 +355,8 @@ fp8_gemm_kernel(const GemmParams P) {
         for (int i = 0; i < kNt; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[i][j][r] += part[i][j][r] * f;
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
     if (!kEach) {
 #pragma unroll
@@ -441,7 +454,7 @@ int launch_tile(GemmParams P, hipStream_t st) {
 template <int KIND, int OUT>
 int launch_plan(const Plan& p, const GemmParams& P, hipStream_t st) {
   // f32 scales take a second set of accumulators: narrower tiles
-  if (p.bm == 256) return KIND == kScaleE8M0 ? launch_tile<256, 256, 128, 64, kScaleE8M0, OUT>(P, st) : launch_tile<256, 128, 64, 64, kScaleF32, OUT>(P, st);
+  if (p.bm == 256) return KIND == kScaleE8M0 ? launch_tile<256, 256, 128, 128, kScaleE8M0, OUT>(P, st) : launch_tile<256, 128, 64, 64, kScaleF32, OUT>(P, st);
   if (p.bm == 128) return launch_tile<128, 128, 64, 64, KIND, OUT>(P, st);
   if (p.bm == 64) return launch_tile<64, 128, 64, 32, KIND, OUT>(P, st);
   return launch_tile<32, 64, 32, 32, KIND, OUT>(P, st);
