@@ -12,6 +12,7 @@
 // are stored in the order piece ^ (row / 2 % 8): 16 rows' reads of one piece fall on different banks
 // (rows are half the banks' span apart; with row % 8 two of 16 met on each bank).
 #include <algorithm>
+#include <type_traits>
 
 #include "dsa_common.h"
 #include "fp8_block.h"
@@ -36,8 +37,14 @@ struct GemmParams {
   int64_t out_stride;
 };
 
-// 16 bytes from base + offset into LDS at lds + 16 * lane, for the lanes in `mask`, without registers; the
-// kernel waits for them itself (vmcnt). To be called with every lane active.
+// 16 bytes a lane from base + offset into LDS at lds + 16 * lane, without registers; the kernel
+// waits for them itself (vmcnt).
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base),
+               "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
+// The same for the lanes in `mask` (every lane is active at the call).
 __device__ __forceinline__ void dma16(const uint8_t* base, uint32_t offset, uint32_t lds, uint64_t mask) {
   asm volatile("s_mov_b64 exec, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1" ::"v"(offset),
                "s"(base), "s"(mask), "{m0}"(__builtin_amdgcn_readfirstlane(lds))
@@ -158,32 +165,30 @@ fp8_gemm_kernel(const GemmParams P) {
   for (int i = 0; i < kPerB; ++i) off_b[i] = offset(i, P.n - 1 - n0, P.b_stride);
   const uint8_t* tile_a = P.a + (int64_t)m0 * P.a_stride;
   const uint8_t* tile_b = P.b + (int64_t)n0 * P.b_stride;
-  // the lanes of a copy of block kb whose pieces lie inside K
-  auto lanes_of = [&](int kb) -> uint64_t {
-    return (kb + 1) * kBlock <= P.k ? ~0ull : __builtin_amdgcn_ballot_w64(kb * kBlock + 16 * piece < P.k);
-  };
+  // the lanes whose pieces of the last block lie inside K
+  const int full = P.k / kBlock;  // whole blocks
+  const uint64_t tail = __builtin_amdgcn_ballot_w64(16 * piece < P.k % kBlock);
   const uint32_t dst0 = lds_addr(smem) + wave * 1024;
-  auto issue_a = [&](int kb, int buf, int i, uint64_t mask) {
-    dma16(tile_a + (int64_t)kb * kBlock, off_a[i], dst0 + buf * kStage + i * kWaves * 1024, mask);
+  auto issue_a = [&](int kb, int buf, int i, auto... mask) {
+    dma16(tile_a + (int64_t)kb * kBlock, off_a[i], dst0 + buf * kStage + i * kWaves * 1024, mask...);
   };
-  auto issue_b = [&](int kb, int buf, int i, uint64_t mask) {
-    dma16(tile_b + (int64_t)kb * kBlock, off_b[i], dst0 + buf * kStage + BM * kBlock + i * kWaves * 1024, mask);
+  auto issue_b = [&](int kb, int buf, int i, auto... mask) {
+    dma16(tile_b + (int64_t)kb * kBlock, off_b[i], dst0 + buf * kStage + BM * kBlock + i * kWaves * 1024, mask...);
   };
-  // zeros where a block lies past the end of K
-  auto clear_tail = [&](int kb, int buf) {
-    if (kb * kBlock + 16 * piece >= P.k) {
+  // zeros where the last block lies past the end of K
+  auto clear_tail = [&](int buf) {
+    if (16 * piece >= P.k % kBlock) {
       uint8_t* z = smem + buf * kStage + wave * 1024 + lane * 16;
 #pragma unroll
       for (int i = 0; i < kPerA + kPerB; ++i) *reinterpret_cast<v4i*>(z + i * kWaves * 1024) = (v4i){0, 0, 0, 0};
     }
   };
   auto issue = [&](int kb, int buf) {
-    const uint64_t mask = lanes_of(kb);
+    const uint64_t mask = kb < full ? ~0ull : tail;
 #pragma unroll
     for (int i = 0; i < kPerA; ++i) issue_a(kb, buf, i, mask);
 #pragma unroll
     for (int i = 0; i < kPerB; ++i) issue_b(kb, buf, i, mask);
-    if (mask != ~0ull) clear_tail(kb, buf);
   };
 
   // activation scales: thread t brings half t % 2 of a chunk of row t / 2. (Its addresses are made anew from an
@@ -250,6 +255,7 @@ fp8_gemm_kernel(const GemmParams P) {
   const int steps = kb1 - kb0;
   if (steps > 0) {
     issue(kb0, 0);
+    if (kb0 == full) clear_tail(0);
     if (brings) keep_chunk(load_chunk(kb0), 0);
     sb = load_weight_scales(kb0);
     asm volatile("" : "+v"(sb));
@@ -269,10 +275,19 @@ fp8_gemm_kernel(const GemmParams P) {
   asm volatile("" : "+s"(out), "+s"(out_stride));
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
   Chunk next_chunk = {};
-  for (int s = 0; s < steps; ++s) {
+  // One step: block s is multiplied, block s + 2 sent for. LAST: it may be short, or there is none.
+  auto step = [&](int s, auto last) {
+    constexpr bool LAST = decltype(last)::value;
     const int buf = s & 1;
-    const bool more = s + 2 < steps;
-    const uint64_t mask = more ? lanes_of(kb0 + s + 2) : 0ull;
+    const uint64_t mask = s + 2 >= steps ? 0ull : kb0 + s + 2 < full ? ~0ull : tail;
+    auto send_a = [&](int i) {
+      if constexpr (LAST) issue_a(kb0 + s + 2, buf, i, mask);
+      else issue_a(kb0 + s + 2, buf, i);
+    };
+    auto send_b = [&](int i) {
+      if constexpr (LAST) issue_b(kb0 + s + 2, buf, i, mask);
+      else issue_b(kb0 + s + 2, buf, i);
+    };
     cb = __builtin_amdgcn_readlane(sb, s % kScales);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
@@ -295,29 +310,33 @@ fp8_gemm_kernel(const GemmParams P) {
               else if (KIND == kScaleE8M0) asm volatile("" : "+v"(acc[x][y]));
               else asm volatile("" : "+v"(part[x][y]));
             }
-          if (kSpread && more) meet<kPerB>();  // all but the weights of block s + 2
-          else meet<0>();
-          // the next chunk of scales: sent for at a chunk's first step, kept at its second
-          if (s % kScales == 1) {
-            asm volatile("" : "+v"(sb_next));
+          // The next chunk of scales: sent for at a chunk's first step, kept at its second.
+          if (__builtin_expect((unsigned)(s + 1) % kScales < 3, 0)) {
+            if (s % kScales == 1) {
+              asm volatile("" : "+v"(sb_next));
 #pragma unroll
-            for (int x = 0; x < kPieces; ++x) asm volatile("" : "+v"(next_chunk.v[x]));
-            if (brings) keep_chunk(next_chunk, ((s / kScales) & 1) ^ 1);
+              for (int x = 0; x < kPieces; ++x) asm volatile("" : "+v"(next_chunk.v[x]));
+              if (brings) keep_chunk(next_chunk, ((s / kScales) & 1) ^ 1);
+            } else if (s % kScales == 0) {
+              if (s + kScales < steps) {
+                sb_next = load_weight_scales(kb0 + s + kScales);
+                if (brings) next_chunk = load_chunk(kb0 + s + kScales);
+              }
+            } else {
+              sb = sb_next;
+            }
+            asm volatile("" : "+v"(sb));  // (what was loaded is waited for here, not at every step)
           }
-          if (s % kScales == kScales - 1) {
-            sb = sb_next;
-            asm volatile("" : "+v"(sb));  // (a branch: as a select it would wait for loads at every step)
+          if (LAST) {
+            if (s + 1 < steps && kb0 + s + 1 == full) clear_tail(buf ^ 1);
+            __builtin_amdgcn_s_waitcnt(0);
           }
-          if (s % kScales == 0 && s + kScales < steps) {
-            sb_next = load_weight_scales(kb0 + s + kScales);
-            if (brings) next_chunk = load_chunk(kb0 + s + kScales);
-          }
-          if (more && mask != ~0ull) clear_tail(kb0 + s + 2, buf);
-          if (!kSpread && more) {
+          meet<kSpread ? kPerB : 0>();  // all but the weights of block s + 2
+          if (!kSpread) {
 #pragma unroll
-            for (int x = 0; x < kPerA; ++x) issue_a(kb0 + s + 2, buf, x, mask);
+            for (int x = 0; x < kPerA; ++x) send_a(x);
 #pragma unroll
-            for (int x = 0; x < kPerB; ++x) issue_b(kb0 + s + 2, buf, x, mask);
+            for (int x = 0; x < kPerB; ++x) send_b(x);
           }
           if (!kEach) {
 #pragma unroll
@@ -327,12 +346,12 @@ fp8_gemm_kernel(const GemmParams P) {
         if (kSpread && g / 2 == 1) {
           constexpr int kNow = kPerB / (2 * kNt);
 #pragma unroll
-          for (int x = 0; x < kNow; ++x) issue_b(kb0 + s + 2, buf, ((g - 2) * kNt + i) * kNow + x, mask);
+          for (int x = 0; x < kNow; ++x) send_b(((g - 2) * kNt + i) * kNow + x);
         }
         if (kSpread && g >= kGroups - 2) {
           constexpr int kNow = kPerA / (2 * kNt);
 #pragma unroll
-          for (int x = 0; x < kNow; ++x) issue_a(kb0 + s + 2, buf, ((g - kGroups + 2) * kNt + i) * kNow + x, mask);
+          for (int x = 0; x < kNow; ++x) send_a(((g - kGroups + 2) * kNt + i) * kNow + x);
         }
         if (g == 0) fb[1][i] = operand(buf, BM + wn + 32 * i, 1);
         if (g == kGroups - kAhead) fb[0][i] = operand(buf ^ 1, BM + wn + 32 * i, 0);
@@ -362,7 +381,11 @@ fp8_gemm_kernel(const GemmParams P) {
 #pragma unroll
       for (int j = 0; j < kMt; ++j) ca[j] = na[j];
     }
-  }
+  };
+  const int plain = min(steps, full - kb0) - 2;  // steps that send for a whole block
+  int s = 0;
+  for (; s < plain; ++s) step(s, std::false_type{});
+  for (; s < steps; ++s) step(s, std::true_type{});
 
   // lane (c32, half): row c32 of an activation tile, columns 8g + 4 half .. + 3 of a weight tile
   if (P.splits > 1) out = static_cast<float*>(out) + (int64_t)split * P.m * P.n;
