@@ -52,13 +52,20 @@ __device__ __forceinline__ void dma16(const uint8_t* base, uint32_t offset, uint
 }
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)reinterpret_cast<uintptr_t>(p); }
 
-// All of this wave's loads but the last LEFT and its LDS accesses are done, then all waves' are. (The wait is a builtin:
-// the compiler's own counting of what is under way starts anew behind it.)
+// At most LEFT of this wave's loads are under way, and none of its LDS accesses. (A builtin: the compiler's own
+// counting of what is under way takes note of it.)
+template <int LEFT>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(LEFT < 64, "the counter's range");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((LEFT & 15) | (LEFT >> 4 << 14));
+  asm volatile("" ::: "memory");
+}
+
+// The same, and then for every wave of the workgroup.
 template <int LEFT>
 __device__ __forceinline__ void meet() {
-  static_assert(LEFT < 16, "low bits of the count");
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(LEFT);
+  wait_loads<LEFT>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -72,19 +79,19 @@ __device__ __forceinline__ uint32_t load_scale(const void* s, int64_t i) {
 
 __device__ __forceinline__ int pack2(float a, float b) { return __builtin_bit_cast(int, (v2bf){(__bf16)a, (__bf16)b}); }
 
+// 16 bytes of results from element `at` on, of which `left` lie inside the row.
 template <int OUT>
-__device__ __forceinline__ void store4(void* out, int64_t at, bool whole, int left, const float* v) {
+__device__ __forceinline__ void store16(void* out, int64_t at, bool whole, int left, v4i v) {
   if (OUT == kOutBf16) {
     uint16_t* o = static_cast<uint16_t*>(out) + at;
-    const v2i p = {pack2(v[0], v[1]), pack2(v[2], v[3])};
-    if (whole) *reinterpret_cast<v2i*>(o) = p;
+    if (whole) *reinterpret_cast<v4i*>(o) = v;
     else
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < left) o[j] = (uint16_t)((uint32_t)p[j >> 1] >> (16 * (j & 1)));
+      for (int j = 0; j < 8; ++j)
+        if (j < left) o[j] = (uint16_t)((uint32_t)v[j >> 1] >> (16 * (j & 1)));
   } else {
-    float* o = static_cast<float*>(out) + at;
-    if (whole) *reinterpret_cast<v4f*>(o) = (v4f){v[0], v[1], v[2], v[3]};
+    int* o = static_cast<int*>(out) + at;
+    if (whole) *reinterpret_cast<v4i*>(o) = v;
     else
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -92,15 +99,34 @@ __device__ __forceinline__ void store4(void* out, int64_t at, bool whole, int le
   }
 }
 
-// Bytes of a tile's activation scales that lie in LDS at a time, two such chunks: 32 e8m0 or
-// 8 f32 blocks of each row. Rows are 36 bytes apart, so that 32 rows' reads of one block fall
-// on different banks.
-constexpr int kMaxStride = 1 << 23;  // a tile's offsets are 32-bit
-constexpr int kScaleChunk = 32, kScaleRow = 36;
+template <int OUT>
+__device__ __forceinline__ void store4(void* out, int64_t at, bool whole, int left, const float* v) {
+  if (OUT == kOutF32) {
+    store16<OUT>(out, at, whole, left, (v4i){__float_as_int(v[0]), __float_as_int(v[1]), __float_as_int(v[2]), __float_as_int(v[3])});
+    return;
+  }
+  uint16_t* o = static_cast<uint16_t*>(out) + at;
+  const v2i p = {pack2(v[0], v[1]), pack2(v[2], v[3])};
+  if (whole) *reinterpret_cast<v2i*>(o) = p;
+  else
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) o[j] = (uint16_t)((uint32_t)p[j >> 1] >> (16 * (j & 1)));
+}
 
-template <int BM, int BN>
+constexpr int kMaxStride = 1 << 23;  // a tile's offsets are 32-bit
+constexpr int kBand = 4;             // activation tiles of a band
+
+// Activation scales of a tile lie in LDS in chunks, two at a time: 32 e8m0 or 16 f32 blocks of each
+// row. Rows are an odd number of words apart, so that 32 rows' reads of one block fall on different banks.
+template <int KIND>
+constexpr int kScaleChunk = KIND == kScaleF32 ? 64 : 32;
+template <int KIND>
+constexpr int kScaleRow = kScaleChunk<KIND> + 4;
+
+template <int BM, int BN, int STAGES, int KIND>
 constexpr int gemm_smem() {
-  return 2 * (BM + BN) * kBlock + 2 * BM * kScaleRow;
+  return STAGES * (BM + BN) * kBlock + 2 * BM * kScaleRow<KIND>;
 }
 
 // 16 bytes of scales from element i of a row of n, at any address.
@@ -125,28 +151,38 @@ __device__ __forceinline__ v4i load_scale_piece(const void* row, int i, int n) {
   return v;
 }
 
-// A tile of BM activation rows and BN weight rows; a wave takes WM x WN of it.
+// A tile of BM activation rows and BN weight rows; a wave takes WM x WN of it. STAGES blocks of both lie in
+// LDS: one is multiplied, the others are on their way or wait.
 //
 // Operands are read from LDS a few products ahead of those that run. Where the reads
 // of block s end and those of block s + 1 begin, the waves meet, once a block: all have read block
-// s by then, and block s + 1 has landed; block s + 2 is sent for in block s's place.
-template <int BM, int BN, int WM, int WN, int KIND, int OUT>
+// s by then, and block s + 1 has landed; block s + STAGES is sent for in block s's place.
+template <int BM, int BN, int WM, int WN, int STAGES, int KIND, int OUT>
 __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) __attribute__((amdgpu_waves_per_eu(WM * WN > 128 * 64 ? 1 : 2)))
 fp8_gemm_kernel(const GemmParams P) {
   constexpr int kWaves = (BM / WM) * (BN / WN);
   constexpr int kMt = WM / 32, kNt = WN / 32;
   constexpr int kStage = (BM + BN) * kBlock;
   constexpr int kPerA = BM / 8 / kWaves, kPerB = BN / 8 / kWaves;  // instructions of a stage: eight rows each
-  constexpr int kScales = KIND == kScaleF32 ? kScaleChunk / 4 : kScaleChunk;
+  constexpr int kChunk = kScaleChunk<KIND>, kRow = kScaleRow<KIND>;
+  constexpr int kScales = KIND == kScaleF32 ? kChunk / 4 : kChunk, kRowPieces = kChunk / 16;
   static_assert(kPerA * kWaves * 8 == BM && kPerB * kWaves * 8 == BN, "rows dealt out evenly");
   static_assert(kWaves % 2 == 0, "a wave's rows of a stage have one order of pieces");
   static_assert(kBlock % WN == 0, "one weight scale a wave");
-  constexpr int kThreads = kWaves * 64, kPieces = (2 * BM + kThreads - 1) / kThreads;  // of a scale chunk, a thread
-  static_assert(2 * BM % (kPieces * 64) == 0, "whole waves bring scales");
+  static_assert(64 % kScales == 0 && kScales >= 4, "weight scales are replaced where a chunk is");
+  constexpr int kThreads = kWaves * 64, kPieces = (kRowPieces * BM + kThreads - 1) / kThreads;  // of a scale chunk, a thread
+  static_assert(kRowPieces * BM % (kPieces * 64) == 0, "whole waves bring scales");
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = blockIdx.x % (P.mtiles * P.ntiles), split = blockIdx.x / (P.mtiles * P.ntiles);
-  const int m0 = (tile % P.mtiles) * BM, n0 = (tile / P.mtiles) * BN;
+  // Workgroups go to the eight XCDs in turn: each XCD takes a run of neighbouring tiles, in bands of four activation
+  // tiles, so that the tiles at work beside one L2 share their rows. (Against tiles dealt out one by one: 8192^3 / 2
+  // of work the same, 2048 x 8192 x 8192 4% less, 333 x 8192 x 8192 40 -> 60 us without.)
+  const int tiles = P.mtiles * P.ntiles;
+  const int xcd = blockIdx.x & 7, share = gridDim.x >> 3, rest = gridDim.x & 7;
+  const int at = xcd * share + min(xcd, rest) + (blockIdx.x >> 3);
+  const int split = at / tiles, tile = at - split * tiles;
+  const int band = tile / (kBand * P.ntiles), in_band = tile - band * kBand * P.ntiles, wide = min(kBand, P.mtiles - kBand * band);
+  const int m0 = (kBand * band + in_band % wide) * BM, n0 = in_band / wide * BN;
   const int kb0 = (int)((int64_t)P.kblocks * split / P.splits), kb1 = (int)((int64_t)P.kblocks * (split + 1) / P.splits);
   const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
   const int c32 = lane & 31, half = lane >> 5;
@@ -169,11 +205,11 @@ fp8_gemm_kernel(const GemmParams P) {
   const int full = P.k / kBlock;  // whole blocks
   const uint64_t tail = __builtin_amdgcn_ballot_w64(16 * piece < P.k % kBlock);
   const uint32_t dst0 = lds_addr(smem) + wave * 1024;
-  auto issue_a = [&](int kb, int buf, int i, auto... mask) {
-    dma16(tile_a + (int64_t)kb * kBlock, off_a[i], dst0 + buf * kStage + i * kWaves * 1024, mask...);
-  };
-  auto issue_b = [&](int kb, int buf, int i, auto... mask) {
-    dma16(tile_b + (int64_t)kb * kBlock, off_b[i], dst0 + buf * kStage + BM * kBlock + i * kWaves * 1024, mask...);
+  // copy i of block kb: the activations' first
+  auto copy = [&](int kb, int buf, int i, auto... mask) {
+    const uint32_t dst = dst0 + buf * kStage + i * kWaves * 1024;
+    if (i < kPerA) dma16(tile_a + (int64_t)kb * kBlock, off_a[i < kPerA ? i : 0], dst, mask...);
+    else dma16(tile_b + (int64_t)kb * kBlock, off_b[i < kPerA ? 0 : i - kPerA], dst, mask...);
   };
   // zeros where the last block lies past the end of K
   auto clear_tail = [&](int buf) {
@@ -183,18 +219,17 @@ fp8_gemm_kernel(const GemmParams P) {
       for (int i = 0; i < kPerA + kPerB; ++i) *reinterpret_cast<v4i*>(z + i * kWaves * 1024) = (v4i){0, 0, 0, 0};
     }
   };
-  auto issue = [&](int kb, int buf) {
+  auto issue = [&](int kb, int buf, int copies) {
     const uint64_t mask = kb < full ? ~0ull : tail;
 #pragma unroll
-    for (int i = 0; i < kPerA; ++i) issue_a(kb, buf, i, mask);
-#pragma unroll
-    for (int i = 0; i < kPerB; ++i) issue_b(kb, buf, i, mask);
+    for (int i = 0; i < kPerA + kPerB; ++i)
+      if (i < copies) copy(kb, buf, i, mask);
   };
 
-  // activation scales: thread t brings half t % 2 of a chunk of row t / 2. (Its addresses are made anew from an
-  // opaque copy of the thread's number: kept in registers they would be spilled.)
-  uint8_t* scale_lds = smem + 2 * kStage;
-  const bool brings = kPieces * kThreads == 2 * BM || (int)threadIdx.x < 2 * BM;
+  // activation scales: thread t brings piece t % kRowPieces of a chunk of row t / kRowPieces. (Its addresses are made
+  // anew from an opaque copy of the thread's number: kept in registers they would be spilled.)
+  uint8_t* scale_lds = smem + STAGES * kStage;
+  const bool brings = kPieces * kThreads == kRowPieces * BM || (int)threadIdx.x < kRowPieces * BM;
   struct Chunk {
     v4i v[kPieces];
   };
@@ -204,10 +239,10 @@ fp8_gemm_kernel(const GemmParams P) {
     for (int i = 0; i < kPieces; ++i) {
       int t = threadIdx.x + i * kThreads;
       asm volatile("" : "+v"(t));
-      const int64_t row = (int64_t)min(m0 + t / 2, P.m - 1) * P.sa_stride;
+      const int64_t row = (int64_t)min(m0 + t / kRowPieces, P.m - 1) * P.sa_stride;
       c.v[i] = load_scale_piece<KIND>(KIND == kScaleF32 ? (const void*)(static_cast<const uint32_t*>(P.sa) + row)
                                                         : (const void*)(static_cast<const uint8_t*>(P.sa) + row),
-                                      kb + (t & 1) * (kScales / 2), P.kblocks);
+                                      kb + t % kRowPieces * (kScales / kRowPieces), P.kblocks);
     }
     return c;
   };
@@ -216,19 +251,19 @@ fp8_gemm_kernel(const GemmParams P) {
     for (int i = 0; i < kPieces; ++i) {
       int t = threadIdx.x + i * kThreads;
       asm volatile("" : "+v"(t));
-      uint32_t* d = reinterpret_cast<uint32_t*>(scale_lds + which * BM * kScaleRow + (t / 2) * kScaleRow + (t & 1) * 16);
+      uint32_t* d = reinterpret_cast<uint32_t*>(scale_lds + which * BM * kRow + t / kRowPieces * kRow + t % kRowPieces * 16);
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] = (uint32_t)c.v[i][j];
     }
   };
   // the scale of this lane's row in activation tile j at block kb
   auto row_scale = [&](int step, int j) -> uint32_t {
-    const uint8_t* p = scale_lds + ((step / kScales) & 1) * BM * kScaleRow + (wm + 32 * j + c32) * kScaleRow;
+    const uint8_t* p = scale_lds + ((step / kScales) & 1) * BM * kRow + (wm + 32 * j + c32) * kRow;
     return KIND == kScaleF32 ? reinterpret_cast<const uint32_t*>(p)[step % kScales] : (uint32_t)p[step % kScales];
   };
-  // a chunk of the wave's one weight scale a block, a lane each
+  // the wave's one weight scale a block, 64 blocks a lane each
   const int64_t sb_at = (int64_t)min((n0 + wn) / kBlock, (P.n - 1) / kBlock) * P.sb_stride;
-  auto load_weight_scales = [&](int kb) { return load_scale<KIND>(P.sb, sb_at + min(kb + lane % kScales, P.kblocks - 1)); };
+  auto load_weight_scales = [&](int kb) { return load_scale<KIND>(P.sb, sb_at + min(kb + lane, P.kblocks - 1)); };
 
   v16f acc[kNt][kMt], part[kNt][kMt];
 #pragma unroll
@@ -245,22 +280,49 @@ fp8_gemm_kernel(const GemmParams P) {
   };
   // A step's groups: half h of activation tile j times all weight tiles. Group g's activations lie in
   // slot g % kSlots and are read kAhead groups before; weights a half before.
-  constexpr int kGroups = 2 * kMt, kAhead = kMt == 4 ? 3 : kMt, kSlots = kMt == 4 ? 4 : kGroups;
+  // (as far ahead as registers allow)
+  constexpr bool kTight = kMt == 4 || (KIND == kScaleF32 && kMt == 2);
+  constexpr int kGroups = 2 * kMt, kAhead = kTight ? kMt - 1 : kMt, kSlots = kTight ? kMt : kGroups;
   v8i fa[kSlots], fb[2][kNt];
-  // scales of this block, and of the next ones; those of four tiles are replaced one by one behind their last use
+  // scales of this block, and of the next ones (replaced one by one behind their last use where tiles are read that late)
   constexpr bool kEach = kAhead < kMt;
-  constexpr bool kSpread = kMt == 4;  // copies sent between the products
+  // Copies are sent between the products: a wave that sent all of its own at once would stand until they are taken.
+  // Two meetings a block (kTwice): its weights' place is free early, its activations' at the second. Else the copies of
+  // block s + STAGES are dealt out over the kSend products behind the meeting, the last of them in the next step.
+  constexpr bool kTwice = kMt == 4;
+  constexpr int kSlotsAll = kGroups * kNt, kMeetAt = (kGroups - kAhead) * kNt, kCopies = kPerA + kPerB;
+  constexpr int kSend = STAGES > 2 ? kSlotsAll : kSlotsAll / 2, kSendHere = kSlotsAll - kMeetAt;
+  constexpr int kCopiesHere = kSendHere >= kSend ? kCopies : kSendHere * kCopies / kSend;  // before the step ends
   uint32_t ca[kMt], na[kMt], cb, sb = 0, sb_next = 0;
+  // f32 scales: a tile's sums over a block join the others while the next tile's products run
+  constexpr bool kDelay = KIND == kScaleF32 && kMt > 1;
+  float join = 0.f;
+  if (kDelay)
+#pragma unroll
+    for (int i = 0; i < kNt; ++i) part[i][kMt - 1] = (v16f){};
+  auto join_tile = [&](int j, float f) {
+#pragma unroll
+    for (int i = 0; i < kNt; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] += part[i][j][r] * f;
+  };
 
   const int steps = kb1 - kb0;
   if (steps > 0) {
-    issue(kb0, 0);
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i)
+      if (i < steps) issue(kb0 + i, i, i < STAGES - 1 || kTwice ? kCopies : kCopiesHere);
     if (kb0 == full) clear_tail(0);
-    if (brings) keep_chunk(load_chunk(kb0), 0);
+    Chunk c0 = {}, c1 = {};
     sb = load_weight_scales(kb0);
-    asm volatile("" : "+v"(sb));
+    if (brings) {
+      c0 = load_chunk(kb0);
+      if (steps > kScales) c1 = load_chunk(kb0 + kScales);
+      keep_chunk(c0, 0);
+      keep_chunk(c1, 1);
+    }
+    asm volatile("" ::"v"(sb));  // (waited for here)
     meet<0>();
-    if (steps > 1) issue(kb0 + 1, 1);
 #pragma unroll
     for (int i = 0; i < kNt; ++i) fb[0][i] = operand(0, BM + wn + 32 * i, 0);
 #pragma unroll
@@ -275,27 +337,30 @@ fp8_gemm_kernel(const GemmParams P) {
   asm volatile("" : "+s"(out), "+s"(out_stride));
   __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
   Chunk next_chunk = {};
-  // One step: block s is multiplied, block s + 2 sent for. LAST: it may be short, or there is none.
+  int buf = 0;  // block s's place
+  // One step: block s is multiplied, block s + STAGES sent for (and the rest of the one before).
+  // LAST: one of them may be short, or not there.
   auto step = [&](int s, auto last) {
     constexpr bool LAST = decltype(last)::value;
-    const int buf = s & 1;
-    const uint64_t mask = s + 2 >= steps ? 0ull : kb0 + s + 2 < full ? ~0ull : tail;
-    auto send_a = [&](int i) {
-      if constexpr (LAST) issue_a(kb0 + s + 2, buf, i, mask);
-      else issue_a(kb0 + s + 2, buf, i);
+    const int buf1 = buf + 1 < STAGES ? buf + 1 : 0, buf0 = buf > 0 ? buf - 1 : STAGES - 1, kb2 = kb0 + s + STAGES;
+    const uint64_t mask = kb2 < min(kb1, full) ? ~0ull : kb2 < kb1 ? tail : 0ull;
+    const uint64_t mask0 = kb2 - 1 < min(kb1, full) ? ~0ull : kb2 - 1 < kb1 ? tail : 0ull;
+    auto send = [&](int i) {
+      if constexpr (LAST) copy(kb2, buf, i, mask);
+      else copy(kb2, buf, i);
     };
-    auto send_b = [&](int i) {
-      if constexpr (LAST) issue_b(kb0 + s + 2, buf, i, mask);
-      else issue_b(kb0 + s + 2, buf, i);
+    auto send_rest = [&](int i) {
+      if constexpr (LAST) copy(kb2 - 1, buf0, i, mask0);
+      else copy(kb2 - 1, buf0, i);
     };
-    cb = __builtin_amdgcn_readlane(sb, s % kScales);
+    cb = __builtin_amdgcn_readlane(sb, s % 64);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
       const int h = g / kMt, j = g % kMt, t = g + kAhead;
 #pragma unroll
       for (int i = 0; i < kNt; ++i) {  // one product, and what is sent for meanwhile
-        if (kSpread && g == 2 && i == 0) {
-          // every wave has read the block's weights: those of block s + 2 take their place
+        if (kTwice && g == 2 && i == 0) {
+          // every wave has read the block's weights: those of block s + STAGES take their place
           asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
         if (g == kGroups - kAhead && i == 0) {
@@ -310,55 +375,61 @@ fp8_gemm_kernel(const GemmParams P) {
               else if (KIND == kScaleE8M0) asm volatile("" : "+v"(acc[x][y]));
               else asm volatile("" : "+v"(part[x][y]));
             }
-          // The next chunk of scales: sent for at a chunk's first step, kept at its second.
-          if (__builtin_expect((unsigned)(s + 1) % kScales < 3, 0)) {
-            if (s % kScales == 1) {
-              asm volatile("" : "+v"(sb_next));
-#pragma unroll
-              for (int x = 0; x < kPieces; ++x) asm volatile("" : "+v"(next_chunk.v[x]));
+          // The chunk of scales after the next: sent for at a chunk's first step, kept at its second.
+          if (__builtin_expect((unsigned)(s + 1) % kScales < 3 && s + 1 >= kScales, 0)) {
+            if (s % kScales == 0) {
+              if (s % 64 == kScales % 64 && s + 64 - kScales < steps) sb_next = load_weight_scales(kb0 + s + 64 - kScales);
+              if (s + kScales < steps && brings) next_chunk = load_chunk(kb0 + s + kScales);
+            } else if (s % kScales == 1) {
               if (brings) keep_chunk(next_chunk, ((s / kScales) & 1) ^ 1);
-            } else if (s % kScales == 0) {
-              if (s + kScales < steps) {
-                sb_next = load_weight_scales(kb0 + s + kScales);
-                if (brings) next_chunk = load_chunk(kb0 + s + kScales);
-              }
-            } else {
+              asm volatile("" ::"v"(sb_next));  // (waited for here, not where it is used)
+            } else if (s % 64 == 63) {
               sb = sb_next;
             }
-            asm volatile("" : "+v"(sb));  // (what was loaded is waited for here, not at every step)
           }
-          if (LAST) {
-            if (s + 1 < steps && kb0 + s + 1 == full) clear_tail(buf ^ 1);
-            __builtin_amdgcn_s_waitcnt(0);
-          }
-          meet<kSpread ? kPerB : 0>();  // all but the weights of block s + 2
-          if (!kSpread) {
-#pragma unroll
-            for (int x = 0; x < kPerA; ++x) send_a(x);
-#pragma unroll
-            for (int x = 0; x < kPerB; ++x) send_b(x);
+          if (LAST && s + 1 < steps && kb0 + s + 1 == full) clear_tail(buf1);
+          // the blocks behind the next may still be on their way
+          if (kTwice) {
+            if (LAST) wait_loads<0>();
+            meet<kPerB>();
+          } else if (LAST) {
+            const int left = steps - 2 - s;
+            if (left >= STAGES - 2) wait_loads<(STAGES - 2) * (kPerA + kPerB)>();
+            else if (STAGES > 4 && left == 2) wait_loads<2 * (kPerA + kPerB)>();
+            else if (STAGES > 3 && left == 1) wait_loads<kPerA + kPerB>();
+            else wait_loads<0>();
+            meet<(STAGES - 2) * (kPerA + kPerB)>();
+          } else {
+            meet<(STAGES - 2) * (kPerA + kPerB)>();
           }
           if (!kEach) {
 #pragma unroll
             for (int x = 0; x < kMt; ++x) na[x] = row_scale(s + 1, x);
           }
         }
-        if (kSpread && g / 2 == 1) {
-          constexpr int kNow = kPerB / (2 * kNt);
+        if (kTwice) {
+          constexpr int kNowA = kPerA / (2 * kNt), kNowB = kPerB / (2 * kNt);
+          if (g / 2 == 1)
 #pragma unroll
-          for (int x = 0; x < kNow; ++x) send_b(((g - 2) * kNt + i) * kNow + x);
-        }
-        if (kSpread && g >= kGroups - 2) {
-          constexpr int kNow = kPerA / (2 * kNt);
+            for (int x = 0; x < kNowB; ++x) send(kPerA + ((g - 2) * kNt + i) * kNowB + x);
+          if (g >= kGroups - 2)
 #pragma unroll
-          for (int x = 0; x < kNow; ++x) send_a(((g - kGroups + 2) * kNt + i) * kNow + x);
+            for (int x = 0; x < kNowA; ++x) send(((g - kGroups + 2) * kNt + i) * kNowA + x);
+        } else {
+          const int q = g * kNt + i, r = q >= kMeetAt ? q - kMeetAt : q + kSendHere;  // products since the meeting
+#pragma unroll
+          for (int x = 0; x < kCopies; ++x)
+            if (r < kSend && x >= r * kCopies / kSend && x < (r + 1) * kCopies / kSend) {
+              if (q >= kMeetAt) send(x);
+              else send_rest(x);
+            }
         }
         if (g == 0) fb[1][i] = operand(buf, BM + wn + 32 * i, 1);
-        if (g == kGroups - kAhead) fb[0][i] = operand(buf ^ 1, BM + wn + 32 * i, 0);
+        if (g == kGroups - kAhead) fb[0][i] = operand(buf1, BM + wn + 32 * i, 0);
         if (i == 0) {
           if (kEach && g >= kGroups - kAhead) ca[g - (kGroups - kAhead)] = row_scale(s + 1, g - (kGroups - kAhead));
           if (kEach && g == 0) ca[kMt - 1] = row_scale(s, kMt - 1);
-          fa[t % kSlots] = t < kGroups ? operand(buf, wm + 32 * (t % kMt), t / kMt) : operand(buf ^ 1, wm + 32 * (t % kMt), 0);
+          fa[t % kSlots] = t < kGroups ? operand(buf, wm + 32 * (t % kMt), t / kMt) : operand(buf1, wm + 32 * (t % kMt), 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         if (KIND == kScaleE8M0)
@@ -368,12 +439,13 @@ fp8_gemm_kernel(const GemmParams P) {
                                                                        0, 127, 0, 127);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (KIND == kScaleF32 && h == 1) {
-        const float f = __uint_as_float(ca[j]) * __uint_as_float(cb);
-#pragma unroll
-        for (int i = 0; i < kNt; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] += part[i][j][r] * f;
+      if (kDelay && (g == 0 || h == 1)) {
+        if (g == 0) join_tile(kMt - 1, join);
+        else if (j > 0) join_tile(j - 1, join);
+        if (h == 1) join = __uint_as_float(ca[j]) * __uint_as_float(cb);
+        __builtin_amdgcn_sched_barrier(0);
+      } else if (KIND == kScaleF32 && h == 1) {
+        join_tile(j, __uint_as_float(ca[j]) * __uint_as_float(cb));
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -381,27 +453,45 @@ fp8_gemm_kernel(const GemmParams P) {
 #pragma unroll
       for (int j = 0; j < kMt; ++j) ca[j] = na[j];
     }
+    buf = buf1;
   };
-  const int plain = min(steps, full - kb0) - 2;  // steps that send for a whole block
+  const int plain = min(steps, full - kb0) - STAGES;  // steps that send for a whole block
   int s = 0;
   for (; s < plain; ++s) step(s, std::false_type{});
   for (; s < steps; ++s) step(s, std::true_type{});
+  if (kDelay) join_tile(kMt - 1, join);
 
-  // lane (c32, half): row c32 of an activation tile, columns 8g + 4 half .. + 3 of a weight tile
+  // Lane (c32, half) holds row c32 of an activation tile, columns 8g + 4 half .. + 3 of a weight tile: 32 rows at a
+  // time they change places in LDS (a part of its own for each wave), so that a store takes 16 bytes a lane and whole rows.
+  // (From the registers, 8 bytes a lane and 32 rows to a store, 256 x 256 results took 10.8 us.)
+  constexpr int kSize = OUT == kOutBf16 ? 2 : 4, kEach16 = 16 / kSize, kPitch = WN * kSize + 16, kRowChunks = WN * kSize / 16;
+  static_assert(kWaves * 32 * kPitch <= STAGES * kStage, "the stages' place");
   if (P.splits > 1) out = static_cast<float*>(out) + (int64_t)split * P.m * P.n;
-  const bool aligned = !((reinterpret_cast<uintptr_t>(out) & (OUT == kOutBf16 ? 7 : 15)) | (out_stride & 3));
+  const bool aligned = !((reinterpret_cast<uintptr_t>(out) & 15) | (out_stride & (kEach16 - 1)));
+  meet<0>();
+  uint8_t* mine = smem + wave * 32 * kPitch;
 #pragma unroll
   for (int j = 0; j < kMt; ++j) {
-    const int m = m0 + wm + 32 * j + c32;
-    if (m >= P.m) continue;
 #pragma unroll
     for (int i = 0; i < kNt; ++i)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int n = n0 + wn + 32 * i + 8 * g + 4 * half;
-        const float v[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        if (n < P.n) store4<OUT>(out, (int64_t)m * out_stride + n, aligned && n + 4 <= P.n, P.n - n, v);
+        uint8_t* d = mine + c32 * kPitch + (32 * i + 8 * g + 4 * half) * kSize;
+        const v16f& v = acc[i][j];
+        if (OUT == kOutBf16)
+          *reinterpret_cast<v2i*>(d) = (v2i){pack2(v[4 * g], v[4 * g + 1]), pack2(v[4 * g + 2], v[4 * g + 3])};
+        else
+          *reinterpret_cast<v4f*>(d) = (v4f){v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
       }
+    wait_loads<63>();  // (LDS only; the wave's own accesses are in order)
+#pragma unroll
+    for (int x = 0; x < 32 * kRowChunks / 64; ++x) {
+      const int at16 = 64 * x + lane, row = at16 / kRowChunks, col = at16 % kRowChunks * kEach16;
+      const v4i v = *reinterpret_cast<const v4i*>(mine + row * kPitch + col * kSize);
+      const int m = m0 + wm + 32 * j + row, n = n0 + wn + col;
+      if (m < P.m && n < P.n) store16<OUT>(out, (int64_t)m * out_stride + n, aligned && n + kEach16 <= P.n, P.n - n, v);
+    }
+    wait_loads<63>();
   }
 }
 
@@ -457,10 +547,10 @@ int device_cus() {
   return n;
 }
 
-template <int BM, int BN, int WM, int WN, int KIND, int OUT>
+template <int BM, int BN, int WM, int WN, int STAGES, int KIND, int OUT>
 int launch_tile(GemmParams P, hipStream_t st) {
-  constexpr int kSmem = gemm_smem<BM, BN>();
-  auto kern = fp8_gemm_kernel<BM, BN, WM, WN, KIND, OUT>;
+  constexpr int kSmem = gemm_smem<BM, BN, STAGES, KIND>();
+  auto kern = fp8_gemm_kernel<BM, BN, WM, WN, STAGES, KIND, OUT>;
   if (kSmem > 64 * 1024) {
     const hipError_t e =
         hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kSmem);
@@ -477,10 +567,10 @@ int launch_tile(GemmParams P, hipStream_t st) {
 template <int KIND, int OUT>
 int launch_plan(const Plan& p, const GemmParams& P, hipStream_t st) {
   // f32 scales take a second set of accumulators: narrower tiles
-  if (p.bm == 256) return KIND == kScaleE8M0 ? launch_tile<256, 256, 128, 128, kScaleE8M0, OUT>(P, st) : launch_tile<256, 128, 64, 64, kScaleF32, OUT>(P, st);
-  if (p.bm == 128) return launch_tile<128, 128, 64, 64, KIND, OUT>(P, st);
-  if (p.bm == 64) return launch_tile<64, 128, 64, 32, KIND, OUT>(P, st);
-  return launch_tile<32, 64, 32, 32, KIND, OUT>(P, st);
+  if (p.bm == 256) return KIND == kScaleE8M0 ? launch_tile<256, 256, 128, 128, 2, kScaleE8M0, OUT>(P, st) : launch_tile<256, 128, 64, 64, 2, kScaleF32, OUT>(P, st);
+  if (p.bm == 128) return launch_tile<128, 128, 64, 64, 2, KIND, OUT>(P, st);
+  if (p.bm == 64) return launch_tile<64, 128, 64, 32, 2, KIND, OUT>(P, st);
+  return launch_tile<32, 64, 32, 32, 2, KIND, OUT>(P, st);
 }
 
 }  // namespace
