@@ -134,21 +134,25 @@ template <int KIND>
 __device__ __forceinline__ v4i load_scale_piece(const void* row, int i, int n) {
   constexpr int kSize = KIND == kScaleF32 ? 4 : 1;
   const uint8_t* p = static_cast<const uint8_t*>(row) + (int64_t)i * kSize;
-  v4i v = {0, 0, 0, 0};
+  uint64_t v[2] = {0, 0};
   if (i + 16 / kSize <= n) {
-    __builtin_memcpy(&v, p, 16);
+    __builtin_memcpy(v, p, 16);
   } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (KIND == kScaleF32) {
-        if (i + j < n) v[j] = reinterpret_cast<const int*>(p)[j];
-      } else {
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-          if (i + 4 * j + b < n) v[j] |= (int)((uint32_t)p[4 * j + b] << (8 * b));
+#pragma unroll 1
+    for (int j = 0; j < 8; j += kSize) {  // an element of each half
+      if (i + j / kSize < n) {
+        uint32_t x = 0;
+        __builtin_memcpy(&x, p + j, kSize);
+        v[0] |= (uint64_t)x << (8 * j);
       }
+      if (i + (j + 8) / kSize < n) {
+        uint32_t x = 0;
+        __builtin_memcpy(&x, p + 8 + j, kSize);
+        v[1] |= (uint64_t)x << (8 * j);
+      }
+    }
   }
-  return v;
+  return (v4i){(int)v[0], (int)(v[0] >> 32), (int)v[1], (int)(v[1] >> 32)};
 }
 
 // A tile of BM activation rows and BN weight rows; a wave takes WM x WN of it. STAGES blocks of both lie in
@@ -484,12 +488,22 @@ fp8_gemm_kernel(const GemmParams P) {
           *reinterpret_cast<v4f*>(d) = (v4f){v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
       }
     wait_loads<63>();  // (LDS only; the wave's own accesses are in order)
+    auto row_of = [&](int x) { return (64 * x + lane) / kRowChunks; };
+    auto col_of = [&](int x) { return (64 * x + lane) % kRowChunks * kEach16; };
+    auto held = [&](int x) { return *reinterpret_cast<const v4i*>(mine + row_of(x) * kPitch + col_of(x) * kSize); };
+    const int m = m0 + wm + 32 * j, n = n0 + wn;
+    constexpr int kStores = 32 * kRowChunks / 64;
+    if (aligned && n + WN <= P.n) {
+      uint8_t* to = static_cast<uint8_t*>(out) + ((int64_t)m * out_stride + n) * kSize;
 #pragma unroll
-    for (int x = 0; x < 32 * kRowChunks / 64; ++x) {
-      const int at16 = 64 * x + lane, row = at16 / kRowChunks, col = at16 % kRowChunks * kEach16;
-      const v4i v = *reinterpret_cast<const v4i*>(mine + row * kPitch + col * kSize);
-      const int m = m0 + wm + 32 * j + row, n = n0 + wn + col;
-      if (m < P.m && n < P.n) store16<OUT>(out, (int64_t)m * out_stride + n, aligned && n + kEach16 <= P.n, P.n - n, v);
+      for (int x = 0; x < kStores; ++x)
+        if (m + row_of(x) < P.m) *reinterpret_cast<v4i*>(to + (row_of(x) * out_stride + col_of(x)) * kSize) = held(x);
+    } else {
+#pragma unroll 1
+      for (int x = 0; x < kStores; ++x)
+        if (m + row_of(x) < P.m && n + col_of(x) < P.n)
+          store16<OUT>(out, (int64_t)(m + row_of(x)) * out_stride + n + col_of(x), aligned && n + col_of(x) + kEach16 <= P.n,
+                       P.n - n - col_of(x), held(x));
     }
     wait_loads<63>();
   }
