@@ -646,7 +646,7 @@ DSA_API int dsa_act_quant(const void* x, int64_t x_stride, int64_t rows, int dim
                           void* stream);
 
 /* Workspace bytes dsa_fp8_gemm needs for this shape on the current device (0: none). */
-DSA_API size_t dsa_fp8_gemm_workspace_bytes(int m, int n, int k);
+DSA_API size_t dsa_fp8_gemm_workspace_bytes(int m, int n, int k, int scale_kind);
 
 /* Product of block-scaled fp8 matrices:
  *   out[i, j] = sum_kb a_scale[i, kb] b_scale[j / 128, kb] sum_{t in block kb} a[i, t] b[j, t]

@@ -1137,8 +1137,8 @@ def act_quant(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.
     return codes, scales
 
 
-def fp8_gemm_workspace_bytes(m: int, n: int, k: int) -> int:
-    return int(_lib.load().dsa_fp8_gemm_workspace_bytes(int(m), int(n), int(k)))
+def fp8_gemm_workspace_bytes(m: int, n: int, k: int, scale_dtype: torch.dtype = torch.float8_e8m0fnu) -> int:
+    return int(_lib.load().dsa_fp8_gemm_workspace_bytes(int(m), int(n), int(k), _SCALE_KINDS[scale_dtype]))
 
 
 def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -1167,10 +1167,10 @@ def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
         out_stride = _rows2d(out, "out", (torch.bfloat16, torch.float32), (M, N))
         _gpu(a, out)
     if dev == _CURRENT_DEVICE():
-        need = (_lib._lib or _lib.load()).dsa_fp8_gemm_workspace_bytes(M, N, K)
+        need = (_lib._lib or _lib.load()).dsa_fp8_gemm_workspace_bytes(M, N, K, kind)
     else:  # the size goes by the current device's CUs
         with torch.cuda.device(dev):
-            need = fp8_gemm_workspace_bytes(M, N, K)
+            need = fp8_gemm_workspace_bytes(M, N, K, a_scale.dtype)
     ws_ptr, ws_bytes = None, 0
     if need:
         if (workspace is None or workspace.numel() * workspace.element_size() < need or workspace.data_ptr() % 16

@@ -62,12 +62,13 @@ def test_gemm_refusals(lib):
          [(0, P, 1), (0, TWO, 1), (1, 240, 1), (1, 264, 1), (2, P, 1), (2, TWO, 1), (3, 1, 1), (4, P, 1), (4, TWO, 1), (5, 240, 1),
           (5, 264, 1), (6, P, 1), (6, TWO, 1), (7, 1, 1), (8, 2, 1), (9, -1, 1), (9, 0, 0), (10, -1, 1), (10, 0, 0), (11, 0, 1),
           (11, 200, 2), (12, P, 1), (12, ODD, 1), (13, 299, 1)])
-    assert lib.dsa_fp8_gemm_workspace_bytes(0, 8, 8) == 0 and lib.dsa_fp8_gemm_workspace_bytes(8, 8, -1) == 0
+    assert lib.dsa_fp8_gemm_workspace_bytes(0, 8, 8, 0) == 0 and lib.dsa_fp8_gemm_workspace_bytes(8, 8, -1, 0) == 0
+    assert lib.dsa_fp8_gemm_workspace_bytes(8, 8, 8192, 2) == 0
 
 
 def test_gemm_refuses_a_workspace_too_small_or_unaligned(lib):
     m, n, k = 100, 256, 8192  # few tiles of many blocks: split over K
-    need = lib.dsa_fp8_gemm_workspace_bytes(m, n, k)
+    need = lib.dsa_fp8_gemm_workspace_bytes(m, n, k, 0)
     assert need > 0
     args = [ONE, k, ONE, 64, ONE, k, ONE, 64, 0, m, n, k, ONE, n, 0, ONE, need, P]
     _bad(lib, "dsa_fp8_gemm", args, [(15, P, 4), (16, need - 1, 4), (15, ctypes.c_void_p(24), 1)])
