@@ -566,7 +566,7 @@ constexpr Tile kTilesE8M0[] = {
 constexpr Tile kTilesF32[] = {
     {32, 64, 3, 3, 2.3f, 0.04f, 0.28f, 1.2f, 0.f},    {64, 64, 3, 2, 2.6f, 0.08f, 0.235f, 1.35f, 0.f},
     {64, 128, 2, 2, 2.1f, 0.085f, 0.41f, 1.7f, 0.f},  {64, 128, 3, 1, 2.2f, 0.38f, 0.f, 0.f, 2.4f},
-    {128, 128, 3, 1, 1.9f, 0.63f, 0.f, 3.9f, 0.f},    {256, 128, 2, 1, 0.55f, 1.05f, 0.f, 5.9f, 0.f}};
+    {256, 128, 2, 1, 0.55f, 1.05f, 0.f, 5.9f, 0.f}};
 // A second launch adds up the parts of K: so much, and more by their MB.
 constexpr float kSumBase = 2.9f, kSumPerMB[2] = {0.33f, 0.25f};
 
@@ -660,7 +660,6 @@ int launch_plan(const Plan& p, int kind, const GemmParams& P, int dev, hipStream
     case 1: return launch_tile<64, 64, 32, 32, 3, kScaleF32, OUT>(P, dev, st);
     case 2: return launch_tile<64, 128, 32, 64, 2, kScaleF32, OUT>(P, dev, st);
     case 3: return launch_tile<64, 128, 32, 64, 3, kScaleF32, OUT>(P, dev, st);
-    case 4: return launch_tile<128, 128, 64, 64, 3, kScaleF32, OUT>(P, dev, st);
     default: return launch_tile<256, 128, 64, 64, 2, kScaleF32, OUT>(P, dev, st);
   }
 }

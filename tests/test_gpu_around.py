@@ -176,6 +176,59 @@ def test_gemm_large(cuda, M, N, K, kind):
     check_product(out[rows], a[rows], sa[rows], b, sb)
 
 
+@pytest.mark.parametrize("M,N,K", [(33, 129, 16528), (1000, 1000, 8336), (130, 8200, 8848), (65, 8200, 16528), (257, 16400, 8336),
+                                   (1030, 2100, 8336), (2050, 2100, 1168), (500, 8200, 8848), (2050, 4100, 8336)])
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+def test_gemm_long(cuda, M, N, K, kind):
+    """More blocks of K than a wave's register of weight scales and the chunks of activation scales hold, a short
+    last one, whole and in parts, in every tile there is."""
+    print(f"gemm long {M} {N} {K} {kind}", flush=True)
+    a, sa, b, sb = product(gen(cuda, K), M, N, K, kind)
+    out = ops.fp8_gemm(a, sa, b, sb)
+    rows = torch.cat([torch.arange(0, M, 37, device=cuda), torch.arange(M - 33, M, device=cuda)])
+    check_product(out[rows], a[rows], sa[rows], b, sb)
+
+
+@pytest.mark.parametrize("K", [128, 1152])
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+def test_gemm_far_rows(cuda, K, kind):
+    """Rows whose offsets pass 32 bits, in the operands (2^23 bytes apart, the most) and in the result."""
+    print(f"gemm far {K} {kind}", flush=True)
+    M, N = 600, 40
+    a, sa, b, sb = product(gen(cuda, 9), M, N, K, kind)
+    want = ops.fp8_gemm(a, sa, b, sb)
+    check_product(want, a, sa, b, sb)
+    far = torch.empty(M << 23, dtype=torch.uint8, device=cuda).as_strided((M, K), (1 << 23, 1))
+    far.copy_(a.view(torch.uint8))
+    out = torch.empty((M << 22) + N, dtype=BF, device=cuda).as_strided((M, N), (1 << 22, 1))
+    assert torch.equal(ops.fp8_gemm(far, sa, b, sb, out=out), want)
+    # the weights' rows too: the product the other way round, with the activations' scales of the weights' rows
+    b2, sb2 = ops.act_quant(torch.randn(M, K, device=cuda, generator=gen(cuda, 10)).to(BF), scale_dtype=sb.dtype)
+    want = ops.fp8_gemm(b, sb.expand(N, -1).contiguous(), b2, sb2[:5].contiguous())
+    far.copy_(b2.view(torch.uint8))
+    assert torch.equal(ops.fp8_gemm(b, sb.expand(N, -1).contiguous(), far, sb2[:5].contiguous()), want)
+
+
+def test_far_rows_of_norm_and_rope(cuda):
+    """Rows 2^31 elements apart."""
+    g = gen(cuda, 12)
+    base = torch.empty((2 << 31) + 1024, dtype=BF, device=cuda)
+    x = base.as_strided((3, 1000), (1 << 31, 1))
+    near = rnd(g, 3, 1000).to(BF)
+    x.copy_(near)
+    w = rnd(g, 1000).to(BF)
+    want = ops.rms_norm(near, w, 1e-6)
+    assert torch.equal(ops.rms_norm(x, w, 1e-6), want)
+    for got, exp in zip(ops.act_quant(x), ops.act_quant(near)):
+        assert torch.equal(got.view(torch.uint8), exp.view(torch.uint8))
+    t, pos = table(cuda, 50, 64), torch.tensor([0, 7, 49], device=cuda)
+    q = base.as_strided((3, 5, 64), (1 << 31, 96, 1))
+    close = q.contiguous()
+    want = ops.rope(close, pos, t, out=torch.empty_like(close))
+    assert torch.equal(ops.rope(q, pos, t), want) and torch.equal(q, want)
+    assert torch.equal(ops.rms_norm(near, w, 1e-6, out=x), ops.rms_norm(near, w, 1e-6)) and x.stride(0) == 1 << 31
+
+
 def test_gemm_strides_and_neighbours(cuda):
     """Rows inside wider ones, outputs inside wider ones: what lies beside them stays."""
     g = gen(cuda, 6)
@@ -251,6 +304,39 @@ def test_rope_sizes(cuda, T, H, rot, head, pairs, out_pairs):
     assert torch.equal(k_all[..., :head + 8 - rot], kept[1][..., :head + 8 - rot])
     q1 = ops.rope(kept[0][..., head - rot:].contiguous(), pos, t, interleaved=pairs, out_interleaved=out_pairs)
     assert torch.equal(q1, outs[0])
+
+
+def test_rope_many_heads_a_lane(cuda):
+    """Enough tokens for several heads a lane, and a count of heads that these do not divide."""
+    for T, H, rot in ((8200, 7, 64), (4099, 17, 64), (8200, 9, 40), (40000, 3, 30), (20000, 1, 128)):
+        print(f"rope many {T} {H} {rot}", flush=True)
+        g = gen(cuda, T)
+        q, k = rnd(g, T, H, rot).to(BF), rnd(g, T, 1, rot + 8).to(BF)[..., 8:]
+        t, pos = table(cuda, 5000, rot), torch.randint(0, 5000, (T,), generator=g, device=cuda)
+        wants = [A.rope(x, t, pos, True, False) for x in (q, k)]
+        for got, (want, err) in zip(ops.rope(q, pos, t, k=k, interleaved=True, out_interleaved=False), wants):
+            assert A.within_bf16(got, want, err)
+
+
+def test_rope_heads_outside(cuda):
+    """Heads outside tokens in memory (a view [T, H, rot] of [H, T, rot]), in place and not."""
+    g = gen(cuda, 4)
+    x = rnd(g, 6, 33, 64).to(BF)
+    q, t, pos = x.transpose(0, 1), table(cuda, 64, 64), torch.arange(33, device=cuda)
+    want, err = A.rope(q, t, pos, True, True)
+    assert A.within_bf16(ops.rope(q, pos, t, out=torch.empty_like(q)), want, err)
+    assert A.within_bf16(ops.rope(q, pos, t), want, err)
+
+
+def test_rope_refuses_shared_outputs(cuda):
+    q, t, pos = torch.zeros(4, 1, 64, dtype=BF, device=cuda), table(cuda, 8, 64), torch.arange(4, device=cuda)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.rope(q.expand(4, 3, 64), pos, t)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.rope(q.clone(), pos, t, out=q[:1].expand(4, 1, 64))
+    # read alike, they are fine
+    got = ops.rope(q.expand(4, 3, 64), pos, t, out=torch.empty(4, 3, 64, dtype=BF, device=cuda))
+    assert torch.all(got == 0)
 
 
 def test_rope_empty(cuda):
