@@ -1,10 +1,11 @@
-"""The four DeepGEMM entry points the DSA indexer calls, on MI355X.
+"""The four DeepGEMM entry points the DSA indexer calls, and the block-scaled fp8 product, on MI355X.
 
 Same names, arguments and results as the calls at
 dlengine/runtime/layers/backends/dsa/indexer/lightning.py:633 (``get_num_sms``),
 :668-676 (``get_paged_mqa_logits_metadata``), :1395-1406
 (``fp8_paged_mqa_logits``) and :1212-1219 (``fp8_mqa_logits``, prefill), so the
-caller's code stays unchanged.
+caller's code stays unchanged. ``fp8_gemm_nt`` is the product that the projections
+around the attention go through.
 """
 from __future__ import annotations
 
@@ -75,3 +76,14 @@ def fp8_mqa_logits(q: torch.Tensor, kv: tuple[torch.Tensor, torch.Tensor], weigh
     out = torch.empty(q.shape[0], keys.shape[0], dtype=torch.float32, device=q.device)
     ops.mqa_logits(q, keys, scales, weights, cu_seq_len_k_start, cu_seq_len_k_end, out, clean_logits)
     return out
+
+
+def fp8_gemm_nt(a: tuple[torch.Tensor, torch.Tensor], b: tuple[torch.Tensor, torch.Tensor], d: torch.Tensor) -> None:
+    """d [M, N] (bf16 or f32) = a @ b.T of block-scaled fp8 matrices.
+
+    a = (codes [M, K] float8_e4m3fn, scales [M, ceil(K / 128)]); b = (codes [N, K], scales
+    [ceil(N / 128), ceil(K / 128)]); scales float32, in rows or in columns, or float8_e8m0fnu.
+    """
+    (x, sx), (w, sw) = a, b
+    rows = [s if s.dim() != 2 or s.stride(1) == 1 else s.contiguous() for s in (sx, sw)]
+    ops.fp8_gemm(x, rows[0], w, rows[1], out=d)
