@@ -496,10 +496,14 @@ fp8_gemm_kernel(const GemmParams P) {
     const int m = m0 + wm + 32 * j, n = n0 + wn;
     constexpr int kStores = 32 * kRowChunks / 64;
     if (aligned && n + WN <= P.n) {
+      // Results are streamed past the L2, where they would take the place of rows that neighbouring tiles share (8192 x
+      // 24576 x 1536 353 -> 318 us, f32 scales 504 -> 419; parts of K too, 333 x 2112 x
+      // 8192 20.0 -> 19.3).
       uint8_t* to = static_cast<uint8_t*>(out) + ((int64_t)m * out_stride + n) * kSize;
 #pragma unroll
       for (int x = 0; x < kStores; ++x)
-        if (m + row_of(x) < P.m) *reinterpret_cast<v4i*>(to + (row_of(x) * out_stride + col_of(x)) * kSize) = held(x);
+        if (m + row_of(x) < P.m)
+          __builtin_nontemporal_store(held(x), reinterpret_cast<v4i*>(to + (row_of(x) * out_stride + col_of(x)) * kSize));
     } else {
 #pragma unroll 1
       for (int x = 0; x < kStores; ++x)
