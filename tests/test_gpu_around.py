@@ -189,6 +189,22 @@ def test_gemm_long(cuda, M, N, K, kind):
     check_product(out[rows], a[rows], sa[rows], b, sb)
 
 
+@pytest.mark.parametrize("M,N,K", [(32, 8200, 1536), (3, 2112, 1168), (1, 31, 1008), (32, 33, 400), (5, 24576, 128), (9, 100, 96),
+                                   (1, 8192, 8192), (20, 4100, 3600), (32, 2112, 8208), (2, 576, 16400)])
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+def test_gemm_few_rows(cuda, M, N, K, kind):
+    """Few rows, on both sides of the choice between waves over K and tiles; an odd result in between others."""
+    print(f"gemm few {M} {N} {K} {kind}", flush=True)
+    ops_ = product(gen(cuda, M + K), M, N, K, kind)
+    want = ops.fp8_gemm(*ops_)
+    check_product(want, *ops_)
+    check_product(ops.fp8_gemm(*ops_, out_dtype=F32), *ops_)
+    wide = torch.full((M + 2, N + 3), 3.0, dtype=BF, device=cuda)
+    assert torch.equal(ops.fp8_gemm(*ops_, out=wide[1:M + 1, 1:N + 1]), want)
+    wide[1:M + 1, 1:N + 1] = 3.0
+    assert torch.all(wide == 3.0)
+
+
 @pytest.mark.parametrize("K", [128, 1152])
 @pytest.mark.parametrize("kind", ["f32", "e8m0"])
 def test_gemm_far_rows(cuda, K, kind):
