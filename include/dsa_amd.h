@@ -654,10 +654,12 @@ DSA_API size_t dsa_fp8_gemm_workspace_bytes(int m, int n, int k, int scale_kind)
  *   b        [n, k] e4m3fn, row stride b_stride bytes;  b_scale [ceil(n / 128), ceil(k / 128)]
  *   out      [m, n] bf16, or f32 when out_is_f32, row stride out_stride elements
  * Scales are of scale_kind, their strides in elements; float32 ones may be any numbers, byte
- * 255 of an e8m0 one is NaN. k a multiple of 16; a and b rows 16-byte aligned.
+ * 255 of an e8m0 one is NaN. k a multiple of 16; a and b rows 16-byte aligned and at most 2^23
+ * bytes apart.
  * Products of 64 neighbouring k are summed by the matrix instruction, which drops what lies
- * more than 13 bits below the largest of them; those sums are added in f32. A NaN code or
- * scale gives NaN in the rows or columns that it belongs to.
+ * more than 13 bits below the largest of them; those sums are added in f32. Two f32 scales are
+ * multiplied in f32 before a block's sum is multiplied by them. A NaN code or scale gives NaN in
+ * the rows or columns that it belongs to.
  * workspace: dsa_fp8_gemm_workspace_bytes, 16-byte aligned (NULL where that is 0); calls that
  * share one must be ordered. The result does not depend on what it held. Stands beside dsa_mqa_logits as the
  * second of DeepGEMM's fp8 products (its fp8_gemm_nt). */
@@ -675,7 +677,9 @@ DSA_API int dsa_fp8_gemm(const uint8_t* a, int64_t a_stride, const void* a_scale
  * Pair p of a head is dims (2p, 2p + 1) when interleaved, else (p, p + rot_dim / 2), and
  * (a, b) becomes (a cos - b sin, b cos + a sin); out_interleaved says the same of the output.
  * f32, rounded once. rot_dim even, at most 512; a multiple of 8 with 16-byte aligned rows
- * takes wide loads. An output is its input, with the same strides, or does not overlap it.
+ * takes wide loads. An output is its input, with the same strides, or does not overlap it; its
+ * rows lie apart, all heads of a token within its stride or all tokens of a head within its
+ * (inputs may repeat rows). Fewer than 2^31 heads of all tokens.
  * Beside dsa_indexer_q_prologue, whose rotation is fused for the indexer's own heads. */
 DSA_API int dsa_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads, void* q_out,
                      int64_t q_out_token_stride, int64_t q_out_head_stride, const void* k,

@@ -7,10 +7,29 @@
 //
 // The products run on v_mfma_scale_f32_32x32x64_f8f6f4 with the weights as its rows, so that
 // a lane ends up with one activation row's results for four neighbouring columns at a time.
-// A workgroup's tiles of a and b go straight from HBM into LDS, a block of 128 deep, two
-// buffers deep: while one is multiplied the next is on its way. A row's eight 16-byte pieces
+// e8m0 scales are the instruction's own, and all of K runs into one accumulator. f32 scales take a
+// second one: a block's sums times sa sb are added to the first by vector instructions.
+//
+// Three kernels share that: tiles staged through LDS; waves over K for up to 32 rows; and the
+// sum of a product's parts where K is split. A cost fitted to measurements chooses (plan_of).
+//
+// Tiles: a workgroup's blocks of 128 of a and b go straight from memory into LDS, two or three
+// blocks deep: while one is multiplied the others are on their way. A row's eight 16-byte pieces
 // are stored in the order piece ^ (row / 2 % 8): 16 rows' reads of one piece fall on different banks
-// (rows are half the banks' span apart; with row % 8 two of 16 met on each bank).
+// (rows are half the banks' span apart; with row % 8 two of 16 met on each bank: 1e8 conflict
+// cycles in 8192 x 8192 x 16384, now 2e6).
+//
+// What bounds it, measured: 8192 x 8192 x 16384 (e8m0) 745-765 us, 2.9 PFLOP/s, where the library's product with one
+// scale a matrix takes 720-765 on the same cards and one with a scale per 32 elements 1450. Products run in 79% of a
+// SIMD's cycles, and the clock gives way under their power: without any copies it takes 698, with all data in L2 780 of then
+// 811, without scales 3% less; persistent workgroups, which close the gaps between tiles, gain nothing. Steps that
+// took the first kernel's 1125 there: operands read ahead of their products 875, copies sent between products 840,
+// four waves of 128 x 128 rather than eight of 128 x 64 811, a main loop without rare branches and masks 744. f32
+// scales: 8192^3 575 us against 397 (second accumulators leave no room for waves of 128 x 128, and those of 64 x 64 read
+// twice as much LDS per product; a third stage, 128 x 64 a wave and other orders of the sums changed nothing or lost).
+// Short K is bound by a tile's start and end (256 x 256: 6.7 and 4 us around 12 steps of 1.4 for 8192 x 24576 x 1536,
+// 318 us); few tiles of long K by the steps of one tile (0.49 us for 128^3, one wave a SIMD) and the
+// second launch: 333 x 2112 x 8192, four parts of K, 15 + 4 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -181,8 +200,8 @@ fp8_gemm_kernel(const GemmParams P) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go to the eight XCDs in turn: each XCD takes a run of neighbouring tiles, in bands of four activation
-  // tiles, so that the tiles at work beside one L2 share their rows. (Against tiles dealt out one by one: 8192^3 / 2
-  // of work the same, 2048 x 8192 x 8192 4% less, 333 x 8192 x 8192 40 -> 60 us without.)
+  // tiles, so that the tiles at work beside one L2 share their rows. (Against tiles dealt out to the XCDs one by one, 2048 x 8192 x 8192 takes
+  // 4% less and 333 x 8192 x 8192 40 us rather than 60.)
   const int tiles = P.mtiles * P.ntiles;
   const int xcd = blockIdx.x & 7, share = gridDim.x >> 3, rest = gridDim.x & 7;
   const int at = xcd * share + min(xcd, rest) + (blockIdx.x >> 3);

@@ -10,6 +10,12 @@
 // and its largest magnitude four shuffles. Codes and the bf16 output are each rounded
 // once, from the same f32 y. The sum of squares is f32 in a fixed order: a row's results do
 // not depend on the rows beside it.
+//
+// Memory bounds the norm of many rows: 8192 x 8192 with residual, its sum, fp8 and bf16 out, 604 MB, in
+// 109-111 us (5.5 TB/s; a plain copy reaches 5.1). Few rows are one pass of latencies: 4 x 8192
+// in 4.0 us, of which an empty launch is more than half. A wave a row up to 512 elements, then as many
+// waves as give a lane one or two loads: 1000 x 512 in 3.1 us. Reading the weights before the sum made
+// nothing faster (4 rows 4.2 us either way). The rounding alone: 5001 x 1600, 24 MB, in 6.1-6.5 us.
 #include "dsa_common.h"
 #include "fp8_block.h"
 #include "../../include/dsa_amd.h"

@@ -35,7 +35,7 @@ def quantize_weight(weight: torch.Tensor, scale_dtype: torch.dtype = torch.float
     scale = full.abs().amax(dim=(1, 3)).clamp_min(2.0 ** -40) / 448.0
     if scale_dtype is torch.float8_e8m0fnu:
         bits = scale.view(torch.int32)  # positive: the exponent, one more where a fraction is left
-        byte = (bits >> 23) + ((bits & 0x7FFFFF) != 0).to(torch.int32)
+        byte = ((bits >> 23) + ((bits & 0x7FFFFF) != 0).to(torch.int32)).clamp_max(254)
         stored, scale = byte.to(torch.uint8).view(scale_dtype), (byte << 23).view(torch.float32)
     else:
         stored = scale
@@ -88,6 +88,12 @@ class MlaProjections:
         returns (q_idx [T, 64, 128] fp8, weights [T, 64] f32, q_mla [T, H, 576] bf16, residual): the step's arguments
         and the residual stream, which is ``residual`` itself, updated, or ``hidden`` where there is none yet."""
         T, rank, H = hidden.shape[0], self.q_rank, self.heads
+        q_idx = torch.empty(T, IDX_HEADS, ops.INDEXER_HEAD_DIM, dtype=torch.float8_e4m3fn, device=hidden.device)
+        weights = torch.empty(T, IDX_HEADS, dtype=torch.float32, device=hidden.device)
+        q_mla = torch.empty(T, H, ops.MLA_D_QK, dtype=torch.bfloat16, device=hidden.device)
+        stream = hidden if residual is None else residual
+        if T == 0:
+            return q_idx, weights, q_mla, stream
         h = torch.empty_like(hidden)
         coded = ops.rms_norm_quant(hidden, self.norm, self.eps, out=h, residual=residual, residual_out=residual,
                                    scale_dtype=self.scale_dtype)
@@ -96,7 +102,6 @@ class MlaProjections:
         kv = c.new_empty(T, ops.MLA_D_QK)
         ops.rms_norm(c[:, rank:rank + KV_RANK], self.kv_norm, self.eps, out=kv[:, :KV_RANK])
         q = self.q(*c_q).view(T, H, self.nope + ROT)
-        q_mla = c.new_empty(T, H, ops.MLA_D_QK)
         q_mla[..., :KV_RANK] = torch.bmm(q[..., :self.nope].transpose(0, 1), self.k_up).transpose(0, 1)
         at = rank + KV_RANK
         ops.rope(q[..., self.nope:], positions, self.cos_sin_cache, out=q_mla[..., KV_RANK:],
@@ -104,14 +109,12 @@ class MlaProjections:
         ops.mla_kv_store(kv, kv_cache, slot_mapping)
         ops.indexer_k_transform_store(c[:, at + ROT:], self.idx_norm, self.idx_bias, self.eps, positions,
                                       self.cos_sin_cache, indexer_cache, slot_mapping, page_size)
-        q_idx = torch.empty(T, IDX_HEADS, ops.INDEXER_HEAD_DIM, dtype=torch.float8_e4m3fn, device=hidden.device)
-        weights = torch.empty(T, IDX_HEADS, dtype=torch.float32, device=hidden.device)
         ops.indexer_q_prologue(self.idx_q(*c_q).view(T, IDX_HEADS, ops.INDEXER_HEAD_DIM), h @ self.idx_gate.t(),
                                IDX_HEADS ** -0.5 * ops.INDEXER_HEAD_DIM ** -0.5, self.cos_sin_cache, positions, q_idx,
                                weights, self.interleaved)
-        return q_idx, weights, q_mla, hidden if residual is None else residual
+        return q_idx, weights, q_mla, stream
 
     def output(self, o: torch.Tensor) -> torch.Tensor:
         """The step's attention output [T, H, 512] bf16 -> [T, D] bf16."""
-        v = torch.bmm(o.transpose(0, 1), self.v_up).transpose(0, 1).reshape(o.shape[0], -1)
+        v = torch.bmm(o.transpose(0, 1), self.v_up).transpose(0, 1).flatten(1)
         return self.o(*ops.act_quant(v, scale_dtype=self.scale_dtype))

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from nanoengine_amd import _lib, ops
+from nanoengine_amd import _lib, deep_gemm, ops, projections
 from oracle import around_oracle as A
 
 ONE = ctypes.c_void_p(16)   # a non-null, aligned address that is never dereferenced
@@ -13,6 +13,7 @@ ODD = ctypes.c_void_p(17)
 TWO = ctypes.c_void_p(18)
 P = None
 BF, FP8, E8M0, F32 = torch.bfloat16, torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.float32
+KINDS = {"f32": F32, "e8m0": E8M0}
 
 
 @pytest.fixture(scope="module")
@@ -62,6 +63,8 @@ def test_gemm_refusals(lib):
          [(0, P, 1), (0, TWO, 1), (1, 240, 1), (1, 264, 1), (2, P, 1), (2, TWO, 1), (3, 1, 1), (4, P, 1), (4, TWO, 1), (5, 240, 1),
           (5, 264, 1), (6, P, 1), (6, TWO, 1), (7, 1, 1), (8, 2, 1), (9, -1, 1), (9, 0, 0), (10, -1, 1), (10, 0, 0), (11, 0, 1),
           (11, 200, 2), (12, P, 1), (12, ODD, 1), (13, 299, 1)])
+    far = 2 ** 23 + 16
+    _bad(lib, "dsa_fp8_gemm", args, [(1, far, 2), (5, far, 2), (1, 2 ** 40, 2)])
     assert lib.dsa_fp8_gemm_workspace_bytes(0, 8, 8, 0) == 0 and lib.dsa_fp8_gemm_workspace_bytes(8, 8, -1, 0) == 0
     assert lib.dsa_fp8_gemm_workspace_bytes(8, 8, 8192, 2) == 0
 
@@ -80,6 +83,8 @@ def test_rope_refusals(lib):
          [(0, P, 1), (0, ODD, 1), (3, -1, 1), (4, P, 1), (4, ODD, 1), (7, P, 1), (7, ODD, 1), (10, -1, 1), (11, P, 1), (11, ODD, 1),
           (14, -1, 1), (14, 2 ** 31, 1), (14, 0, 0), (15, 63, 1), (15, 0, 1), (15, 514, 2), (16, P, 1), (16, TWO, 1), (17, 0, 1),
           (18, P, 1), (18, TWO, 1)])
+    # output rows that share elements: of heads, of tokens, of the key; and more heads than an index holds
+    _bad(lib, "dsa_rope", args, [(6, 0, 1), (6, 63, 1), (5, 0, 1), (5, 639, 1), (12, 0, 1), (12, 63, 1), (14, 2 ** 28, 2)])
     a = list(args)
     a[18], a[19] = ctypes.c_void_p(20), 1  # int64 positions at a 4-byte address
     assert lib.dsa_rope(*a) == 1
@@ -119,6 +124,35 @@ def test_adapters_refuse_bad_tensors():
                       ({"k": q[..., :32]}, "k must be"), ({"k_out": q}, "needs k"), ({"k": q[:, :1], "k_out": q}, "k_out"), ({}, "GPU only")):
         with pytest.raises(RuntimeError, match=match):
             ops.rope(**{**dict(q=q, positions=pos, cos_sin_cache=t), **kw})
+
+
+def test_layer_refuses_weights_that_do_not_fit():
+    D, rank, H, nope, v = 256, 128, 2, 64, 32
+    shapes = dict(norm=(D,), a=(rank + 704, D), q_norm=(rank,), kv_norm=(512,), q=(H * (nope + 64), rank), k_up=(H, nope, 512),
+                  v_up=(H, 512, v), o=(D, H * v), idx_q=(8192, rank), idx_gate=(64, D), idx_norm=(128,), idx_bias=(128,))
+    good = {k: torch.zeros(s) for k, s in shapes.items()}
+    layer = projections.MlaProjections(**good, cos_sin_cache=torch.zeros(8, 64))
+    assert layer.q.codes.shape == (H * (nope + 64), rank) and layer.a.scales.shape == (7, 2)
+    for name in ("a", "kv_norm", "q", "k_up", "v_up", "o", "idx_q", "idx_gate"):
+        with pytest.raises(ValueError, match="must be"):
+            projections.MlaProjections(**{**good, name: good[name][..., 1:]}, cos_sin_cache=torch.zeros(8, 64))
+    with pytest.raises(ValueError, match="scale_dtype"):
+        projections.quantize_weight(good["a"], torch.float16)
+    x, s = torch.zeros(3, 256, dtype=FP8), torch.zeros(3, 2)
+    with pytest.raises(RuntimeError, match="share K"):
+        deep_gemm.fp8_gemm_nt((x, s), (x[:, :128], s[:1, :1]), torch.zeros(3, 3))
+
+
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+def test_weights_are_rounded_by_the_rule_of_activations(kind):
+    w = torch.randn(200, 300, generator=torch.Generator().manual_seed(0))
+    w[:128, 128:256] = 0
+    codes, scales = projections.quantize_weight(w, KINDS[kind])
+    want = A.scale_values(A.quantise_weight(w, kind)[1])
+    assert torch.all((A.scale_values(scales) - want).abs() <= (2 * A.EPS32 if kind == "f32" else 0) * want)
+    full = A.scale_values(scales).repeat_interleave(128, 0)[:200].repeat_interleave(128, 1)[:, :300]
+    tol = torch.maximum(A.HALF_FP8 * w.double().abs(), 2.0 ** -10 * full) * (1 + 3 * A.EPS32) + 3 * A.EPS32 * w.double().abs()
+    assert torch.all((codes.double() * full - w.double()).abs() <= tol)
 
 
 # ------------------------------------------------------------------ the oracle's format

@@ -193,6 +193,57 @@ def test_two_streams_at_once(cuda):
         assert all(torch.equal(o, want[i]) for o in got[i])
 
 
+def test_split_product_captured(cuda):
+    """A product in parts of K, whose workspace comes from the graph's pool: replays between eager calls of the same, with
+    inputs that change under the graph."""
+    g = torch.Generator(device=cuda).manual_seed(8)
+    xs = [torch.randn(100, 8192, generator=g, device=cuda).to(BF) for _ in range(2)]
+    w = projections.Fp8Linear(torch.randn(300, 8192, generator=g, device=cuda))
+    assert ops.fp8_gemm_workspace_bytes(100, 300, 8192) > 0
+    want = [w(*ops.act_quant(x)) for x in xs]
+    x, out = xs[0].clone(), torch.empty(100, 300, dtype=BF, device=cuda)
+    codes, scales = ops.act_quant(x)
+    torch.cuda.synchronize()
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        w(*ops.act_quant(x, codes, scales), out=out)
+        with torch.cuda.graph(graph, stream=s):
+            w(*ops.act_quant(x, codes, scales), out=out)
+    torch.cuda.synchronize()
+    for turn in range(4):
+        x.copy_(xs[turn % 2])
+        out.zero_()
+        other = w(*ops.act_quant(xs[1 - turn % 2]))
+        graph.replay()
+        assert torch.equal(w(*ops.act_quant(xs[1 - turn % 2])), want[1 - turn % 2])
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[turn % 2]) and torch.equal(other, want[1 - turn % 2])
+
+
+def test_no_tokens(cuda):
+    layer, _ = make_layer(cuda, E8M0)
+    b = Batch(cuda)
+    none = torch.empty(0, dtype=torch.int64, device=cuda)
+    before = b.kv.clone()
+    q_idx, w, q, _ = layer.inputs(b.x0[:0], None, none, none, b.kv, b.idx)
+    assert q_idx.shape == (0, 64, 128) and w.shape == (0, 64) and q.shape == (0, H, 576)
+    assert layer.output(torch.empty(0, H, 512, dtype=BF, device=cuda)).shape == (0, D) and torch.equal(b.kv, before)
+
+
+def test_padded_tokens_write_nothing(cuda):
+    """Rows of a padded batch (slot -1, any position, NaN in the hidden states) leave the caches and the other rows alone."""
+    layer, _ = make_layer(cuda, E8M0)
+    b, c = Batch(cuda), Batch(cuda)
+    pos, slots = b.before[:5], b.slots(b.seq, b.before)[:5]
+    want = layer.inputs(b.x0[:5], None, pos, slots, b.kv, b.idx)
+    x = torch.cat([b.x0[:5], torch.full((3, D), float("nan"), dtype=BF, device=cuda)])
+    pad = torch.tensor([-1, 7 * CTX, 0], device=cuda)
+    got = layer.inputs(x, None, torch.cat([pos, pad]), torch.cat([slots, torch.full_like(pad, -1)]), c.kv, c.idx)
+    for w, g in zip(want[:3], got[:3]):
+        assert torch.equal(w.view(torch.uint8), g[:5].view(torch.uint8))
+    assert torch.equal(b.kv, c.kv) and torch.equal(b.idx, c.idx)
+
+
 def test_fp8_gemm_nt(cuda):
     g = torch.Generator(device=cuda).manual_seed(6)
     for kind, dtype in ((F32, BF), (E8M0, F32)):
