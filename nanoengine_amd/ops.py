@@ -8,6 +8,8 @@ synchronises the host, so the calls are capturable in a HIP graph.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -474,12 +476,12 @@ def _rope_cache(cos_sin_cache: torch.Tensor) -> torch.Tensor:
 
 
 def _positions(positions: torch.Tensor, n: int) -> tuple[torch.Tensor, int]:
-    if not (positions.dim() == 1 and positions.shape[0] == n):
+    s, dtype = positions.shape, positions.dtype
+    if not (len(s) == 1 and s[0] == n):
         _fail(f"positions must be 1-D of length {n}")
-    if not (positions.dtype in (torch.int32, torch.int64)):
-        _fail(f"positions dtype {positions.dtype}")
-    p = positions.contiguous()
-    return p, int(p.dtype == torch.int64)
+    if not (dtype is torch.int32 or dtype is torch.int64):
+        _fail(f"positions dtype {dtype}")
+    return positions if positions.is_contiguous() else positions.contiguous(), int(dtype is torch.int64)
 
 
 def indexer_q_prologue(query: torch.Tensor, gate_weight: torch.Tensor, weight_scale: float,
@@ -777,7 +779,10 @@ def _launch(index: int, name: str, *args) -> None:
         with torch.cuda.device(index):
             _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
     elif _RAW_STREAM is not None:
-        _lib.call(name, *args, _RAW_STREAM(index))
+        # (_lib.call without packing the arguments once more)
+        status = getattr(_lib._lib or _lib.load(), name)(*args, _RAW_STREAM(index))
+        if status != 0:
+            _lib.check(status, name)
     else:
         _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
 
@@ -1044,15 +1049,20 @@ _SCALE_KINDS = {torch.float32: 0, torch.float8_e8m0fnu: 1, torch.uint8: 1}
 
 def _rows2d(t: torch.Tensor, name: str, dtypes, shape=None) -> int:
     """Row stride of a 2-D tensor with a contiguous last dim, of this shape where one is given."""
-    s, st = t.shape, t.stride()
-    if not (len(s) == 2 and t.dtype in dtypes and (st[1] == 1 or s[1] == 1) and (shape is None or s == shape)):
-        want = "2-D" if shape is None else str(list(shape))
-        _fail(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)} {want} with a contiguous "
-              f"last dim, got {t.dtype} {tuple(s)}")
-    return st[0] if s[0] > 1 else s[1]
+    s = t.shape
+    if t.dtype in dtypes and (len(s) == 2 if shape is None else s == shape):
+        if t.is_contiguous():
+            return s[1]
+        st = t.stride()
+        if st[1] == 1 or s[1] == 1:
+            return st[0] if s[0] > 1 else s[1]
+    want = "2-D" if shape is None else str(list(shape))
+    _fail(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)} {want} with a contiguous "
+          f"last dim, got {t.dtype} {tuple(s)}")
 
 
 _BF16 = (torch.bfloat16,)
+_WEIGHTS = (torch.bfloat16, torch.float32)
 
 
 def _coded(rows: int, dim: int, codes: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, int]:
@@ -1068,28 +1078,32 @@ def _norm(x, weight, eps, out, residual, residual_out, codes, scales) -> None:
     stride = _rows2d(x, "x", _BF16)
     shape = x.shape
     rows, dim = shape
-    if not (weight.dim() == 1 and weight.shape[0] == dim and weight.dtype in (torch.bfloat16, torch.float32)
-            and weight.is_contiguous()):
+    if not (weight.shape == (dim,) and weight.dtype in _WEIGHTS and weight.is_contiguous()):
         _fail(f"weight must be contiguous bfloat16 or float32 [{dim}]")
     tensors = [x, weight]
     res_stride = sum_stride = out_stride = code_stride = scale_stride = kind = 0
+    res_ptr = sum_ptr = out_ptr = code_ptr = scale_ptr = None
     if residual is not None:
         res_stride = _rows2d(residual, "residual", _BF16, shape)
+        res_ptr = residual.data_ptr()
         tensors.append(residual)
     if residual_out is not None:
         if residual is None:
             _fail("residual_out needs a residual")
-        sum_stride = _rows2d(residual_out, "residual_out", _BF16, shape)
+        sum_stride = res_stride if residual_out is residual else _rows2d(residual_out, "residual_out", _BF16, shape)
+        sum_ptr = residual_out.data_ptr()
         tensors.append(residual_out)
     if out is not None:
         out_stride = _rows2d(out, "out", _BF16, shape)
+        out_ptr = out.data_ptr()
         tensors.append(out)
     if codes is not None:
         code_stride, scale_stride, kind = _coded(rows, dim, codes, scales)
+        code_ptr, scale_ptr = codes.data_ptr(), scales.data_ptr()
         tensors += (codes, scales)
-    _launch(_gpu(*tensors), "dsa_rms_norm", x.data_ptr(), stride, _ptr(residual), res_stride, _ptr(residual_out),
-            sum_stride, weight.data_ptr(), int(weight.dtype is torch.float32), float(eps), rows, dim, _ptr(out),
-            out_stride, _ptr(codes), code_stride, _ptr(scales), scale_stride, kind)
+    _launch(_gpu(*tensors), "dsa_rms_norm", x.data_ptr(), stride, res_ptr, res_stride, sum_ptr, sum_stride,
+            weight.data_ptr(), int(weight.dtype is torch.float32), float(eps), rows, dim, out_ptr, out_stride, code_ptr,
+            code_stride, scale_ptr, scale_stride, kind)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, out: torch.Tensor | None = None, *,
@@ -1120,7 +1134,8 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, codes: tor
     """``rms_norm`` rounded to fp8 by blocks of 128: codes [T, D] float8_e4m3fn and scales [T, ceil(D / 128)],
     float32 (amax / 448) or float8_e8m0fnu (the power of two above), the operands of ``fp8_gemm``. ``out`` receives
     the bf16 norm too when given. ``scale_dtype`` is that of scales that are not given (see dsa_rms_norm)."""
-    codes, scales = _new_codes(x, codes, scales, scale_dtype)
+    if codes is None or scales is None:
+        codes, scales = _new_codes(x, codes, scales, scale_dtype)
     _norm(x, weight, eps, out, residual, residual_out, codes, scales)
     return codes, scales
 
@@ -1128,7 +1143,8 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, codes: tor
 def act_quant(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None, *,
               scale_dtype: torch.dtype = torch.float8_e8m0fnu) -> tuple[torch.Tensor, torch.Tensor]:
     """x [T, D] bf16 (row stride free) rounded to fp8 by blocks of 128, as in ``rms_norm_quant`` (see dsa_act_quant)."""
-    codes, scales = _new_codes(x, codes, scales, scale_dtype)
+    if codes is None or scales is None:
+        codes, scales = _new_codes(x, codes, scales, scale_dtype)
     stride = _rows2d(x, "x", _BF16)
     rows, dim = x.shape
     code_stride, scale_stride, kind = _coded(rows, dim, codes, scales)
@@ -1139,6 +1155,13 @@ def act_quant(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.
 
 def fp8_gemm_workspace_bytes(m: int, n: int, k: int, scale_dtype: torch.dtype = torch.float8_e8m0fnu) -> int:
     return int(_lib.load().dsa_fp8_gemm_workspace_bytes(int(m), int(n), int(k), _SCALE_KINDS[scale_dtype]))
+
+
+@functools.lru_cache(maxsize=4096)
+def _gemm_workspace(device: int, m: int, n: int, k: int, scale_dtype: torch.dtype) -> int:
+    """``fp8_gemm_workspace_bytes`` on a device: it goes by the device's CUs, and asking takes a tenth of a small call."""
+    with torch.cuda.device(device):
+        return fp8_gemm_workspace_bytes(m, n, k, scale_dtype)
 
 
 def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
@@ -1166,11 +1189,7 @@ def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     else:
         out_stride = _rows2d(out, "out", (torch.bfloat16, torch.float32), (M, N))
         _gpu(a, out)
-    if dev == _CURRENT_DEVICE():
-        need = (_lib._lib or _lib.load()).dsa_fp8_gemm_workspace_bytes(M, N, K, kind)
-    else:  # the size goes by the current device's CUs
-        with torch.cuda.device(dev):
-            need = fp8_gemm_workspace_bytes(M, N, K, a_scale.dtype)
+    need = _gemm_workspace(dev, M, N, K, a_scale.dtype)
     ws_ptr, ws_bytes = None, 0
     if need:
         if (workspace is None or workspace.numel() * workspace.element_size() < need or workspace.data_ptr() % 16
@@ -1203,31 +1222,34 @@ def rope(q: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor, 
     other (``interleaved``) or in halves, in the output as in the input unless ``out_interleaved`` says
     otherwise. ``out`` and ``k_out`` default to q and k (in place). Returns out, or (out, k_out) (see dsa_rope)."""
     q_t, q_h = _heads3d(q, "q")
-    T, H, rot = q.shape
+    shape = q.shape
+    T, H, rot = shape
     if out is None or out is q:
         out, o_t, o_h = q, q_t, q_h
     else:
-        o_t, o_h = _heads3d(out, "out", q.shape)
+        o_t, o_h = _heads3d(out, "out", shape)
     table = cos_sin_cache if cos_sin_cache.dim() == 2 else cos_sin_cache.reshape(cos_sin_cache.shape[0], -1)
-    if not (table.shape[1] == rot and table.dtype is torch.float32 and table.is_contiguous()):
+    max_pos, width = table.shape
+    if not (width == rot and table.dtype is torch.float32 and table.is_contiguous()):
         _fail(f"cos_sin_cache must be contiguous float32 [max_pos, {rot}], got {table.dtype} {tuple(cos_sin_cache.shape)}")
     pos, wide = _positions(positions, T)
     tensors = [q, out, table, pos]
     k_args = (None, 0, 0, 0, None, 0, 0)
     if k is not None:
         k_t, k_h = _heads3d(k, "k")
-        Hk = k.shape[1]
-        if k.shape != (T, Hk, rot):
-            _fail(f"k must be bfloat16 [{T}, Hk, {rot}], got {tuple(k.shape)}")
+        k_shape = k.shape
+        Hk = k_shape[1]
+        if k_shape[0] != T or k_shape[2] != rot:
+            _fail(f"k must be bfloat16 [{T}, Hk, {rot}], got {tuple(k_shape)}")
         if k_out is None or k_out is k:
             k_out, ko_t, ko_h = k, k_t, k_h
         else:
-            ko_t, ko_h = _heads3d(k_out, "k_out", k.shape)
+            ko_t, ko_h = _heads3d(k_out, "k_out", k_shape)
         tensors += (k, k_out)
         k_args = (k.data_ptr(), k_t, k_h, Hk, k_out.data_ptr(), ko_t, ko_h)
     elif k_out is not None:
         _fail("k_out needs k")
     _launch(_gpu(*tensors), "dsa_rope", q.data_ptr(), q_t, q_h, H, out.data_ptr(), o_t, o_h, *k_args, T, rot,
-            table.data_ptr(), table.shape[0], pos.data_ptr(), wide, int(bool(interleaved)),
+            table.data_ptr(), max_pos, pos.data_ptr(), wide, int(bool(interleaved)),
             int(bool(interleaved if out_interleaved is None else out_interleaved)))
     return out if k is None else (out, k_out)
