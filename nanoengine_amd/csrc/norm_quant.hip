@@ -12,10 +12,10 @@
 // not depend on the rows beside it.
 //
 // Memory bounds the norm of many rows: 8192 x 8192 with residual, its sum, fp8 and bf16 out, 604 MB, in
-// 109-111 us (5.5 TB/s; a plain copy reaches 5.1). Few rows are one pass of latencies: 4 x 8192
+// 105 us (5.8 TB/s; a plain copy reaches 5.1). Few rows are one pass of latencies: 4 x 8192
 // in 4.0 us, of which an empty launch is more than half. A wave a row up to 512 elements, then as many
 // waves as give a lane one or two loads: 1000 x 512 in 3.1 us. Reading the weights before the sum made
-// nothing faster (4 rows 4.2 us either way). The rounding alone: 5001 x 1600, 24 MB, in 6.1-6.5 us.
+// nothing faster (4 rows 4.2 us either way). The rounding alone: 5001 x 1600, 24 MB, in 5.9 us.
 #include "dsa_common.h"
 #include "fp8_block.h"
 #include "../../include/dsa_amd.h"
@@ -63,10 +63,12 @@ __device__ __forceinline__ v4i load8(const uint16_t* row, int i, int n) {
   return r;
 }
 
+// Outputs are streamed past the L2, which has nothing more to do with them (8192 x 8192 110 -> 105 us, 5001 x 1600 6.5 -> 5.9;
+// inputs read so cost more, 118 and 7.0).
 template <bool VEC>
 __device__ __forceinline__ void store8(uint16_t* row, int i, int n, v4i v) {
   if (VEC) {
-    if (i < n) *reinterpret_cast<v4i*>(row + i) = v;
+    if (i < n) __builtin_nontemporal_store(v, reinterpret_cast<v4i*>(row + i));
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -94,7 +96,7 @@ __device__ __forceinline__ v4i pack8(const float* x) {
 template <bool VEC>
 __device__ __forceinline__ void store_codes(uint8_t* row, int i, int n, uint2 c) {
   if (VEC) {
-    if (i < n) *reinterpret_cast<uint2*>(row + i) = c;
+    if (i < n) __builtin_nontemporal_store((uint64_t)c.y << 32 | c.x, reinterpret_cast<uint64_t*>(row + i));
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)

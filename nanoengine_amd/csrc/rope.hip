@@ -10,8 +10,8 @@
 // A lane takes four pairs of a token (eight neighbouring lanes a line of 128 bytes of a head
 // of 64) and turns them in HEADS heads with one read of their cosines and sines. f32
 // arithmetic, one rounding to bf16. What bounds it is memory for many rows and the launch
-// for few: 8192 tokens x 129 heads of 64 in rows of 192, 270 MB, in 60 us (4.5 TB/s; scaling the
-// same parts of rows in place takes 52); 4 tokens of 128 heads in 2.9 us, most of which is a launch.
+// for few: 8192 tokens x 129 heads of 64 in rows of 192, 270 MB, in 59 us (4.5 TB/s; a plain copy
+// of whole rows reaches 5.1); 4 tokens of 128 heads in 2.9 us, most of which is a launch.
 #include "dsa_common.h"
 #include "../../include/dsa_amd.h"
 
@@ -23,7 +23,7 @@ constexpr int kMaxRot = 512;  // a row within one wave
 // From as many lanes as the card holds at a time (256 CUs of 2048), a lane takes four heads:
 // the loads in flight that a lane's second turn would have given, and a quarter of the
 // positions and angles read. 8192 tokens x 129 heads of 64: 65 us against 81 with one head a
-// lane (two: 68, eight: 75; all before neighbours shared their stores); 1024: 9.2 and 9.9. Below, more lanes hide more:
+// lane (two: 68, eight: 75; all with warm caches and before what load_pairs says); 1024: 9.2 and 9.9. Below, more lanes hide more:
 // 128 x 129, 4.2 and 3.5.
 constexpr int64_t kManyLanes = 256 * 2048;
 constexpr int kManyHeads = 4;
@@ -59,20 +59,21 @@ __device__ __forceinline__ int neighbour(int v) { return __builtin_amdgcn_mov_dp
 
 // Pairs p .. p + 3 of a row (half = rot / 2 pairs). VEC: rot a multiple of eight, rows 16-byte aligned.
 // Halves take 8 bytes a lane from each; where half is a multiple of eight, two neighbouring lanes share 16 of one half
-// and 16 of the other (8192 tokens x 129 heads, stored so: 60 us against 65).
+// and 16 of the other (8192 tokens x 129 heads, stored so: 70 us against 73). Each element is read once, past the L2:
+// 70 -> 59 (stores past it too: 63).
 template <bool PAIRS, bool VEC>
 __device__ __forceinline__ void load_pairs(const uint16_t* row, int p, int half, float* a, float* b) {
   if (VEC) {
     if (p >= half) return;
     if (PAIRS) {
-      const v4i v = *reinterpret_cast<const v4i*>(row + 2 * p);
+      const v4i v = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(row + 2 * p));
 #pragma unroll
       for (int j = 0; j < 4; ++j) a[j] = lo_f32(v[j]), b[j] = hi_f32(v[j]);
     } else {
       v2i u, w;
       if (half % 8 == 0) {
         const bool odd = p & 4;
-        const v4i own = *reinterpret_cast<const v4i*>(row + (odd ? half + p - 4 : p));
+        const v4i own = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(row + (odd ? half + p - 4 : p)));
         const int got0 = neighbour(odd ? own[0] : own[2]), got1 = neighbour(odd ? own[1] : own[3]);
         u = odd ? (v2i){got0, got1} : (v2i){own[0], own[1]};
         w = odd ? (v2i){own[2], own[3]} : (v2i){got0, got1};
