@@ -12,10 +12,10 @@
 // not depend on the rows beside it.
 //
 // Memory bounds the norm of many rows: 8192 x 8192 with residual, its sum, fp8 and bf16 out, 604 MB, in
-// 105 us (5.8 TB/s; a plain copy reaches 5.1). Few rows are one pass of latencies: 4 x 8192
-// in 4.0 us, of which an empty launch is more than half. A wave a row up to 512 elements, then as many
-// waves as give a lane one or two loads: 1000 x 512 in 3.1 us. Reading the weights before the sum made
-// nothing faster (4 rows 4.2 us either way). The rounding alone: 5001 x 1600, 24 MB, in 5.9 us.
+// 102 us (5.9 TB/s; a plain copy reaches 5.1). Few rows are one pass of latencies: 4 x 8192
+// in 3.8 us, of which an empty launch is more than half. A wave a row up to 512 elements (1000 x 512 in
+// 2.9 us), then as many waves as give a lane one load up to 8192 (with half as many waves 4 x 8192 takes 4.2 and
+// 8192 x 8192 105). Reading the weights before the sum made nothing faster. The rounding alone: 5001 x 1600, 24 MB, in 5.9 us.
 #include "dsa_common.h"
 #include "fp8_block.h"
 #include "../../include/dsa_amd.h"
@@ -221,8 +221,8 @@ void norm_by_dim(const NormParams& P, bool vec, bool wf32, hipStream_t st) {
   const int lanes = (P.dim + kLane - 1) / kLane;
   if (lanes <= 64) launch_norm<64, 1, KIND>(P, vec, wf32, st);
   else if (lanes <= 256) launch_norm<256, 1, KIND>(P, vec, wf32, st);
-  else if (lanes <= 512) launch_norm<256, 2, KIND>(P, vec, wf32, st);
-  else if (lanes <= 1024) launch_norm<512, 2, KIND>(P, vec, wf32, st);
+  else if (lanes <= 512) launch_norm<512, 1, KIND>(P, vec, wf32, st);
+  else if (lanes <= 1024) launch_norm<1024, 1, KIND>(P, vec, wf32, st);
   else if (lanes <= 2048) launch_norm<1024, 2, KIND>(P, vec, wf32, st);
   else launch_norm<1024, 4, KIND>(P, vec, wf32, st);
 }
