@@ -25,10 +25,9 @@
 // 811, without scales 3% less; persistent workgroups, which close the gaps between tiles, gain nothing. Steps that
 // took the first kernel's 1125 there: operands read ahead of their products 875, copies sent between products 840,
 // four waves of 128 x 128 rather than eight of 128 x 64 811, a main loop without rare branches and masks 744. f32
-// scales: 8192^3 575 us against 397 (second accumulators leave no room for waves of 128 x 128, and those of 64 x 64 read
-// twice as much LDS per product; a third stage, 128 x 64 a wave and other orders of the sums changed nothing or lost).
-// Short K is bound by a tile's start and end (256 x 256: 6.7 and 4 us around 12 steps of 1.4 for 8192 x 24576 x 1536,
-// 318 us); few tiles of long K by the steps of one tile (0.49 us for 128^3, one wave a SIMD) and the
+// scales: 8192^3 462 us against 387; with 64 x 64 a wave, whose sums join while the next tile's products run, 573, of
+// which copies are 115 and the joining 80. (128 x 64 with all of its second accumulators does not fit the registers, 909.)
+// Short K is bound by a tile's start and end (8192 x 24576 x 1536 298 us where its operations take 189); few tiles of long K by the steps of one tile (0.49 us for 128^3, one wave a SIMD) and the
 // second launch: 333 x 2112 x 8192, four parts of K, 15 + 4 us.
 #include <algorithm>
 #include <atomic>
@@ -138,16 +137,17 @@ __device__ __forceinline__ void store4(void* out, int64_t at, bool whole, int le
 constexpr int kMaxStride = 1 << 23;  // a tile's offsets are 32-bit
 constexpr int kBand = 4;             // activation tiles of a band
 
-// Activation scales of a tile lie in LDS in chunks, two at a time: 32 e8m0 or 16 f32 blocks of each
-// row. Rows are an odd number of words apart, so that 32 rows' reads of one block fall on different banks.
-template <int KIND>
-constexpr int kScaleChunk = KIND == kScaleF32 ? 64 : 32;
-template <int KIND>
-constexpr int kScaleRow = kScaleChunk<KIND> + 4;
+// Activation scales of a tile lie in LDS in chunks, two at a time: 32 e8m0 or 16 f32 blocks (8 beside the widest
+// tile's stages) of each row. Rows are an odd number of words apart, so that 32 rows' reads of one block fall on
+// different banks.
+template <int BM, int BN, int KIND>
+constexpr int kScaleChunk = KIND == kScaleF32 && BM * BN < 256 * 256 ? 64 : 32;
+template <int BM, int BN, int KIND>
+constexpr int kScaleRow = kScaleChunk<BM, BN, KIND> + 4;
 
 template <int BM, int BN, int STAGES, int KIND>
 constexpr int gemm_smem() {
-  return STAGES * (BM + BN) * kBlock + 2 * BM * kScaleRow<KIND>;
+  return STAGES * (BM + BN) * kBlock + 2 * BM * kScaleRow<BM, BN, KIND>;
 }
 
 // 16 bytes of scales from element i of a row of n, at any address.
@@ -189,7 +189,7 @@ fp8_gemm_kernel(const GemmParams P) {
   constexpr int kMt = WM / 32, kNt = WN / 32;
   constexpr int kStage = (BM + BN) * kBlock;
   constexpr int kPerA = BM / 8 / kWaves, kPerB = BN / 8 / kWaves;  // instructions of a stage: eight rows each
-  constexpr int kChunk = kScaleChunk<KIND>, kRow = kScaleRow<KIND>;
+  constexpr int kChunk = kScaleChunk<BM, BN, KIND>, kRow = kScaleRow<BM, BN, KIND>;
   constexpr int kScales = KIND == kScaleF32 ? kChunk / 4 : kChunk, kRowPieces = kChunk / 16;
   static_assert(kPerA * kWaves * 8 == BM && kPerB * kWaves * 8 == BN, "rows dealt out evenly");
   static_assert(kWaves % 2 == 0, "a wave's rows of a stage have one order of pieces");
@@ -290,7 +290,7 @@ fp8_gemm_kernel(const GemmParams P) {
   const int64_t sb_at = (int64_t)min((n0 + wn) / kBlock, (P.n - 1) / kBlock) * P.sb_stride;
   auto load_weight_scales = [&](int kb) { return load_scale<KIND>(P.sb, sb_at + min(kb + lane, P.kblocks - 1)); };
 
-  v16f acc[kNt][kMt], part[kNt][kMt];
+  v16f acc[kNt][kMt], part[kNt][kMt];  // (kByTile: one tile's part)
 #pragma unroll
   for (int i = 0; i < kNt; ++i)
 #pragma unroll
@@ -307,7 +307,13 @@ fp8_gemm_kernel(const GemmParams P) {
   // slot g % kSlots and are read kAhead groups before; weights a half before.
   // (as far ahead as registers allow)
   constexpr bool kTight = kMt == 4 || (KIND == kScaleF32 && kMt == 2);
-  constexpr int kGroups = 2 * kMt, kAhead = kTight ? kMt - 1 : kMt, kSlots = kTight ? kMt : kGroups;
+  // f32 scales and the widest tile: both halves of an activation tile follow one another, and its sums join the others
+  // before the next tile's take their registers
+  constexpr bool kByTile = KIND == kScaleF32 && kMt == 4;
+  constexpr int kGroups = 2 * kMt, kAhead = kByTile ? 1 : kTight ? kMt - 1 : kMt;
+  constexpr int kSlots = kByTile ? 2 : kTight ? kMt : kGroups;
+  auto tile_of = [](int g) { return kByTile ? g / 2 : g % kMt; };
+  auto half_of = [](int g) { return kByTile ? g % 2 : g / kMt; };
   v8i fa[kSlots], fb[2][kNt];
   // scales of this block, and of the next ones (replaced one by one behind their last use where tiles are read that late)
   constexpr bool kEach = kAhead < kMt;
@@ -320,7 +326,7 @@ fp8_gemm_kernel(const GemmParams P) {
   constexpr int kCopiesHere = kSendHere >= kSend ? kCopies : kSendHere * kCopies / kSend;  // before the step ends
   uint32_t ca[kMt], na[kMt], cb, sb = 0, sb_next = 0;
   // f32 scales: a tile's sums over a block join the others while the next tile's products run
-  constexpr bool kDelay = KIND == kScaleF32 && kMt > 1;
+  constexpr bool kDelay = KIND == kScaleF32 && kMt > 1 && !kByTile;
   float join = 0.f;
   if (kDelay)
 #pragma unroll
@@ -329,7 +335,7 @@ fp8_gemm_kernel(const GemmParams P) {
 #pragma unroll
     for (int i = 0; i < kNt; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] += part[i][j][r] * f;
+      for (int r = 0; r < 16; ++r) acc[i][j][r] += part[i][kByTile ? 0 : j][r] * f;
   };
 
   const int steps = kb1 - kb0;
@@ -351,7 +357,7 @@ fp8_gemm_kernel(const GemmParams P) {
 #pragma unroll
     for (int i = 0; i < kNt; ++i) fb[0][i] = operand(0, BM + wn + 32 * i, 0);
 #pragma unroll
-    for (int g = 0; g < kAhead; ++g) fa[g % kSlots] = operand(0, wm + 32 * (g % kMt), g / kMt);
+    for (int g = 0; g < kAhead; ++g) fa[g % kSlots] = operand(0, wm + 32 * tile_of(g), half_of(g));
 #pragma unroll
     for (int j = 0; j < kMt; ++j) ca[j] = row_scale(0, j);
   }
@@ -381,7 +387,7 @@ fp8_gemm_kernel(const GemmParams P) {
     cb = __builtin_amdgcn_readlane(sb, s % 64);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-      const int h = g / kMt, j = g % kMt, t = g + kAhead;
+      const int h = half_of(g), j = tile_of(g), t = g + kAhead;
 #pragma unroll
       for (int i = 0; i < kNt; ++i) {  // one product, and what is sent for meanwhile
         if (kTwice && g == 2 && i == 0) {
@@ -397,7 +403,7 @@ fp8_gemm_kernel(const GemmParams P) {
 #pragma unroll
             for (int y = 0; y < kMt; ++y) {
               if (WM * WN > 128 * 64) asm volatile("" : "+a"(acc[x][y]));
-              else if (KIND == kScaleE8M0) asm volatile("" : "+v"(acc[x][y]));
+              else if (KIND == kScaleE8M0 || kByTile) asm volatile("" : "+v"(acc[x][y]));
               else asm volatile("" : "+v"(part[x][y]));
             }
           // The chunk of scales after the next: sent for at a chunk's first step, kept at its second.
@@ -432,14 +438,16 @@ fp8_gemm_kernel(const GemmParams P) {
             for (int x = 0; x < kMt; ++x) na[x] = row_scale(s + 1, x);
           }
         }
-        if (kTwice) {
-          constexpr int kNowA = kPerA / (2 * kNt), kNowB = kPerB / (2 * kNt);
+        if constexpr (kTwice) {
+          constexpr int kLate = kAhead < 2 ? 1 : 2;  // groups behind the meeting
+          constexpr int kNowA = kPerA / (kLate * kNt), kNowB = kPerB / (2 * kNt);
+          static_assert(kNowA * kLate * kNt == kPerA && kNowB * 2 * kNt == kPerB, "copies dealt out evenly");
           if (g / 2 == 1)
 #pragma unroll
             for (int x = 0; x < kNowB; ++x) send(kPerA + ((g - 2) * kNt + i) * kNowB + x);
-          if (g >= kGroups - 2)
+          if (g >= kGroups - kLate)
 #pragma unroll
-            for (int x = 0; x < kNowA; ++x) send(((g - kGroups + 2) * kNt + i) * kNowA + x);
+            for (int x = 0; x < kNowA; ++x) send(((g - kGroups + kLate) * kNt + i) * kNowA + x);
         } else {
           const int q = g * kNt + i, r = q >= kMeetAt ? q - kMeetAt : q + kSendHere;  // products since the meeting
 #pragma unroll
@@ -452,16 +460,21 @@ fp8_gemm_kernel(const GemmParams P) {
         if (g == 0) fb[1][i] = operand(buf, BM + wn + 32 * i, 1);
         if (g == kGroups - kAhead) fb[0][i] = operand(buf1, BM + wn + 32 * i, 0);
         if (i == 0) {
-          if (kEach && g >= kGroups - kAhead) ca[g - (kGroups - kAhead)] = row_scale(s + 1, g - (kGroups - kAhead));
-          if (kEach && g == 0) ca[kMt - 1] = row_scale(s, kMt - 1);
-          fa[t % kSlots] = t < kGroups ? operand(buf, wm + 32 * (t % kMt), t / kMt) : operand(buf1, wm + 32 * (t % kMt), 0);
+          if (kByTile) {
+            if (h == 0 && j + 1 < kMt) ca[j + 1] = row_scale(s, j + 1);
+            if (g == kGroups - 1) na[0] = row_scale(s + 1, 0);
+          } else if (kEach) {
+            if (g >= kGroups - kAhead) ca[g - (kGroups - kAhead)] = row_scale(s + 1, g - (kGroups - kAhead));
+            if (g == 0) ca[kMt - 1] = row_scale(s, kMt - 1);
+          }
+          fa[t % kSlots] = operand(t < kGroups ? buf : buf1, wm + 32 * tile_of(t % kGroups), half_of(t % kGroups));
         }
         __builtin_amdgcn_sched_barrier(0);
         if (KIND == kScaleE8M0)
           acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h][i], fa[g % kSlots], acc[i][j], 0, 0, 0, cb, 0, ca[j]);
         else
-          part[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h][i], fa[g % kSlots], h ? part[i][j] : (v16f){}, 0, 0,
-                                                                       0, 127, 0, 127);
+          part[i][kByTile ? 0 : j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+              fb[h][i], fa[g % kSlots], h ? part[i][kByTile ? 0 : j] : (v16f){}, 0, 0, 0, 127, 0, 127);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (kDelay && (g == 0 || h == 1)) {
@@ -474,6 +487,7 @@ fp8_gemm_kernel(const GemmParams P) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    if (kByTile) ca[0] = na[0];
     if (!kEach) {
 #pragma unroll
       for (int j = 0; j < kMt; ++j) ca[j] = na[j];
@@ -647,13 +661,14 @@ fp8_gemm_sum_kernel(const float* __restrict__ part, int splits, int m, int n, vo
   store4<OUT>(out, row * out_stride + c, aligned && whole, n - c, v);
 }
 
-// The tiles there are, and what a product of G of them takes, in us: fitted to 8000 runs of 440 shapes (1 to 8192
-// rows, 64 to 24576 columns, 128 to 8192 deep), of which the choice is 1.6% slower than the best on average.
+// The tiles there are, and what a product of G of them takes, in us: fitted to measurements of several hundred shapes (1 to
+// 8192 rows, 64 to 24576 columns, 128 to 8192 deep), of which the choice is 1% slower than the best on average.
 //   n = ceil(G / CUs) tiles a CU, r = ceil(n / resident) of them after one another, steps blocks of K each:
 //   base + n (per_tile + steps per_step) + r (per_round + steps per_round_step)
 // Small tiles keep every CU and its memory path busy where there are few rows (1 x 8192 x 1536 by 32 x 64 tiles of
 // three stages 7.7 us, of two 9.3); large ones read less from L2 per product (2048 x 8192 x 8192 by 256 x 256 104 us,
-// by 128 x 128 143). f32 scales cost registers and vector instructions: narrower tiles.
+// by 128 x 128 143). The widest tile has four waves of 128 x 128, or eight of 128 x 64: these read more from LDS (8192^3 387
+// and 394 us) but begin and end a tile sooner (8192 x 24576 x 1536 318 and 298). f32 scales leave room for the latter only.
 struct Tile {
   int bm, bn, stages, resident;
   float base, per_step, per_round_step, per_tile, per_round;
@@ -662,11 +677,11 @@ constexpr Tile kTilesE8M0[] = {
     {32, 64, 3, 4, 3.0f, 0.05f, 0.20f, 1.25f, 0.f},   {64, 64, 3, 3, 2.85f, 0.11f, 0.12f, 1.1f, 1.1f},
     {64, 128, 3, 2, 3.0f, 0.20f, 0.10f, 1.4f, 1.4f},  {128, 128, 2, 2, 1.9f, 0.21f, 0.36f, 2.1f, 1.7f},
     {128, 128, 3, 1, 1.7f, 0.42f, 0.f, 4.8f, 0.f},    {256, 128, 2, 1, 0.8f, 0.86f, 0.f, 6.0f, 0.f},
-    {256, 256, 2, 1, 0.f, 1.2f, 0.f, 12.9f, 0.f}};
+    {256, 256, 2, 1, 0.f, 1.25f, 0.f, 10.1f, 0.f},    {256, 256, 2, 1, 0.f, 1.19f, 0.f, 12.2f, 0.f}};
 constexpr Tile kTilesF32[] = {
     {32, 64, 3, 3, 2.3f, 0.04f, 0.28f, 1.2f, 0.f},    {64, 64, 3, 2, 2.6f, 0.08f, 0.235f, 1.35f, 0.f},
     {64, 128, 2, 2, 2.1f, 0.085f, 0.41f, 1.7f, 0.f},  {64, 128, 3, 1, 2.2f, 0.38f, 0.f, 0.f, 2.4f},
-    {256, 128, 2, 1, 0.55f, 1.05f, 0.f, 5.9f, 0.f}};
+    {256, 128, 2, 1, 0.55f, 1.05f, 0.f, 5.9f, 0.f},   {256, 256, 2, 1, 0.f, 1.6f, 0.f, 9.0f, 0.f}};
 // A second launch adds up the parts of K: so much, and more by their MB.
 constexpr float kSumBase = 2.9f, kSumPerMB[2] = {0.33f, 0.25f};
 
@@ -772,6 +787,7 @@ int launch_plan(const Plan& p, int kind, const GemmParams& P, int dev, hipStream
       case 3: return launch_tile<128, 128, 64, 64, 2, kScaleE8M0, OUT>(P, dev, st);
       case 4: return launch_tile<128, 128, 64, 64, 3, kScaleE8M0, OUT>(P, dev, st);
       case 5: return launch_tile<256, 128, 64, 64, 2, kScaleE8M0, OUT>(P, dev, st);
+      case 6: return launch_tile<256, 256, 128, 64, 2, kScaleE8M0, OUT>(P, dev, st);
       default: return launch_tile<256, 256, 128, 128, 2, kScaleE8M0, OUT>(P, dev, st);
     }
   }
@@ -780,7 +796,8 @@ int launch_plan(const Plan& p, int kind, const GemmParams& P, int dev, hipStream
     case 1: return launch_tile<64, 64, 32, 32, 3, kScaleF32, OUT>(P, dev, st);
     case 2: return launch_tile<64, 128, 32, 64, 2, kScaleF32, OUT>(P, dev, st);
     case 3: return launch_tile<64, 128, 32, 64, 3, kScaleF32, OUT>(P, dev, st);
-    default: return launch_tile<256, 128, 64, 64, 2, kScaleF32, OUT>(P, dev, st);
+    case 4: return launch_tile<256, 128, 64, 64, 2, kScaleF32, OUT>(P, dev, st);
+    default: return launch_tile<256, 256, 128, 64, 2, kScaleF32, OUT>(P, dev, st);
   }
 }
 

@@ -177,7 +177,8 @@ def test_gemm_large(cuda, M, N, K, kind):
 
 
 @pytest.mark.parametrize("M,N,K", [(33, 129, 16528), (1000, 1000, 8336), (130, 8200, 8848), (65, 8200, 16528), (257, 16400, 8336),
-                                   (1030, 2100, 8336), (2050, 2100, 1168), (500, 8200, 8848), (2050, 4100, 8336)])
+                                   (1030, 2100, 8336), (1000, 520, 1168), (2050, 2100, 1168), (500, 8200, 8848),
+                                   (2050, 4100, 8336)])
 @pytest.mark.parametrize("kind", ["f32", "e8m0"])
 def test_gemm_long(cuda, M, N, K, kind):
     """More blocks of K than a wave's register of weight scales and the chunks of activation scales hold, a short
