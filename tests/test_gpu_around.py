@@ -165,7 +165,7 @@ def test_gemm_sizes(cuda, M, N, K, kind):
     check_product(ops.fp8_gemm(*ops_, out_dtype=F32), *ops_)
 
 
-@pytest.mark.parametrize("M,N,K", [(4096, 4096, 256), (4100, 4090, 400)])
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 256), (4100, 4090, 400), (4096, 4100, 16), (4100, 4104, 144)])
 @pytest.mark.parametrize("kind", ["f32", "e8m0"])
 def test_gemm_large(cuda, M, N, K, kind):
     """Enough tiles for the widest form, whole and ragged: rows from every part against the exact sums."""
@@ -283,6 +283,47 @@ def test_gemm_nan_stays_in_its_row_and_column(cuda):
             sa[1, 2] = float("nan")
         want[1] = True
         assert torch.equal(ops.fp8_gemm(a, sa, b, sb).isnan(), want)
+
+
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+def test_gemm_workspace(cuda, kind):
+    """What a workspace held does not matter, nor that calls of several shapes share it; one that does not fit is not used."""
+    need = []
+    ops_ = [product(gen(cuda, 9 + i), M, N, 8192, kind) for i, (M, N) in enumerate(((100, 300), (40, 576), (70, 129)))]
+    for a, sa, b, sb in ops_:
+        need.append(ops.fp8_gemm_workspace_bytes(a.shape[0], b.shape[0], a.shape[1], sa.dtype))
+    assert min(need) > 0
+    want = [ops.fp8_gemm(*o) for o in ops_]
+    check_product(want[0], *ops_[0])
+    shared = torch.full((max(need) + 32,), 0xff, dtype=torch.uint8, device=cuda)
+    for _ in range(2):
+        for o, w in zip(ops_, want):
+            assert torch.equal(ops.fp8_gemm(*o, workspace=shared), w)
+    edge = shared[:max(need)]
+    shared[max(need):] = 0x55
+    for o, w in zip(ops_, want):
+        assert torch.equal(ops.fp8_gemm(*o, workspace=edge), w)
+    assert torch.all(shared[max(need):] == 0x55)
+    shared.fill_(7)
+    for bad in (shared[:min(need) - 1], shared[8:], torch.empty(max(need), dtype=torch.uint8)):
+        assert torch.equal(ops.fp8_gemm(*ops_[0], workspace=bad), want[0])
+    assert torch.all(shared == 7)
+
+
+@pytest.mark.parametrize("kind", ["f32", "e8m0"])
+def test_gemm_nan_in_the_widest_tile(cuda, kind):
+    M, N, K = 4100, 4090, 400
+    a, sa, b, sb = product(gen(cuda, 21), M, N, K, kind)
+    a.view(torch.uint8)[M - 3, K - 1] = 0x7f
+    b.view(torch.uint8)[N - 2, 5] = 0xff
+    if kind == "e8m0":
+        sa.view(torch.uint8)[300, 2] = 255
+    else:
+        sa[300, 2] = float("nan")
+    bad = ops.fp8_gemm(a, sa, b, sb).isnan()
+    want = torch.zeros_like(bad)
+    want[M - 3], want[300], want[:, N - 2] = True, True, True
+    assert torch.equal(bad, want)
 
 
 def test_gemm_empty(cuda):

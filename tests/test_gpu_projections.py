@@ -172,8 +172,7 @@ def test_layer_captured(cuda):
 
 
 def test_two_streams_at_once(cuda):
-    """Products in parts on two streams, each with a workspace from its own stream's pool; and a captured one that shares
-    neither with an eager call."""
+    """Products in parts on two streams at once, each with a workspace from its own stream's pool."""
     g = torch.Generator(device=cuda).manual_seed(5)
     a, sa = ops.act_quant(torch.randn(20, 8192, generator=g, device=cuda).to(BF))
     ws = [projections.Fp8Linear(torch.randn(300, 8192, generator=g, device=cuda)) for _ in range(2)]
