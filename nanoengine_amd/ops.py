@@ -1062,7 +1062,7 @@ def _rows2d(t: torch.Tensor, name: str, dtypes, shape=None) -> int:
 
 
 _BF16 = (torch.bfloat16,)
-_WEIGHTS = (torch.bfloat16, torch.float32)
+_BF16_F32 = (torch.bfloat16, torch.float32)
 
 
 def _coded(rows: int, dim: int, codes: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, int]:
@@ -1078,7 +1078,7 @@ def _norm(x, weight, eps, out, residual, residual_out, codes, scales) -> None:
     stride = _rows2d(x, "x", _BF16)
     shape = x.shape
     rows, dim = shape
-    if not (weight.shape == (dim,) and weight.dtype in _WEIGHTS and weight.is_contiguous()):
+    if not (weight.shape == (dim,) and weight.dtype in _BF16_F32 and weight.is_contiguous()):
         _fail(f"weight must be contiguous bfloat16 or float32 [{dim}]")
     tensors = [x, weight]
     res_stride = sum_stride = out_stride = code_stride = scale_stride = kind = 0
@@ -1171,25 +1171,27 @@ def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     b_scale [ceil(N / 128), ceil(K / 128)], both scales float32 or both float8_e8m0fnu (uint8: the same bytes). out
     is bf16 or float32 (``out_dtype`` when it is not given). K a multiple of 16 (see dsa_fp8_gemm)."""
     a_stride, b_stride = _rows2d(a, "a", _FP8_TYPES), _rows2d(b, "b", _FP8_TYPES)
-    (M, K), (N, Kb) = a.shape, b.shape
+    M, K = a.shape
+    N, Kb = b.shape
     if K != Kb:
         _fail(f"a and b must share K, got {K} and {Kb}")
-    kind = _SCALE_KINDS.get(a_scale.dtype)
+    scale_dtype = a_scale.dtype
+    kind = _SCALE_KINDS.get(scale_dtype)
     if kind is None or kind != _SCALE_KINDS.get(b_scale.dtype):
-        _fail(f"a_scale and b_scale must both be float32 or both float8_e8m0fnu, got {a_scale.dtype} and {b_scale.dtype}")
+        _fail(f"a_scale and b_scale must both be float32 or both float8_e8m0fnu, got {scale_dtype} and {b_scale.dtype}")
     blocks = -(-K // FP8_BLOCK)
     sa_stride = _rows2d(a_scale, "a_scale", _SCALE_KINDS, (M, blocks))
     sb_stride = _rows2d(b_scale, "b_scale", _SCALE_KINDS, (-(-N // FP8_BLOCK), blocks))
-    dev = _gpu(a, a_scale, b, b_scale)
     if out is None:
-        if out_dtype not in (torch.bfloat16, torch.float32):
+        if out_dtype not in _BF16_F32:
             _fail(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
+        dev = _gpu(a, a_scale, b, b_scale)
         out = a.new_empty((M, N), dtype=out_dtype)
         out_stride = N
     else:
-        out_stride = _rows2d(out, "out", (torch.bfloat16, torch.float32), (M, N))
-        _gpu(a, out)
-    need = _gemm_workspace(dev, M, N, K, a_scale.dtype)
+        out_stride = _rows2d(out, "out", _BF16_F32, (M, N))
+        dev = _gpu(a, a_scale, b, b_scale, out)
+    need = _gemm_workspace(dev, M, N, K, scale_dtype)
     ws_ptr, ws_bytes = None, 0
     if need:
         if (workspace is None or workspace.numel() * workspace.element_size() < need or workspace.data_ptr() % 16
@@ -1204,13 +1206,17 @@ def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
 
 def _heads3d(t: torch.Tensor, name: str, shape=None) -> tuple[int, int]:
     """(token stride, head stride) of a bf16 tensor [T, H, rot] with a contiguous last dim."""
-    s, st = t.shape, t.stride()
-    if not (len(s) == 3 and t.dtype is torch.bfloat16 and (st[2] == 1 or s[2] == 1) and (shape is None or s == shape)):
-        want = "[T, H, rot_dim]" if shape is None else str(list(shape))
-        _fail(f"{name} must be bfloat16 {want} with a contiguous last dim, got {t.dtype} {tuple(s)}")
-    # torch leaves the stride of a single head or token free
-    head = st[1] if s[1] > 1 else s[2]
-    return (st[0] if s[0] > 1 else s[1] * head), head
+    s = t.shape
+    if t.dtype in _BF16 and (len(s) == 3 if shape is None else s == shape):
+        token, head, element = t.stride()
+        tokens, heads, rot = s
+        if element == 1 or rot == 1:
+            # torch leaves the stride of a single head or token free
+            if heads <= 1:
+                head = rot
+            return (token if tokens > 1 else heads * head), head
+    want = "[T, H, rot_dim]" if shape is None else str(list(shape))
+    _fail(f"{name} must be bfloat16 {want} with a contiguous last dim, got {t.dtype} {tuple(s)}")
 
 
 def rope(q: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor, out: torch.Tensor | None = None, *,
@@ -1228,13 +1234,13 @@ def rope(q: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor, 
         out, o_t, o_h = q, q_t, q_h
     else:
         o_t, o_h = _heads3d(out, "out", shape)
-    table = cos_sin_cache if cos_sin_cache.dim() == 2 else cos_sin_cache.reshape(cos_sin_cache.shape[0], -1)
-    max_pos, width = table.shape
-    if not (width == rot and table.dtype is torch.float32 and table.is_contiguous()):
+    table, t_shape = cos_sin_cache, cos_sin_cache.shape
+    if len(t_shape) != 2:
+        table = cos_sin_cache.reshape(t_shape[0], -1)
+        t_shape = table.shape
+    if not (t_shape[1] == rot and table.dtype is torch.float32 and table.is_contiguous()):
         _fail(f"cos_sin_cache must be contiguous float32 [max_pos, {rot}], got {table.dtype} {tuple(cos_sin_cache.shape)}")
     pos, wide = _positions(positions, T)
-    tensors = [q, out, table, pos]
-    k_args = (None, 0, 0, 0, None, 0, 0)
     if k is not None:
         k_t, k_h = _heads3d(k, "k")
         k_shape = k.shape
@@ -1245,11 +1251,16 @@ def rope(q: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor, 
             k_out, ko_t, ko_h = k, k_t, k_h
         else:
             ko_t, ko_h = _heads3d(k_out, "k_out", k_shape)
-        tensors += (k, k_out)
-        k_args = (k.data_ptr(), k_t, k_h, Hk, k_out.data_ptr(), ko_t, ko_h)
+        dev = _gpu(q, out, table, pos, k, k_out)
+        k_ptr, ko_ptr = k.data_ptr(), k_out.data_ptr()
     elif k_out is not None:
         _fail("k_out needs k")
-    _launch(_gpu(*tensors), "dsa_rope", q.data_ptr(), q_t, q_h, H, out.data_ptr(), o_t, o_h, *k_args, T, rot,
-            table.data_ptr(), max_pos, pos.data_ptr(), wide, int(bool(interleaved)),
-            int(bool(interleaved if out_interleaved is None else out_interleaved)))
+    else:
+        dev = _gpu(q, out, table, pos)
+        k_ptr = ko_ptr = None
+        k_t = k_h = Hk = ko_t = ko_h = 0
+    pairs = 1 if interleaved else 0
+    _launch(dev, "dsa_rope", q.data_ptr(), q_t, q_h, H, out.data_ptr(), o_t, o_h, k_ptr, k_t, k_h, Hk, ko_ptr, ko_t, ko_h,
+            T, rot, table.data_ptr(), t_shape[0], pos.data_ptr(), wide, pairs,
+            pairs if out_interleaved is None else int(bool(out_interleaved)))
     return out if k is None else (out, k_out)
