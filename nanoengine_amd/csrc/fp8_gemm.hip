@@ -625,15 +625,18 @@ __global__ void __launch_bounds__(kFewWaves * 64) fp8_gemm_few_kernel(const Gemm
   store4<OUT>(P.out, (int64_t)c32 * P.out_stride + n, aligned && n + 4 <= P.n, P.n - n, r);
 }
 
-// out = the sum of the splits' partial sums, in order; eight parts' loads in flight at once.
+// out = the sum of the splits' partial sums, in order; eight parts' loads in flight at once. They are read once, past the L2
+// (333 x 2112 x 8192, cold, 19.6 -> 18.1 us); single waves spread evenly over the CUs (0.2 us).
+constexpr int kSumThreads = 64;
+
 template <int OUT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kSumThreads)
 fp8_gemm_sum_kernel(const float* __restrict__ part, int splits, int m, int n, void* __restrict__ out, int64_t out_stride) {
-  const int per_row = (n + 3) / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / per_row;
-  if (row >= m) return;
-  const int c = (int)(i - row * per_row) * 4;
+  // (few tiles are split: the results are far fewer than 2^32)
+  const uint32_t per_row = (n + 3) / 4, i = blockIdx.x * kSumThreads + threadIdx.x, in_order = i / per_row;
+  if (in_order >= (uint32_t)m) return;
+  const int64_t row = in_order;
+  const int c = (int)(i - in_order * per_row) * 4;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
   const bool whole = n % 4 == 0;
   const float* p = part + row * n + c;
@@ -644,7 +647,7 @@ fp8_gemm_sum_kernel(const float* __restrict__ part, int splits, int m, int n, vo
     for (int k = 0; k < 8; ++k) {
       const float* q = p + min(s + k, splits - 1) * step;
       if (whole) {
-        x[k] = *reinterpret_cast<const v4f*>(q);
+        x[k] = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(q));
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[k][j] = q[min(c + j, n - 1) - c];
@@ -804,8 +807,8 @@ int launch_plan(const Plan& p, int kind, const GemmParams& P, int dev, hipStream
 template <int OUT>
 void launch_sum(const void* part, int splits, int m, int n, void* out, int64_t out_stride, hipStream_t st) {
   const int64_t threads = (int64_t)m * ((n - 1) / 4 + 1);
-  hipLaunchKernelGGL(fp8_gemm_sum_kernel<OUT>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st,
-                     static_cast<const float*>(part), splits, m, n, out, out_stride);
+  hipLaunchKernelGGL(fp8_gemm_sum_kernel<OUT>, dim3((unsigned)((threads + kSumThreads - 1) / kSumThreads)),
+                     dim3(kSumThreads), 0, st, static_cast<const float*>(part), splits, m, n, out, out_stride);
 }
 
 }  // namespace
