@@ -19,16 +19,17 @@
 // (rows are half the banks' span apart; with row % 8 two of 16 met on each bank: 1e8 conflict
 // cycles in 8192 x 8192 x 16384, now 2e6).
 //
-// What bounds it, measured: 8192 x 8192 x 16384 (e8m0) 745-765 us, 2.9 PFLOP/s, where the library's product with one
-// scale a matrix takes 720-765 on the same cards and one with a scale per 32 elements 1450. Products run in 79% of a
-// SIMD's cycles, and the clock gives way under their power: without any copies it takes 698, with all data in L2 780 of then
-// 811, without scales 3% less; persistent workgroups, which close the gaps between tiles, gain nothing. Steps that
-// took the first kernel's 1125 there: operands read ahead of their products 875, copies sent between products 840,
-// four waves of 128 x 128 rather than eight of 128 x 64 811, a main loop without rare branches and masks 744. f32
-// scales: 8192^3 462 us against 387; with 64 x 64 a wave, whose sums join while the next tile's products run, 573, of
-// which copies are 115 and the joining 80. (128 x 64 with all of its second accumulators does not fit the registers, 909.)
-// Short K is bound by a tile's start and end (8192 x 24576 x 1536 298 us where its operations take 189); few tiles of long K by the steps of one tile (0.49 us for 128^3, one wave a SIMD) and the
-// second launch: 333 x 2112 x 8192, four parts of K, 15 + 4 us.
+// What bounds it, measured: 8192 x 8192 x 16384 (e8m0) 745-765 us, 2.9 PFLOP/s, where the library's product with
+// one scale a matrix takes 720-765 on the same cards and one with a scale per 32 elements 1450. Products run in 79% of
+// a SIMD's cycles, and the clock gives way under their power: without any copies it takes 698, with all data in L2 780
+// of then 811, without scales 3% less; persistent workgroups, which close the gaps between tiles, gain nothing. Steps
+// that brought it there from the first kernel's 1125: operands read ahead of their products 875, copies sent between
+// products 840, four waves of 128 x 128 rather than eight of 128 x 64 811, a main loop without rare branches and masks
+// 744. f32 scales: 8192^3 462 us against 387; with 64 x 64 a wave, whose sums join while the next tile's products run,
+// 573, of which copies are 115 and the joining 80. (128 x 64 with all of its second accumulators does not fit the
+// registers, 909.) Short K is bound by a tile's start and end (8192 x 24576 x 1536 298 us where its operations take
+// 189); few tiles of long K by the steps of one tile (0.49 us for 128^3, one wave a SIMD) and the second launch: 333 x
+// 2112 x 8192, four parts of K, 15 + 4 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -122,7 +123,8 @@ __device__ __forceinline__ void store16(void* out, int64_t at, bool whole, int l
 template <int OUT>
 __device__ __forceinline__ void store4(void* out, int64_t at, bool whole, int left, const float* v) {
   if (OUT == kOutF32) {
-    store16<OUT>(out, at, whole, left, (v4i){__float_as_int(v[0]), __float_as_int(v[1]), __float_as_int(v[2]), __float_as_int(v[3])});
+    store16<OUT>(out, at, whole, left,
+                 (v4i){__float_as_int(v[0]), __float_as_int(v[1]), __float_as_int(v[2]), __float_as_int(v[3])});
     return;
   }
   uint16_t* o = static_cast<uint16_t*>(out) + at;
@@ -183,7 +185,8 @@ __device__ __forceinline__ v4i load_scale_piece(const void* row, int i, int n) {
 // of block s end and those of block s + 1 begin, the waves meet, once a block: all have read block
 // s by then, and block s + 1 has landed; block s + STAGES is sent for in block s's place.
 template <int BM, int BN, int WM, int WN, int STAGES, int KIND, int OUT>
-__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) __attribute__((amdgpu_waves_per_eu(WM * WN > 128 * 64 ? 1 : 2)))
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64)
+    __attribute__((amdgpu_waves_per_eu(WM * WN > 128 * 64 ? 1 : 2)))
 fp8_gemm_kernel(const GemmParams P) {
   constexpr int kWaves = (BM / WM) * (BN / WN);
   constexpr int kMt = WM / 32, kNt = WN / 32;
@@ -200,13 +203,14 @@ fp8_gemm_kernel(const GemmParams P) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go to the eight XCDs in turn: each XCD takes a run of neighbouring tiles, in bands of four activation
-  // tiles, so that the tiles at work beside one L2 share their rows. (Against tiles dealt out to the XCDs one by one, 2048 x 8192 x 8192 takes
-  // 4% less and 333 x 8192 x 8192 40 us rather than 60.)
+  // tiles, so that the tiles at work beside one L2 share their rows. (Against tiles dealt out to the XCDs one by one,
+  // 2048 x 8192 x 8192 takes 4% less and 333 x 8192 x 8192 40 us rather than 60.)
   const int tiles = P.mtiles * P.ntiles;
   const int xcd = blockIdx.x & 7, share = gridDim.x >> 3, rest = gridDim.x & 7;
   const int at = xcd * share + min(xcd, rest) + (blockIdx.x >> 3);
   const int split = at / tiles, tile = at - split * tiles;
-  const int band = tile / (kBand * P.ntiles), in_band = tile - band * kBand * P.ntiles, wide = min(kBand, P.mtiles - kBand * band);
+  const int band = tile / (kBand * P.ntiles), in_band = tile - band * kBand * P.ntiles;
+  const int wide = min(kBand, P.mtiles - kBand * band);
   const int m0 = (kBand * band + in_band % wide) * BM, n0 = in_band / wide * BN;
   const int kb0 = (int)((int64_t)P.kblocks * split / P.splits), kb1 = (int)((int64_t)P.kblocks * (split + 1) / P.splits);
   const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
@@ -300,7 +304,8 @@ fp8_gemm_kernel(const GemmParams P) {
   const uint32_t at0 = c32 * kBlock + 16 * ((2 * half) ^ ((lane >> 1) & 7));
   auto operand = [&](int buf, int row, int h) {
     const uint8_t* rows = smem + (buf * kStage + row * kBlock);
-    const v4i x = *reinterpret_cast<const v4i*>(rows + (at0 ^ (64 * h))), y = *reinterpret_cast<const v4i*>(rows + (at0 ^ (64 * h + 16)));
+    const v4i x = *reinterpret_cast<const v4i*>(rows + (at0 ^ (64 * h)));
+    const v4i y = *reinterpret_cast<const v4i*>(rows + (at0 ^ (64 * h + 16)));
     return (v8i){x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
   };
   // A step's groups: half h of activation tile j times all weight tiles. Group g's activations lie in
@@ -471,7 +476,8 @@ fp8_gemm_kernel(const GemmParams P) {
         }
         __builtin_amdgcn_sched_barrier(0);
         if (KIND == kScaleE8M0)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h][i], fa[g % kSlots], acc[i][j], 0, 0, 0, cb, 0, ca[j]);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h][i], fa[g % kSlots], acc[i][j], 0, 0, 0, cb, 0,
+                                                                      ca[j]);
         else
           part[i][kByTile ? 0 : j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
               fb[h][i], fa[g % kSlots], h ? part[i][kByTile ? 0 : j] : (v16f){}, 0, 0, 0, 127, 0, 127);
@@ -503,7 +509,8 @@ fp8_gemm_kernel(const GemmParams P) {
   // Lane (c32, half) holds row c32 of an activation tile, columns 8g + 4 half .. + 3 of a weight tile: 32 rows at a
   // time they change places in LDS (a part of its own for each wave), so that a store takes 16 bytes a lane and whole rows.
   // (From the registers, 8 bytes a lane and 32 rows to a store, 256 x 256 results took 10.8 us.)
-  constexpr int kSize = OUT == kOutBf16 ? 2 : 4, kEach16 = 16 / kSize, kPitch = WN * kSize + 16, kRowChunks = WN * kSize / 16;
+  constexpr int kSize = OUT == kOutBf16 ? 2 : 4, kEach16 = 16 / kSize;
+  constexpr int kPitch = WN * kSize + 16, kRowChunks = WN * kSize / 16;
   static_assert(kWaves * 32 * kPitch <= STAGES * kStage, "the stages' place");
   if (P.splits > 1) out = static_cast<float*>(out) + (int64_t)split * P.m * P.n;
   const bool aligned = !((reinterpret_cast<uintptr_t>(out) & 15) | (out_stride & (kEach16 - 1)));
@@ -549,11 +556,12 @@ fp8_gemm_kernel(const GemmParams P) {
 }
 
 // Up to 32 rows: a workgroup takes 32 columns, its eight waves parts of K, and operands go from memory straight into
-// the registers of the products; the waves' sums meet in LDS, in order. No copies to wait for ahead of the first product, no
-// second launch: 1 x 8192 x 1536 in 5.0 us (by tiles 8.1), 16 x 2112 x 1536 4.9 (7.9). (The products and their groups of 64
-// elements are the tiles'; within a group a lane's pieces may come in any order, so a load takes 32 neighbouring
-// bytes of each row. Rows' lines are read by four loads: they have to stay in L1 meanwhile, 1 x 8192 x 8192 14.0 us, 25.0 with
-// loads that pass it. Several blocks at a time in a wave are slower, 17.6 with two: it is waves that hide the reads.)
+// the registers of the products; the waves' sums meet in LDS, in order. No copies to wait for ahead of the first
+// product, no second launch: 1 x 8192 x 1536 in 5.0 us (by tiles 8.1), 16 x 2112 x 1536 4.9 (7.9). (The products and
+// their groups of 64 elements are the tiles'; within a group a lane's pieces may come in any order, so a load takes 32
+// neighbouring bytes of each row. Rows' lines are read by four loads: they have to stay in L1 meanwhile, 1 x 8192 x
+// 8192 14.0 us, 25.0 with loads that pass it. Several blocks at a time in a wave are slower, 17.6 with two: it is
+// waves that hide the reads.)
 constexpr int kFew = 32, kFewWaves = 8;
 
 template <int KIND, int OUT>
@@ -573,8 +581,9 @@ __global__ void __launch_bounds__(kFewWaves * 64) fp8_gemm_few_kernel(const Gemm
     v16f part = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const v8i fa = {x[2 * h][0], x[2 * h][1], x[2 * h][2], x[2 * h][3], x[2 * h + 1][0], x[2 * h + 1][1], x[2 * h + 1][2], x[2 * h + 1][3]};
-      const v8i fb = {y[2 * h][0], y[2 * h][1], y[2 * h][2], y[2 * h][3], y[2 * h + 1][0], y[2 * h + 1][1], y[2 * h + 1][2], y[2 * h + 1][3]};
+      const v4i x0 = x[2 * h], x1 = x[2 * h + 1], y0 = y[2 * h], y1 = y[2 * h + 1];
+      const v8i fa = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+      const v8i fb = {y0[0], y0[1], y0[2], y0[3], y1[0], y1[1], y1[2], y1[3]};
       if (KIND == kScaleE8M0) acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb, fa, acc, 0, 0, 0, cb, 0, ca);
       else part = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb, fa, part, 0, 0, 0, 127, 0, 127);
     }
@@ -608,7 +617,8 @@ __global__ void __launch_bounds__(kFewWaves * 64) fp8_gemm_few_kernel(const Gemm
 
   // Lane (c32, half) holds row c32, columns 8g + 4 half .. + 3.
 #pragma unroll
-  for (int g = 0; g < 4; ++g) sums[wave * 256 + g * 64 + lane] = (v4f){acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+  for (int g = 0; g < 4; ++g)
+    sums[wave * 256 + g * 64 + lane] = (v4f){acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
   __syncthreads();
   if (threadIdx.x >= 256 || c32 >= P.m) return;
   v4f v = sums[threadIdx.x];
@@ -688,8 +698,8 @@ constexpr Tile kTilesF32[] = {
 // A second launch adds up the parts of K: so much, and more by their MB.
 constexpr float kSumBase = 2.9f, kSumPerMB[2] = {0.33f, 0.25f};
 
-// The same of the kernel for few rows, a part of K a wave: base + steps (per_step + rounds (per_round + rows per_row)). Fitted
-// to 1 to 32 rows of 180 shapes, of which the choice is 2% slower than the best on average.
+// The same of the kernel for few rows, a part of K a wave: base + steps (per_step + rounds (per_round + rows per_row)).
+// Fitted to 1 to 32 rows of 180 shapes, of which the choice is 2% slower than the best on average.
 constexpr struct {
   float base, per_step, per_round, per_row;
 } kFewCost = {2.0f, 0.36f, 1.0f, 0.02f};

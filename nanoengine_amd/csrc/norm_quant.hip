@@ -12,10 +12,11 @@
 // not depend on the rows beside it.
 //
 // Memory bounds the norm of many rows: 8192 x 8192 with residual, its sum, fp8 and bf16 out, 604 MB, in
-// 102 us (5.9 TB/s; a plain copy reaches 5.1). Few rows are one pass of latencies: 4 x 8192
-// in 3.8 us, of which an empty launch is more than half. A wave a row up to 512 elements (1000 x 512 in
-// 2.9 us), then as many waves as give a lane one load up to 8192 (with half as many waves 4 x 8192 takes 4.2 and
-// 8192 x 8192 105). Reading the weights before the sum made nothing faster. The rounding alone: 5001 x 1600, 24 MB, in 5.9 us.
+// 102 us (5.9 TB/s; a plain copy reaches 5.1). Few rows are one pass of latencies: 4 x 8192 in 3.8 us,
+// of which an empty launch is more than half. A wave a row up to 512 elements (1000 x 512 in 2.9 us),
+// then as many waves as give a lane one load up to 8192 (with half as many waves 4 x 8192 takes 4.2 and
+// 8192 x 8192 105). Reading the weights before the sum made nothing faster. The rounding alone: 5001 x
+// 1600, 24 MB, in 5.9 us.
 #include "dsa_common.h"
 #include "fp8_block.h"
 #include "../../include/dsa_amd.h"
@@ -63,8 +64,8 @@ __device__ __forceinline__ v4i load8(const uint16_t* row, int i, int n) {
   return r;
 }
 
-// Outputs are streamed past the L2, which has nothing more to do with them (8192 x 8192 110 -> 105 us, 5001 x 1600 6.5 -> 5.9;
-// inputs read so cost more, 118 and 7.0).
+// Outputs are streamed past the L2, which has nothing more to do with them (8192 x 8192 110 -> 105 us, 5001 x
+// 1600 6.5 -> 5.9; inputs read so cost more, 118 and 7.0).
 template <bool VEC>
 __device__ __forceinline__ void store8(uint16_t* row, int i, int n, v4i v) {
   if (VEC) {

@@ -20,11 +20,10 @@ namespace {
 
 constexpr int kRopeThreads = 256;
 constexpr int kMaxRot = 512;  // a row within one wave
-// From as many lanes as the card holds at a time (256 CUs of 2048), a lane takes four heads:
-// the loads in flight that a lane's second turn would have given, and a quarter of the
-// positions and angles read. 8192 tokens x 129 heads of 64: 65 us against 81 with one head a
-// lane (two: 68, eight: 75; all with warm caches and before what load_pairs says); 1024: 9.2 and 9.9. Below, more lanes hide more:
-// 128 x 129, 4.2 and 3.5.
+// From as many lanes as the card holds at a time (256 CUs of 2048), a lane takes four heads: the loads in flight that
+// a lane's second turn would have given, and a quarter of the positions and angles read. 8192 tokens x 129 heads of
+// 64: 65 us against 81 with one head a lane (two: 68, eight: 75; all with warm caches and before what load_pairs
+// says); 1024 tokens: 9.2 and 9.9. Below, more lanes hide more: 128 tokens, 4.2 and 3.5.
 constexpr int64_t kManyLanes = 256 * 2048;
 constexpr int kManyHeads = 4;
 
@@ -109,7 +108,8 @@ __device__ __forceinline__ void store_pairs(uint16_t* row, int p, int half, cons
       if (half % 8 == 0) {
         const bool odd = p & 4;
         const int got0 = neighbour(odd ? x[0] : y[0]), got1 = neighbour(odd ? x[1] : y[1]);
-        *reinterpret_cast<v4i*>(row + (odd ? half + p - 4 : p)) = odd ? (v4i){got0, got1, y[0], y[1]} : (v4i){x[0], x[1], got0, got1};
+        *reinterpret_cast<v4i*>(row + (odd ? half + p - 4 : p)) =
+            odd ? (v4i){got0, got1, y[0], y[1]} : (v4i){x[0], x[1], got0, got1};
       } else {
         *reinterpret_cast<v2i*>(row + p) = x;
         *reinterpret_cast<v2i*>(row + half + p) = y;
