@@ -555,67 +555,23 @@ fp8_gemm_kernel(const GemmParams P) {
   }
 }
 
-// Up to 32 rows: a workgroup takes 32 columns, its eight waves parts of K, and operands go from memory straight into
-// the registers of the products; the waves' sums meet in LDS, in order. No copies to wait for ahead of the first
-// product, no second launch: 1 x 8192 x 1536 in 5.0 us (by tiles 8.1), 16 x 2112 x 1536 4.9 (7.9). (The products and
-// their groups of 64 elements are the tiles'; within a group a lane's pieces may come in any order, so a load takes 32
-// neighbouring bytes of each row. Rows' lines are read by four loads: they have to stay in L1 meanwhile, 1 x 8192 x
-// 8192 14.0 us, 25.0 with loads that pass it. Several blocks at a time in a wave are slower, 17.6 with two: it is
-// waves that hide the reads.)
-constexpr int kFew = 32, kFewWaves = 8;
+// Up to 32 rows: a workgroup takes 32 columns, its four or eight waves parts of K, each with two blocks of 128 of its own
+// on their way into LDS in whole lines while a third is multiplied; the waves' sums meet in LDS, in order. No meetings of
+// waves until then, no second launch: 1 x 8192 x 1536 in 5.0 us (by tiles 8.0), 32 x 576 x 1536 4.0 (7.5), 16 x 2112 x
+// 8192 8.3 (10.8), 8 x 8192 x 8192 13.8 (15.4). What bounds it is the start (2 us beside the launch) and then what a CU can
+// fetch, 0.5 us a block of K for each of eight waves. (Straight into registers a load touches 32 rows, and where
+// these lie a power of two apart their lines crowd each other out of L1 before the next load wants them: 16 x 2112 x 8192
+// 15.4, 1 x 8192 x 1536 the same 5.0.)
+constexpr int kFew = 32;
+constexpr int kFewBlocks = 16;                                       // of K, a wave at most
+constexpr int kFewStage = 2 * kFew * kBlock;                         // a block of weights and of activations
+constexpr int kFewWave = 2 * kFewStage + kFewBlocks * kFew * 4;      // and the activations' scales
 
-template <int KIND, int OUT>
-__global__ void __launch_bounds__(kFewWaves * 64) fp8_gemm_few_kernel(const GemmParams P) {
-  __shared__ v4f sums[kFewWaves * 256];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c32 = lane & 31, half = lane >> 5;
-  const int n0 = blockIdx.x * kFew;
-  const int kb0 = (int)((int64_t)P.kblocks * wave / kFewWaves), kb1 = (int)((int64_t)P.kblocks * (wave + 1) / kFewWaves);
-  // rows past the matrix repeat its last one: their results are not stored
-  const uint8_t* a = P.a + (int64_t)min(c32, P.m - 1) * P.a_stride + 16 * half;
-  const uint8_t* b = P.b + (int64_t)min(n0 + c32, P.n - 1) * P.b_stride + 16 * half;
-  const int64_t sa = (int64_t)min(c32, P.m - 1) * P.sa_stride, sb = (int64_t)(n0 / kBlock) * P.sb_stride;
-
-  v16f acc = {};
-  auto multiply = [&](const v4i (&x)[4], const v4i (&y)[4], uint32_t ca, uint32_t cb) {
-    v16f part = {};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const v4i x0 = x[2 * h], x1 = x[2 * h + 1], y0 = y[2 * h], y1 = y[2 * h + 1];
-      const v8i fa = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-      const v8i fb = {y0[0], y0[1], y0[2], y0[3], y1[0], y1[1], y1[2], y1[3]};
-      if (KIND == kScaleE8M0) acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb, fa, acc, 0, 0, 0, cb, 0, ca);
-      else part = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb, fa, part, 0, 0, 0, 127, 0, 127);
-    }
-    if (KIND == kScaleF32) {
-      const float f = __uint_as_float(ca) * __uint_as_float(cb);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[r] += part[r] * f;
-    }
-  };
-  const int full = min(kb1, P.k / kBlock);
-  for (int kb = kb0; kb < full; ++kb) {
-    v4i x[4], y[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const v4i*>(b + (int64_t)kb * kBlock + 32 * j);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const v4i*>(a + (int64_t)kb * kBlock + 32 * j);
-    multiply(x, y, load_scale<KIND>(P.sa, sa + kb), load_scale<KIND>(P.sb, sb + kb));
-  }
-  if (full < kb1) {  // a last block that ends inside: zeros past the end
-    const int k = P.k / kBlock;
-    v4i x[4], y[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool in = k * kBlock + 32 * j + 16 * half < P.k;
-      const v4i zero = {0, 0, 0, 0};
-      y[j] = in ? *reinterpret_cast<const v4i*>(b + (int64_t)k * kBlock + 32 * j) : zero;
-      x[j] = in ? *reinterpret_cast<const v4i*>(a + (int64_t)k * kBlock + 32 * j) : zero;
-    }
-    multiply(x, y, load_scale<KIND>(P.sa, sa + k), load_scale<KIND>(P.sb, sb + k));
-  }
-
-  // Lane (c32, half) holds row c32, columns 8g + 4 half .. + 3.
+// The waves' sums of a workgroup's 32 columns, in order, to the result. Lane (c32, half) holds row c32, columns 8g + 4 half
+// .. + 3.
+template <int WAVES, int OUT>
+__device__ __forceinline__ void join_waves(const GemmParams& P, v4f* sums, const v16f& acc) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c32 = lane & 31, half = lane >> 5, n0 = blockIdx.x * kFew;
 #pragma unroll
   for (int g = 0; g < 4; ++g)
     sums[wave * 256 + g * 64 + lane] = (v4f){acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
@@ -623,7 +579,7 @@ __global__ void __launch_bounds__(kFewWaves * 64) fp8_gemm_few_kernel(const Gemm
   if (threadIdx.x >= 256 || c32 >= P.m) return;
   v4f v = sums[threadIdx.x];
 #pragma unroll
-  for (int w = 1; w < kFewWaves; ++w) {
+  for (int w = 1; w < WAVES; ++w) {
     const v4f x = sums[w * 256 + threadIdx.x];
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] += x[j];
@@ -633,6 +589,99 @@ __global__ void __launch_bounds__(kFewWaves * 64) fp8_gemm_few_kernel(const Gemm
   const bool aligned = !((reinterpret_cast<uintptr_t>(P.out) & (OUT == kOutBf16 ? 7 : 15)) | (P.out_stride & 3));
   const float r[4] = {v[0], v[1], v[2], v[3]};
   store4<OUT>(P.out, (int64_t)c32 * P.out_stride + n, aligned && n + 4 <= P.n, P.n - n, r);
+}
+
+template <int WAVES, int KIND, int OUT>
+__global__ void __launch_bounds__(WAVES * 64) fp8_gemm_few_kernel(const GemmParams P) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c32 = lane & 31, half = lane >> 5;
+  const int n0 = blockIdx.x * kFew;
+  const int kb0 = (int)((int64_t)P.kblocks * wave / WAVES), kb1 = (int)((int64_t)P.kblocks * (wave + 1) / WAVES);
+  const int steps = kb1 - kb0, full = P.k / kBlock;
+  uint8_t* mine = smem + wave * kFewWave;
+  uint32_t* scales = reinterpret_cast<uint32_t*>(mine + 2 * kFewStage);
+
+  // copy i brings rows 8i .. 8i + 7, pieces in the tiles' order; rows past the matrix repeat its last one
+  const int piece0 = (lane & 7) ^ (lane >> 4), piece1 = piece0 ^ 4;
+  uint32_t off_a[4], off_b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 8 * i + (lane >> 3), piece = i & 1 ? piece1 : piece0;
+    off_a[i] = (uint32_t)min(row, P.m - 1) * (uint32_t)P.a_stride + 16 * piece;
+    off_b[i] = (uint32_t)min(row, P.n - 1 - n0) * (uint32_t)P.b_stride + 16 * piece;
+  }
+  const uint8_t* tile_b = P.b + (int64_t)n0 * P.b_stride;
+  const uint64_t tail0 = __builtin_amdgcn_ballot_w64(16 * piece0 < P.k % kBlock);
+  const uint64_t tail1 = __builtin_amdgcn_ballot_w64(16 * piece1 < P.k % kBlock);
+  auto issue = [&](int s) {
+    const int kb = kb0 + s, buf = s & 1;
+    const uint32_t dst = lds_addr(mine) + buf * kFewStage;
+    const bool whole = kb < full;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t mask = whole ? ~0ull : i & 1 ? tail1 : tail0;
+      dma16(tile_b + (int64_t)kb * kBlock, off_b[i], dst + i * 1024, mask);
+      dma16(P.a + (int64_t)kb * kBlock, off_a[i], dst + 4096 + i * 1024, mask);
+    }
+    if (!whole) {
+      const v4i zero = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (16 * (i & 1 ? piece1 : piece0) >= P.k % kBlock) {
+          uint8_t* z = mine + buf * kFewStage + i * 1024 + lane * 16;
+          *reinterpret_cast<v4i*>(z) = zero;
+          *reinterpret_cast<v4i*>(z + 4096) = zero;
+        }
+    }
+  };
+  for (int s = 0; s < min(steps, 2); ++s) issue(s);
+  // scales: of the activations in LDS, [block][row]; of the weights one a lane
+  const int64_t sb_at = (int64_t)(n0 / kBlock) * P.sb_stride, sa_at = (int64_t)min(c32, P.m - 1) * P.sa_stride;
+  uint32_t sb = load_scale<KIND>(P.sb, sb_at + min(kb0 + lane, P.kblocks - 1));
+  uint32_t sa[kFewBlocks / 2];
+#pragma unroll
+  for (int t = 0; t < kFewBlocks / 2; ++t) sa[t] = load_scale<KIND>(P.sa, sa_at + min(kb0 + 2 * t + half, P.kblocks - 1));
+#pragma unroll
+  for (int t = 0; t < kFewBlocks / 2; ++t) scales[(2 * t + half) * kFew + c32] = sa[t];
+  asm volatile("" : "+v"(sb));  // (waited for here)
+  wait_loads<0>();
+
+  const uint32_t at0 = c32 * kBlock + 16 * ((2 * half) ^ ((lane >> 1) & 7));
+  v16f acc = {};
+  for (int s = 0; s < steps; ++s) {
+    if (s + 1 < steps) wait_loads<8>();  // the next block may still be on its way
+    else wait_loads<0>();
+    const uint8_t* rows = mine + s % 2 * kFewStage;
+    v8i fa[2], fb[2];
+    auto operand = [&](int at) {
+      const v4i p = *reinterpret_cast<const v4i*>(rows + at), q = *reinterpret_cast<const v4i*>(rows + (at ^ 16));
+      return (v8i){p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
+    };
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      fb[h] = operand(at0 ^ (64 * h));
+      fa[h] = operand(4096 + (at0 ^ (64 * h)));
+    }
+    const uint32_t ca = scales[s * kFew + c32], cb = __builtin_amdgcn_readlane(sb, s);
+    wait_loads<63>();  // the block is in registers: its place is free
+    if (s + 2 < steps) issue(s + 2);
+    if (KIND == kScaleE8M0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h], fa[h], acc, 0, 0, 0, cb, 0, ca);
+    } else {
+      v16f part = {};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        part = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h], fa[h], part, 0, 0, 0, 127, 0, 127);
+      const float f = __uint_as_float(ca) * __uint_as_float(cb);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[r] += part[r] * f;
+    }
+  }
+  __syncthreads();
+  join_waves<WAVES, OUT>(P, reinterpret_cast<v4f*>(smem), acc);
 }
 
 // out = the sum of the splits' partial sums, in order; eight parts' loads in flight at once. They are read once, past the L2
@@ -698,28 +747,23 @@ constexpr Tile kTilesF32[] = {
 // A second launch adds up the parts of K: so much, and more by their MB.
 constexpr float kSumBase = 2.9f, kSumPerMB[2] = {0.33f, 0.25f};
 
-// The same of the kernel for few rows, a part of K a wave: base + steps (per_step + rounds (per_round + rows per_row)).
-// Fitted to 1 to 32 rows of 180 shapes, of which the choice is 2% slower than the best on average.
-constexpr struct {
-  float base, per_step, per_round, per_row;
-} kFewCost = {2.0f, 0.36f, 1.0f, 0.02f};
 constexpr int kFewTile = -1;
 
 struct Plan {
-  int tile, splits;
+  int tile, splits;  // kFewTile: by the kernel for few rows, and its waves
 };
 
 Plan plan_of(int m, int n, int k, int kind, int cus) {
   const int kblocks = (k + kBlock - 1) / kBlock;
+  // Few rows: the kernel of their own as far as a wave's scales reach, 1.40 times as fast as the best tile over 110 shapes (64 to
+  // 24576 columns, 128 to 16384 deep). Eight waves where they leave half of the CUs idle and K is long (2112 x 8192: 8.0 us, by
+  // four 8.4 to 9.7), or too long for four; four elsewhere, of which a CU holds two groups (8 x 8192 x 8192 13.8, by eight 14.8).
+  if (m <= kFew && kblocks <= 8 * kFewBlocks)
+    return {kFewTile, kblocks > 4 * kFewBlocks || (kblocks > 16 && ((n - 1) / kFew + 1) * 2 <= cus) ? 8 : 4};
   const Tile* tiles = kind == kScaleF32 ? kTilesF32 : kTilesE8M0;
   const int count = kind == kScaleF32 ? (int)(sizeof(kTilesF32) / sizeof(Tile)) : (int)(sizeof(kTilesE8M0) / sizeof(Tile));
   Plan best = {0, 1};
   double least = 1e300;
-  if (m <= kFew) {
-    const double rounds = std::ceil(((n - 1) / kFew + 1.0) / cus), steps = (kblocks - 1) / kFewWaves + 1;
-    least = kFewCost.base + steps * (kFewCost.per_step + rounds * (kFewCost.per_round + m * kFewCost.per_row));
-    best.tile = kFewTile;
-  }
   for (int t = 0; t < count; ++t) {
     const Tile& T = tiles[t];
     const double all = ((m - 1) / T.bm + 1.0) * ((n - 1) / T.bn + 1.0);
@@ -738,7 +782,9 @@ Plan plan_of(int m, int n, int k, int kind, int cus) {
   return best;
 }
 
-size_t workspace_of(const Plan& p, int m, int n) { return p.splits > 1 ? (size_t)p.splits * m * n * sizeof(float) : 0; }
+size_t workspace_of(const Plan& p, int m, int n) {
+  return p.tile != kFewTile && p.splits > 1 ? (size_t)p.splits * m * n * sizeof(float) : 0;
+}
 
 constexpr int kMaxDevices = 64;
 
@@ -759,21 +805,24 @@ int current_device() {
   return hipGetDevice(&dev) == hipSuccess ? dev : -1;
 }
 
+// A kernel's use of more LDS than 64 KB has to be asked for, once a device (`known`: those that were).
+int allow_smem(const void* kern, int bytes, int dev, std::atomic<uint64_t>& known) {
+  const uint64_t bit = dev >= 0 && dev < kMaxDevices ? 1ull << dev : 0;
+  if (bytes <= 64 * 1024 || (known.load(std::memory_order_relaxed) & bit)) return kOk;
+  const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return set_error(kLaunchFailed, "dsa_fp8_gemm: %s", hipGetErrorString(e));
+  known.fetch_or(bit, std::memory_order_relaxed);
+  return kOk;
+}
+
 template <int BM, int BN, int WM, int WN, int STAGES, int KIND, int OUT>
 int launch_tile(GemmParams P, int dev, hipStream_t st) {
   constexpr int kSmem = gemm_smem<BM, BN, STAGES, KIND>();
   static_assert(kSmem <= 160 * 1024, "LDS of a CU");
   auto kern = fp8_gemm_kernel<BM, BN, WM, WN, STAGES, KIND, OUT>;
-  if (kSmem > 64 * 1024) {
-    static std::atomic<uint64_t> done{0};  // devices that know
-    const uint64_t bit = dev >= 0 && dev < kMaxDevices ? 1ull << dev : 0;
-    if (!(done.load(std::memory_order_relaxed) & bit)) {
-      const hipError_t e =
-          hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-      if (e != hipSuccess) return set_error(kLaunchFailed, "dsa_fp8_gemm: %s", hipGetErrorString(e));
-      done.fetch_or(bit, std::memory_order_relaxed);
-    }
-  }
+  static std::atomic<uint64_t> known{0};
+  const int rc = allow_smem(reinterpret_cast<const void*>(kern), kSmem, dev, known);
+  if (rc != kOk) return rc;
   P.mtiles = (P.m - 1) / BM + 1;
   P.ntiles = (P.n - 1) / BN + 1;
   const int64_t groups = (int64_t)P.mtiles * P.ntiles * P.splits;
@@ -782,16 +831,24 @@ int launch_tile(GemmParams P, int dev, hipStream_t st) {
   return check_launch("dsa_fp8_gemm");
 }
 
-template <int KIND, int OUT>
-int launch_few(const GemmParams& P, hipStream_t st) {
-  hipLaunchKernelGGL((fp8_gemm_few_kernel<KIND, OUT>), dim3((P.n - 1) / kFew + 1), dim3(kFewWaves * 64), 0, st, P);
+template <int WAVES, int KIND, int OUT>
+int launch_few(const GemmParams& P, int dev, hipStream_t st) {
+  constexpr int kSmem = WAVES * kFewWave;
+  auto kern = fp8_gemm_few_kernel<WAVES, KIND, OUT>;
+  static std::atomic<uint64_t> known{0};
+  const int rc = allow_smem(reinterpret_cast<const void*>(kern), kSmem, dev, known);
+  if (rc != kOk) return rc;
+  hipLaunchKernelGGL(kern, dim3((P.n - 1) / kFew + 1), dim3(WAVES * 64), kSmem, st, P);
   return check_launch("dsa_fp8_gemm");
 }
 
 template <int OUT>
 int launch_plan(const Plan& p, int kind, const GemmParams& P, int dev, hipStream_t st) {
-  if (p.tile == kFewTile)
-    return kind == kScaleE8M0 ? launch_few<kScaleE8M0, OUT>(P, st) : launch_few<kScaleF32, OUT>(P, st);
+  if (p.tile == kFewTile) {
+    if (kind == kScaleE8M0)
+      return p.splits == 8 ? launch_few<8, kScaleE8M0, OUT>(P, dev, st) : launch_few<4, kScaleE8M0, OUT>(P, dev, st);
+    return p.splits == 8 ? launch_few<8, kScaleF32, OUT>(P, dev, st) : launch_few<4, kScaleF32, OUT>(P, dev, st);
+  }
   if (kind == kScaleE8M0) {
     switch (p.tile) {
       case 0: return launch_tile<32, 64, 32, 32, 3, kScaleE8M0, OUT>(P, dev, st);
@@ -862,9 +919,9 @@ int dsa_fp8_gemm(const uint8_t* a, int64_t a_stride, const void* a_scale, int64_
   if (need && (reinterpret_cast<uintptr_t>(workspace) & 15))
     return set_error(kInvalidArgument, "dsa_fp8_gemm: the workspace must be 16-byte aligned");
   GemmParams P = {a, b, m > 1 ? a_stride : k, n > 1 ? b_stride : k, a_scale, b_scale, a_scale_stride, b_scale_stride,
-                  m, n, k, kblocks, 0, 0, p.splits, out, out_stride};
+                  m, n, k, kblocks, 0, 0, p.tile == kFewTile ? 1 : p.splits, out, out_stride};
   const hipStream_t st = (hipStream_t)stream;
-  if (p.splits == 1)
+  if (p.tile == kFewTile || p.splits == 1)
     return out_is_f32 ? launch_plan<kOutF32>(p, scale_kind, P, dev, st) : launch_plan<kOutBf16>(p, scale_kind, P, dev, st);
   P.out = workspace;
   P.out_stride = n;
