@@ -555,43 +555,52 @@ fp8_gemm_kernel(const GemmParams P) {
   }
 }
 
-// Up to 32 rows: a workgroup takes 32 columns, its four or eight waves parts of K, each with two blocks of 128 of its own
-// on their way into LDS in whole lines while a third is multiplied; the waves' sums meet in LDS, in order. No meetings of
-// waves until then, no second launch: 1 x 8192 x 1536 in 5.0 us (by tiles 8.0), 32 x 576 x 1536 4.0 (7.5), 16 x 2112 x
-// 8192 8.3 (10.8), 8 x 8192 x 8192 13.8 (15.4). What bounds it is the start (2 us beside the launch) and then what a CU can
-// fetch, 0.5 us a block of K for each of eight waves. (Straight into registers a load touches 32 rows, and where
-// these lie a power of two apart their lines crowd each other out of L1 before the next load wants them: 16 x 2112 x 8192
-// 15.4, 1 x 8192 x 1536 the same 5.0.)
-constexpr int kFew = 32;
-constexpr int kFewBlocks = 16;                                       // of K, a wave at most
-constexpr int kFewStage = 2 * kFew * kBlock;                         // a block of weights and of activations
-constexpr int kFewWave = 2 * kFewStage + kFewBlocks * kFew * 4;      // and the activations' scales
+// Few rows: a workgroup takes 32 columns, its four or eight waves parts of K, each with two blocks of 128 of its own on
+// their way into LDS in whole lines while a third is multiplied; the waves' sums meet in LDS, in order. No meetings of
+// waves until then, no second launch: 1 x 8192 x 1536 in 4.0 us (by tiles 8.0), 32 x 576 x 1536 4.0 (7.5), 16 x 2112 x
+// 8192 7.7 (10.8), 8 x 8192 x 8192 13.4 (15.4; its bytes take 13.0). What bounds it is the start (under 2 us beside the
+// launch) and then memory, or what few CUs can fetch: 0.5 us a block of K for each of eight waves. (Straight into
+// registers a load touches 32 rows, and where these lie a power of two apart their lines crowd each other out of L1
+// before the next load wants them: 16 x 2112 x 8192 15.4, 1 x 8192 x 1536 4.6.)
+constexpr int kFew = 32;         // columns, and rows of one activation tile: there are one or two
+constexpr int kFewBlocks = 16;   // of K, a wave at most
+template <int TILES>
+constexpr int kFewStage = (1 + TILES) * kFew * kBlock;  // a block of weights and of activations
+template <int TILES>
+constexpr int kFewWave = 2 * kFewStage<TILES> + kFewBlocks * TILES * kFew * 4;  // and the activations' scales
 
 // The waves' sums of a workgroup's 32 columns, in order, to the result. Lane (c32, half) holds row c32, columns 8g + 4 half
 // .. + 3.
-template <int WAVES, int OUT>
-__device__ __forceinline__ void join_waves(const GemmParams& P, v4f* sums, const v16f& acc) {
+template <int WAVES, int TILES, int OUT>
+__device__ __forceinline__ void join_waves(const GemmParams& P, v4f* sums, const v16f* acc) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c32 = lane & 31, half = lane >> 5, n0 = blockIdx.x * kFew;
 #pragma unroll
-  for (int g = 0; g < 4; ++g)
-    sums[wave * 256 + g * 64 + lane] = (v4f){acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+  for (int t = 0; t < TILES; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      sums[(t * WAVES + wave) * 256 + g * 64 + lane] =
+          (v4f){acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]};
   __syncthreads();
-  if (threadIdx.x >= 256 || c32 >= P.m) return;
-  v4f v = sums[threadIdx.x];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) {
-    const v4f x = sums[w * 256 + threadIdx.x];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] += x[j];
-  }
   const int n = n0 + 8 * wave + 4 * half;
-  if (n >= P.n) return;
+  if (threadIdx.x >= 256 || n >= P.n) return;
   const bool aligned = !((reinterpret_cast<uintptr_t>(P.out) & (OUT == kOutBf16 ? 7 : 15)) | (P.out_stride & 3));
-  const float r[4] = {v[0], v[1], v[2], v[3]};
-  store4<OUT>(P.out, (int64_t)c32 * P.out_stride + n, aligned && n + 4 <= P.n, P.n - n, r);
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    const int m = t * kFew + c32;
+    if (m >= P.m) return;
+    v4f v = sums[t * WAVES * 256 + threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+      const v4f x = sums[(t * WAVES + w) * 256 + threadIdx.x];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += x[j];
+    }
+    const float r[4] = {v[0], v[1], v[2], v[3]};
+    store4<OUT>(P.out, (int64_t)m * P.out_stride + n, aligned && n + 4 <= P.n, P.n - n, r);
+  }
 }
 
-template <int WAVES, int KIND, int OUT>
+template <int WAVES, int TILES, int KIND, int OUT>
 __global__ void __launch_bounds__(WAVES * 64) fp8_gemm_few_kernel(const GemmParams P) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -599,61 +608,62 @@ __global__ void __launch_bounds__(WAVES * 64) fp8_gemm_few_kernel(const GemmPara
   const int n0 = blockIdx.x * kFew;
   const int kb0 = (int)((int64_t)P.kblocks * wave / WAVES), kb1 = (int)((int64_t)P.kblocks * (wave + 1) / WAVES);
   const int steps = kb1 - kb0, full = P.k / kBlock;
-  uint8_t* mine = smem + wave * kFewWave;
-  uint32_t* scales = reinterpret_cast<uint32_t*>(mine + 2 * kFewStage);
+  constexpr int kStage = kFewStage<TILES>, kRows = TILES * kFew, kCopies = 4 + 4 * TILES;
+  uint8_t* mine = smem + wave * kFewWave<TILES>;
+  uint32_t* scales = reinterpret_cast<uint32_t*>(mine + 2 * kStage);
 
   // copy i brings rows 8i .. 8i + 7, pieces in the tiles' order; rows past the matrix repeat its last one
   const int piece0 = (lane & 7) ^ (lane >> 4), piece1 = piece0 ^ 4;
-  uint32_t off_a[4], off_b[4];
+  uint32_t off_a[4 * TILES], off_b[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4 * TILES; ++i) {
     const int row = 8 * i + (lane >> 3), piece = i & 1 ? piece1 : piece0;
     off_a[i] = (uint32_t)min(row, P.m - 1) * (uint32_t)P.a_stride + 16 * piece;
-    off_b[i] = (uint32_t)min(row, P.n - 1 - n0) * (uint32_t)P.b_stride + 16 * piece;
+    if (i < 4) off_b[i] = (uint32_t)min(row, P.n - 1 - n0) * (uint32_t)P.b_stride + 16 * piece;
   }
   const uint8_t* tile_b = P.b + (int64_t)n0 * P.b_stride;
   const uint64_t tail0 = __builtin_amdgcn_ballot_w64(16 * piece0 < P.k % kBlock);
   const uint64_t tail1 = __builtin_amdgcn_ballot_w64(16 * piece1 < P.k % kBlock);
   auto issue = [&](int s) {
     const int kb = kb0 + s, buf = s & 1;
-    const uint32_t dst = lds_addr(mine) + buf * kFewStage;
+    const uint32_t dst = lds_addr(mine) + buf * kStage;
     const bool whole = kb < full;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4 * TILES; ++i) {
       const uint64_t mask = whole ? ~0ull : i & 1 ? tail1 : tail0;
-      dma16(tile_b + (int64_t)kb * kBlock, off_b[i], dst + i * 1024, mask);
+      if (i < 4) dma16(tile_b + (int64_t)kb * kBlock, off_b[i], dst + i * 1024, mask);
       dma16(P.a + (int64_t)kb * kBlock, off_a[i], dst + 4096 + i * 1024, mask);
     }
     if (!whole) {
       const v4i zero = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (16 * (i & 1 ? piece1 : piece0) >= P.k % kBlock) {
-          uint8_t* z = mine + buf * kFewStage + i * 1024 + lane * 16;
-          *reinterpret_cast<v4i*>(z) = zero;
-          *reinterpret_cast<v4i*>(z + 4096) = zero;
-        }
+      for (int i = 0; i < kCopies; ++i)
+        if (16 * (i & 1 ? piece1 : piece0) >= P.k % kBlock)
+          *reinterpret_cast<v4i*>(mine + buf * kStage + i * 1024 + lane * 16) = zero;
     }
   };
   for (int s = 0; s < min(steps, 2); ++s) issue(s);
   // scales: of the activations in LDS, [block][row]; of the weights one a lane
-  const int64_t sb_at = (int64_t)(n0 / kBlock) * P.sb_stride, sa_at = (int64_t)min(c32, P.m - 1) * P.sa_stride;
+  const int row = lane % kRows, first = lane / kRows;
+  const int64_t sb_at = (int64_t)(n0 / kBlock) * P.sb_stride, sa_at = (int64_t)min(row, P.m - 1) * P.sa_stride;
   uint32_t sb = load_scale<KIND>(P.sb, sb_at + min(kb0 + lane, P.kblocks - 1));
-  uint32_t sa[kFewBlocks / 2];
+  constexpr int kEach = 64 / kRows;  // blocks at a time
+  uint32_t sa[kFewBlocks / kEach];
 #pragma unroll
-  for (int t = 0; t < kFewBlocks / 2; ++t) sa[t] = load_scale<KIND>(P.sa, sa_at + min(kb0 + 2 * t + half, P.kblocks - 1));
+  for (int t = 0; t < kFewBlocks / kEach; ++t)
+    sa[t] = load_scale<KIND>(P.sa, sa_at + min(kb0 + kEach * t + first, P.kblocks - 1));
 #pragma unroll
-  for (int t = 0; t < kFewBlocks / 2; ++t) scales[(2 * t + half) * kFew + c32] = sa[t];
+  for (int t = 0; t < kFewBlocks / kEach; ++t) scales[(kEach * t + first) * kRows + row] = sa[t];
   asm volatile("" : "+v"(sb));  // (waited for here)
   wait_loads<0>();
 
   const uint32_t at0 = c32 * kBlock + 16 * ((2 * half) ^ ((lane >> 1) & 7));
-  v16f acc = {};
+  v16f acc[TILES] = {};
   for (int s = 0; s < steps; ++s) {
-    if (s + 1 < steps) wait_loads<8>();  // the next block may still be on its way
+    if (s + 1 < steps) wait_loads<kCopies>();  // the next block may still be on its way
     else wait_loads<0>();
-    const uint8_t* rows = mine + s % 2 * kFewStage;
-    v8i fa[2], fb[2];
+    const uint8_t* rows = mine + s % 2 * kStage;
+    v8i fa[TILES][2], fb[2];
     auto operand = [&](int at) {
       const v4i p = *reinterpret_cast<const v4i*>(rows + at), q = *reinterpret_cast<const v4i*>(rows + (at ^ 16));
       return (v8i){p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
@@ -661,27 +671,34 @@ __global__ void __launch_bounds__(WAVES * 64) fp8_gemm_few_kernel(const GemmPara
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       fb[h] = operand(at0 ^ (64 * h));
-      fa[h] = operand(4096 + (at0 ^ (64 * h)));
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) fa[t][h] = operand((1 + t) * 4096 + (at0 ^ (64 * h)));
     }
-    const uint32_t ca = scales[s * kFew + c32], cb = __builtin_amdgcn_readlane(sb, s);
+    uint32_t ca[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) ca[t] = scales[s * kRows + t * kFew + c32];
+    const uint32_t cb = __builtin_amdgcn_readlane(sb, s);
     wait_loads<63>();  // the block is in registers: its place is free
     if (s + 2 < steps) issue(s + 2);
-    if (KIND == kScaleE8M0) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h], fa[h], acc, 0, 0, 0, cb, 0, ca);
-    } else {
-      v16f part = {};
+    for (int t = 0; t < TILES; ++t) {
+      if (KIND == kScaleE8M0) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        part = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h], fa[h], part, 0, 0, 0, 127, 0, 127);
-      const float f = __uint_as_float(ca) * __uint_as_float(cb);
+        for (int h = 0; h < 2; ++h)
+          acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h], fa[t][h], acc[t], 0, 0, 0, cb, 0, ca[t]);
+      } else {
+        v16f part = {};
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[r] += part[r] * f;
+        for (int h = 0; h < 2; ++h)
+          part = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[h], fa[t][h], part, 0, 0, 0, 127, 0, 127);
+        const float f = __uint_as_float(ca[t]) * __uint_as_float(cb);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[t][r] += part[r] * f;
+      }
     }
   }
   __syncthreads();
-  join_waves<WAVES, OUT>(P, reinterpret_cast<v4f*>(smem), acc);
+  join_waves<WAVES, TILES, OUT>(P, reinterpret_cast<v4f*>(smem), acc);
 }
 
 // out = the sum of the splits' partial sums, in order; eight parts' loads in flight at once. They are read once, past the L2
@@ -755,11 +772,16 @@ struct Plan {
 
 Plan plan_of(int m, int n, int k, int kind, int cus) {
   const int kblocks = (k + kBlock - 1) / kBlock;
-  // Few rows: the kernel of their own as far as a wave's scales reach, 1.40 times as fast as the best tile over 110 shapes (64 to
-  // 24576 columns, 128 to 16384 deep). Eight waves where they leave half of the CUs idle and K is long (2112 x 8192: 8.0 us, by
-  // four 8.4 to 9.7), or too long for four; four elsewhere, of which a CU holds two groups (8 x 8192 x 8192 13.8, by eight 14.8).
+  // Few rows: the kernel of their own as far as a wave's scales reach. Up to 32: 1.4 times as fast as the best tile over 110
+  // shapes (64 to 24576 columns, 128 to 16384 deep). Eight waves where they leave half of the CUs idle and K is long
+  // (2112 x 8192: 6.9 us, by four 8.4), or too long for four; four elsewhere, of which a CU holds two groups
+  // (8192 x 8192 13.4, by eight 14.8). Up to 64 where every group has a CU at once (64 x 8192 x 1536 6.2 us, by tiles 8.3;
+  // 64 x 24576 x 1536 14.8 and 11.3), and K is short or half of the CUs have one (64 x 576 x 8192 11.1 and 9.0).
+  const int groups = (n - 1) / kFew + 1;
   if (m <= kFew && kblocks <= 8 * kFewBlocks)
-    return {kFewTile, kblocks > 4 * kFewBlocks || (kblocks > 16 && ((n - 1) / kFew + 1) * 2 <= cus) ? 8 : 4};
+    return {kFewTile, kblocks > 4 * kFewBlocks || (kblocks > 16 && groups <= cus / 2) ? 8 : 4};
+  if (m > kFew && m <= 2 * kFew && groups <= cus && kblocks <= 4 * kFewBlocks && (kblocks <= 32 || groups > cus / 2))
+    return {kFewTile, 4};
   const Tile* tiles = kind == kScaleF32 ? kTilesF32 : kTilesE8M0;
   const int count = kind == kScaleF32 ? (int)(sizeof(kTilesF32) / sizeof(Tile)) : (int)(sizeof(kTilesE8M0) / sizeof(Tile));
   Plan best = {0, 1};
@@ -831,10 +853,11 @@ int launch_tile(GemmParams P, int dev, hipStream_t st) {
   return check_launch("dsa_fp8_gemm");
 }
 
-template <int WAVES, int KIND, int OUT>
+template <int WAVES, int TILES, int KIND, int OUT>
 int launch_few(const GemmParams& P, int dev, hipStream_t st) {
-  constexpr int kSmem = WAVES * kFewWave;
-  auto kern = fp8_gemm_few_kernel<WAVES, KIND, OUT>;
+  constexpr int kSmem = WAVES * kFewWave<TILES>;
+  static_assert(kSmem <= 160 * 1024 && WAVES >= 4, "LDS of a CU, and 256 threads to join");
+  auto kern = fp8_gemm_few_kernel<WAVES, TILES, KIND, OUT>;
   static std::atomic<uint64_t> known{0};
   const int rc = allow_smem(reinterpret_cast<const void*>(kern), kSmem, dev, known);
   if (rc != kOk) return rc;
@@ -846,8 +869,12 @@ template <int OUT>
 int launch_plan(const Plan& p, int kind, const GemmParams& P, int dev, hipStream_t st) {
   if (p.tile == kFewTile) {
     if (kind == kScaleE8M0)
-      return p.splits == 8 ? launch_few<8, kScaleE8M0, OUT>(P, dev, st) : launch_few<4, kScaleE8M0, OUT>(P, dev, st);
-    return p.splits == 8 ? launch_few<8, kScaleF32, OUT>(P, dev, st) : launch_few<4, kScaleF32, OUT>(P, dev, st);
+      return P.m > kFew        ? launch_few<4, 2, kScaleE8M0, OUT>(P, dev, st)
+             : p.splits == 8 ? launch_few<8, 1, kScaleE8M0, OUT>(P, dev, st)
+                             : launch_few<4, 1, kScaleE8M0, OUT>(P, dev, st);
+    return P.m > kFew        ? launch_few<4, 2, kScaleF32, OUT>(P, dev, st)
+           : p.splits == 8 ? launch_few<8, 1, kScaleF32, OUT>(P, dev, st)
+                           : launch_few<4, 1, kScaleF32, OUT>(P, dev, st);
   }
   if (kind == kScaleE8M0) {
     switch (p.tile) {

@@ -191,7 +191,9 @@ def test_gemm_long(cuda, M, N, K, kind):
 
 
 @pytest.mark.parametrize("M,N,K", [(32, 8200, 1536), (3, 2112, 1168), (1, 31, 1008), (32, 33, 400), (5, 24576, 128), (9, 100, 96),
-                                   (1, 8192, 8192), (20, 4100, 3600), (32, 2112, 8208), (2, 576, 16400)])
+                                   (1, 8192, 8192), (20, 4100, 3600), (32, 2112, 8208), (2, 576, 16400), (1, 64, 16384),
+                                   (31, 576, 16144), (33, 129, 16), (64, 2100, 1536), (40, 8200, 3600), (63, 4100, 8080),
+                                   (50, 8100, 400), (64, 300, 4096), (64, 8192, 8192), (65, 300, 1536)])
 @pytest.mark.parametrize("kind", ["f32", "e8m0"])
 def test_gemm_few_rows(cuda, M, N, K, kind):
     """Few rows, on both sides of the choice between waves over K and tiles; an odd result in between others."""
