@@ -10,7 +10,7 @@
 // e8m0 scales are the instruction's own, and all of K runs into one accumulator. f32 scales take a
 // second one: a block's sums times sa sb are added to the first by vector instructions.
 //
-// Three kernels share that: tiles staged through LDS; waves over K for up to 32 rows; and the
+// Three kernels share that: tiles staged through LDS; waves over K for up to 64 rows; and the
 // sum of a product's parts where K is split. A cost fitted to measurements chooses (plan_of).
 //
 // Tiles: a workgroup's blocks of 128 of a and b go straight from memory into LDS, two or three
@@ -19,7 +19,7 @@
 // (rows are half the banks' span apart; with row % 8 two of 16 met on each bank: 1e8 conflict
 // cycles in 8192 x 8192 x 16384, now 2e6).
 //
-// What bounds it, measured: 8192 x 8192 x 16384 (e8m0) 745-765 us, 2.9 PFLOP/s, where the library's product with
+// What bounds it, measured: 8192 x 8192 x 16384 (e8m0) 735-765 us, 2.9 to 3.0 PFLOP/s, where the library's product with
 // one scale a matrix takes 720-765 on the same cards and one with a scale per 32 elements 1450. Products run in 79% of
 // a SIMD's cycles, and the clock gives way under their power: without any copies it takes 698, with all data in L2 780
 // of then 811, without scales 3% less; persistent workgroups, which close the gaps between tiles, gain nothing. Steps
