@@ -559,7 +559,7 @@ fp8_gemm_kernel(const GemmParams P) {
 // their way into LDS in whole lines while a third is multiplied; the waves' sums meet in LDS, in order. No meetings of
 // waves until then, no second launch: 1 x 8192 x 1536 in 4.0 us (by tiles 8.0), 32 x 576 x 1536 4.0 (7.5), 16 x 2112 x
 // 8192 7.7 (10.8), 8 x 8192 x 8192 13.4 (15.4; its bytes take 13.0). What bounds it is the start (under 2 us beside the
-// launch) and then memory, or what few CUs can fetch: 0.5 us a block of K for each of eight waves. (Straight into
+// launch) and then memory, or what few CUs can fetch: 0.3 us a block of K for each of four waves. (Straight into
 // registers a load touches 32 rows, and where these lie a power of two apart their lines crowd each other out of L1
 // before the next load wants them: 16 x 2112 x 8192 15.4, 1 x 8192 x 1536 4.6.)
 constexpr int kFew = 32;         // columns, and rows of one activation tile: there are one or two
@@ -773,13 +773,12 @@ struct Plan {
 Plan plan_of(int m, int n, int k, int kind, int cus) {
   const int kblocks = (k + kBlock - 1) / kBlock;
   // Few rows: the kernel of their own as far as a wave's scales reach. Up to 32: 1.4 times as fast as the best tile over 110
-  // shapes (64 to 24576 columns, 128 to 16384 deep). Eight waves where they leave half of the CUs idle and K is long
-  // (2112 x 8192: 6.9 us, by four 8.4), or too long for four; four elsewhere, of which a CU holds two groups
-  // (8192 x 8192 13.4, by eight 14.8). Up to 64 where every group has a CU at once (64 x 8192 x 1536 6.2 us, by tiles 8.3;
-  // 64 x 24576 x 1536 14.8 and 11.3), and K is short or half of the CUs have one (64 x 576 x 8192 11.1 and 9.0).
+  // shapes (64 to 24576 columns, 128 to 16384 deep), by four waves, of which a CU holds two groups (32 x 8192 x 8192
+  // 13.5 us, by eight 15.6), and by eight where K is too long for four. Up to 64 where every group has a CU at once (64 x
+  // 8192 x 1536 6.2 us, by tiles 8.3; 64 x 24576 x 1536 14.8 and 11.3), and K is short or half of the CUs have one (64 x 576
+  // x 8192 11.1 and 9.0).
   const int groups = (n - 1) / kFew + 1;
-  if (m <= kFew && kblocks <= 8 * kFewBlocks)
-    return {kFewTile, kblocks > 4 * kFewBlocks || (kblocks > 16 && groups <= cus / 2) ? 8 : 4};
+  if (m <= kFew && kblocks <= 8 * kFewBlocks) return {kFewTile, kblocks > 4 * kFewBlocks ? 8 : 4};
   if (m > kFew && m <= 2 * kFew && groups <= cus && kblocks <= 4 * kFewBlocks && (kblocks <= 32 || groups > cus / 2))
     return {kFewTile, 4};
   const Tile* tiles = kind == kScaleF32 ? kTilesF32 : kTilesE8M0;

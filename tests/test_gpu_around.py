@@ -251,7 +251,7 @@ def test_far_rows_of_norm_and_rope(cuda):
 def test_gemm_strides_and_neighbours(cuda):
     """Rows inside wider ones, outputs inside wider ones: what lies beside them stays."""
     g = gen(cuda, 6)
-    for M, N, K, kind in ((5, 200, 272, "e8m0"), (130, 333, 1152, "f32")):
+    for M, N, K, kind in ((5, 200, 272, "e8m0"), (130, 333, 1152, "f32"), (7, 203, 272, "f32"), (45, 203, 1040, "e8m0")):
         a, sa, b, sb = product(g, M, N, K, kind)
         want = ops.fp8_gemm(a, sa, b, sb)
 
@@ -270,7 +270,7 @@ def test_gemm_strides_and_neighbours(cuda):
 
 def test_gemm_nan_stays_in_its_row_and_column(cuda):
     g = gen(cuda, 7)
-    for M, N, K, kind in ((40, 300, 400, "e8m0"), (200, 300, 1040, "f32")):
+    for M, N, K, kind in ((40, 300, 400, "e8m0"), (200, 300, 1040, "f32"), (20, 300, 400, "f32"), (20, 300, 8208, "e8m0")):
         a, sa, b, sb = product(g, M, N, K, kind)
         a.view(torch.uint8)[M - 3, K - 1] = 0x7f
         b.view(torch.uint8)[N - 2, 5] = 0xff
