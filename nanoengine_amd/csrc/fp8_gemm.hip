@@ -558,7 +558,7 @@ fp8_gemm_kernel(const GemmParams P) {
 // Few rows: a workgroup takes 32 columns, its four or eight waves parts of K, each with two blocks of 128 of its own on
 // their way into LDS in whole lines while a third is multiplied; the waves' sums meet in LDS, in order. No meetings of
 // waves until then, no second launch: 1 x 8192 x 1536 in 4.0 us (by tiles 8.0), 32 x 576 x 1536 4.0 (7.5), 16 x 2112 x
-// 8192 7.7 (10.8), 8 x 8192 x 8192 13.4 (15.4; its bytes take 13.0). What bounds it is the start (under 2 us beside the
+// 8192 7.1 (10.8), 8 x 8192 x 8192 13.3 (15.4; its bytes take 13.0). What bounds it is the start (under 2 us beside the
 // launch) and then memory, or what few CUs can fetch: 0.3 us a block of K for each of four waves. (Straight into
 // registers a load touches 32 rows, and where these lie a power of two apart their lines crowd each other out of L1
 // before the next load wants them: 16 x 2112 x 8192 15.4, 1 x 8192 x 1536 4.6.)
@@ -627,15 +627,20 @@ __global__ void __launch_bounds__(WAVES * 64) fp8_gemm_few_kernel(const GemmPara
   auto issue = [&](int s) {
     const int kb = kb0 + s, buf = s & 1;
     const uint32_t dst = lds_addr(mine) + buf * kStage;
-    const bool whole = kb < full;
+    if (kb < full) {
 #pragma unroll
-    for (int i = 0; i < 4 * TILES; ++i) {
-      const uint64_t mask = whole ? ~0ull : i & 1 ? tail1 : tail0;
-      if (i < 4) dma16(tile_b + (int64_t)kb * kBlock, off_b[i], dst + i * 1024, mask);
-      dma16(P.a + (int64_t)kb * kBlock, off_a[i], dst + 4096 + i * 1024, mask);
-    }
-    if (!whole) {
+      for (int i = 0; i < 4 * TILES; ++i) {
+        if (i < 4) dma16(tile_b + (int64_t)kb * kBlock, off_b[i], dst + i * 1024);
+        dma16(P.a + (int64_t)kb * kBlock, off_a[i], dst + 4096 + i * 1024);
+      }
+    } else {
       const v4i zero = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 4 * TILES; ++i) {
+        const uint64_t mask = i & 1 ? tail1 : tail0;
+        if (i < 4) dma16(tile_b + (int64_t)kb * kBlock, off_b[i], dst + i * 1024, mask);
+        dma16(P.a + (int64_t)kb * kBlock, off_a[i], dst + 4096 + i * 1024, mask);
+      }
 #pragma unroll
       for (int i = 0; i < kCopies; ++i)
         if (16 * (i & 1 ? piece1 : piece0) >= P.k % kBlock)
