@@ -113,12 +113,8 @@ __device__ __forceinline__ void quantise(const float* y, int i, int n, uint8_t* 
   for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(y[j]));
 #pragma unroll
   for (int off = 1; off < 16; off <<= 1) amax = fmaxf(amax, shfl_xor(amax, off));
-  float inv;
-  const uint32_t s = block_scale<KIND>(amax, &inv);
-  uint2 c;
-  c.x = f32x4_to_fp8(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
-  c.y = f32x4_to_fp8(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv);
-  store_codes<VEC>(codes, i, n, c);
+  const uint32_t s = block_scale<KIND>(amax);
+  store_codes<VEC>(codes, i, n, block_codes<KIND>(y, s));
   if (i % kBlock == 0 && i < n) {
     if (KIND == kScaleF32) static_cast<uint32_t*>(scales)[i / kBlock] = s;
     else static_cast<uint8_t*>(scales)[i / kBlock] = (uint8_t)s;
