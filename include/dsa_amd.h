@@ -329,6 +329,16 @@ DSA_API int dsa_indexer_k_transform_store(const void* key, int64_t key_row_strid
                                           int slot_is_64, int num_tokens, uint8_t* cache,
                                           int page_size, void* stream);
 
+/* The same for keys of either layout: dims 0..63 are interleaved pairs when rope_interleaved, else
+ * already in the half layout. It has to be that of the queries (dsa_indexer_q_prologue): of different
+ * ones, each key dim meets another pair's query dim. */
+DSA_API int dsa_indexer_k_transform_store_layout(const void* key, int64_t key_row_stride,
+                                                 const float* ln_weight, const float* ln_bias, float eps,
+                                                 const float* cos_sin_cache, int64_t cache_positions,
+                                                 const void* positions, int pos_is_64, const void* slots,
+                                                 int slot_is_64, int num_tokens, int rope_interleaved,
+                                                 uint8_t* cache, int page_size, void* stream);
+
 /* Ragged fp8 MQA logits (prefill indexer).
  *   q        [num_rows, 64, 128] e4m3fn, contiguous, 16-byte aligned
  *   kv       [num_keys, 128] e4m3fn, contiguous, 16-byte aligned; kv_scale [num_keys] f32

@@ -61,6 +61,8 @@ SIGNATURES = {
     "dsa_prefill_windows": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P, _P, _P, _P]),
     "dsa_indexer_k_transform_store": (c_int, [_P, c_int64, _P, _P, c_float, _P, c_int64, _P, c_int, _P, c_int,
                                               c_int, _P, c_int, _P]),
+    "dsa_indexer_k_transform_store_layout": (c_int, [_P, c_int64, _P, _P, c_float, _P, c_int64, _P, c_int, _P, c_int,
+                                                     c_int, c_int, _P, c_int, _P]),
     "dsa_batch_tables": (c_int, [_P, _P, c_int, _P, c_int64, c_int, c_int, _P, c_int64, _P, _P, c_int, _P, c_int, _P,
                                  c_int64, _P, _P, c_int, _P, _P]),
     "dsa_mla_kv_store_fp4": (c_int, [_P, c_int64, _P, c_int, c_int, _P, c_int64, c_int, c_int64, _P]),

@@ -14,8 +14,8 @@
 //   4. per (token, head) row: sf = 2^ceil(log2(max(amax, 1e-4) / 448)),
 //      code = e4m3fn(x / sf); weights[t, h] = gate[t, h] * weight_scale * sf.
 // Key (dlengine/runtime/kernel/triton/generic/indexer_transform.py:156-288):
-//   LayerNorm(weight, bias, eps) rounded to bf16, steps 1-2 above, the
-//   Hadamard of step 3 kept in f32, then the quantisation of step 4 written to
+//   LayerNorm(weight, bias, eps) rounded to bf16, steps 1-2 above (of either
+//   layout, the query's), the Hadamard of step 3 kept in f32, then the quantisation of step 4 written to
 //   the split page layout [page_size x 128 fp8][page_size x f32 scale].
 //
 // Data layout: one row of 128 values per 16 lanes (8 consecutive values per
@@ -188,7 +188,8 @@ indexer_k_transform_store_kernel(const uint16_t* __restrict__ key, int64_t key_s
                                  const float* __restrict__ ln_w, const float* __restrict__ ln_b, float eps,
                                  const float* __restrict__ cos_sin, int64_t cache_positions,
                                  const void* __restrict__ positions, int pos_is_64, const void* __restrict__ slots,
-                                 int slot_is_64, int num_tokens, uint8_t* __restrict__ cache, int page_size) {
+                                 int slot_is_64, int num_tokens, int interleaved, uint8_t* __restrict__ cache,
+                                 int page_size) {
 #pragma clang fp contract(off)
   const int lane = threadIdx.x & 63;
   const int gl = threadIdx.x & 15;
@@ -223,8 +224,8 @@ indexer_k_transform_store_kernel(const uint16_t* __restrict__ key, int64_t key_s
     const float y1 = (c[2 * q + 1] * inv_std) * wv[2 * q + 1] + bv[2 * q + 1];
     w[q] = pack_bf16_rne(y0, y1);
   }
-  // the projection's rope dims are interleaved pairs (indexer_transform.py:183-186)
-  interleaved_to_half(w, lane, gl);
+  // the reference's projection gives interleaved pairs (indexer_transform.py:183-186)
+  if (interleaved) interleaved_to_half(w, lane, gl);
   unpack8(w, x);
   int64_t pos = load_index(positions, pos_is_64, tok);
   pos = pos < 0 ? 0 : (pos >= cache_positions ? cache_positions - 1 : pos);
@@ -268,10 +269,11 @@ int dsa_indexer_q_prologue(const void* q, const void* gate, int64_t gate_token_s
   return check_launch("dsa_indexer_q_prologue");
 }
 
-int dsa_indexer_k_transform_store(const void* key, int64_t key_row_stride, const float* ln_weight,
-                                  const float* ln_bias, float eps, const float* cos_sin_cache, int64_t cache_positions,
-                                  const void* positions, int pos_is_64, const void* slots, int slot_is_64,
-                                  int num_tokens, uint8_t* cache, int page_size, void* stream) {
+int dsa_indexer_k_transform_store_layout(const void* key, int64_t key_row_stride, const float* ln_weight,
+                                         const float* ln_bias, float eps, const float* cos_sin_cache,
+                                         int64_t cache_positions, const void* positions, int pos_is_64,
+                                         const void* slots, int slot_is_64, int num_tokens, int rope_interleaved,
+                                         uint8_t* cache, int page_size, void* stream) {
   using namespace dsa;
   if (num_tokens < 0 || page_size <= 0 || cache_positions <= 0 || key_row_stride < 128)
     return set_error(kInvalidArgument, "dsa_indexer_k_transform_store: bad sizes");
@@ -287,8 +289,17 @@ int dsa_indexer_k_transform_store(const void* key, int64_t key_row_stride, const
   hipLaunchKernelGGL(indexer_k_transform_store_kernel, dim3((num_tokens + kRowsPerBlock - 1) / kRowsPerBlock),
                      dim3(256), 0, (hipStream_t)stream, static_cast<const uint16_t*>(key), key_row_stride, ln_weight,
                      ln_bias, eps, cos_sin_cache, cache_positions, positions, pos_is_64, slots, slot_is_64,
-                     num_tokens, cache, page_size);
+                     num_tokens, rope_interleaved, cache, page_size);
   return check_launch("dsa_indexer_k_transform_store");
+}
+
+int dsa_indexer_k_transform_store(const void* key, int64_t key_row_stride, const float* ln_weight,
+                                  const float* ln_bias, float eps, const float* cos_sin_cache, int64_t cache_positions,
+                                  const void* positions, int pos_is_64, const void* slots, int slot_is_64,
+                                  int num_tokens, uint8_t* cache, int page_size, void* stream) {
+  return dsa_indexer_k_transform_store_layout(key, key_row_stride, ln_weight, ln_bias, eps, cos_sin_cache, cache_positions,
+                                              positions, pos_is_64, slots, slot_is_64, num_tokens, 1, cache, page_size,
+                                              stream);
 }
 
 }  // extern "C"

@@ -512,9 +512,10 @@ def indexer_q_prologue(query: torch.Tensor, gate_weight: torch.Tensor, weight_sc
 
 def indexer_k_transform_store(key: torch.Tensor, ln_weight: torch.Tensor, ln_bias: torch.Tensor, eps: float,
                               positions: torch.Tensor, cos_sin_cache: torch.Tensor, cache: torch.Tensor,
-                              slot_mapping: torch.Tensor, page_size: int) -> None:
+                              slot_mapping: torch.Tensor, page_size: int, rope_interleaved: bool = True) -> None:
     """LayerNorm -> RoPE -> Hadamard-128 -> UE8M0 fp8 quant -> split-page store of
-    indexer keys [T, 128] bf16 (see dsa_indexer_k_transform_store)."""
+    indexer keys [T, 128] bf16, whose rotated dims have the layout of the queries'
+    (see dsa_indexer_k_transform_store, dsa_indexer_k_transform_store_layout)."""
     if not (key.dim() == 2 and key.shape[1] == INDEXER_HEAD_DIM and key.dtype == torch.bfloat16
             and key.stride(1) == 1):
         _fail("fused Indexer K path requires a bfloat16 [T, 128] key", ValueError)
@@ -527,9 +528,9 @@ def indexer_k_transform_store(key: torch.Tensor, ln_weight: torch.Tensor, ln_bia
     pos, pos64 = _positions(positions, key.shape[0])
     slots, is64 = _slots(slot_mapping, key.shape[0])
     dev = _check_cuda(key, lw, lb, cs, pos, slots, cache)
-    _lib.call("dsa_indexer_k_transform_store", key.data_ptr(), key.stride(0), lw.data_ptr(), lb.data_ptr(),
+    _lib.call("dsa_indexer_k_transform_store_layout", key.data_ptr(), key.stride(0), lw.data_ptr(), lb.data_ptr(),
               float(eps), cs.data_ptr(), cs.shape[0], pos.data_ptr(), pos64, slots.data_ptr(), is64, key.shape[0],
-              cache.data_ptr(), int(page_size), _stream(dev))
+              int(bool(rope_interleaved)), cache.data_ptr(), int(page_size), _stream(dev))
 
 
 # --------------------------------------------------------------------------- prefill indexer

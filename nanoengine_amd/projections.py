@@ -59,13 +59,16 @@ class MlaProjections:
     norm [D]; a [q_rank + 512 + 64 + 128, D] (query latent, kv latent, rotated key, indexer key); q_norm [q_rank];
     kv_norm [512]; q [H * (nope + 64), q_rank]; k_up [H, nope, 512]; v_up [H, 512, v]; o [D, H * v];
     idx_q [64 * 128, q_rank]; idx_gate [64, D]; idx_norm, idx_bias [128]. ``cos_sin_cache``: ``rotary.cos_sin_cache``.
-    ``sm_scale`` of the attention is the step's own argument."""
+    ``interleaved`` says whether the pairs of the MLA's rotated dims (the tails of q's heads and the shared key) lie beside each
+    other or in halves, ``indexer_interleaved`` the same of the indexer's (the heads' first 64 dims and its key's): as the
+    MLA's unless given. ``sm_scale`` of the attention is the step's own argument."""
 
     def __init__(self, *, norm, a, q_norm, kv_norm, q, k_up, v_up, o, idx_q, idx_gate, idx_norm, idx_bias,
                  cos_sin_cache: torch.Tensor, eps: float = 1e-6, interleaved: bool = True,
-                 scale_dtype: torch.dtype = torch.float8_e8m0fnu):
+                 scale_dtype: torch.dtype = torch.float8_e8m0fnu, indexer_interleaved: bool | None = None):
         self.heads, self.nope = k_up.shape[0], k_up.shape[1]
         self.q_rank, self.eps, self.interleaved, self.scale_dtype = q_norm.shape[0], eps, interleaved, scale_dtype
+        self.indexer_interleaved = interleaved if indexer_interleaved is None else indexer_interleaved
         D = norm.shape[0]
         want = {"a": (a, (self.q_rank + KV_RANK + ROT + ops.INDEXER_HEAD_DIM, D)), "kv_norm": (kv_norm, (KV_RANK,)),
                 "q": (q, (self.heads * (self.nope + ROT), self.q_rank)), "k_up": (k_up, (self.heads, self.nope, KV_RANK)),
@@ -108,10 +111,11 @@ class MlaProjections:
                  k=c[:, at:at + ROT].unsqueeze(1), k_out=kv[:, KV_RANK:].unsqueeze(1), interleaved=self.interleaved)
         ops.mla_kv_store(kv, kv_cache, slot_mapping)
         ops.indexer_k_transform_store(c[:, at + ROT:], self.idx_norm, self.idx_bias, self.eps, positions,
-                                      self.cos_sin_cache, indexer_cache, slot_mapping, page_size)
+                                      self.cos_sin_cache, indexer_cache, slot_mapping, page_size,
+                                      self.indexer_interleaved)
         ops.indexer_q_prologue(self.idx_q(*c_q).view(T, IDX_HEADS, ops.INDEXER_HEAD_DIM), h @ self.idx_gate.t(),
                                IDX_HEADS ** -0.5 * ops.INDEXER_HEAD_DIM ** -0.5, self.cos_sin_cache, positions, q_idx,
-                               weights, self.interleaved)
+                               weights, self.indexer_interleaved)
         return q_idx, weights, q_mla, stream
 
     def output(self, o: torch.Tensor) -> torch.Tensor:

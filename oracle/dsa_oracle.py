@@ -620,10 +620,11 @@ def indexer_q_prologue(q_bf16: np.ndarray, gate_bf16: np.ndarray, weight_scale: 
 
 
 def indexer_k_transform(key_bf16: np.ndarray, ln_w: np.ndarray, ln_b: np.ndarray, eps: float,
-                        cos_sin: np.ndarray, positions: np.ndarray):
+                        cos_sin: np.ndarray, positions: np.ndarray, rope_interleaved: bool = True):
     """Indexer key transform (indexer_transform.py:156-260): LayerNorm (biased
-    variance, 1/sqrt(var + eps)) rounded to bf16, RoPE on the interleaved
-    leading 64 dims rounded to bf16, Hadamard kept in f32, UE8M0 quantisation.
+    variance, 1/sqrt(var + eps)) rounded to bf16, RoPE on the leading 64 dims
+    (interleaved pairs, or already in halves) rounded to bf16, Hadamard kept in
+    f32, UE8M0 quantisation.
 
     key_bf16 [T, 128] uint16. Returns (codes uint8 [T, 128], scales f32 [T])."""
     x = bf16_to_f32(key_bf16).astype(np.float32)
@@ -634,7 +635,8 @@ def indexer_k_transform(key_bf16: np.ndarray, ln_w: np.ndarray, ln_b: np.ndarray
     y = ((c * inv_std[:, None]).astype(np.float32) * np.asarray(ln_w, dtype=np.float32)).astype(np.float32)
     y = bf16_to_f32(f32_to_bf16(y + np.asarray(ln_b, dtype=np.float32)))
     cs = np.asarray(cos_sin, dtype=np.float32)[np.asarray(positions, dtype=np.int64)]
-    rot = rope_neox(interleaved_to_half(y[:, :64]), cs[:, :32], cs[:, 32:])
+    rope = interleaved_to_half(y[:, :64]) if rope_interleaved else y[:, :64]
+    rot = rope_neox(rope, cs[:, :32], cs[:, 32:])
     y = np.concatenate([bf16_to_f32(f32_to_bf16(rot)), y[:, 64:]], axis=-1)
     return _quant_ue8m0_f32(hadamard128(y))
 
