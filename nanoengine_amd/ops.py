@@ -788,6 +788,13 @@ def _launch(index: int, name: str, *args) -> None:
         _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
 
 
+def _whole(workspace: torch.Tensor, need: int, index: int) -> bool:
+    """Whether the workspace holds ``need`` bytes in one piece, 16-byte aligned, on GPU ``index``. (Expanded, it has fewer bytes
+    than elements; strided, the bytes between them are someone else's.)"""
+    return (workspace.numel() * workspace.element_size() >= need and workspace.is_contiguous()
+            and workspace.data_ptr() % 16 == 0 and workspace.get_device() == index)
+
+
 def mla_fp4_geometry(k_cache: torch.Tensor) -> tuple[int, int]:
     """(block stride in bytes, rows per block) of a 4-bit MLA cache view
     [num_blocks, block_size, (1,) 400] whose block stride may include a padding row."""
@@ -1195,8 +1202,7 @@ def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     need = _gemm_workspace(dev, M, N, K, scale_dtype)
     ws_ptr, ws_bytes = None, 0
     if need:
-        if (workspace is None or workspace.numel() * workspace.element_size() < need or workspace.data_ptr() % 16
-                or workspace.get_device() != dev):
+        if workspace is None or not _whole(workspace, need, dev):
             workspace = a.new_empty((need,), dtype=torch.uint8)
         ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     _launch(dev, "dsa_fp8_gemm", a.data_ptr(), a_stride, a_scale.data_ptr(), sa_stride, b.data_ptr(), b_stride,
