@@ -179,6 +179,7 @@ def indexer_topk(q_fp8: torch.Tensor, kv_cache: torch.Tensor, weights: torch.Ten
         workspace = torch.zeros(need, dtype=torch.uint8, device=dev)
     if not (workspace.dtype == torch.uint8 and workspace.numel() >= need):
         _fail(f"workspace needs {need} bytes")
+    _ws_args(workspace, dev)
     _lib.call("dsa_indexer_topk", q_fp8.data_ptr(), kv_cache.data_ptr(),
               weights.data_ptr(), cl.data_ptr(), bt.data_ptr(), bt.stride(0), B, n, H, D, page_size,
               int(max_context_len), int(top_k), out_physical.data_ptr(),
@@ -228,11 +229,16 @@ def topk_workspace(batch: int, device: torch.device) -> torch.Tensor:
     return ws
 
 
-def _ws_args(ws):
+def _ws_args(ws, dev: torch.device):
     """(pointer, bytes) for a workspace tensor; False for none. Aligned rows of up
     to 64K scores need none; longer or unaligned rows without one take the full
-    multi-pass exact select."""
-    return (None, 0) if ws is None or ws is False else (ws.data_ptr(), ws.numel())
+    multi-pass exact select. One with holes (expanded, strided) has fewer bytes of
+    its own than elements, and is refused."""
+    if ws is None or ws is False:
+        return None, 0
+    if not (ws.is_contiguous() and ws.device == dev):
+        _fail(f"workspace must be contiguous on {dev}, got strides {ws.stride()} on {ws.device}")
+    return ws.data_ptr(), ws.numel()
 
 
 def topk_transform(scores: torch.Tensor, seq_lens: torch.Tensor, page_tables: torch.Tensor,
@@ -260,7 +266,7 @@ def topk_transform(scores: torch.Tensor, seq_lens: torch.Tensor, page_tables: to
         workspace = topk_workspace(B, dev)
     _lib.call("dsa_topk_transform", scores.data_ptr(), scores.stride(0), seq_lens.data_ptr(),
               page_tables.data_ptr(), page_tables.stride(0), out_page_indices.data_ptr(),
-              _ptr(out_raw_indices), B, scores.shape[1], int(page_size), int(top_k), *_ws_args(workspace),
+              _ptr(out_raw_indices), B, scores.shape[1], int(page_size), int(top_k), *_ws_args(workspace, dev),
               _stream(dev))
 
 
@@ -281,7 +287,7 @@ def topk_transform_raw(scores: torch.Tensor, seq_lens: torch.Tensor, out_indices
     if workspace is None:
         workspace = topk_workspace(B, dev)
     _lib.call("dsa_topk_transform", scores.data_ptr(), scores.stride(0), seq_lens.data_ptr(), None, 0,
-              out_indices.data_ptr(), None, B, scores.shape[1], 1, int(top_k), *_ws_args(workspace),
+              out_indices.data_ptr(), None, B, scores.shape[1], 1, int(top_k), *_ws_args(workspace, dev),
               _stream(dev))
 
 
@@ -305,7 +311,7 @@ def indexer_select(logits: torch.Tensor, context_lens: torch.Tensor, out_indices
     if workspace is None:
         workspace = topk_workspace(R, dev)
     _lib.call("dsa_indexer_select", logits.data_ptr(), logits.stride(0), context_lens.data_ptr(),
-              out_indices.data_ptr(), R, logits.shape[1], int(top_k), *_ws_args(workspace), _stream(dev))
+              out_indices.data_ptr(), R, logits.shape[1], int(top_k), *_ws_args(workspace, dev), _stream(dev))
 
 
 def topk_transform_ragged(scores: torch.Tensor, seq_lens: torch.Tensor, row_starts: torch.Tensor,
@@ -327,7 +333,7 @@ def topk_transform_ragged(scores: torch.Tensor, seq_lens: torch.Tensor, row_star
         workspace = topk_workspace(B, dev)
     _lib.call("dsa_topk_transform_ragged", scores.data_ptr(), scores.stride(0), seq_lens.data_ptr(),
               row_starts.data_ptr(), offsets.data_ptr(), out_indices.data_ptr(), B, scores.shape[1],
-              int(top_k), *_ws_args(workspace), _stream(dev))
+              int(top_k), *_ws_args(workspace, dev), _stream(dev))
 
 
 def topk_to_physical(topk_indices: torch.Tensor, block_table: torch.Tensor, block_size: int,
@@ -408,7 +414,8 @@ def sparse_mla_decode(q: torch.Tensor, k_cache: torch.Tensor, indices: torch.Ten
     if num_splits is None:
         num_splits = sparse_mla_num_splits(T, H, topk, dev)
     need = sparse_mla_workspace_bytes(T, H, num_splits)
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need
+                 or not workspace.is_contiguous() or workspace.device != dev):
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     ws_ptr = workspace.data_ptr() if (need and workspace is not None) else None
     ws_bytes = workspace.numel() * workspace.element_size() if (need and workspace is not None) else 0
@@ -597,7 +604,7 @@ def mqa_topk(q_fp8: torch.Tensor, kv_fp8: torch.Tensor, kv_scale: torch.Tensor, 
         workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
     _lib.call("dsa_mqa_topk", q_fp8.data_ptr(), kv2.data_ptr(), sc.data_ptr(),
               weights.data_ptr(), weights.stride(0), ks.data_ptr(), ke.data_ptr(), m, n, INDEXER_HEADS,
-              int(max_len), int(top_k), out.data_ptr(), *_ws_args(workspace), _stream(dev))
+              int(max_len), int(top_k), out.data_ptr(), *_ws_args(workspace, dev), _stream(dev))
 
 
 def mla_prefill_kv(k_cache: torch.Tensor, block_table: torch.Tensor, cu_seqlens_q: torch.Tensor,
@@ -753,8 +760,8 @@ def sparse_mla_prefill_paged(q: torch.Tensor, k_cache: torch.Tensor, block_table
               block_table.shape[1], cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
               int(cu_seqlens_q.dtype == torch.int64), num_seqs,
               int(total_k), f2.data_ptr(), f2.stride(0), f2.shape[0], indices.data_ptr(), indices.stride(0), T, H,
-              topk, float(sm_scale), out.data_ptr(), max_logits.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
-              workspace.numel(), _stream(dev))
+              topk, float(sm_scale), out.data_ptr(), max_logits.data_ptr(), lse.data_ptr(), *_ws_args(workspace, dev),
+              _stream(dev))
     return out, max_logits, lse
 
 
@@ -887,8 +894,7 @@ def sparse_mla_decode_fp4(q: torch.Tensor, k_cache: torch.Tensor, indices: torch
             with torch.cuda.device(dev):
                 need = sparse_mla_workspace_bytes(T, H, num_splits)
     if need:
-        if (workspace is None or workspace.numel() * workspace.element_size() < need
-                or workspace.data_ptr() % 16 or workspace.get_device() != dev):
+        if workspace is None or not _whole(workspace, need, dev):
             workspace = k_cache.new_empty((need,))
         ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     _launch(dev, "dsa_sparse_mla_decode_fp4", q.data_ptr(), stride[0] if T > 1 else 0, stride[1],
