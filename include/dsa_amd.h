@@ -640,7 +640,8 @@ DSA_API int dsa_batch_tables(const int32_t* cached_lens, const int32_t* new_lens
  *                same f32 y
  *   scales       [rows, ceil(dim / 128)] of scale_kind, row stride scale_stride elements
  *                (NULL exactly when codes is)
- * One of out and codes at least. 1 <= dim <= 32768; rows that are 16-byte aligned (codes
+ * One of out and codes at least. 1 <= dim <= 32768. A launch holds fewer than 2^32 threads, of which a
+ * row takes 64 (dim <= 512), 256 (<= 2048), 512 (<= 4096) or 1024. Rows that are 16-byte aligned (codes
  * 8-byte) and a dim that is a multiple of 8 take wide loads, others narrow ones. Apart from
  * the pairs named, outputs must not overlap inputs. */
 DSA_API int dsa_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
@@ -650,7 +651,7 @@ DSA_API int dsa_rms_norm(const void* x, int64_t x_stride, const void* residual, 
                          int scale_kind, void* stream);
 
 /* The fp8 rounding alone: x [rows, dim] bf16 to codes and scales as in dsa_rms_norm
- * (any dim), such as the attention's output before the output projection. */
+ * (any dim; fewer than 2^28 blocks), such as the attention's output before the output projection. */
 DSA_API int dsa_act_quant(const void* x, int64_t x_stride, int64_t rows, int dim, uint8_t* codes,
                           int64_t code_stride, void* scales, int64_t scale_stride, int scale_kind,
                           void* stream);
@@ -665,7 +666,7 @@ DSA_API size_t dsa_fp8_gemm_workspace_bytes(int m, int n, int k, int scale_kind)
  *   out      [m, n] bf16, or f32 when out_is_f32, row stride out_stride elements
  * Scales are of scale_kind, their strides in elements; float32 ones may be any numbers, byte
  * 255 of an e8m0 one is NaN. k a multiple of 16; a and b rows 16-byte aligned and at most 2^23
- * bytes apart.
+ * bytes apart. Where m <= 32, n stays below 2^28: a launch holds fewer than 2^32 threads.
  * Products of 64 neighbouring k are summed by the matrix instruction, which drops what lies
  * more than 13 bits below the largest of them; those sums are added in f32. Two f32 scales are
  * multiplied in f32 before a block's sum is multiplied by them. A NaN code or scale gives NaN in
@@ -689,7 +690,8 @@ DSA_API int dsa_fp8_gemm(const uint8_t* a, int64_t a_stride, const void* a_scale
  * f32, rounded once. rot_dim even, at most 512; a multiple of 8 with 16-byte aligned rows
  * takes wide loads. An output is its input, with the same strides, or does not overlap it; its
  * rows lie apart, all heads of a token within its stride or all tokens of a head within its
- * (inputs may repeat rows). Fewer than 2^31 heads of all tokens.
+ * (inputs may repeat rows). Fewer than 2^31 heads of all tokens, and of 2^32 threads: rot_dim / 8 of them,
+ * rounded up to a power of two, for every four heads of a token (of q, and of k).
  * Beside dsa_indexer_q_prologue, whose rotation is fused for the indexer's own heads. */
 DSA_API int dsa_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads, void* q_out,
                      int64_t q_out_token_stride, int64_t q_out_head_stride, const void* k,

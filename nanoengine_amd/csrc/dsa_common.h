@@ -25,6 +25,9 @@ enum Status : int {
 int set_error(int code, const char* fmt, ...);
 int check_launch(const char* what);
 
+// A launch holds fewer than 2^32 threads.
+inline bool launch_holds(int64_t groups, int threads) { return groups * threads < (int64_t)1 << 32; }
+
 // Monotone uint32 key of a float: larger float -> larger key. NaN ranks as -inf.
 __device__ __forceinline__ uint32_t order_key(float x) {
   uint32_t u = __float_as_uint(x);

@@ -851,9 +851,11 @@ int launch_tile(GemmParams P, int dev, hipStream_t st) {
   if (rc != kOk) return rc;
   P.mtiles = (P.m - 1) / BM + 1;
   P.ntiles = (P.n - 1) / BN + 1;
+  constexpr int kThreads = (BM / WM) * (BN / WN) * 64;
   const int64_t groups = (int64_t)P.mtiles * P.ntiles * P.splits;
-  if (groups > INT32_MAX) return set_error(kUnsupported, "dsa_fp8_gemm: more than 2^31 tiles");
-  hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3((BM / WM) * (BN / WN) * 64), kSmem, st, P);
+  if (!launch_holds(groups, kThreads))
+    return set_error(kUnsupported, "dsa_fp8_gemm: %lld tiles take 2^32 threads or more", (long long)groups);
+  hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(kThreads), kSmem, st, P);
   return check_launch("dsa_fp8_gemm");
 }
 
@@ -861,11 +863,14 @@ template <int WAVES, int TILES, int KIND, int OUT>
 int launch_few(const GemmParams& P, int dev, hipStream_t st) {
   constexpr int kSmem = WAVES * kFewWave<TILES>;
   static_assert(kSmem <= 160 * 1024 && WAVES >= 4, "LDS of a CU, and 256 threads to join");
+  const int64_t groups = (P.n - 1) / kFew + 1;
+  if (!launch_holds(groups, WAVES * 64))
+    return set_error(kUnsupported, "dsa_fp8_gemm: %d columns of few rows take 2^32 threads or more", P.n);
   auto kern = fp8_gemm_few_kernel<WAVES, TILES, KIND, OUT>;
   static std::atomic<uint64_t> known{0};
   const int rc = allow_smem(reinterpret_cast<const void*>(kern), kSmem, dev, known);
   if (rc != kOk) return rc;
-  hipLaunchKernelGGL(kern, dim3((P.n - 1) / kFew + 1), dim3(WAVES * 64), kSmem, st, P);
+  hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(WAVES * 64), kSmem, st, P);
   return check_launch("dsa_fp8_gemm");
 }
 

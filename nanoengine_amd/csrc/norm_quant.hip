@@ -204,24 +204,28 @@ act_quant_kernel(const uint16_t* __restrict__ x, int64_t x_stride, int64_t block
 }
 
 template <int THREADS, int CHUNKS, int KIND>
-void launch_norm(const NormParams& P, bool vec, bool wf32, hipStream_t st) {
+int launch_norm(const NormParams& P, bool vec, bool wf32, hipStream_t st) {
   constexpr int kRows = THREADS < 256 ? 256 / THREADS : 1;
-  const dim3 grid((unsigned)((P.rows + kRows - 1) / kRows)), block(THREADS < 256 ? 256 : THREADS);
+  const int64_t groups = (P.rows + kRows - 1) / kRows;
+  if (!launch_holds(groups, kRows * THREADS))
+    return set_error(kUnsupported, "dsa_rms_norm: %lld rows of %d take 2^32 threads or more", (long long)P.rows, P.dim);
+  const dim3 grid((unsigned)groups), block(kRows * THREADS);
   if (vec && wf32) hipLaunchKernelGGL((rms_norm_kernel<THREADS, CHUNKS, KIND, true, true>), grid, block, 0, st, P);
   else if (vec) hipLaunchKernelGGL((rms_norm_kernel<THREADS, CHUNKS, KIND, true, false>), grid, block, 0, st, P);
   else if (wf32) hipLaunchKernelGGL((rms_norm_kernel<THREADS, CHUNKS, KIND, false, true>), grid, block, 0, st, P);
   else hipLaunchKernelGGL((rms_norm_kernel<THREADS, CHUNKS, KIND, false, false>), grid, block, 0, st, P);
+  return check_launch("dsa_rms_norm");
 }
 
 template <int KIND>
-void norm_by_dim(const NormParams& P, bool vec, bool wf32, hipStream_t st) {
+int norm_by_dim(const NormParams& P, bool vec, bool wf32, hipStream_t st) {
   const int lanes = (P.dim + kLane - 1) / kLane;
-  if (lanes <= 64) launch_norm<64, 1, KIND>(P, vec, wf32, st);
-  else if (lanes <= 256) launch_norm<256, 1, KIND>(P, vec, wf32, st);
-  else if (lanes <= 512) launch_norm<512, 1, KIND>(P, vec, wf32, st);
-  else if (lanes <= 1024) launch_norm<1024, 1, KIND>(P, vec, wf32, st);
-  else if (lanes <= 2048) launch_norm<1024, 2, KIND>(P, vec, wf32, st);
-  else launch_norm<1024, 4, KIND>(P, vec, wf32, st);
+  if (lanes <= 64) return launch_norm<64, 1, KIND>(P, vec, wf32, st);
+  if (lanes <= 256) return launch_norm<256, 1, KIND>(P, vec, wf32, st);
+  if (lanes <= 512) return launch_norm<512, 1, KIND>(P, vec, wf32, st);
+  if (lanes <= 1024) return launch_norm<1024, 1, KIND>(P, vec, wf32, st);
+  if (lanes <= 2048) return launch_norm<1024, 2, KIND>(P, vec, wf32, st);
+  return launch_norm<1024, 4, KIND>(P, vec, wf32, st);
 }
 
 bool aligned(const void* p, int64_t stride, int elements) {  // 2-byte or 1-byte elements, `elements` to a load
@@ -262,9 +266,8 @@ int dsa_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t 
   const bool vec = dim % kLane == 0 && aligned(x, x_stride, 8) && aligned(residual, residual_stride, 8) &&
                    aligned(residual_out, residual_out_stride, 8) && aligned(out, out_stride, 8) &&
                    aligned(weight, 0, 8) && aligned(codes, code_stride, 4);
-  if (scale_kind == kScaleF32) norm_by_dim<kScaleF32>(P, vec, weight_is_f32, (hipStream_t)stream);
-  else norm_by_dim<kScaleE8M0>(P, vec, weight_is_f32, (hipStream_t)stream);
-  return check_launch("dsa_rms_norm");
+  return scale_kind == kScaleF32 ? norm_by_dim<kScaleF32>(P, vec, weight_is_f32, (hipStream_t)stream)
+                                 : norm_by_dim<kScaleE8M0>(P, vec, weight_is_f32, (hipStream_t)stream);
 }
 
 int dsa_act_quant(const void* x, int64_t x_stride, int64_t rows, int dim, uint8_t* codes, int64_t code_stride,
@@ -282,7 +285,8 @@ int dsa_act_quant(const void* x, int64_t x_stride, int64_t rows, int dim, uint8_
     return set_error(kInvalidArgument, "dsa_act_quant: pointers must be aligned to their elements");
   const int64_t blocks = rows * per_row;
   const int64_t groups = (blocks + kQuantThreads / 16 - 1) / (kQuantThreads / 16);
-  if (groups > INT32_MAX) return set_error(kUnsupported, "dsa_act_quant: more than 2^31 groups of blocks");
+  if (!launch_holds(groups, kQuantThreads))
+    return set_error(kUnsupported, "dsa_act_quant: %lld blocks of 128 take 2^32 threads or more", (long long)blocks);
   const bool vec = dim % kLane == 0 && aligned(x, x_stride, 8) && aligned(codes, code_stride, 4);
   const dim3 grid((unsigned)groups), block(kQuantThreads);
   const hipStream_t st = (hipStream_t)stream;

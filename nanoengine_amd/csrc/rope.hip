@@ -173,17 +173,21 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams P) 
 }
 
 template <int HEADS>
-void launch_rope(RopeParams P, bool pairs, bool out_pairs, bool vec, hipStream_t st) {
+int launch_rope(RopeParams P, bool pairs, bool out_pairs, bool vec, hipStream_t st) {
   P.q_groups = (P.heads[0] + HEADS - 1) / HEADS;
   P.groups = P.q_groups + (P.heads[1] + HEADS - 1) / HEADS;
-  const int64_t threads = P.tokens * P.groups * P.lanes;
-  const dim3 grid((unsigned)((threads + kRopeThreads - 1) / kRopeThreads)), block(kRopeThreads);
+  const int64_t groups = (P.tokens * P.groups * P.lanes + kRopeThreads - 1) / kRopeThreads;
+  if (!launch_holds(groups, kRopeThreads))
+    return set_error(kUnsupported, "dsa_rope: %lld tokens of %d heads take 2^32 threads or more", (long long)P.tokens,
+                     P.heads[0] + P.heads[1]);
+  const dim3 grid((unsigned)groups), block(kRopeThreads);
 #define DSA_ROPE(A, B, V) hipLaunchKernelGGL((rope_kernel<A, B, V, HEADS>), grid, block, 0, st, P)
   if (pairs && out_pairs) { if (vec) DSA_ROPE(true, true, true); else DSA_ROPE(true, true, false); }
   else if (pairs) { if (vec) DSA_ROPE(true, false, true); else DSA_ROPE(true, false, false); }
   else if (out_pairs) { if (vec) DSA_ROPE(false, true, true); else DSA_ROPE(false, true, false); }
   else { if (vec) DSA_ROPE(false, false, true); else DSA_ROPE(false, false, false); }
 #undef DSA_ROPE
+  return check_launch("dsa_rope");
 }
 
 // Rows of rot elements that do not share any: heads within a token's step or tokens within a head's.
@@ -239,7 +243,6 @@ extern "C" int dsa_rope(const void* q, int64_t q_token_stride, int64_t q_head_st
   if (num_tokens * (q_heads + k_heads) >= INT32_MAX - kRopeThreads)
     return set_error(kUnsupported, "dsa_rope: 2^31 heads of all tokens or more");
   const bool many = num_tokens * (q_heads + k_heads) * lanes >= kManyLanes;
-  if (many) launch_rope<kManyHeads>(P, interleaved, out_interleaved, vec, (hipStream_t)stream);
-  else launch_rope<1>(P, interleaved, out_interleaved, vec, (hipStream_t)stream);
-  return check_launch("dsa_rope");
+  return many ? launch_rope<kManyHeads>(P, interleaved, out_interleaved, vec, (hipStream_t)stream)
+              : launch_rope<1>(P, interleaved, out_interleaved, vec, (hipStream_t)stream);
 }
