@@ -27,12 +27,12 @@ IDX_HEADS = 64
 
 def quantize_weight(weight: torch.Tensor, scale_dtype: torch.dtype = torch.float8_e8m0fnu):
     """[N, K] -> (codes [N, K] float8_e4m3fn, scales [ceil(N / 128), ceil(K / 128)]): a scale per 128 x 128 block, by
-    the rule of ``ops.act_quant`` (max(amax, 2^-40) / 448, or the power of two above)."""
+    the rule of ``ops.act_quant`` (max(amax, 2^-40) / 448, or the power of two above; a NaN counts for no scale)."""
     if scale_dtype not in (torch.float32, torch.float8_e8m0fnu):
         raise ValueError(f"scale_dtype must be float32 or float8_e8m0fnu, got {scale_dtype}")
     (N, K), B = weight.shape, ops.FP8_BLOCK
     full = torch.nn.functional.pad(weight.float(), (0, -K % B, 0, -N % B)).view(-(-N // B), B, -(-K // B), B)
-    scale = full.abs().amax(dim=(1, 3)).clamp_min(2.0 ** -40) / 448.0
+    scale = full.abs().masked_fill(full.isnan(), 0.0).amax(dim=(1, 3)).clamp_min(2.0 ** -40) / 448.0
     if scale_dtype is torch.float8_e8m0fnu:
         bits = scale.view(torch.int32)  # positive: the exponent, one more where a fraction is left
         byte = ((bits >> 23) + ((bits & 0x7FFFFF) != 0).to(torch.int32)).clamp_max(254)
