@@ -47,6 +47,8 @@ class Fp8Linear:
     """x @ weight.T with the weight in fp8 by blocks of 128 x 128."""
 
     def __init__(self, weight: torch.Tensor, scale_dtype: torch.dtype = torch.float8_e8m0fnu):
+        if weight.shape[1] % 16:
+            raise ValueError(f"fp8 products take a depth that is a multiple of 16, got {list(weight.shape)}")
         self.codes, self.scales = quantize_weight(weight, scale_dtype)
 
     def __call__(self, codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -58,7 +60,8 @@ class MlaProjections:
 
     norm [D]; a [q_rank + 512 + 64 + 128, D] (query latent, kv latent, rotated key, indexer key); q_norm [q_rank];
     kv_norm [512]; q [H * (nope + 64), q_rank]; k_up [H, nope, 512]; v_up [H, 512, v]; o [D, H * v];
-    idx_q [64 * 128, q_rank]; idx_gate [64, D]; idx_norm, idx_bias [128]. ``cos_sin_cache``: ``rotary.cos_sin_cache``.
+    idx_q [64 * 128, q_rank]; idx_gate [64, D]; idx_norm, idx_bias [128]. D, q_rank and H * v are multiples of 16.
+    ``cos_sin_cache``: ``rotary.cos_sin_cache``.
     ``interleaved`` says whether the pairs of the MLA's rotated dims (the tails of q's heads and the shared key) lie beside each
     other or in halves, ``indexer_interleaved`` the same of the indexer's (the heads' first 64 dims and its key's): as the
     MLA's unless given. ``sm_scale`` of the attention is the step's own argument."""
@@ -83,14 +86,20 @@ class MlaProjections:
         self.k_up, self.v_up = k_up.to(bf16).contiguous(), v_up.to(bf16).contiguous()
         self.idx_gate = idx_gate.to(bf16).contiguous()
         self.idx_norm, self.idx_bias = idx_norm.float().contiguous(), idx_bias.float().contiguous()
-        self.cos_sin_cache = cos_sin_cache
+        self.cos_sin_cache = ops._rope_cache(cos_sin_cache)
 
     def inputs(self, hidden: torch.Tensor, residual: torch.Tensor | None, positions: torch.Tensor,
                slot_mapping: torch.Tensor, kv_cache: torch.Tensor, indexer_cache: torch.Tensor, page_size: int = 64):
         """hidden [T, D] bf16 of one layer's tokens. Writes their rows of both caches at ``slot_mapping`` (-1: none) and
         returns (q_idx [T, 64, 128] fp8, weights [T, 64] f32, q_mla [T, H, 576] bf16, residual): the step's arguments
-        and the residual stream, which is ``residual`` itself, updated, or ``hidden`` where there is none yet."""
+        and the residual stream, which is ``residual`` itself, updated, or ``hidden`` where there is none yet. Arguments
+        that do not fit are refused before it is updated."""
         T, rank, H = hidden.shape[0], self.q_rank, self.heads
+        ops._positions(positions, T)
+        ops._slots(slot_mapping, T)
+        ops.mla_kv_geometry(kv_cache)
+        ops._key_pages(indexer_cache, page_size, ops.INDEXER_ROW_BYTES)
+        ops._gpu(hidden, positions, slot_mapping, kv_cache, indexer_cache)
         q_idx = torch.empty(T, IDX_HEADS, ops.INDEXER_HEAD_DIM, dtype=torch.float8_e4m3fn, device=hidden.device)
         weights = torch.empty(T, IDX_HEADS, dtype=torch.float32, device=hidden.device)
         q_mla = torch.empty(T, H, ops.MLA_D_QK, dtype=torch.bfloat16, device=hidden.device)
