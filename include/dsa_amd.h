@@ -659,6 +659,11 @@ DSA_API int dsa_act_quant(const void* x, int64_t x_stride, int64_t rows, int dim
 /* Workspace bytes dsa_fp8_gemm needs for this shape on the current device (0: none). */
 DSA_API size_t dsa_fp8_gemm_workspace_bytes(int m, int n, int k, int scale_kind);
 
+/* How dsa_fp8_gemm works on this shape on a device of `cus` compute units (0: the current one): out[0..4] = the
+ * rows and columns of a workgroup's results, its waves, the blocks of K that lie in LDS at a time, and the
+ * parts of K that are summed by a second launch (1: none). 32 columns: the form for few rows, a part of K a wave. */
+DSA_API int dsa_fp8_gemm_plan(int m, int n, int k, int scale_kind, int cus, int* out);
+
 /* Product of block-scaled fp8 matrices:
  *   out[i, j] = sum_kb a_scale[i, kb] b_scale[j / 128, kb] sum_{t in block kb} a[i, t] b[j, t]
  *   a        [m, k] e4m3fn, row stride a_stride bytes;  a_scale [m, ceil(k / 128)]

@@ -77,6 +77,7 @@ SIGNATURES = {
                              _P, c_int64, _P, c_int64, c_int, _P]),
     "dsa_act_quant": (c_int, [_P, c_int64, c_int64, c_int, _P, c_int64, _P, c_int64, c_int, _P]),
     "dsa_fp8_gemm_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "dsa_fp8_gemm_plan": (c_int, [c_int, c_int, c_int, c_int, c_int, _P]),
     "dsa_fp8_gemm": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int, c_int, c_int, c_int, _P,
                              c_int64, c_int, _P, c_size_t, _P]),
     "dsa_rope": (c_int, [_P, c_int64, c_int64, c_int, _P, c_int64, c_int64, _P, c_int64, c_int64, c_int, _P, c_int64,

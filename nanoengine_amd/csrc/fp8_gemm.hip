@@ -754,18 +754,23 @@ fp8_gemm_sum_kernel(const float* __restrict__ part, int splits, int m, int n, vo
 // by 128 x 128 143). The widest tile has four waves of 128 x 128, or eight of 128 x 64: these read more from LDS (8192^3 387
 // and 394 us) but begin and end a tile sooner (8192 x 24576 x 1536 318 and 298). f32 scales leave room for the latter only.
 struct Tile {
-  int bm, bn, stages, resident;
+  int bm, bn, wm, wn, stages, resident;
   float base, per_step, per_round_step, per_tile, per_round;
 };
 constexpr Tile kTilesE8M0[] = {
-    {32, 64, 3, 4, 3.0f, 0.05f, 0.20f, 1.25f, 0.f},   {64, 64, 3, 3, 2.85f, 0.11f, 0.12f, 1.1f, 1.1f},
-    {64, 128, 3, 2, 3.0f, 0.20f, 0.10f, 1.4f, 1.4f},  {128, 128, 2, 2, 1.9f, 0.21f, 0.36f, 2.1f, 1.7f},
-    {128, 128, 3, 1, 1.7f, 0.42f, 0.f, 4.8f, 0.f},    {256, 128, 2, 1, 0.8f, 0.86f, 0.f, 6.0f, 0.f},
-    {256, 256, 2, 1, 0.f, 1.25f, 0.f, 10.1f, 0.f},    {256, 256, 2, 1, 0.f, 1.19f, 0.f, 12.2f, 0.f}};
+    {32, 64, 32, 32, 3, 4, 3.0f, 0.05f, 0.20f, 1.25f, 0.f},   {64, 64, 32, 32, 3, 3, 2.85f, 0.11f, 0.12f, 1.1f, 1.1f},
+    {64, 128, 32, 64, 3, 2, 3.0f, 0.20f, 0.10f, 1.4f, 1.4f},  {128, 128, 64, 64, 2, 2, 1.9f, 0.21f, 0.36f, 2.1f, 1.7f},
+    {128, 128, 64, 64, 3, 1, 1.7f, 0.42f, 0.f, 4.8f, 0.f},    {256, 128, 64, 64, 2, 1, 0.8f, 0.86f, 0.f, 6.0f, 0.f},
+    {256, 256, 128, 64, 2, 1, 0.f, 1.25f, 0.f, 10.1f, 0.f},   {256, 256, 128, 128, 2, 1, 0.f, 1.19f, 0.f, 12.2f, 0.f}};
 constexpr Tile kTilesF32[] = {
-    {32, 64, 3, 3, 2.3f, 0.04f, 0.28f, 1.2f, 0.f},    {64, 64, 3, 2, 2.6f, 0.08f, 0.235f, 1.35f, 0.f},
-    {64, 128, 2, 2, 2.1f, 0.085f, 0.41f, 1.7f, 0.f},  {64, 128, 3, 1, 2.2f, 0.38f, 0.f, 0.f, 2.4f},
-    {256, 128, 2, 1, 0.55f, 1.05f, 0.f, 5.9f, 0.f},   {256, 256, 2, 1, 0.f, 1.6f, 0.f, 9.0f, 0.f}};
+    {32, 64, 32, 32, 3, 3, 2.3f, 0.04f, 0.28f, 1.2f, 0.f},    {64, 64, 32, 32, 3, 2, 2.6f, 0.08f, 0.235f, 1.35f, 0.f},
+    {64, 128, 32, 64, 2, 2, 2.1f, 0.085f, 0.41f, 1.7f, 0.f},  {64, 128, 32, 64, 3, 1, 2.2f, 0.38f, 0.f, 0.f, 2.4f},
+    {256, 128, 64, 64, 2, 1, 0.55f, 1.05f, 0.f, 5.9f, 0.f},   {256, 256, 128, 64, 2, 1, 0.f, 1.6f, 0.f, 9.0f, 0.f}};
+template <int KIND>
+constexpr int kTileCount = KIND == kScaleF32 ? sizeof(kTilesF32) / sizeof(Tile) : sizeof(kTilesE8M0) / sizeof(Tile);
+template <int KIND, int I>
+constexpr Tile kTile = KIND == kScaleF32 ? kTilesF32[I] : kTilesE8M0[I];
+constexpr const Tile* tiles_of(int kind) { return kind == kScaleF32 ? kTilesF32 : kTilesE8M0; }
 // A second launch adds up the parts of K: so much, and more by their MB.
 constexpr float kSumBase = 2.9f, kSumPerMB[2] = {0.33f, 0.25f};
 
@@ -786,8 +791,8 @@ Plan plan_of(int m, int n, int k, int kind, int cus) {
   if (m <= kFew && kblocks <= 8 * kFewBlocks) return {kFewTile, kblocks > 4 * kFewBlocks ? 8 : 4};
   if (m > kFew && m <= 2 * kFew && groups <= cus && kblocks <= 4 * kFewBlocks && (kblocks <= 32 || groups > cus / 2))
     return {kFewTile, 4};
-  const Tile* tiles = kind == kScaleF32 ? kTilesF32 : kTilesE8M0;
-  const int count = kind == kScaleF32 ? (int)(sizeof(kTilesF32) / sizeof(Tile)) : (int)(sizeof(kTilesE8M0) / sizeof(Tile));
+  const Tile* tiles = tiles_of(kind);
+  const int count = kind == kScaleF32 ? kTileCount<kScaleF32> : kTileCount<kScaleE8M0>;
   Plan best = {0, 1};
   double least = 1e300;
   for (int t = 0; t < count; ++t) {
@@ -841,8 +846,10 @@ int allow_smem(const void* kern, int bytes, int dev, std::atomic<uint64_t>& know
   return kOk;
 }
 
-template <int BM, int BN, int WM, int WN, int STAGES, int KIND, int OUT>
+template <int KIND, int I, int OUT>
 int launch_tile(GemmParams P, int dev, hipStream_t st) {
+  constexpr Tile T = kTile<KIND, I>;
+  constexpr int BM = T.bm, BN = T.bn, WM = T.wm, WN = T.wn, STAGES = T.stages;
   constexpr int kSmem = gemm_smem<BM, BN, STAGES, KIND>();
   static_assert(kSmem <= 160 * 1024, "LDS of a CU");
   auto kern = fp8_gemm_kernel<BM, BN, WM, WN, STAGES, KIND, OUT>;
@@ -874,6 +881,15 @@ int launch_few(const GemmParams& P, int dev, hipStream_t st) {
   return check_launch("dsa_fp8_gemm");
 }
 
+// The kernel of tile `tile`.
+template <int KIND, int OUT, int I = 0>
+int launch_one(int tile, const GemmParams& P, int dev, hipStream_t st) {
+  if constexpr (I + 1 < kTileCount<KIND>) {
+    if (tile != I) return launch_one<KIND, OUT, I + 1>(tile, P, dev, st);
+  }
+  return launch_tile<KIND, I, OUT>(P, dev, st);
+}
+
 template <int OUT>
 int launch_plan(const Plan& p, int kind, const GemmParams& P, int dev, hipStream_t st) {
   if (p.tile == kFewTile) {
@@ -885,26 +901,7 @@ int launch_plan(const Plan& p, int kind, const GemmParams& P, int dev, hipStream
            : p.splits == 8 ? launch_few<8, 1, kScaleF32, OUT>(P, dev, st)
                            : launch_few<4, 1, kScaleF32, OUT>(P, dev, st);
   }
-  if (kind == kScaleE8M0) {
-    switch (p.tile) {
-      case 0: return launch_tile<32, 64, 32, 32, 3, kScaleE8M0, OUT>(P, dev, st);
-      case 1: return launch_tile<64, 64, 32, 32, 3, kScaleE8M0, OUT>(P, dev, st);
-      case 2: return launch_tile<64, 128, 32, 64, 3, kScaleE8M0, OUT>(P, dev, st);
-      case 3: return launch_tile<128, 128, 64, 64, 2, kScaleE8M0, OUT>(P, dev, st);
-      case 4: return launch_tile<128, 128, 64, 64, 3, kScaleE8M0, OUT>(P, dev, st);
-      case 5: return launch_tile<256, 128, 64, 64, 2, kScaleE8M0, OUT>(P, dev, st);
-      case 6: return launch_tile<256, 256, 128, 64, 2, kScaleE8M0, OUT>(P, dev, st);
-      default: return launch_tile<256, 256, 128, 128, 2, kScaleE8M0, OUT>(P, dev, st);
-    }
-  }
-  switch (p.tile) {
-    case 0: return launch_tile<32, 64, 32, 32, 3, kScaleF32, OUT>(P, dev, st);
-    case 1: return launch_tile<64, 64, 32, 32, 3, kScaleF32, OUT>(P, dev, st);
-    case 2: return launch_tile<64, 128, 32, 64, 2, kScaleF32, OUT>(P, dev, st);
-    case 3: return launch_tile<64, 128, 32, 64, 3, kScaleF32, OUT>(P, dev, st);
-    case 4: return launch_tile<256, 128, 64, 64, 2, kScaleF32, OUT>(P, dev, st);
-    default: return launch_tile<256, 256, 128, 64, 2, kScaleF32, OUT>(P, dev, st);
-  }
+  return kind == kScaleE8M0 ? launch_one<kScaleE8M0, OUT>(p.tile, P, dev, st) : launch_one<kScaleF32, OUT>(p.tile, P, dev, st);
 }
 
 template <int OUT>
@@ -923,6 +920,22 @@ size_t dsa_fp8_gemm_workspace_bytes(int m, int n, int k, int scale_kind) {
   using namespace dsa;
   if (m <= 0 || n <= 0 || k <= 0 || (scale_kind != kScaleF32 && scale_kind != kScaleE8M0)) return 0;
   return workspace_of(plan_of(m, n, k, scale_kind, device_cus(current_device())), m, n);
+}
+
+int dsa_fp8_gemm_plan(int m, int n, int k, int scale_kind, int cus, int* out) {
+  using namespace dsa;
+  if (m <= 0 || n <= 0 || k <= 0 || cus < 0 || (scale_kind != kScaleF32 && scale_kind != kScaleE8M0) || !out)
+    return set_error(kInvalidArgument, "dsa_fp8_gemm_plan: bad arguments");
+  const Plan p = plan_of(m, n, k, scale_kind, cus ? cus : device_cus(current_device()));
+  if (p.tile == kFewTile) {
+    const int few[5] = {m > kFew ? 2 * kFew : kFew, kFew, p.splits, 2, 1};
+    std::copy(few, few + 5, out);
+  } else {
+    const Tile& T = tiles_of(scale_kind)[p.tile];
+    const int tile[5] = {T.bm, T.bn, T.bm / T.wm * (T.bn / T.wn), T.stages, p.splits};
+    std::copy(tile, tile + 5, out);
+  }
+  return kOk;
 }
 
 int dsa_fp8_gemm(const uint8_t* a, int64_t a_stride, const void* a_scale, int64_t a_scale_stride, const uint8_t* b,

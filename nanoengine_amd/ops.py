@@ -8,6 +8,7 @@ synchronises the host, so the calls are capturable in a HIP graph.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 
 import torch
@@ -1169,6 +1170,15 @@ def act_quant(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.
 
 def fp8_gemm_workspace_bytes(m: int, n: int, k: int, scale_dtype: torch.dtype = torch.float8_e8m0fnu) -> int:
     return int(_lib.load().dsa_fp8_gemm_workspace_bytes(int(m), int(n), int(k), _SCALE_KINDS[scale_dtype]))
+
+
+def fp8_gemm_plan(m: int, n: int, k: int, scale_dtype: torch.dtype = torch.float8_e8m0fnu,
+                  cus: int = 0) -> tuple[int, int, int, int, int]:
+    """(rows, columns, waves, blocks staged, parts of K) of the kernel that ``fp8_gemm`` takes for a shape, on the current
+    device or one of ``cus`` compute units (see dsa_fp8_gemm_plan)."""
+    out = (ctypes.c_int * 5)()
+    _lib.call("dsa_fp8_gemm_plan", int(m), int(n), int(k), _SCALE_KINDS[scale_dtype], int(cus), ctypes.addressof(out))
+    return tuple(out)
 
 
 @functools.lru_cache(maxsize=4096)
