@@ -197,6 +197,7 @@ fp8_gemm_kernel(const GemmParams P) {
   static_assert(kPerA * kWaves * 8 == BM && kPerB * kWaves * 8 == BN, "rows dealt out evenly");
   static_assert(kWaves % 2 == 0, "a wave's rows of a stage have one order of pieces");
   static_assert(kBlock % WN == 0, "one weight scale a wave");
+  static_assert(STAGES == 2 || STAGES == 3, "one block on its way behind the next, or none");
   static_assert(64 % kScales == 0 && kScales >= 4, "weight scales are replaced where a chunk is");
   constexpr int kThreads = kWaves * 64, kPieces = (kRowPieces * BM + kThreads - 1) / kThreads;  // of a scale chunk, a thread
   static_assert(kRowPieces * BM % (kPieces * 64) == 0, "whole waves bring scales");
@@ -429,10 +430,7 @@ fp8_gemm_kernel(const GemmParams P) {
             if (LAST) wait_loads<0>();
             meet<kPerB>();
           } else if (LAST) {
-            const int left = steps - 2 - s;
-            if (left >= STAGES - 2) wait_loads<(STAGES - 2) * (kPerA + kPerB)>();
-            else if (STAGES > 4 && left == 2) wait_loads<2 * (kPerA + kPerB)>();
-            else if (STAGES > 3 && left == 1) wait_loads<kPerA + kPerB>();
+            if (steps - 2 - s >= STAGES - 2) wait_loads<(STAGES - 2) * (kPerA + kPerB)>();
             else wait_loads<0>();
             meet<(STAGES - 2) * (kPerA + kPerB)>();
           } else {
