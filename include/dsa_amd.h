@@ -643,7 +643,7 @@ DSA_API int dsa_batch_tables(const int32_t* cached_lens, const int32_t* new_lens
  * One of out and codes at least. 1 <= dim <= 32768. A launch holds fewer than 2^32 threads, of which a
  * row takes 64 (dim <= 512), 256 (<= 2048), 512 (<= 4096) or 1024. Rows that are 16-byte aligned (codes
  * 8-byte) and a dim that is a multiple of 8 take wide loads, others narrow ones. Apart from
- * the pairs named, outputs must not overlap inputs. */
+ * the pairs named, of the same row stride, outputs overlap neither inputs nor one another. */
 DSA_API int dsa_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                          void* residual_out, int64_t residual_out_stride, const void* weight,
                          int weight_is_f32, float eps, int64_t rows, int dim, void* out, int64_t out_stride,

@@ -255,6 +255,12 @@ int dsa_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t 
   if (rows > 1 && (x_stride < dim || (residual && residual_stride < dim) || (residual_out && residual_out_stride < dim) ||
                    (out && out_stride < dim) || (codes && (code_stride < dim || scale_stride < blocks))))
     return set_error(kInvalidArgument, "dsa_rms_norm: rows overlap");
+  if (out && out == residual_out)
+    return set_error(kInvalidArgument, "dsa_rms_norm: out and residual_out are the same memory");
+  if (rows > 1 && ((out && out == x && out_stride != x_stride) ||
+                   (residual_out && ((residual_out == x && residual_out_stride != x_stride) ||
+                                     (residual_out == residual && residual_out_stride != residual_stride)))))
+    return set_error(kInvalidArgument, "dsa_rms_norm: in place, rows need the same stride");
   if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) |
         reinterpret_cast<uintptr_t>(residual_out) | reinterpret_cast<uintptr_t>(out)) & 1) ||
       (reinterpret_cast<uintptr_t>(weight) & (weight_is_f32 ? 3 : 1)) ||

@@ -197,6 +197,12 @@ bool rope_apart(int64_t tokens, int64_t token, int64_t heads, int64_t head, int 
   return (head >= rot && token >= (heads - 1) * head + rot) || (token >= rot && head >= (tokens - 1) * token + rot);
 }
 
+// In place, every row is where it was.
+bool rope_in_place(const void* x, int64_t tokens, int64_t token, int64_t heads, int64_t head, const void* out, int64_t out_token,
+                   int64_t out_head) {
+  return heads == 0 || x != out || ((tokens <= 1 || token == out_token) && (heads <= 1 || head == out_head));
+}
+
 bool rope_aligned(const void* p, int64_t token, int64_t head) {
   return !p || (!(reinterpret_cast<uintptr_t>(p) & 15) && !(token & 7) && !(head & 7));
 }
@@ -226,6 +232,9 @@ extern "C" int dsa_rope(const void* q, int64_t q_token_stride, int64_t q_head_st
   if (!rope_apart(num_tokens, q_out_token_stride, q_heads, q_out_head_stride, rot_dim) ||
       !rope_apart(num_tokens, k_out_token_stride, k_heads, k_out_head_stride, rot_dim))
     return set_error(kInvalidArgument, "dsa_rope: output rows overlap");
+  if (!rope_in_place(q, num_tokens, q_token_stride, q_heads, q_head_stride, q_out, q_out_token_stride, q_out_head_stride) ||
+      !rope_in_place(k, num_tokens, k_token_stride, k_heads, k_head_stride, k_out, k_out_token_stride, k_out_head_stride))
+    return set_error(kInvalidArgument, "dsa_rope: in place, rows need the same strides");
   int lanes = 1, shift = 0;
   while (lanes * 8 < rot_dim) lanes <<= 1, ++shift;
   RopeParams P = {{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k)},
