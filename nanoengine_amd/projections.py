@@ -32,7 +32,8 @@ def quantize_weight(weight: torch.Tensor, scale_dtype: torch.dtype = torch.float
         raise ValueError(f"scale_dtype must be float32 or float8_e8m0fnu, got {scale_dtype}")
     (N, K), B = weight.shape, ops.FP8_BLOCK
     full = torch.nn.functional.pad(weight.float(), (0, -K % B, 0, -N % B)).view(-(-N // B), B, -(-K // B), B)
-    scale = full.abs().masked_fill(full.isnan(), 0.0).amax(dim=(1, 3)).clamp_min(2.0 ** -40) / 448.0
+    top = full.abs().masked_fill(full.isnan(), 0.0).amax(dim=(1, 3)).clamp_min(2.0 ** -40)
+    scale = top / torch.full_like(top, 448.0)  # (by a number, torch multiplies with its rounded inverse on the GPU)
     if scale_dtype is torch.float8_e8m0fnu:
         bits = scale.view(torch.int32)  # positive: the exponent, one more where a fraction is left
         byte = ((bits >> 23) + ((bits & 0x7FFFFF) != 0).to(torch.int32)).clamp_max(254)

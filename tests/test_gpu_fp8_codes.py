@@ -39,3 +39,15 @@ def test_codes_of_the_norm(cuda, scale_dtype):
     tall = (x * weight).float()[:, :1000]
     codes, scales = projections.quantize_weight(tall, scale_dtype)
     assert torch.equal(codes.view(torch.uint8).cpu(), quotient_codes(tall, scales.repeat_interleave(128, dim=0)[:64]))
+
+
+def test_scales_are_the_rounded_quotient(cuda):
+    """float32 scales of activations and of weights: max(amax, 2^-40) / 448 rounded once, on whichever device."""
+    g = torch.Generator(device=cuda).manual_seed(9)
+    x = torch.randn(512, 1600, generator=g, device=cuda).to(BF)
+    blocks = torch.nn.functional.pad(x.double().abs().cpu(), (0, 64)).view(512, 13, 128)
+    want = (blocks.amax(-1).clamp_min(2.0 ** -40) / 448).float()
+    assert torch.equal(ops.act_quant(x, scale_dtype=F32)[1].cpu(), want)
+    want = blocks.view(4, 128, 13, 128).amax((1, 3)).clamp_min(2.0 ** -40)
+    for w in (x, x.cpu()):
+        assert torch.equal(projections.quantize_weight(w, F32)[1].cpu(), (want / 448).float())
