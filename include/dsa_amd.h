@@ -641,9 +641,11 @@ DSA_API int dsa_batch_tables(const int32_t* cached_lens, const int32_t* new_lens
  *   scales       [rows, ceil(dim / 128)] of scale_kind, row stride scale_stride elements
  *                (NULL exactly when codes is)
  * One of out and codes at least. 1 <= dim <= 32768. A launch holds fewer than 2^32 threads, of which a
- * row takes 64 (dim <= 512), 256 (<= 2048), 512 (<= 4096) or 1024. Rows that are 16-byte aligned (codes
- * 8-byte) and a dim that is a multiple of 8 take wide loads, others narrow ones. Apart from
- * the pairs named, of the same row stride, outputs overlap neither inputs nor one another. */
+ * row takes 64 (dim <= 512), 256 (<= 2048), 512 (<= 4096) or 1024. The sum of squares is f32: a row
+ * whose own passes 2^128 (elements of 2^64) gives zeros, and one whose own vanishes, with eps 0,
+ * infinities or NaN. Rows that are 16-byte aligned (codes 8-byte) and a dim that is a multiple of 8
+ * take wide loads, others narrow ones. Apart from the pairs named, of the same row stride, outputs
+ * overlap neither inputs nor one another. */
 DSA_API int dsa_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                          void* residual_out, int64_t residual_out_stride, const void* weight,
                          int weight_is_f32, float eps, int64_t rows, int dim, void* out, int64_t out_stride,

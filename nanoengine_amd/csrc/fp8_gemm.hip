@@ -19,8 +19,8 @@
 // (rows are half the banks' span apart; with row % 8 two of 16 met on each bank: 1e8 conflict
 // cycles in 8192 x 8192 x 16384, now 2e6).
 //
-// What bounds it, measured: 8192 x 8192 x 16384 (e8m0) 735-765 us, 2.9 to 3.0 PFLOP/s, where the library's product with
-// one scale a matrix takes 720-765 on the same cards and one with a scale per 32 elements 1450. Products run in 79% of
+// What bounds it, measured: 8192 x 8192 x 16384 (e8m0) 735 to 780 us by card, 2.8 to 3.0 PFLOP/s, where the library's product
+// with one scale a matrix takes 720 to 770 and one with a scale per 32 elements 1450. Products run in 79% of
 // a SIMD's cycles, and the clock gives way under their power: without any copies it takes 698, with all data in L2 780
 // of then 811, without scales 3% less; persistent workgroups, which close the gaps between tiles, gain nothing. Steps
 // that brought it there from the first kernel's 1125: operands read ahead of their products 875, copies sent between
@@ -29,7 +29,7 @@
 // 573, of which copies are 115 and the joining 80. (128 x 64 with all of its second accumulators does not fit the
 // registers, 909.) Short K is bound by a tile's start and end (8192 x 24576 x 1536 298 us where its operations take
 // 189); few tiles of long K by the steps of one tile (0.49 us for 128^3, one wave a SIMD) and the second launch: 333 x
-// 2112 x 8192, four parts of K, 15 + 4 us.
+// 2112 x 8192, four parts of K, 14 to 16 + 4 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -744,7 +744,8 @@ fp8_gemm_sum_kernel(const float* __restrict__ part, int splits, int m, int n, vo
 }
 
 // The tiles there are, and what a product of G of them takes, in us: fitted to measurements of several hundred shapes (1 to
-// 8192 rows, 64 to 24576 columns, 128 to 8192 deep), of which the choice is 1% slower than the best on average.
+// 8192 rows, 64 to 24576 columns, 128 to 8192 deep). Over 360 others the choice takes 1.004 times the best form's time in the
+// mean, above 64 rows 1.007, and 1.17 at worst.
 //   n = ceil(G / CUs) tiles a CU, r = ceil(n / resident) of them after one another, steps blocks of K each:
 //   base + n (per_tile + steps per_step) + r (per_round + steps per_round_step)
 // Small tiles keep every CU and its memory path busy where there are few rows (1 x 8192 x 1536 by 32 x 64 tiles of
@@ -780,8 +781,8 @@ struct Plan {
 
 Plan plan_of(int m, int n, int k, int kind, int cus) {
   const int kblocks = (k + kBlock - 1) / kBlock;
-  // Few rows: the kernel of their own as far as a wave's scales reach. Up to 32: 1.4 times as fast as the best tile over 110
-  // shapes (64 to 24576 columns, 128 to 16384 deep), by four waves, of which a CU holds two groups (32 x 8192 x 8192
+  // Few rows: the kernel of their own as far as a wave's scales reach. Up to 32: 1.4 times as fast as the best tile over 125
+  // shapes (64 to 24576 columns, 128 to 8192 deep), by four waves, of which a CU holds two groups (32 x 8192 x 8192
   // 13.5 us, by eight 15.6), and by eight where K is too long for four. Up to 64 where every group has a CU at once (64 x
   // 8192 x 1536 6.2 us, by tiles 8.3; 64 x 24576 x 1536 14.8 and 11.3), and K is short or half of the CUs have one (64 x 576
   // x 8192 11.1 and 9.0).
