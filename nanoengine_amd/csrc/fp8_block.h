@@ -35,8 +35,8 @@ __device__ __forceinline__ uint32_t block_scale(float amax) {
 
 // Eight elements of a block over its scale, in two words of four codes. For a power of two that is a product with its exact
 // inverse (byte 254 has a subnormal one, which the products keep). For a float32 scale q = y (1 / s) is off by a step or so,
-// which gives codes next to a tie their neighbours' value (1 of 2000 in rows of bf16); the remainder y - q s is exact in
-// one fused operation, and q + remainder (1 / s) is y / s rounded once (Markstein, 1990: IBM J. Res. Dev. 34). Eight
+// which gives codes next to a tie their neighbours' value (1 of 2000 in rows of bf16); the remainder q s - y is exact in
+// one fused operation, and q - remainder (1 / s) is y / s rounded once (Markstein, 1990: IBM J. Res. Dev. 34). Eight
 // divisions instead took 8192 x 8192 from 38 to 47 us. (Remainders lose bits where |q| is far below the smallest code's
 // half, 2^-10. An infinite scale counts as 0 in them: what is finite over it is 0.)
 template <int KIND>
@@ -47,7 +47,7 @@ __device__ __forceinline__ uint2 block_codes(const float* y, uint32_t scale) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float first = y[j] * inv;
-      q[j] = fmaf(fmaf(-first, by, y[j]), inv, first);
+      q[j] = fmaf(-fmaf(first, by, -y[j]), inv, first);  // (so written, a zero keeps its sign)
     }
   } else {
     const float inv = __uint_as_float(scale < 254u ? (254u - scale) << 23 : 0x400000u);

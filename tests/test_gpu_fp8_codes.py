@@ -51,3 +51,16 @@ def test_scales_are_the_rounded_quotient(cuda):
     want = blocks.view(4, 128, 13, 128).amax((1, 3)).clamp_min(2.0 ** -40)
     for w in (x, x.cpu()):
         assert torch.equal(projections.quantize_weight(w, F32)[1].cpu(), (want / 448).float())
+
+
+@pytest.mark.parametrize("scale_dtype", [F32, E8M0])
+def test_signs_of_zeros(cuda, scale_dtype):
+    """Zeros, and what is rounded to zero, keep their sign, as a quotient does; over an infinite scale too."""
+    x = torch.zeros(3, 128, dtype=BF, device=cuda)
+    x[:, 1], x[:, 2], x[:, 3], x[:, 4] = -0.0, -1e-30, 1e-30, -3.0
+    x[1, 5] = 1e30
+    x[2, 6] = float("inf")
+    codes, scales = ops.act_quant(x, scale_dtype=scale_dtype)
+    got, want = codes.view(torch.uint8).cpu(), quotient_codes(x, scales)
+    got[2, 6] = want[2, 6] = 0  # (NaN; its sign is free)
+    assert torch.equal(got, want)
