@@ -6,8 +6,10 @@
 
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 namespace dsa {
@@ -68,6 +70,9 @@ __device__ __forceinline__ uint32_t f32x4_to_fp8(float a, float b, float c, floa
   w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
   return (uint32_t)w;
 }
+
+// Two floats -> two bf16 in a word (round to nearest even).
+__device__ __forceinline__ int pack2(float a, float b) { return __builtin_bit_cast(int, (v2bf){(__bf16)a, (__bf16)b}); }
 
 __device__ __forceinline__ float bf16_to_f32(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
 

@@ -43,8 +43,6 @@ namespace dsa {
 namespace {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
-typedef int v2i __attribute__((ext_vector_type(2)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 struct GemmParams {
   const uint8_t *a, *b;
@@ -97,8 +95,6 @@ template <int KIND>
 __device__ __forceinline__ uint32_t load_scale(const void* s, int64_t i) {
   return KIND == kScaleF32 ? static_cast<const uint32_t*>(s)[i] : (uint32_t)static_cast<const uint8_t*>(s)[i];
 }
-
-__device__ __forceinline__ int pack2(float a, float b) { return __builtin_bit_cast(int, (v2bf){(__bf16)a, (__bf16)b}); }
 
 // 16 bytes of results from element `at` on, of which `left` lie inside the row.
 template <int OUT>

@@ -40,7 +40,6 @@ namespace dsa {
 namespace {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
-typedef int v2i __attribute__((ext_vector_type(2)));
 
 constexpr int kPage = 64, kDim = 128, kHeads = 64;
 constexpr int kCodeBytes = kPage * kIdx4KeyBytes;                        // 4096

@@ -85,12 +85,10 @@ __device__ __forceinline__ void unpack8(v4i v, float* x) {
   }
 }
 
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ v4i pack8(const float* x) {
   v4i v;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    v[j] = __builtin_bit_cast(int, (v2bf){(__bf16)x[2 * j], (__bf16)x[2 * j + 1]});
+  for (int j = 0; j < 4; ++j) v[j] = pack2(x[2 * j], x[2 * j + 1]);
   return v;
 }
 

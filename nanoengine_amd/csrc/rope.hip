@@ -44,14 +44,8 @@ struct RopeParams {
   int q_groups;
 };
 
-typedef int v2i __attribute__((ext_vector_type(2)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-
 __device__ __forceinline__ float lo_f32(int v) { return __uint_as_float((uint32_t)v << 16); }
 __device__ __forceinline__ float hi_f32(int v) { return __uint_as_float((uint32_t)v & 0xffff0000u); }
-__device__ __forceinline__ int pack2(float a, float b) {
-  return __builtin_bit_cast(int, (v2bf){(__bf16)a, (__bf16)b});
-}
 
 // The value of the other lane of two neighbours (both of them active).
 __device__ __forceinline__ int neighbour(int v) { return __builtin_amdgcn_mov_dpp(v, 0xb1, 15, 15, true); }

@@ -81,8 +81,6 @@
 namespace dsa {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
-typedef int v2i __attribute__((ext_vector_type(2)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef unsigned short v2u16 __attribute__((ext_vector_type(2)));
 
 constexpr int kMlaThreads = 512;
@@ -430,7 +428,6 @@ __device__ __forceinline__ void issue_index(const MlaParams& P, uint8_t* smem, c
                           (c.lane & (kFreshKeys - 1));
   dma4(src, __builtin_amdgcn_readfirstlane(lds_addr(smem + kRingOff + (j % kRingSlots) * 256)));
 }
-
 
 // Start of iteration t (both roles, every wave): the index load of block t+4;
 // this wave's share of block t+1's rows.
