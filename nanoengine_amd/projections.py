@@ -96,17 +96,17 @@ class MlaProjections:
         and the residual stream, which is ``residual`` itself, updated, or ``hidden`` where there is none yet. Arguments
         that do not fit are refused before it is updated."""
         T, rank, H = hidden.shape[0], self.q_rank, self.heads
-        ops._positions(positions, T)
-        ops._slots(slot_mapping, T)
-        ops.mla_kv_geometry(kv_cache)
-        ops._key_pages(indexer_cache, page_size, ops.INDEXER_ROW_BYTES)
-        ops._gpu(hidden, positions, slot_mapping, kv_cache, indexer_cache)
         q_idx = torch.empty(T, IDX_HEADS, ops.INDEXER_HEAD_DIM, dtype=torch.float8_e4m3fn, device=hidden.device)
         weights = torch.empty(T, IDX_HEADS, dtype=torch.float32, device=hidden.device)
         q_mla = torch.empty(T, H, ops.MLA_D_QK, dtype=torch.bfloat16, device=hidden.device)
         stream = hidden if residual is None else residual
         if T == 0:
             return q_idx, weights, q_mla, stream
+        ops._positions(positions, T)
+        ops._slots(slot_mapping, T)
+        ops.mla_kv_geometry(kv_cache)
+        ops._key_pages(indexer_cache, page_size, ops.INDEXER_ROW_BYTES)
+        ops._gpu(hidden, positions, slot_mapping, kv_cache, indexer_cache)
         h = torch.empty_like(hidden)
         coded = ops.rms_norm_quant(hidden, self.norm, self.eps, out=h, residual=residual, residual_out=residual,
                                    scale_dtype=self.scale_dtype)

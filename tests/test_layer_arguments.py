@@ -46,3 +46,11 @@ def test_arguments_before_the_residual(monkeypatch):
     assert not reached
     with pytest.raises(RuntimeError, match="reached"):
         layer.inputs(**good)
+
+
+def test_no_tokens_ask_for_nothing():
+    layer = projections.MlaProjections(**weights(), cos_sin_cache=torch.zeros(8, 64))
+    hidden = torch.zeros(0, 256, dtype=BF)
+    for positions in (torch.zeros(0, dtype=torch.int64), torch.zeros(5, dtype=torch.int64), None):
+        q_idx, w, q, stream = layer.inputs(hidden, None, positions, positions, None, None)
+        assert q_idx.shape == (0, 64, 128) and w.shape == (0, 64) and q.shape == (0, 2, 576) and stream is hidden
